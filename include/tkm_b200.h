@@ -39,7 +39,9 @@ const char *tkb_version(void);
 /* Message describing the last failing call made from this host thread. */
 const char *tkb_last_error(void);
 /* Synchronizes `stream`, reads and clears the device error word (0 = none).
- * Bit 0: a bounded wait inside a kernel timed out; bit 1: bad launch. */
+ * Bit 0: a bounded wait inside a kernel timed out; bit 1: bad launch;
+ * bit 2: device data named a page, slot or row that does not exist (the
+ * access was left out). */
 int tkb_device_error(unsigned int *code, void *stream);
 /* Number of kernels this library launched since load (all entry points). */
 unsigned long long tkb_launch_count(void);
@@ -243,6 +245,119 @@ size_t tkb_lmhead_ce_workspace(int rows, int V);
 int tkb_lmhead_ce(const void *X, long long ldx, const void *W, long long ldw, const float *bias,
                   const int32_t *labels, void *dlogits, long long ldd, float *loss, int *correct,
                   void *workspace, size_t workspace_bytes, int rows, int d, int V, void *stream);
+
+/* ------------------------------------------------------------ paged key-value cache
+ * Generation (no counterpart in the reference, which runs whole sequences
+ * only).  The cache of one attention layer: a pool of pages, each holding
+ * page_size tokens of every kv head, and per sequence the list of its pages.
+ *   k, v         [n_pages][Hkv][page_size][D] of `dtype`, pages page_stride
+ *                elements apart (so K and V, or several layers, may share one
+ *                pool); 16-byte aligned, page_stride a multiple of 16 bytes.
+ *   pos          [n_pages][Hkv][page_size] position of the token a slot
+ *                holds, or NULL (needed by tkb_kv_evict).
+ *   weight       [n_pages][Hkv][page_size] accumulated attention weight of a
+ *                slot, or NULL (needed by tkb_kv_evict).
+ *   block_table  [B][max_pages]; slot j of sequence b lies in page
+ *                block_table[b][j / page_size].  Only the entries that the
+ *                lengths reach are read.
+ *   seq_lens     [B] tokens each sequence holds (0 allowed).
+ * page_size: a multiple of 16, at most 1024; D 64 or 128; B at most 4096.
+ * The struct itself is read on the host, during the call; everything it
+ * points to is device memory and is read when the kernels run, so a captured
+ * CUDA graph follows the lengths and tables.  A page outside [0, n_pages)
+ * or a length above max_pages * page_size sets bit 2 of the device error
+ * word: such slots count as not held, such rows are not written.  Sequences
+ * may share pages that only tkb_paged_attn_decode without `accumulate` reads. */
+typedef struct {
+    void *k, *v;
+    int32_t *pos;
+    float *weight;
+    const int32_t *block_table;
+    const int32_t *seq_lens;
+    long long page_stride;
+    int n_pages, page_size, max_pages;
+    int B, Hkv, D, dtype;
+} tkb_kv_cache;
+
+/* Lengths on the device: seq_lens[b] = min(seq_lens[b] + n_b, limit) and
+ * seen[b] += n_b (seen, the tokens a sequence has had so far, may be NULL),
+ * with n_b = row_start[b + 1] - row_start[b], or `add` when row_start is
+ * NULL.  Before a step: add 1 with limit max_pages * page_size (a sequence
+ * that would pass the limit sets bit 2 of the device error word); after an
+ * eviction: add 0 with limit `budget`. */
+int tkb_kv_lens(int32_t *seq_lens, int32_t *seen, const int32_t *row_start, int add, int limit, int B, void *stream);
+
+/* New tokens enter the cache.  Packed rows qkv [rows][(Hq + 2*Hkv)*D]
+ * (qkv_stride elements apart) get tkb_qkv_prep_fwd's bias, QKNorm and RoPE
+ * (same parameters), except that the position is the token's own:
+ * row_start [B + 1] gives the rows of each sequence (NULL: row b belongs to
+ * sequence b and rows == B); with n_b rows, row i of sequence b goes to slot
+ * seq_lens[b] - n_b + i and stands at position seen[b] - n_b + i (seen NULL:
+ * seq_lens).  seq_lens and seen therefore already count the new rows
+ * (tkb_kv_lens).  K and V go to the slot, the position to pos, 0 to weight
+ * (where present).  out (may be NULL) gets the prepared row: its Hq*D query
+ * columns, or with out_full the whole packed row, as tkb_gqa_attn_fwd and
+ * tkb_paged_attn_decode take it.  Rows that have no slot (n_b > seq_lens[b],
+ * a bad page) set bit 2 of the device error word; their out is written. */
+int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stride, const float *bias,
+                  const float *qk_gain, void *out, long long out_stride, int out_full, const int32_t *row_start,
+                  const int32_t *seen, int rows, int Hq, int has_qknorm, int has_rope, float theta,
+                  float rope_scale, float low_freq_factor, float high_freq_factor,
+                  float original_context_length, void *stream);
+
+/* Attention of one new token per sequence over its cached tokens: for query
+ * head h (kv head h / (Hq/Hkv)) s_j = scale * q . k_j over the seq_lens[b]
+ * slots, out = sum_j softmax(s)_j v_j, lse = ln sum_j exp(s_j).  q and out
+ * [B] rows of Hq*D (q_stride, out_stride elements apart, 16-byte aligned),
+ * lse [B][Hq] fp32 (may be NULL).  A sequence that holds nothing gets out 0
+ * and lse -inf.  With `accumulate`, weight[slot] of each kv head also grows by
+ * the sum over its query heads of softmax(s)_slot.  The work is cut over the
+ * cached lengths and joined in a fixed order: equal inputs give equal bits.
+ * workspace: tkb_paged_attn_decode_workspace bytes, 256-byte aligned, zeroed
+ * before its first use; every call leaves it fit for the next one.  Calls
+ * that may overlap need workspaces of their own. */
+size_t tkb_paged_attn_decode_workspace(const tkb_kv_cache *cache, int Hq, int accumulate);
+int tkb_paged_attn_decode(const tkb_kv_cache *cache, const void *q, long long q_stride, void *out,
+                          long long out_stride, float *lse, int Hq, float scale, int accumulate,
+                          void *workspace, size_t workspace_bytes, void *stream);
+
+/* Eviction by accumulated attention weight.  Every (sequence, kv head) that
+ * holds more than `budget` tokens keeps budget of them: those within the
+ * newest `recent` positions (pos >= seen[b] - recent) and the first `sinks`
+ * (pos < sinks), then the others by weight, largest first, equal weights by
+ * the lower slot (a NaN weight counts as the lowest).  Kept tokens in slots
+ * budget and above move, with pos and weight, into the freed slots below, in
+ * ascending order; slots budget and above are then free.  Slots hold no
+ * order: positions do.  recent + sinks <= budget.  seq_lens is left as it is,
+ * since layers share it: call tkb_kv_lens(seq_lens, NULL, NULL, 0, budget, B)
+ * after the last layer.  workspace: tkb_kv_evict_workspace bytes, 16-byte
+ * aligned; no state is kept in it. */
+size_t tkb_kv_evict_workspace(const tkb_kv_cache *cache);
+int tkb_kv_evict(const tkb_kv_cache *cache, const int32_t *seen, int budget, int recent, int sinks,
+                 void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------ sampling
+ * One token per row of logits [rows][V] (ld elements apart) from given
+ * uniform numbers u[rows] in [0, 1); temperature, top_k, top_p, min_p are per
+ * row, each array may be NULL (1, off, off, off).  With x the row, m its
+ * maximum: every token has the whole weight w = rint(exp(-(m - x) * (1/T)) *
+ * 2^31), so that sums of weights are exact and the result does not depend on
+ * their order.  In the order of falling logits, equal ones by index, the
+ * tokens kept are those of weight > 0 that are among the first top_k
+ * (top_k <= 0: all); whose preceding weights sum to less than top_p times
+ * the weight of those (top_p >= 1: all; the first always); and whose weight
+ * is at least min_p * 2^31.  The token is the first in index order at
+ * which the running sum of kept weights passes u times their total.
+ *   token[r]   the token, -1 when no logit is above -inf
+ *   logprob[r] ln of its share of the kept weight (may be NULL)
+ *   kept[r]    number of tokens kept (may be NULL)
+ * temperature 0 (or anything not above 0) takes the largest logit, the lowest
+ * index among equals, with logprob 0.  NaN logits count as -inf; +inf shares
+ * the whole weight.  top_p and u act as multiples of 2^-32.
+ * V at most 2^20. */
+int tkb_sample_logits(const void *logits, long long ld, const float *u, const float *temperature,
+                      const int32_t *top_k, const float *top_p, const float *min_p, int32_t *token,
+                      float *logprob, int32_t *kept, int rows, int V, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

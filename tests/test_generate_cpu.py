@@ -1,0 +1,120 @@
+"""Refusals of the generation entry points: bad arguments are turned down
+with a message before any CUDA call."""
+import ctypes
+
+import pytest
+
+import tokamak_b200
+from tokamak_b200.ops import _KVCacheStruct
+
+vp = ctypes.c_void_p
+
+
+def cache(**over):
+    f = dict(k=256, v=256, pos=256, weight=256, block_table=256, seq_lens=256, page_stride=2 * 16 * 64, n_pages=8,
+             page_size=16, max_pages=4, B=2, Hkv=2, D=64, dtype=1)
+    f.update(over)
+    return _KVCacheStruct(*[f[n] for n, _ in _KVCacheStruct._fields_])
+
+
+def decode(c, Hq=4, q=256, out=256, stride=256, acc=0, ws=256, n=1 << 30):
+    L = tokamak_b200.lib()
+    return L.tkb_paged_attn_decode(ctypes.byref(c) if c else None, vp(q), stride, vp(out), stride, None, Hq, 0.1, acc,
+                                   vp(ws), n, None)
+
+
+def append(c, rows=2, Hq=4, qkv=256, stride=8 * 64, out=256, out_stride=8 * 64, full=1, start=None, theta=1e4):
+    L = tokamak_b200.lib()
+    return L.tkb_kv_append(ctypes.byref(c), vp(qkv), stride, None, None, vp(out), out_stride, full, start, None, rows,
+                           Hq, 0, 1, theta, 1.0, 1.0, 4.0, 8192.0, None)
+
+
+def evict(c, budget=16, recent=4, sinks=4, seen=256, ws=256, n=1 << 30):
+    return tokamak_b200.lib().tkb_kv_evict(ctypes.byref(c), vp(seen), budget, recent, sinks, vp(ws), n, None)
+
+
+def message():
+    return tokamak_b200.lib().tkb_last_error().decode()
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(k=0), -1), (dict(seq_lens=0), -1), (dict(block_table=0), -1), (dict(k=264), -1), (dict(dtype=7), -1),
+    (dict(B=0), -1), (dict(B=5000), -3), (dict(D=96), -3), (dict(page_size=24), -1), (dict(page_size=2048), -1),
+    (dict(page_size=0), -1), (dict(page_stride=2 * 16 * 64 - 8), -1), (dict(page_stride=2 * 16 * 64 + 4), -1),
+    (dict(max_pages=1 << 28), -1), (dict(n_pages=0), -1), (dict(Hkv=0), -1)])
+def test_bad_caches(over, code):
+    c = cache(**over)
+    assert decode(c) == code and message()
+    assert append(c) == code and evict(c) == code
+    L = tokamak_b200.lib()
+    assert L.tkb_paged_attn_decode_workspace(ctypes.byref(c), 4, 0) == 0
+    assert L.tkb_kv_evict_workspace(ctypes.byref(c)) == 0
+
+
+def test_decode_refusals():
+    assert decode(None) == -1
+    assert decode(cache(), Hq=3) == -1 and "multiple" in message()
+    assert decode(cache(), Hq=0) == -1
+    assert decode(cache(), q=0) == -1 and decode(cache(), out=0) == -1
+    assert decode(cache(), q=264) == -1 and decode(cache(), stride=128) == -1 and decode(cache(), stride=260) == -1
+    assert decode(cache(weight=0), acc=1) == -1 and "weight" in message()
+    assert decode(cache(), ws=0) == -4 and decode(cache(), n=8) == -4 and decode(cache(), ws=272) == -4
+
+
+def test_append_refusals():
+    assert append(cache(), rows=3) == -1 and "row_start" in message()
+    assert append(cache(), rows=0) == -1 and append(cache(), Hq=0) == -1
+    assert append(cache(), qkv=0) == -1 and append(cache(), qkv=264) == -1
+    assert append(cache(), stride=8 * 64 - 8) == -1 and append(cache(), stride=8 * 64 + 4) == -1
+    assert append(cache(), out_stride=4 * 64) == -1
+    assert append(cache(), theta=0.0) == -1
+
+
+def test_evict_refusals():
+    assert evict(cache(pos=0)) == -1 and evict(cache(weight=0)) == -1 and evict(cache(), seen=0) == -1
+    assert evict(cache(), budget=0) == -1 and evict(cache(), budget=7) == -1 and evict(cache(), recent=-1) == -1
+    assert evict(cache(), ws=0) == -4 and evict(cache(), n=4) == -4
+
+
+def test_lens_refusals():
+    L = tokamak_b200.lib()
+    assert L.tkb_kv_lens(None, None, None, 1, 10, 4, None) == -1
+    assert L.tkb_kv_lens(vp(256), None, None, 1, 10, 0, None) == -1
+    assert L.tkb_kv_lens(vp(256), None, None, -1, 10, 4, None) == -1
+
+
+def test_sample_refusals():
+    L = tokamak_b200.lib()
+
+    def call(logits=256, ld=100, u=256, token=256, rows=2, V=100, dtype=0):
+        return L.tkb_sample_logits(vp(logits), ld, vp(u), None, None, None, None, vp(token), None, None, rows, V, dtype,
+                                   None)
+    assert call(logits=0) == -1 and call(u=0) == -1 and call(token=0) == -1
+    assert call(rows=0) == -1 and call(V=0) == -1 and call(ld=99) == -1 and call(dtype=3) == -1
+    assert call(V=(1 << 20) + 1, ld=1 << 21) == -3
+    assert call(logits=258) == -1
+
+
+def test_python_checks():
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, ops
+    k = torch.zeros(4, 2, 16, 64)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    c = ops.KVCache(k, k.clone(), table, lens)
+    assert c.capacity == 32
+    with pytest.raises(TkbError):
+        ops.KVCache(k, k[:, :, :, :32], table, lens)
+    with pytest.raises(TkbError):
+        ops.KVCache(k.transpose(1, 2), k.transpose(1, 2), table, lens)
+    with pytest.raises(TkbError):
+        ops.KVCache(k, k.clone(), table.long(), lens)
+    with pytest.raises(TkbError):
+        ops.KVCache(k, k.clone(), table, lens[:1])
+    with pytest.raises(TkbError):
+        ops.paged_attn_decode(c, torch.zeros(3, 4 * 64), 4)
+    with pytest.raises(TkbError):
+        ops.paged_attn_decode(c, torch.zeros(2, 4 * 64, dtype=torch.bfloat16), 4)
+    with pytest.raises(TkbError):
+        ops.sample_logits(torch.zeros(2, 8), torch.zeros(3))
+    with pytest.raises(TkbError):
+        ops.sample_logits(torch.zeros(2, 8), torch.zeros(2), top_k=torch.zeros(2))

@@ -56,6 +56,13 @@ _SIGS = {
     "tkb_lmhead_ce_workspace": ([_i, _i], _sz),
     "tkb_lmhead_ce": ([_vp, _ll, _vp, _ll, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _sz, _i, _i, _i, _vp], _i),
     "tkb_gemm": ([_vp, _ll, _i, _vp, _ll, _i, _vp, _ll, _i, _i, _vp, _i, _i, _i, _vp, _sz, _vp], _i),
+    "tkb_kv_lens": ([_vp, _vp, _vp, _i, _i, _i, _vp], _i),
+    "tkb_kv_append": ([_vp, _vp, _ll, _vp, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _f, _f, _f, _f, _f, _vp], _i),
+    "tkb_paged_attn_decode_workspace": ([_vp, _i, _i], _sz),
+    "tkb_paged_attn_decode": ([_vp, _vp, _ll, _vp, _ll, _vp, _i, _f, _i, _vp, _sz, _vp], _i),
+    "tkb_kv_evict_workspace": ([_vp], _sz),
+    "tkb_kv_evict": ([_vp, _vp, _i, _i, _i, _vp, _sz, _vp], _i),
+    "tkb_sample_logits": ([_vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp], _i),
     "tkb_gemm_swiglu": ([_vp, _ll, _vp, _ll, _i, _vp, _vp, _vp, _ll, _vp, _ll, _i, _i, _vp], _i),
 }
 

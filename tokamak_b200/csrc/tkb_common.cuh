@@ -22,6 +22,7 @@ __device__ unsigned int g_device_error = 0;
 enum : unsigned int {
   ERR_WAIT_TIMEOUT = 1u << 0,   // an mbarrier wait ran past its time limit
   ERR_BAD_LAUNCH   = 1u << 1,   // a kernel saw inconsistent launch arguments
+  ERR_BAD_INDEX    = 1u << 2,   // device data named a page, slot or row that does not exist
 };
 
 // Upper bound for any single mbarrier wait.  A correct pipeline never gets

@@ -212,3 +212,131 @@ def lmhead_ce(X, W, labels, bias=None, want_grad=True):
                               dl.stride(0) if dl is not None else 0, _p(loss), _p(corr), _p(ws), nws, rows, d, V,
                               _stream()), "tkb_lmhead_ce")
     return loss, dl, corr
+
+
+class _KVCacheStruct(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
+                ("page_stride", ctypes.c_longlong), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("B", ctypes.c_int), ("Hkv", ctypes.c_int), ("D", ctypes.c_int),
+                ("dtype", ctypes.c_int)]
+
+
+def _expect(t, name, shape, dtype):
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous()):
+        raise TkbError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, "
+                       f"got {t.dtype} {tuple(t.shape)}")
+
+
+class KVCache:
+    """One attention layer's paged key-value cache (tkb_kv_cache): tensors
+    k, v [n_pages, Hkv, page_size, D] (any page stride, the rest contiguous),
+    block_table [B, max_pages] and seq_lens [B] int32, and, for the eviction,
+    pos (int32) and weight (fp32) [n_pages, Hkv, page_size]."""
+
+    def __init__(self, k, v, block_table, seq_lens, pos=None, weight=None):
+        n_pages, Hkv, page, D = k.shape
+        B, max_pages = block_table.shape
+        for t, name in ((k, "k"), (v, "v")):
+            if tuple(t.shape) != (n_pages, Hkv, page, D) or t.dtype != k.dtype or \
+                    t.stride()[1:] != (page * D, D, 1) or t.stride(0) != k.stride(0):
+                raise TkbError(f"{name}: expected {k.dtype} [n_pages, Hkv, page_size, D], contiguous within a page, "
+                               "k and v with the same page stride")
+        _expect(block_table, "block_table", (B, max_pages), torch.int32)
+        _expect(seq_lens, "seq_lens", (B,), torch.int32)
+        _expect(pos, "pos", (n_pages, Hkv, page), torch.int32)
+        _expect(weight, "weight", (n_pages, Hkv, page), torch.float32)
+        self.k, self.v, self.block_table, self.seq_lens, self.pos, self.weight = k, v, block_table, seq_lens, pos, weight
+        self.B, self.Hkv, self.D, self.page_size, self.max_pages = B, Hkv, D, page, max_pages
+        # a single page has no stride of its own
+        stride = k.stride(0) if n_pages > 1 else Hkv * page * D
+        self.struct = _KVCacheStruct(k.data_ptr(), v.data_ptr(), pos.data_ptr() if pos is not None else None,
+                                     weight.data_ptr() if weight is not None else None, block_table.data_ptr(),
+                                     seq_lens.data_ptr(), stride, n_pages, page, max_pages, B, Hkv, D, dtype_code(k))
+        self.ref = ctypes.addressof(self.struct)
+
+    @property
+    def capacity(self):
+        """Tokens a sequence's table has room for."""
+        return self.max_pages * self.page_size
+
+
+def kv_lens(seq_lens, limit, seen=None, add=0, row_start=None):
+    """seq_lens = min(seq_lens + n, limit) and seen += n, on the device (n = add, or row_start's differences)."""
+    check(lib().tkb_kv_lens(_p(seq_lens), _p(seen), _p(row_start), int(add), int(limit), seq_lens.numel(), _stream()),
+          "tkb_kv_lens")
+
+
+def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None, qknorm=False, rope=True,
+              theta=10000.0, rope_scale=1.0, low=1.0, high=4.0, octx=8192.0, full=False, out=None):
+    """Packed rows qkv [rows, (Hq+2Hkv)*D] enter the cache (tkb_kv_append); returns the prepared query columns
+    [rows, Hq*D], or the whole prepared rows with `full`.  seq_lens and seen already count the new rows."""
+    if qkv.dtype != cache.k.dtype:
+        raise TkbError(f"kv_append: rows are {qkv.dtype}, the cache is {cache.k.dtype}")
+    rows = qkv.shape[0]
+    if out is None:
+        out = torch.empty(rows, (Hq + 2 * cache.Hkv if full else Hq) * cache.D, dtype=qkv.dtype, device=qkv.device)
+    check(lib().tkb_kv_append(cache.ref, _p(qkv), qkv.stride(0), _p(bias), _p(qk_gain), _p(out), out.stride(0),
+                              int(full), _p(row_start), _p(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
+                              low, high, octx, _stream()), "tkb_kv_append")
+    return out
+
+
+def paged_attn_workspace(cache, Hq, accumulate=False):
+    """Zeroed workspace of paged_attn_decode; one per stream that calls it."""
+    n = lib().tkb_paged_attn_decode_workspace(cache.ref, Hq, int(accumulate))
+    if n == 0:
+        check(-1, "tkb_paged_attn_decode_workspace")
+    return torch.zeros(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=None, workspace=None):
+    """Attention of one token per sequence over its cache: q [B, Hq*D] -> (out [B, Hq*D], lse [B, Hq] fp32)."""
+    if q.dtype != cache.k.dtype:
+        raise TkbError(f"paged_attn_decode: q is {q.dtype}, the cache is {cache.k.dtype}")
+    if q.shape[0] != cache.B:
+        raise TkbError(f"paged_attn_decode: {q.shape[0]} query rows for {cache.B} sequences")
+    if out is None:
+        out = torch.empty(cache.B, Hq * cache.D, dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty(cache.B, Hq, dtype=torch.float32, device=q.device)
+    if workspace is None:
+        workspace = paged_attn_workspace(cache, Hq, accumulate)
+    check(lib().tkb_paged_attn_decode(cache.ref, _p(q), q.stride(0), _p(out), out.stride(0), _p(lse), Hq,
+                                      cache.D ** -0.5 if scale is None else scale, int(accumulate), _p(workspace),
+                                      workspace.numel(), _stream()), "tkb_paged_attn_decode")
+    return out, lse
+
+
+def kv_evict_workspace(cache):
+    n = lib().tkb_kv_evict_workspace(cache.ref)
+    if n == 0:
+        check(-1, "tkb_kv_evict_workspace")
+    return torch.empty(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def kv_evict(cache, budget, seen, recent=0, sinks=0, workspace=None):
+    """Keep `budget` tokens of every (sequence, kv head) that holds more, by accumulated weight (tkb_kv_evict);
+    kv_lens(cache.seq_lens, budget) after the last layer."""
+    if workspace is None:
+        workspace = kv_evict_workspace(cache)
+    check(lib().tkb_kv_evict(cache.ref, _p(seen), int(budget), int(recent), int(sinks), _p(workspace),
+                             workspace.numel(), _stream()), "tkb_kv_evict")
+
+
+def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """(token int32, logprob fp32, kept int32) per row of logits [rows, V] from uniform numbers u [rows]
+    (tkb_sample_logits); the parameters are per-row tensors (top_k int32, the others fp32) or None."""
+    rows, V = logits.shape
+    if logits.stride(1) != 1:
+        raise TkbError("sample_logits: a row's logits must be contiguous")
+    for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
+        _expect(t, name, (rows,), dt)
+    token = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    kept = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    check(lib().tkb_sample_logits(_p(logits), logits.stride(0) if rows > 1 else V, _p(u), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
+                                  _p(token), _p(logprob), _p(kept), rows, V, dtype_code(logits), _stream()),
+          "tkb_sample_logits")
+    return token, logprob, kept
