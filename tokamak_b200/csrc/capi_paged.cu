@@ -90,9 +90,12 @@ int tkb_kv_append(const tkb_kv_cache* cache, const void* qkv, long long qkv_stri
 }
 
 size_t tkb_paged_attn_decode_workspace(const tkb_kv_cache* cache, int Hq, int accumulate) {
-  (void)accumulate;
-  if (cache_check("tkb_paged_attn_decode_workspace", cache) || Hq <= 0) return 0;
-  return 256;
+  if (cache_check("tkb_paged_attn_decode_workspace", cache)) return 0;
+  if (Hq <= 0 || Hq % cache->Hkv) {
+    fail(TKB_ERR_ARG, "tkb_paged_attn_decode_workspace: Hq (%d) must be a multiple of Hkv (%d)", Hq, cache->Hkv);
+    return 0;
+  }
+  return decode_ws(*cache, Hq, accumulate).bytes;
 }
 
 int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_stride, void* out,
@@ -121,11 +124,19 @@ int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_
   p.out_stride = out_stride;
   p.lse = lse;
   p.Hq = Hq;
+  p.G = Hq / cache->Hkv;
+  p.qblocks = (p.G + QT - 1) / QT;
   p.accumulate = accumulate ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
+  const DecodeWs w = decode_ws(*cache, Hq, accumulate);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.counters = reinterpret_cast<int*>(ws + w.counters);
+  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
+  p.scores = reinterpret_cast<float*>(ws + w.scores);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define CALL(T) paged_decode_t<T>(p, st)
-  return cuda_status(TKB_BY_DTYPE(cache->dtype, CALL), who, 1);
+  return cuda_status(TKB_BY_DTYPE(cache->dtype, CALL), who, accumulate ? 2 : 1);
 #undef CALL
 }
 

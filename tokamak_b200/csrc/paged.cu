@@ -166,6 +166,24 @@ static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
 }
 
 // ============================================================ attention of one token
+// out = softmax(scale q K^T) V for one query row per sequence: every cached K
+// and V value is read once and used by the G query heads of its kv head, so
+// HBM bounds it (4 G FLOP per element read) and the kernel is built around
+// keeping loads in flight.
+//
+// The keys of a unit (sequence, kv head, block of 16 query heads) are cut into
+// tiles of 16 (8 for fp32 rows of 512 bytes).  All units' tiles, in order, are
+// dealt out to one CTA per SM as equal runs, whatever the lengths: a run
+// starts and ends inside a unit, and the parts of a unit that several CTAs
+// took are joined by the CTA that finishes last (a counter in the
+// workspace), in the order of the run, so the result does not depend on who
+// that is.  Inside a run each of the CTA's 8 warps takes every eighth tile
+// with its own ring of cp.async buffers and its own running maximum and sum;
+// they meet only at the end of a unit.  The rings run ahead across units.
+constexpr int DW = 8;                 // warps per CTA
+constexpr int DNT = DW * 32;
+constexpr int QT = 16;                // query heads per unit (rows of the m16n8k16 product)
+
 struct DecodeParams {
   tkb_kv_cache c;
   const void* q;
@@ -173,81 +191,614 @@ struct DecodeParams {
   void* out;
   long long out_stride;
   float* lse;
-  int Hq, accumulate;
+  int Hq, G, qblocks, accumulate;
   float scale_log2;
+  int* counters;                      // per unit, 0 between calls
+  float* part;                        // [2 * grid][QT][D + 2]: O, then m, l of each row
+  float* lse2;                        // accumulate: [B][Hq], in powers of 2
+  float* scores;                      // accumulate: [B][Hq][cap], in powers of 2
 };
 
-// One block per (sequence, kv head); a warp per key, lanes over D.
+template <int D, int ES>
+struct DecodeTile {
+  static constexpr int RB = D * ES;                 // bytes of a row
+  static constexpr int TK = RB <= 256 ? 16 : 8;     // keys per tile
+  static constexpr int HALF = TK * RB;              // bytes of the K (or V) part
+  static constexpr int STAGES = ES == 4 ? 2 : 3 * 8192 / (2 * HALF);
+  static constexpr int RING = DW * STAGES * 2 * HALF;
+  static constexpr int MERGE = DW * 8 * D * 4;      // eight rows of every warp
+  static constexpr int EXTRA = ES == 4 ? QT * D * 4 + DW * QT * TK * 4 : 0;  // q, p
+  static constexpr int SMEM = RING + MERGE + EXTRA;
+};
+
+// Where a flattened tile index lies.
+struct TileAt {
+  int b, u, j;   // sequence, (kv head, query block), tile of the unit
+  int n, nt;     // tokens held, tiles (at least one, so that an empty sequence gets its zeros)
+};
+template <int TK>
+TKB_DEVFN void tile_seq(const tkb_kv_cache& c, TileAt& t) {
+  t.n = t.b < c.B ? held_of(c, t.b) : 0;
+  t.nt = max(1, (t.n + TK - 1) / TK);
+}
+template <int TK>
+TKB_DEVFN void tile_advance(const tkb_kv_cache& c, int units, TileAt& t, int by) {
+  t.j += by;
+  while (t.j >= t.nt && t.b < c.B) {
+    t.j -= t.nt;
+    if (++t.u == units) {
+      t.u = 0;
+      ++t.b;
+      tile_seq<TK>(c, t);
+    }
+  }
+}
+
+TKB_DEVFN void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+TKB_DEVFN void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+TKB_DEVFN void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+TKB_DEVFN void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+TKB_DEVFN void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool BF16>
+TKB_DEVFN void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Byte offset of 16-byte chunk `ch` of row `r` inside a tile half: the chunk
+// index is xored with the row so that eight rows' equal chunks (ldmatrix) lie
+// in eight different bank groups.
+template <int RB>
+TKB_DEVFN int swz(int r, int ch) {
+  return r * RB + ((ch ^ (r & 7)) << 4);
+}
+
+// The 16-bit tile: S = Q K^T and O += P V on m16n8k16 with the query heads as
+// the 16 rows (rows past G are zero).  Thread t holds rows t/4 and t/4 + 8.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int W = 4, E = D / 32;
-  __shared__ float s_m[W], s_l[W], s_o[W][D];
-  const tkb_kv_cache& c = p.c;
-  const int b = blockIdx.x / c.Hkv, h = blockIdx.x % c.Hkv, G = p.Hq / c.Hkv;
-  const int n = held_of(c, b), w = warp_id(), lane = lane_id();
-  const T* K = static_cast<const T*>(c.k);
-  const T* V = static_cast<const T*>(c.v);
-  for (int g = 0; g < G; ++g) {
-    const int hq = h * G + g;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
+struct TileMma {
+  static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  using Cfg = DecodeTile<D, 2>;
+  uint32_t q[D / 16][4];
+  float o[D / 8][4];
+  float m[2], l[2];
+
+  TKB_DEVFN void start(const DecodeParams& p, int b, int h0, int rows, uint8_t*) {
+    const int r = lane_id() >> 2, c = lane_id() & 3;
+    const T* src = static_cast<const T*>(p.q) + b * p.q_stride + static_cast<long long>(h0 + r) * D + 2 * c;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      q[e] = Elem<T>::ld(static_cast<const T*>(p.q) + b * p.q_stride + hq * D + lane * E + e) * p.scale_log2;
-      o[e] = 0.f;
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[k][i] = r + (i & 1) * 8 < rows
+                      ? __ldg(reinterpret_cast<const uint32_t*>(src + (i & 1) * 8 * D + k * 16 + (i >> 1) * 8))
+                      : 0u;
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[d][i] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  }
+
+  // `scores`: where the tile's scores of query head h0 go, or null
+  TKB_DEVFN void tile(const DecodeParams& p, const uint8_t* buf, uint8_t*, int valid, int rows, float* scores,
+                      long long score_stride) {
+    const int lane = lane_id(), mi = lane >> 3, ri = lane & 7;
+    const uint32_t kb = smem_u32(buf), vb = kb + Cfg::HALF;
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t f[4];
+      ldsm4(kb + swz<Cfg::RB>((mi >> 1) * 8 + ri, k * 2 + (mi & 1)), f);
+      mma16816<BF16>(s[0], q[k], f[0], f[1]);
+      mma16816<BF16>(s[1], q[k], f[2], f[3]);
     }
-    for (int j = w; j < n; j += W) {
-      const int page = page_of(c, b, j / c.page_size);
-      if (page < 0) continue;
-      const long long at = page_offset(c, page, h) + static_cast<long long>(j % c.page_size) * D + lane * E;
-      float s = 0.f;
+    const int c = 2 * (lane & 3);
 #pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], Elem<T>::ld(K + at + e), s);
-      s = warp_sum(s);
-      const float mn = fmaxf(m, s), keep = m == -INFINITY ? 0.f : exp2f(m - mn), pr = exp2f(s - mn);
-      l = l * keep + pr;
-      m = mn;
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(pr, Elem<T>::ld(V + at + e), o[e] * keep);
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] *= p.scale_log2;
+        if (valid < 16 && t * 8 + c + (i & 1) >= valid) s[t][i] = -INFINITY;
+      }
+    if (scores) {
+      const int r = lane >> 2;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (r + 8 * i < rows) {
+          float* at = scores + (r + 8 * i) * score_stride + c;
+          *reinterpret_cast<float2*>(at) = make_float2(s[0][2 * i], s[0][2 * i + 1]);
+          *reinterpret_cast<float2*>(at + 8) = make_float2(s[1][2 * i], s[1][2 * i + 1]);
+        }
     }
+    float mn[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float x = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      mn[i] = fmaxf(m[i], x);
+    }
+    if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1])) {
+      // a maximum of -inf stays -inf only while nothing was seen: l and o are 0 then
+      const float k0 = m[0] == -INFINITY ? 0.f : ex2(m[0] - mn[0]), k1 = m[1] == -INFINITY ? 0.f : ex2(m[1] - mn[1]);
+      l[0] *= k0;
+      l[1] *= k1;
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) {
+        o[d][0] *= k0;
+        o[d][1] *= k0;
+        o[d][2] *= k1;
+        o[d][3] *= k1;
+      }
+      m[0] = mn[0];
+      m[1] = mn[1];
+    }
+    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+    uint32_t a[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float p0 = ex2(s[t][0] - m0), p1 = ex2(s[t][1] - m0), p2 = ex2(s[t][2] - m1), p3 = ex2(s[t][3] - m1);
+      l[0] += p0 + p1;
+      l[1] += p2 + p3;
+      // P in 16 bits: the tensor cores take P and V in one type; the sum keeps 32
+      a[2 * t] = pack2<BF16>(p0, p1);
+      a[2 * t + 1] = pack2<BF16>(p2, p3);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      uint32_t f[4];
+      ldsm4_t(vb + swz<Cfg::RB>((mi & 1) * 8 + ri, d * 2 + (mi >> 1)), f);
+      mma16816<BF16>(o[2 * d], a, f[0], f[1]);
+      mma16816<BF16>(o[2 * d + 1], a, f[2], f[3]);
+    }
+  }
+
+  TKB_DEVFN void finish() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+  }
+  // rows 8*half .. 8*half+7 of this warp: O to so[8][D], (m, l) to sml
+  TKB_DEVFN void put(float* so, float2* sml, int half) {
+    const int r = lane_id() >> 2, c = lane_id() & 3;
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+      *reinterpret_cast<float2*>(so + r * D + d * 8 + 2 * c) = half ? make_float2(o[d][2], o[d][3])
+                                                                    : make_float2(o[d][0], o[d][1]);
+    if (c == 0) sml[r] = half ? make_float2(m[1], l[1]) : make_float2(m[0], l[0]);
+  }
+};
+
+// The fp32 tile on FMA units.  Scores: 32 / TK lanes share a key, each with
+// every (32 / TK)-th 16-byte chunk of its row.  Output: each lane owns D / 32
+// columns.  GT: query heads the registers are laid out for.
+template <int D, int GT>
+struct TileFma {
+  using Cfg = DecodeTile<D, 4>;
+  static constexpr int TK = Cfg::TK, PART = 32 / TK, CH = D / 4 / PART, E = D / 32;
+  float o[GT][E], m[GT], l[GT];
+
+  TKB_DEVFN void start(const DecodeParams& p, int b, int h0, int rows, uint8_t* extra) {
+    // the CTA's q, scaled, in shared memory (all warps wrote and read the last one before the merge's barrier)
+    float* sq = reinterpret_cast<float*>(extra);
+    const float* src = static_cast<const float*>(p.q) + b * p.q_stride + static_cast<long long>(h0) * D;
+    for (int i = threadIdx.x; i < rows * D; i += DNT) sq[i] = __ldg(src + i) * p.scale_log2;
     __syncthreads();
-    if (lane == 0) {
-      s_m[w] = m;
-      s_l[w] = l;
-    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) s_o[w][lane * E + e] = o[e];
-    __syncthreads();
-    float M = -INFINITY, Lsum = 0.f;
-    for (int i = 0; i < W; ++i) M = fmaxf(M, s_m[i]);
-    for (int i = 0; i < W; ++i) Lsum += s_m[i] == -INFINITY ? 0.f : s_l[i] * exp2f(s_m[i] - M);
-    const float lse2 = M == -INFINITY ? -INFINITY : M + log2f(Lsum);
-    for (int d = threadIdx.x; d < D; d += 128) {
-      float acc = 0.f;
-      for (int i = 0; i < W; ++i) acc += s_m[i] == -INFINITY ? 0.f : s_o[i][d] * exp2f(s_m[i] - M);
-      Elem<T>::st(static_cast<T*>(p.out) + b * p.out_stride + hq * D + d, M == -INFINITY ? 0.f : acc / Lsum);
+    for (int g = 0; g < GT; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[g][e] = 0.f;
     }
-    if (threadIdx.x == 0 && p.lse) p.lse[b * p.Hq + hq] = lse2 * 0.6931471805599453f;
-    if (p.accumulate)
-      for (int j = w; j < n; j += W) {
-        const int page = page_of(c, b, j / c.page_size);
-        if (page < 0) continue;
-        const int in_page = j % c.page_size;
-        const long long at = page_offset(c, page, h) + static_cast<long long>(in_page) * D + lane * E;
+  }
+
+  TKB_DEVFN void tile(const DecodeParams&, const uint8_t* buf, uint8_t* extra, int valid, int rows, float* scores,
+                      long long score_stride) {
+    const int lane = lane_id(), part = lane % PART;
+    // neighbouring keys in a phase of eight lanes differ in the bit that the swizzle moves by 64 bytes
+    const int kk = lane / PART;
+    const int key = TK == 8 ? ((kk & 1) << 2) | (kk >> 1) : ((kk & 3) << 1) | ((kk >> 2) & 1) | (kk & 8);
+    const float* sq = reinterpret_cast<const float*>(extra);
+    float* sp = reinterpret_cast<float*>(extra + QT * D * 4) + warp_id() * QT * TK;
+    float4 k[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      k[i] = *reinterpret_cast<const float4*>(buf + swz<Cfg::RB>(key, part + PART * i));
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+      if (g < rows) {
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(q[e], Elem<T>::ld(K + at + e), s);
-        s = warp_sum(s);
-        if (lane == 0) c.weight[meta_offset(c, page, h) + in_page] += exp2f(s - lse2);
+        for (int i = 0; i < CH; ++i) {
+          const float4 q = *reinterpret_cast<const float4*>(sq + g * D + (part + PART * i) * 4);
+          s = fmaf(q.x, k[i].x, s);
+          s = fmaf(q.y, k[i].y, s);
+          s = fmaf(q.z, k[i].z, s);
+          s = fmaf(q.w, k[i].w, s);
+        }
+#pragma unroll
+        for (int d = 1; d < PART; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (key >= valid) s = -INFINITY;
+        if (scores && part == 0) scores[g * score_stride + key] = s;
+        float x = s;
+#pragma unroll
+        for (int d = PART; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+        const float mn = fmaxf(m[g], x);
+        const float keep = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn), pr = mn == -INFINITY ? 0.f : ex2(s - mn);
+        m[g] = mn;
+        // every lane adds its own key's share: the lanes of a key carry it PART times
+        l[g] = l[g] * keep + pr;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[g][e] *= keep;
+        if (part == 0) sp[g * TK + key] = pr;
       }
+    }
+    __syncwarp();
+    const uint8_t* vb = buf + Cfg::HALF;
+#pragma unroll
+    for (int j = 0; j < TK; ++j) {
+      float v[E];
+      const uint8_t* at = vb + swz<Cfg::RB>(j, lane * E / 4) + (lane * E % 4) * 4;
+      if constexpr (E == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(at);
+        v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+      } else {
+        const float2 t = *reinterpret_cast<const float2*>(at);
+        v[0] = t.x; v[1] = t.y;
+      }
+#pragma unroll
+      for (int g = 0; g < GT; ++g)
+        if (g < rows) {
+          const float pr = sp[g * TK + j];
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[g][e] = fmaf(pr, v[e], o[g][e]);
+        }
+    }
+    __syncwarp();
   }
+
+  TKB_DEVFN void finish() {
+#pragma unroll
+    for (int g = 0; g < GT; ++g) l[g] = warp_sum(l[g]) * (1.0f / PART);
+  }
+  TKB_DEVFN void put(float* so, float2* sml, int half) {
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const int at = g + 8 * half;
+#pragma unroll
+      for (int x = 0; x < GT; ++x)
+        if (x == at) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) so[g * D + lane_id() * E + e] = o[x][e];
+          if (lane_id() == 0) sml[g] = make_float2(m[x], l[x]);
+        }
+    }
+  }
+};
+
+// One finished output row: lane holds columns lane*E ..
+template <typename T, int E>
+TKB_DEVFN void decode_store(const DecodeParams& p, int b, int hq, int lane, float M, float L, const float (&acc)[E]) {
+  constexpr int D = 32 * E;
+  const float inv = L == 0.f ? 0.f : 1.0f / L;  // nothing held: zeros
+  T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<long long>(hq) * D + lane * E;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = acc[e] * inv;
+  } else {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<uint32_t*>(out + e) = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
+  }
+  if (lane == 0) {
+    const float lse2 = M + lg2(L);  // -inf + -inf when nothing is held
+    if (p.lse) p.lse[static_cast<long long>(b) * p.Hq + hq] = lse2 * 0.6931471805599453f;
+    if (p.accumulate) p.lse2[static_cast<long long>(b) * p.Hq + hq] = lse2;
+  }
+}
+
+// Row g of the part of the unit starting at tile unit0 that CTA i left: in its
+// first slot when its run starts inside the unit or at its start, else in its second.
+template <int D>
+TKB_DEVFN const float* part_at(const DecodeParams& p, int i, long long total, int ctas, long long unit0, int g) {
+  const int slot = 2 * i + (total * i / ctas >= unit0 ? 0 : 1);
+  return p.part + (static_cast<long long>(slot) * QT + g) * (D + 2);
+}
+
+template <typename T, int D, typename Tile>
+__global__ void __launch_bounds__(DNT, 1) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+  using Cfg = DecodeTile<D, static_cast<int>(sizeof(T))>;
+  constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ long long s_start[DW];
+  __shared__ int s_valid[DW][ST];
+  __shared__ float2 s_ml[DW][8];
+  __shared__ long long s_base;
+  __shared__ int s_seq, s_last;
+  const tkb_kv_cache& c = p.c;
+  const int w = warp_id(), lane = lane_id(), tid = threadIdx.x, units = c.Hkv * p.qblocks;
+  uint8_t* ring = smem + w * ST * 2 * Cfg::HALF;
+  float* merge = reinterpret_cast<float*>(smem + Cfg::RING);
+  uint8_t* extra = smem + Cfg::RING + Cfg::MERGE;
+
+  // ---- this CTA's run of tiles: [t0, t1) of all `total` ones
+  long long total = 0, before = 0;
+  const int per = (c.B + DNT - 1) / DNT, s0 = min(c.B, tid * per), s1 = min(c.B, s0 + per);
+  long long mine = 0;
+  for (int b = s0; b < s1; ++b) mine += static_cast<long long>(max(1, (held_of(c, b) + TK - 1) / TK)) * units;
+  long long pre = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, pre, d);
+    if (lane >= d) pre += t;
+  }
+  if (lane == 31) s_start[w] = pre;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < DW; ++i) {
+    if (i < w) before += s_start[i];
+    total += s_start[i];
+  }
+  before += pre - mine;
+  // fewer CTAs than the grid when there is not a tile for every warp
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + DW - 1) / DW));
+  if (static_cast<int>(blockIdx.x) >= ctas) return;
+  const long long t0 = total * blockIdx.x / ctas, t1 = total * (blockIdx.x + 1) / ctas;
+  if (before <= t0 && t0 < before + mine) {
+    long long at = before;
+    int b = s0;
+    for (;; ++b) {
+      const long long nt = static_cast<long long>(max(1, (held_of(c, b) + TK - 1) / TK)) * units;
+      if (t0 < at + nt) break;
+      at += nt;
+    }
+    s_seq = b;
+    s_base = at;
+  }
+  __syncthreads();
+  TileAt cur;
+  cur.b = s_seq;
+  tile_seq<TK>(c, cur);
+  {
+    const long long r = t0 - s_base;
+    cur.u = static_cast<int>(r / cur.nt);
+    cur.j = static_cast<int>(r % cur.nt);
+  }
+
+  // ---- loads: this warp's tiles t0 + w, t0 + w + 8, ...
+  TileAt ld = cur;
+  long long lt = t0 + w;
+  tile_advance<TK>(c, units, ld, w);
+  int lstage = 0;
+  auto issue = [&]() {
+    if (lt < t1) {
+      const int key0 = ld.j * TK;
+      int valid = min(max(ld.n - key0, 0), TK);
+      int page = -1;
+      if (valid > 0) page = page_of(c, ld.b, key0 / c.page_size);
+      if (page < 0) valid = 0;
+      const long long off =
+          page < 0 ? 0 : (page_offset(c, page, ld.u / p.qblocks) + static_cast<long long>(key0 % c.page_size) * D) *
+                             static_cast<long long>(sizeof(T));
+      const uint8_t* gk = static_cast<const uint8_t*>(c.k) + off;
+      const uint8_t* gv = static_cast<const uint8_t*>(c.v) + off;
+      const uint32_t dst = smem_u32(ring + lstage * 2 * Cfg::HALF);
+      constexpr int CPR = Cfg::RB / 16, RPI = 32 / CPR;  // chunks per row, rows per pass of the warp
+#pragma unroll
+      for (int i = 0; i < TK / RPI; ++i) {
+        const int r = i * RPI + lane / CPR, ch = lane % CPR;
+        const int ok = r < valid ? 16 : 0;  // slots past the length are filled with zeros, not read
+        const int go = ok ? r * Cfg::RB + ch * 16 : 0;
+        cp_async16(dst + swz<Cfg::RB>(r, ch), gk + go, ok);
+        cp_async16(dst + Cfg::HALF + swz<Cfg::RB>(r, ch), gv + go, ok);
+      }
+      if (lane == 0) s_valid[w][lstage] = valid;
+      lt += DW;
+      tile_advance<TK>(c, units, ld, DW);
+    }
+    cp_async_commit();
+    lstage = lstage + 1 == ST ? 0 : lstage + 1;
+  };
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) issue();
+
+  Tile tile;
+  long long t = t0;         // first tile of the current unit's part
+  long long mt = t0 + w;    // this warp's next tile
+  int stage = 0;
+  const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
+  while (t < t1) {
+    const long long unit0 = t - cur.j, end = min(t1, unit0 + cur.nt);
+    const int h = cur.u / p.qblocks, g0 = (cur.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = h * p.G + g0;
+    tile.start(p, cur.b, h0, rows, extra);
+    float* scores = p.accumulate ? p.scores + (static_cast<long long>(cur.b) * p.Hq + h0) * cap : nullptr;
+    for (; mt < end; mt += DW) {
+      cp_async_wait<ST - 2>();
+      __syncwarp();
+      const int valid = s_valid[w][stage];
+      const uint8_t* buf = ring + stage * 2 * Cfg::HALF;
+      issue();  // into the stage that the last tile has left
+      tile.tile(p, buf, extra, valid, rows, scores ? scores + (mt - unit0) * TK : nullptr, cap);
+      __syncwarp();
+      stage = stage + 1 == ST ? 0 : stage + 1;
+    }
+    tile.finish();
+
+    // ---- the warps' parts of this unit meet
+    const bool whole = t == unit0 && end == unit0 + cur.nt;
+    const int slot = 2 * blockIdx.x + (t == t0 ? 0 : 1);
+    for (int half = 0; half * 8 < rows; ++half) {
+      tile.put(merge + w * 8 * D, s_ml[w], half);
+      __syncthreads();
+      const int g = w + 8 * half;  // warp w joins row w
+      if (g < rows) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < DW; ++i) M = fmaxf(M, s_ml[i][w].x);
+        float L = 0.f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DW; ++i) {
+          const float f = s_ml[i][w].x == M ? 1.f : ex2(s_ml[i][w].x - M);
+          L = fmaf(f, s_ml[i][w].y, L);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(f, merge[(i * 8 + w) * D + lane * E + e], acc[e]);
+        }
+        if (whole) {
+          decode_store<T, E>(p, cur.b, h0 + g, lane, M, L, acc);
+        } else {
+          float* at = p.part + (static_cast<long long>(slot) * QT + g) * (D + 2);
+#pragma unroll
+          for (int e = 0; e < E; ++e) at[lane * E + e] = acc[e];
+          if (lane == 0) {
+            at[D] = M;
+            at[D + 1] = L;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!whole) {
+      // ---- the CTA that ends last joins the unit's parts, in the order of the run
+      const long long last_tile = unit0 + cur.nt - 1;
+      const int c0 = static_cast<int>(((unit0 + 1) * ctas - 1) / total), c1 = static_cast<int>(((last_tile + 1) * ctas - 1) / total);
+      if (tid == 0) {
+        __threadfence();
+        const int unit = cur.b * units + cur.u;
+        const int done = atomicAdd(&p.counters[unit], 1);
+        s_last = done == c1 - c0;
+        if (s_last) p.counters[unit] = 0;  // for the next call
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        for (int g = w; g < rows; g += DW) {
+          float M = -INFINITY;
+          for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part_at<D>(p, i, total, ctas, unit0, g) + D));
+          M = warp_max(M);
+          float L = 0.f, acc[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+          for (int i = c0; i <= c1; ++i) {
+            const float* at = part_at<D>(p, i, total, ctas, unit0, g);
+            const float mi = __ldcg(at + D), li = __ldcg(at + D + 1);
+            const float f = mi == M ? 1.f : ex2(mi - M);
+            L = fmaf(f, li, L);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, __ldcg(at + lane * E + e), acc[e]);
+          }
+          decode_store<T, E>(p, cur.b, h0 + g, lane, M, L, acc);
+        }
+      }
+    }
+    // next unit
+    t = end;
+    cur.j = 0;
+    if (t < t1 && ++cur.u == units) {
+      cur.u = 0;
+      ++cur.b;
+      tile_seq<TK>(c, cur);
+    }
+  }
+}
+
+// weight[slot] += sum over the group's query heads of exp(s - lse): the second
+// pass of `accumulate`, over the scores the first one kept (4 G bytes per key
+// and kv head beside the 2 D values of K and V).
+__global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant__ DecodeParams p) {
+  const tkb_kv_cache& c = p.c;
+  const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, n = held_of(c, b);
+  const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
+  const float* s = p.scores + (static_cast<long long>(b) * p.Hq + h * p.G) * cap;
+  const float* lse2 = p.lse2 + static_cast<long long>(b) * p.Hq + h * p.G;
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < n; j += gridDim.x * 256) {
+    const int page = page_of(c, b, j / c.page_size);
+    if (page < 0) continue;
+    float sum = 0.f;
+    for (int g = 0; g < p.G; ++g) sum += ex2(s[g * cap + j] - lse2[g]);
+    c.weight[meta_offset(c, page, h) + j % c.page_size] += sum;
+  }
+}
+
+constexpr int kDecodeGrid = 148;  // one CTA per SM
+
+// Workspace: counters, partial results, then (accumulate) lse2 and scores.
+struct DecodeWs {
+  size_t counters, part, lse2, scores, bytes;
+};
+static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  const int G = Hq / c.Hkv;
+  const size_t units = static_cast<size_t>(c.B) * c.Hkv * ((G + QT - 1) / QT);
+  DecodeWs w;
+  w.counters = 0;
+  w.part = up(units * 4);
+  w.lse2 = w.part + up(static_cast<size_t>(2) * kDecodeGrid * QT * (c.D + 2) * 4);
+  w.scores = w.lse2 + (accumulate ? up(static_cast<size_t>(c.B) * Hq * 4) : 0);
+  w.bytes = w.scores + (accumulate ? up(static_cast<size_t>(c.B) * Hq * c.max_pages * c.page_size * 4) : 0);
+  return w;
+}
+
+template <typename T, int D, typename Tile>
+static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
+  using Cfg = DecodeTile<D, static_cast<int>(sizeof(T))>;
+  auto k = paged_decode_kernel<T, D, Tile>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+  if (e != cudaSuccess) return e;
+  const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks *
+                         ((static_cast<long long>(p.c.max_pages) * p.c.page_size + Cfg::TK - 1) / Cfg::TK);
+  const int grid = static_cast<int>(most < kDecodeGrid * DW ? (most + DW - 1) / DW : kDecodeGrid);
+  k<<<grid, DNT, Cfg::SMEM, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+static cudaError_t paged_decode_d(const DecodeParams& p, cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) return paged_decode_launch<T, D, TileMma<T, D>>(p, st);
+  else if (p.G == 1) return paged_decode_launch<T, D, TileFma<D, 1>>(p, st);
+  else if (p.G <= 4) return paged_decode_launch<T, D, TileFma<D, 4>>(p, st);
+  else return paged_decode_launch<T, D, TileFma<D, 16>>(p, st);
 }
 
 template <typename T>
 static cudaError_t paged_decode_t(const DecodeParams& p, cudaStream_t st) {
-  const int grid = p.c.B * p.c.Hkv;
-  if (p.c.D == 64) paged_decode_kernel<T, 64><<<grid, 128, 0, st>>>(p);
-  else paged_decode_kernel<T, 128><<<grid, 128, 0, st>>>(p);
-  return cudaGetLastError();
+  cudaError_t e = p.c.D == 64 ? paged_decode_d<T, 64>(p, st) : paged_decode_d<T, 128>(p, st);
+  if (e == cudaSuccess && p.accumulate) {
+    const long long cap = static_cast<long long>(p.c.max_pages) * p.c.page_size;
+    const int gx = static_cast<int>(cap < 64 * 256 ? (cap + 255) / 256 : 64);
+    paged_weight_kernel<<<dim3(gx, p.c.B * p.c.Hkv), 256, 0, st>>>(p);
+    e = cudaGetLastError();
+  }
+  return e;
 }
 
 // ============================================================ eviction
