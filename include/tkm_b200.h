@@ -354,7 +354,7 @@ int tkb_kv_evict(const tkb_kv_cache *cache, const int32_t *seen, int budget, int
  * temperature 0 (or anything not above 0) takes the largest logit, the lowest
  * index among equals, with logprob 0.  NaN logits count as -inf; +inf shares
  * the whole weight.  top_p and u act as multiples of 2^-32.
- * V at most 2^20. */
+ * V at most 2^18. */
 int tkb_sample_logits(const void *logits, long long ld, const float *u, const float *temperature,
                       const int32_t *top_k, const float *top_p, const float *min_p, int32_t *token,
                       float *logprob, int32_t *kept, int rows, int V, int dtype, void *stream);

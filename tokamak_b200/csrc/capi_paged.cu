@@ -179,13 +179,14 @@ int tkb_sample_logits(const void* logits, long long ld, const float* u, const fl
                       int32_t* kept, int rows, int V, int dtype, void* stream) {
   const char* who = "tkb_sample_logits";
   if (rows <= 0 || V <= 0) return fail(TKB_ERR_ARG, "%s: rows and V must be positive", who);
-  if (V > (1 << 20)) return fail(TKB_ERR_UNSUPPORTED, "%s: V %d > 2^20", who, V);
+  if (V > kSampleMaxV) return fail(TKB_ERR_UNSUPPORTED, "%s: V %d > 2^18", who, V);
+  if (rows > (1 << 26)) return fail(TKB_ERR_UNSUPPORTED, "%s: %d rows > 2^26", who, rows);
   if (!dtype_ok(dtype)) return fail(TKB_ERR_ARG, "%s: bad dtype %d", who, dtype);
   if (!logits || !u || !token) return fail(TKB_ERR_ARG, "%s: null pointer", who);
   if (ld < V) return fail(TKB_ERR_ARG, "%s: ld %lld < V %d", who, ld, V);
   if (reinterpret_cast<uintptr_t>(logits) % dtype_bytes(dtype))
     return fail(TKB_ERR_ARG, "%s: logits not aligned to their type", who);
-  const SampleParams p = {logits, ld, u, temperature, top_k, top_p, min_p, token, logprob, kept, rows, V};
+  const SampleParams p = {logits, ld, u, temperature, top_k, top_p, min_p, token, logprob, kept, rows, V, 0, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define CALL(T) sample_t<T>(p, st)
   return cuda_status(TKB_BY_DTYPE(dtype, CALL), who, 1);
