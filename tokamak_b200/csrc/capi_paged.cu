@@ -142,9 +142,7 @@ int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_
 
 size_t tkb_kv_evict_workspace(const tkb_kv_cache* cache) {
   if (cache_check("tkb_kv_evict_workspace", cache)) return 0;
-  // moves per (sequence, kv head): no more than half of its slots
-  const size_t cap = static_cast<size_t>(cache->max_pages) * cache->page_size / 2;
-  return round256(static_cast<size_t>(cache->B) * cache->Hkv * 2 * cap * 4);
+  return round256(evict_ws(*cache).bytes);
 }
 
 int tkb_kv_evict(const tkb_kv_cache* cache, const int32_t* seen, int budget, int recent, int sinks, void* workspace,
@@ -163,11 +161,13 @@ int tkb_kv_evict(const tkb_kv_cache* cache, const int32_t* seen, int budget, int
   memset(&p, 0, sizeof(p));
   p.c = *cache;
   p.seen = seen;
-  p.lists = static_cast<int32_t*>(workspace);
+  const EvictWs w = evict_ws(*cache);
+  p.lists = static_cast<uint2*>(workspace);
+  if (w.bytes > w.keys) p.keys = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + w.keys);
   p.budget = budget;
   p.recent = recent;
   p.sinks = sinks;
-  p.cap = cache->max_pages * cache->page_size / 2;
+  p.cap = w.cap;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define CALL(T) kv_evict_t<T>(p, st)
   return cuda_status(TKB_BY_DTYPE(cache->dtype, CALL), who, 1);

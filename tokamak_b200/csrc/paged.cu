@@ -177,11 +177,9 @@ static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
 // starts and ends inside a unit, and the parts of a unit that several CTAs
 // took are joined by the CTA that finishes last (a counter in the
 // workspace), in the order of the run, so the result does not depend on who
-// that is.  Inside a run each of the CTA's 8 warps takes every eighth tile
+// that is.  Inside a run the CTA's warps take the tiles in turn, each
 // with its own ring of cp.async buffers and its own running maximum and sum;
 // they meet only at the end of a unit.  The rings run ahead across units.
-constexpr int DW = 8;                 // warps per CTA
-constexpr int DNT = DW * 32;
 constexpr int QT = 16;                // query heads per unit (rows of the m16n8k16 product)
 
 struct DecodeParams {
@@ -204,10 +202,11 @@ struct DecodeTile {
   static constexpr int RB = D * ES;                 // bytes of a row
   static constexpr int TK = RB <= 256 ? 16 : 8;     // keys per tile
   static constexpr int HALF = TK * RB;              // bytes of the K (or V) part
-  static constexpr int STAGES = ES == 4 ? 2 : 3 * 8192 / (2 * HALF);
-  static constexpr int RING = DW * STAGES * 2 * HALF;
-  static constexpr int MERGE = DW * 8 * D * 4;      // eight rows of every warp
-  static constexpr int EXTRA = ES == 4 ? QT * D * 4 + DW * QT * TK * 4 : 0;  // q, p
+  static constexpr int WARPS = D * ES == 128 ? 16 : 8;
+  static constexpr int STAGES = ES == 4 ? 2 : 3;
+  static constexpr int RING = WARPS * STAGES * 2 * HALF;
+  static constexpr int MERGE = WARPS * 8 * D * 4;   // eight rows of every warp
+  static constexpr int EXTRA = ES == 4 ? QT * D * 4 + WARPS * QT * TK * 4 : 0;  // q, p
   static constexpr int SMEM = RING + MERGE + EXTRA;
 };
 
@@ -407,7 +406,7 @@ struct TileFma {
     // the CTA's q, scaled, in shared memory (all warps wrote and read the last one before the merge's barrier)
     float* sq = reinterpret_cast<float*>(extra);
     const float* src = static_cast<const float*>(p.q) + b * p.q_stride + static_cast<long long>(h0) * D;
-    for (int i = threadIdx.x; i < rows * D; i += DNT) sq[i] = __ldg(src + i) * p.scale_log2;
+    for (int i = threadIdx.x; i < rows * D; i += Cfg::WARPS * 32) sq[i] = __ldg(src + i) * p.scale_log2;
     __syncthreads();
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
@@ -533,9 +532,10 @@ TKB_DEVFN const float* part_at(const DecodeParams& p, int i, long long total, in
 }
 
 template <typename T, int D, typename Tile>
-__global__ void __launch_bounds__(DNT, 1) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(DecodeTile<D, static_cast<int>(sizeof(T))>::WARPS * 32, 1)
+    paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeTile<D, static_cast<int>(sizeof(T))>;
-  constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32;
+  constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32, DW = Cfg::WARPS, DNT = DW * 32;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ long long s_start[DW];
   __shared__ int s_valid[DW][ST];
@@ -596,14 +596,23 @@ __global__ void __launch_bounds__(DNT, 1) paged_decode_kernel(const __grid_const
   TileAt ld = cur;
   long long lt = t0 + w;
   tile_advance<TK>(c, units, ld, w);
-  int lstage = 0;
+  int lstage = 0, next_page = -1;
+  // the page of the next tile is looked up while this one is computed
+  auto look_up = [&]() {
+    if (lt < t1 && ld.j * TK < ld.n) next_page = __ldg(c.block_table + static_cast<long long>(ld.b) * c.max_pages + ld.j * TK / c.page_size);
+  };
+  look_up();
   auto issue = [&]() {
     if (lt < t1) {
       const int key0 = ld.j * TK;
-      int valid = min(max(ld.n - key0, 0), TK);
-      int page = -1;
-      if (valid > 0) page = page_of(c, ld.b, key0 / c.page_size);
-      if (page < 0) valid = 0;
+      int valid = min(max(ld.n - key0, 0), TK), page = next_page;
+      if (valid == 0) {
+        page = -1;
+      } else if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.n_pages)) {
+        atomicOr(&g_device_error, ERR_BAD_INDEX);
+        page = -1;
+        valid = 0;
+      }
       const long long off =
           page < 0 ? 0 : (page_offset(c, page, ld.u / p.qblocks) + static_cast<long long>(key0 % c.page_size) * D) *
                              static_cast<long long>(sizeof(T));
@@ -622,6 +631,7 @@ __global__ void __launch_bounds__(DNT, 1) paged_decode_kernel(const __grid_const
       if (lane == 0) s_valid[w][lstage] = valid;
       lt += DW;
       tile_advance<TK>(c, units, ld, DW);
+      look_up();
     }
     cp_async_commit();
     lstage = lstage + 1 == ST ? 0 : lstage + 1;
@@ -658,7 +668,7 @@ __global__ void __launch_bounds__(DNT, 1) paged_decode_kernel(const __grid_const
       tile.put(merge + w * 8 * D, s_ml[w], half);
       __syncthreads();
       const int g = w + 8 * half;  // warp w joins row w
-      if (g < rows) {
+      if (w < 8 && g < rows) {
         float M = -INFINITY;
 #pragma unroll
         for (int i = 0; i < DW; ++i) M = fmaxf(M, s_ml[i][w].x);
@@ -776,8 +786,9 @@ static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks *
                          ((static_cast<long long>(p.c.max_pages) * p.c.page_size + Cfg::TK - 1) / Cfg::TK);
-  const int grid = static_cast<int>(most < kDecodeGrid * DW ? (most + DW - 1) / DW : kDecodeGrid);
-  k<<<grid, DNT, Cfg::SMEM, st>>>(p);
+  constexpr int W = Cfg::WARPS;
+  const int grid = static_cast<int>(most < kDecodeGrid * W ? (most + W - 1) / W : kDecodeGrid);
+  k<<<grid, W * 32, Cfg::SMEM, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -802,11 +813,22 @@ static cudaError_t paged_decode_t(const DecodeParams& p, cudaStream_t st) {
 }
 
 // ============================================================ eviction
+// Per (sequence, kv head): the budget-th largest key by bisection on counts,
+// then the freed slots below the budget and the kept tokens above it, both in
+// ascending order, then the moves.  Reads 8 bytes per slot; the moves (read
+// and written once) are what HBM is busy with, so several CTAs share a unit
+// when there are few units.  They form a cluster: each finds the same cut from
+// the same keys (held in shared memory, or in the workspace when a sequence
+// has room for more than kEvictSmemKeys), and the barrier between the reading of the keys and
+// the moves keeps a fast one from changing what a slow one still reads.
+constexpr int kEvictSmemKeys = 49152;
+
 struct EvictParams {
   tkb_kv_cache c;
   const int32_t* seen;
-  int32_t* lists;  // per (sequence, kv head): `cap` destinations, then `cap` sources
-  int budget, recent, sinks, cap;
+  uint2* lists;     // per unit: `cap` destinations (page, slot in page), then `cap` sources
+  uint32_t* keys;   // per CTA: room for every slot, or null (shared memory)
+  int budget, recent, sinks, cap, split;
 };
 
 // Floats as unsigned numbers of the same order (-0 as +0, NaN below -inf).
@@ -816,111 +838,210 @@ TKB_DEVFN uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Inclusive block-wide prefix sum (blockDim.x = 1024); `sh` holds 32 ints.
-TKB_DEVFN int block_scan(int v, int* sh, int& total) {
-  const int lane = lane_id(), w = warp_id();
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += t;
-  }
+// Sum over the block of a warp-uniform count; `sh` holds two sums used in turn.
+template <int THREADS>
+TKB_DEVFN int evict_count(int v, int* sh, int turn) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if (lane_id() == 0) sh[turn * (THREADS / 32) + warp_id()] = v;
   __syncthreads();
-  if (lane == 31) sh[w] = v;
+  int s = lane_id() < THREADS / 32 ? sh[turn * (THREADS / 32) + lane_id()] : 0;
+  return __reduce_add_sync(0xffffffffu, s);
+}
+// Exclusive prefix over the warps of a warp-uniform count.
+template <int THREADS>
+TKB_DEVFN int evict_prefix(int v, int* sh, int turn, int& total) {
+  if (lane_id() == 0) sh[turn * (THREADS / 32) + warp_id()] = v;
   __syncthreads();
-  int pre = 0, all = 0;
-  for (int i = 0; i < 32; ++i) {
-    const int t = sh[i];
-    if (i < w) pre += t;
-    all += t;
-  }
-  total = all;
-  return v + pre;
+  const int x = lane_id() < THREADS / 32 ? sh[turn * (THREADS / 32) + lane_id()] : 0;
+  total = __reduce_add_sync(0xffffffffu, x);
+  return __reduce_add_sync(0xffffffffu, lane_id() < warp_id() ? x : 0);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(1024) kv_evict_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[256], sh[32], s_bin, s_need;
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int W = THREADS / 32;
+  extern __shared__ __align__(16) uint32_t s_keys[];
+  __shared__ int sh[2 * W];
   const tkb_kv_cache& c = p.c;
-  const int b = blockIdx.x / c.Hkv, h = blockIdx.x % c.Hkv, tid = threadIdx.x;
-  const int n = held_of(c, b);
-  if (n <= p.budget) return;
+  const int unit = blockIdx.x / p.split, rank = blockIdx.x % p.split;
+  const int b = unit / c.Hkv, h = unit % c.Hkv, tid = threadIdx.x, w = warp_id(), lane = lane_id();
+  const int n = held_of(c, b), ps = c.page_size;
+  if (n <= p.budget) return;  // the whole cluster
+  uint32_t* keys = p.keys ? p.keys + static_cast<long long>(blockIdx.x) * c.max_pages * ps : s_keys;
+
+  // ---- keys: protected tokens above all others
   const int newest = p.seen[b] - p.recent;
-  auto key_of = [&](int j) -> uint32_t {
-    const int page = page_of(c, b, j / c.page_size);
-    if (page < 0) return 0u;
-    const long long at = meta_offset(c, page, h) + j % c.page_size;
-    const int pos = c.pos[at];
-    if (pos >= newest || pos < p.sinks) return 0xFFFFFFFFu;
-    return order_key(c.weight[at]);
-  };
-  // the budget-th largest key, eight bits at a time
-  uint32_t prefix = 0, mask = 0;
-  int need = p.budget;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += 1024) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += 1024) {
-      const uint32_t k = key_of(j);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+  const bool by_pos = p.recent > 0 || p.sinks > 0;
+  const int32_t* table = c.block_table + static_cast<long long>(b) * c.max_pages;
+#pragma unroll 4
+  for (int j = tid; j < n; j += THREADS) {
+    const int pg = j / ps, page = __ldg(table + pg);
+    uint32_t k = 0u;
+    if (static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages)) {
+      const long long at = meta_offset(c, page, h) + (j - pg * ps);
+      k = order_key(c.weight[at]);
+      if (by_pos) {
+        const int pos = c.pos[at];
+        if (pos >= newest || pos < p.sinks) k = 0xFFFFFFFFu;
+      }
+    } else {
+      atomicOr(&g_device_error, ERR_BAD_INDEX);
     }
-    __syncthreads();
-    if (tid == 0) {
-      int above = 0, bin = 255;
-      while (above + hist[bin] < need) above += hist[bin--];
-      s_bin = bin;
-      s_need = need - above;
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(s_bin) << shift;
-    mask |= 255u << shift;
-    need = s_need;
-    __syncthreads();
-  }
-  // freed slots below the budget, kept tokens at it and above, both ascending
-  int32_t* to = p.lists + static_cast<long long>(blockIdx.x) * 2 * p.cap;
-  int32_t* from = to + p.cap;
-  int ties = 0, holes = 0, movers = 0;
-  for (int j0 = 0; j0 < n; j0 += 1024) {
-    const int j = j0 + tid;
-    const uint32_t k = j < n ? key_of(j) : 0u;
-    const bool tie = j < n && k == prefix;
-    int total;
-    const int rank = ties + block_scan(tie, sh, total) - tie;
-    ties += total;
-    const bool kept = j < n && (k > prefix || (tie && rank < need));
-    const bool hole = j < n && j < p.budget && !kept, mover = kept && j >= p.budget;
-    const int at = holes + block_scan(hole, sh, total) - hole;
-    holes += total;
-    if (hole) to[at] = j;
-    const int am = movers + block_scan(mover, sh, total) - mover;
-    movers += total;
-    if (mover) from[am] = j;
+    keys[j] = k;
   }
   __syncthreads();
-  const int vecs = c.D * static_cast<int>(sizeof(T)) / 16;
-  for (int i = warp_id(); i < movers; i += 32) {
-    const int dj = to[i], sj = from[i];
-    const int dp = page_of(c, b, dj / c.page_size), sp = page_of(c, b, sj / c.page_size);
-    if (dp < 0 || sp < 0) continue;
-    const long long d0 = page_offset(c, dp, h) + static_cast<long long>(dj % c.page_size) * c.D;
-    const long long s0 = page_offset(c, sp, h) + static_cast<long long>(sj % c.page_size) * c.D;
-    for (int v = lane_id(); v < 2 * vecs; v += 32) {
-      T* pool = static_cast<T*>(v < vecs ? c.k : c.v);
-      const int o = v < vecs ? v : v - vecs;
-      reinterpret_cast<uint4*>(pool + d0)[o] = reinterpret_cast<const uint4*>(pool + s0)[o];
-    }
-    if (lane_id() == 0) {
-      const long long dm = meta_offset(c, dp, h) + dj % c.page_size, sm = meta_offset(c, sp, h) + sj % c.page_size;
-      c.pos[dm] = c.pos[sm];
-      c.weight[dm] = c.weight[sm];
+
+  // ---- the cut: the largest key that at least `budget` tokens reach
+  uint32_t lo = 0, hi = 0xFFFFFFFFu;  // reached by budget tokens at lo; hi: the largest candidate
+  int turn = 0, reach = n;            // tokens with key >= lo
+  while (lo < hi && reach != p.budget) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    int cnt = 0;
+    for (int j = tid; j < n; j += THREADS) cnt += keys[j] >= mid;
+    cnt = evict_count<THREADS>(cnt, sh, turn);
+    turn ^= 1;
+    if (cnt >= p.budget) {
+      lo = mid;
+      reach = cnt;
+    } else {
+      hi = mid - 1;
     }
   }
+  // kept: every key >= lo when just the budget reaches it, else the keys above it and the first `need` equal to it
+  const int chunk = (n + THREADS - 1) / THREADS * 32, j0 = min(n, w * chunk), j1 = min(n, j0 + chunk);
+  int need = n, tie_base = 0;
+  __syncthreads();
+  if (reach != p.budget) {
+    int above = 0, ties = 0, total;
+    for (int j = j0 + lane; j < j1; j += 32) {
+      above += keys[j] > lo;
+      ties += keys[j] == lo;
+    }
+    above = evict_count<THREADS>(above, sh, 0);
+    need = p.budget - above;
+    tie_base = evict_prefix<THREADS>(__reduce_add_sync(0xffffffffu, ties), sh, 1, total);
+    __syncthreads();
+  }
+  // `f(j, kept)` for the warp's slots in order, 32 at a time
+  auto walk = [&](auto f) {
+    int rank_base = tie_base;
+    for (int j = j0; j < j1; j += 32) {
+      const bool in = j + lane < j1;
+      const uint32_t k = in ? keys[j + lane] : 0u;
+      const unsigned m = __ballot_sync(0xffffffffu, in && k == lo);
+      const bool kept = in && (k > lo || (k == lo && rank_base + __popc(m & ((1u << lane) - 1)) < need));
+      rank_base += __popc(m);
+      f(j + lane, in, kept);
+    }
+  };
+  int holes = 0, movers = 0, total;
+  walk([&](int j, bool in, bool kept) {
+    holes += __popc(__ballot_sync(0xffffffffu, in && !kept && j < p.budget));
+    movers += __popc(__ballot_sync(0xffffffffu, kept && j >= p.budget));
+  });
+  int hole_at = evict_prefix<THREADS>(holes, sh, 0, total);
+  int mover_at = evict_prefix<THREADS>(movers, sh, 1, total);  // as many movers as holes
+  // this CTA's share of the moves
+  const int m0 = static_cast<int>(static_cast<long long>(total) * rank / p.split);
+  const int m1 = static_cast<int>(static_cast<long long>(total) * (rank + 1) / p.split);
+  uint2* to = p.lists + static_cast<long long>(unit) * 2 * p.cap;
+  uint2* from = to + p.cap;
+  walk([&](int j, bool in, bool kept) {
+    const bool hole = in && !kept && j < p.budget, mover = kept && j >= p.budget;
+    const unsigned mh = __ballot_sync(0xffffffffu, hole), mm = __ballot_sync(0xffffffffu, mover);
+    const int at = hole ? hole_at + __popc(mh & ((1u << lane) - 1)) : mover_at + __popc(mm & ((1u << lane) - 1));
+    if ((hole || mover) && at >= m0 && at < m1) {
+      const int pg = j / ps;
+      (hole ? to : from)[at] = make_uint2(__ldg(table + pg), j - pg * ps);
+    }
+    hole_at += __popc(mh);
+    mover_at += __popc(mm);
+  });
+  __syncthreads();
+  if (p.split > 1) cluster_sync();  // every CTA of the unit has read its keys
+
+  // ---- the moves
+  for (int i = m0 + tid; i < m1; i += THREADS) {
+    const uint2 d = to[i], s = from[i];
+    if (d.x >= static_cast<unsigned>(c.n_pages) || s.x >= static_cast<unsigned>(c.n_pages)) continue;
+    const long long dm = meta_offset(c, d.x, h) + d.y, sm = meta_offset(c, s.x, h) + s.y;
+    c.pos[dm] = c.pos[sm];
+    c.weight[dm] = c.weight[sm];
+  }
+  const int vecs = c.D * static_cast<int>(sizeof(T)) / 16, per = 2 * vecs;  // a power of two each
+  const int shift = 31 - __clz(per);
+  const long long items = static_cast<long long>(m1 - m0) << shift;
+  constexpr int U = 4;
+  for (long long i0 = tid; i0 < items; i0 += U * THREADS) {
+    uint4 v[U];
+    uint4* dst[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const long long i = i0 + k * THREADS;
+      dst[k] = nullptr;
+      if (i < items) {
+        const int m = m0 + static_cast<int>(i >> shift), o = static_cast<int>(i) & (per - 1);
+        const uint2 d = to[m], s = from[m];
+        if (d.x < static_cast<unsigned>(c.n_pages) && s.x < static_cast<unsigned>(c.n_pages)) {
+          T* pool = static_cast<T*>(o < vecs ? c.k : c.v);
+          const int ch = o & (vecs - 1);
+          dst[k] = reinterpret_cast<uint4*>(pool + page_offset(c, d.x, h) + static_cast<long long>(d.y) * c.D) + ch;
+          v[k] = reinterpret_cast<const uint4*>(pool + page_offset(c, s.x, h) + static_cast<long long>(s.y) * c.D)[ch];
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (dst[k]) *dst[k] = v[k];
+  }
+}
+
+// CTAs per (sequence, kv head): a power of two up to 8 (the portable cluster
+// size) that gives every SM about one.
+static int evict_split(const tkb_kv_cache& c) {
+  int s = 1;
+  while (s < 8 && static_cast<long long>(c.B) * c.Hkv * s * 2 <= 148) s *= 2;
+  return s;
+}
+struct EvictWs {
+  size_t keys, bytes;
+  int cap;
+};
+static EvictWs evict_ws(const tkb_kv_cache& c) {
+  const size_t slots = static_cast<size_t>(c.max_pages) * c.page_size, units = static_cast<size_t>(c.B) * c.Hkv;
+  EvictWs w;
+  w.cap = static_cast<int>(slots / 2);  // moves: at most half of the slots
+  w.keys = (units * 2 * w.cap * sizeof(uint2) + 255) & ~size_t(255);
+  w.bytes = w.keys + (slots > kEvictSmemKeys ? units * evict_split(c) * slots * 4 : 0);
+  return w;
+}
+
+template <typename T, int THREADS>
+static cudaError_t kv_evict_launch(EvictParams p, cudaStream_t st) {
+  const long long slots = static_cast<long long>(p.c.max_pages) * p.c.page_size;
+  p.split = evict_split(p.c);
+  const size_t smem = p.keys ? 0 : static_cast<size_t>(slots) * 4;
+  auto k = kv_evict_kernel<T, THREADS>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSmemKeys * 4);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.c.B) * p.c.Hkv * p.split);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, p);
 }
 
 template <typename T>
 static cudaError_t kv_evict_t(const EvictParams& p, cudaStream_t st) {
-  kv_evict_kernel<T><<<p.c.B * p.c.Hkv, 1024, 0, st>>>(p);
-  return cudaGetLastError();
+  return static_cast<long long>(p.c.max_pages) * p.c.page_size <= 4096 ? kv_evict_launch<T, 256>(p, st)
+                                                                      : kv_evict_launch<T, 1024>(p, st);
 }
 
 }  // namespace tkb
