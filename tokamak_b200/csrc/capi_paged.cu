@@ -112,6 +112,8 @@ int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_
   if ((rc = rows_check(who, "q", q, q_stride, width, cache->dtype))) return rc;
   if ((rc = rows_check(who, "out", out, out_stride, width, cache->dtype))) return rc;
   if (accumulate && !cache->weight) return fail(TKB_ERR_ARG, "%s: accumulate needs the cache's weight", who);
+  if (static_cast<double>(cache->B) * Hq * cache->max_pages * cache->page_size > 8.0 * 0x3FFFFFFF)
+    return fail(TKB_ERR_UNSUPPORTED, "%s: B * Hq * max_pages * page_size above 2^33", who);
   const size_t need = tkb_paged_attn_decode_workspace(cache, Hq, accumulate);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(TKB_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, required", who, need);
@@ -132,6 +134,7 @@ int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.counters = reinterpret_cast<int*>(ws + w.counters);
   p.part = reinterpret_cast<float*>(ws + w.part);
+  p.head = reinterpret_cast<float*>(ws + w.head);
   p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
   p.scores = reinterpret_cast<float*>(ws + w.scores);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -171,15 +171,15 @@ static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
 // HBM bounds it (4 G FLOP per element read) and the kernel is built around
 // keeping loads in flight.
 //
-// The keys of a unit (sequence, kv head, block of 16 query heads) are cut into
-// tiles of 16 (8 for fp32 rows of 512 bytes).  All units' tiles, in order, are
-// dealt out to one CTA per SM as equal runs, whatever the lengths: a run
-// starts and ends inside a unit, and the parts of a unit that several CTAs
-// took are joined by the CTA that finishes last (a counter in the
-// workspace), in the order of the run, so the result does not depend on who
-// that is.  Inside a run the CTA's warps take the tiles in turn, each
-// with its own ring of cp.async buffers and its own running maximum and sum;
-// they meet only at the end of a unit.  The rings run ahead across units.
+// The keys of a unit (sequence, kv head, block of up to 16 query heads) are cut
+// into tiles of 16 (8 for fp32 rows of 512 bytes).  All units' tiles, in order,
+// are dealt out as equal runs, whatever the lengths: to the CTAs, one per SM,
+// and inside a CTA to its warps, each with its own ring of cp.async buffers and
+// its own running maximum and sum.  A unit that lies inside one warp's run is
+// written by that warp at once; the others are parts, at most two per warp,
+// which meet once, at the CTA's end, and where a unit spans CTAs, in the CTA
+// that finishes last (a counter in the workspace), in the order of the run, so
+// the result does not depend on who that is.
 constexpr int QT = 16;                // query heads per unit (rows of the m16n8k16 product)
 
 struct DecodeParams {
@@ -193,21 +193,22 @@ struct DecodeParams {
   float scale_log2;
   int* counters;                      // per unit, 0 between calls
   float* part;                        // [2 * grid][QT][D + 2]: O, then m, l of each row
+  float* head;                        // [grid * 16 warps][QT][D]: first parts, when they are not in shared memory
   float* lse2;                        // accumulate: [B][Hq], in powers of 2
   float* scores;                      // accumulate: [B][Hq][cap], in powers of 2
 };
 
-template <int D, int ES>
+template <int D, int ES, int GT>
 struct DecodeTile {
   static constexpr int RB = D * ES;                 // bytes of a row
   static constexpr int TK = RB <= 256 ? 16 : 8;     // keys per tile
   static constexpr int HALF = TK * RB;              // bytes of the K (or V) part
   static constexpr int WARPS = D * ES == 128 ? 16 : 8;
-  static constexpr int STAGES = ES == 4 ? 2 : 3;
-  static constexpr int RING = WARPS * STAGES * 2 * HALF;
-  static constexpr int MERGE = WARPS * 8 * D * 4;   // eight rows of every warp
-  static constexpr int EXTRA = ES == 4 ? QT * D * 4 + WARPS * QT * TK * 4 : 0;  // q, p
-  static constexpr int SMEM = RING + MERGE + EXTRA;
+  static constexpr int STAGES = ES == 4 && GT > 8 ? 2 : 3;
+  static constexpr int RING = STAGES * 2 * HALF;    // per warp
+  static constexpr int HEAD = GT <= 8 ? GT * D * 4 : 0;                  // per warp: its first part (else in the workspace)
+  static constexpr int EXTRA = ES == 4 ? GT * D * 4 + GT * TK * 4 : 0;   // per warp: q, p
+  static constexpr int SMEM = WARPS * (RING + HEAD + EXTRA);
 };
 
 // Where a flattened tile index lies.
@@ -265,6 +266,29 @@ TKB_DEVFN void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+TKB_DEVFN void decode_lse(const DecodeParams& p, int b, int hq, float M, float L) {
+  const float lse2 = M + lg2(L);  // -inf + -inf when nothing is held
+  if (p.lse) p.lse[static_cast<long long>(b) * p.Hq + hq] = lse2 * 0.6931471805599453f;
+  if (p.accumulate) p.lse2[static_cast<long long>(b) * p.Hq + hq] = lse2;
+}
+// One finished output row: lane holds columns lane*E ..
+template <typename T, int E>
+TKB_DEVFN void decode_store(const DecodeParams& p, int b, int hq, int lane, float M, float L, const float (&acc)[E]) {
+  constexpr int D = 32 * E;
+  const float inv = L == 0.f ? 0.f : 1.0f / L;  // nothing held: zeros
+  T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<long long>(hq) * D + lane * E;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = acc[e] * inv;
+  } else {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<uint32_t*>(out + e) = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
+  }
+  if (lane == 0) decode_lse(p, b, hq, M, L);
+}
+
 // Byte offset of 16-byte chunk `ch` of row `r` inside a tile half: the chunk
 // index is xored with the row so that eight rows' equal chunks (ldmatrix) lie
 // in eight different bank groups.
@@ -275,10 +299,11 @@ TKB_DEVFN int swz(int r, int ch) {
 
 // The 16-bit tile: S = Q K^T and O += P V on m16n8k16 with the query heads as
 // the 16 rows (rows past G are zero).  Thread t holds rows t/4 and t/4 + 8.
-template <typename T, int D>
+template <typename T, int D, int GT>
 struct TileMma {
   static constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  using Cfg = DecodeTile<D, 2>;
+  using Cfg = DecodeTile<D, 2, GT>;
+  static constexpr int GROUP = GT;
   uint32_t q[D / 16][4];
   float o[D / 8][4];
   float m[2], l[2];
@@ -382,14 +407,30 @@ struct TileMma {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     }
   }
-  // rows 8*half .. 8*half+7 of this warp: O to so[8][D], (m, l) to sml
-  TKB_DEVFN void put(float* so, float2* sml, int half) {
+  // O to so[GT][D], (m, l) to sml[GT]
+  TKB_DEVFN void put(float* so, float2* sml) const {
     const int r = lane_id() >> 2, c = lane_id() & 3;
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
-      *reinterpret_cast<float2*>(so + r * D + d * 8 + 2 * c) = half ? make_float2(o[d][2], o[d][3])
-                                                                    : make_float2(o[d][0], o[d][1]);
-    if (c == 0) sml[r] = half ? make_float2(m[1], l[1]) : make_float2(m[0], l[0]);
+    for (int i = 0; i < GT / 8; ++i) {
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+        *reinterpret_cast<float2*>(so + (r + 8 * i) * D + d * 8 + 2 * c) = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+      if (c == 0) sml[r + 8 * i] = make_float2(m[i], l[i]);
+    }
+  }
+  // the finished rows
+  TKB_DEVFN void store(const DecodeParams& p, int b, int h0, int rows) const {
+    const int r = lane_id() >> 2, c = lane_id() & 3;
+#pragma unroll
+    for (int i = 0; i < GT / 8; ++i)
+      if (r + 8 * i < rows) {
+        const float inv = l[i] == 0.f ? 0.f : 1.0f / l[i];
+        T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<long long>(h0 + r + 8 * i) * D + 2 * c;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+          *reinterpret_cast<uint32_t*>(out + d * 8) = pack2<BF16>(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+        if (c == 0) decode_lse(p, b, h0 + r + 8 * i, m[i], l[i]);
+      }
   }
 };
 
@@ -398,16 +439,18 @@ struct TileMma {
 // columns.  GT: query heads the registers are laid out for.
 template <int D, int GT>
 struct TileFma {
-  using Cfg = DecodeTile<D, 4>;
+  using Cfg = DecodeTile<D, 4, GT>;
   static constexpr int TK = Cfg::TK, PART = 32 / TK, CH = D / 4 / PART, E = D / 32;
+  static constexpr int GROUP = GT;
   float o[GT][E], m[GT], l[GT];
 
   TKB_DEVFN void start(const DecodeParams& p, int b, int h0, int rows, uint8_t* extra) {
-    // the CTA's q, scaled, in shared memory (all warps wrote and read the last one before the merge's barrier)
+    // the unit's q, scaled, in the warp's shared memory
     float* sq = reinterpret_cast<float*>(extra);
     const float* src = static_cast<const float*>(p.q) + b * p.q_stride + static_cast<long long>(h0) * D;
-    for (int i = threadIdx.x; i < rows * D; i += Cfg::WARPS * 32) sq[i] = __ldg(src + i) * p.scale_log2;
-    __syncthreads();
+    __syncwarp();
+    for (int i = lane_id(); i < rows * D; i += 32) sq[i] = __ldg(src + i) * p.scale_log2;
+    __syncwarp();
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
       m[g] = -INFINITY;
@@ -424,7 +467,7 @@ struct TileFma {
     const int kk = lane / PART;
     const int key = TK == 8 ? ((kk & 1) << 2) | (kk >> 1) : ((kk & 3) << 1) | ((kk >> 2) & 1) | (kk & 8);
     const float* sq = reinterpret_cast<const float*>(extra);
-    float* sp = reinterpret_cast<float*>(extra + QT * D * 4) + warp_id() * QT * TK;
+    float* sp = reinterpret_cast<float*>(extra + GT * D * 4);
     float4 k[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i)
@@ -486,96 +529,73 @@ struct TileFma {
 #pragma unroll
     for (int g = 0; g < GT; ++g) l[g] = warp_sum(l[g]) * (1.0f / PART);
   }
-  TKB_DEVFN void put(float* so, float2* sml, int half) {
+  TKB_DEVFN void put(float* so, float2* sml) const {
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const int at = g + 8 * half;
+    for (int g = 0; g < GT; ++g) {
 #pragma unroll
-      for (int x = 0; x < GT; ++x)
-        if (x == at) {
-#pragma unroll
-          for (int e = 0; e < E; ++e) so[g * D + lane_id() * E + e] = o[x][e];
-          if (lane_id() == 0) sml[g] = make_float2(m[x], l[x]);
-        }
+      for (int e = 0; e < E; ++e) so[g * D + lane_id() * E + e] = o[g][e];
+      if (lane_id() == 0) sml[g] = make_float2(m[g], l[g]);
     }
+  }
+  TKB_DEVFN void store(const DecodeParams& p, int b, int h0, int rows) const {
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+      if (g < rows) decode_store<float, E>(p, b, h0 + g, lane_id(), m[g], l[g], o[g]);
   }
 };
 
-// One finished output row: lane holds columns lane*E ..
-template <typename T, int E>
-TKB_DEVFN void decode_store(const DecodeParams& p, int b, int hq, int lane, float M, float L, const float (&acc)[E]) {
-  constexpr int D = 32 * E;
-  const float inv = L == 0.f ? 0.f : 1.0f / L;  // nothing held: zeros
-  T* out = static_cast<T*>(p.out) + b * p.out_stride + static_cast<long long>(hq) * D + lane * E;
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = acc[e] * inv;
-  } else {
-    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-      *reinterpret_cast<uint32_t*>(out + e) = pack2<BF16>(acc[e] * inv, acc[e + 1] * inv);
-  }
-  if (lane == 0) {
-    const float lse2 = M + lg2(L);  // -inf + -inf when nothing is held
-    if (p.lse) p.lse[static_cast<long long>(b) * p.Hq + hq] = lse2 * 0.6931471805599453f;
-    if (p.accumulate) p.lse2[static_cast<long long>(b) * p.Hq + hq] = lse2;
-  }
-}
-
-// Row g of the part of the unit starting at tile unit0 that CTA i left: in its
-// first slot when its run starts inside the unit or at its start, else in its second.
-template <int D>
-TKB_DEVFN const float* part_at(const DecodeParams& p, int i, long long total, int ctas, long long unit0, int g) {
-  const int slot = 2 * i + (total * i / ctas >= unit0 ? 0 : 1);
-  return p.part + (static_cast<long long>(slot) * QT + g) * (D + 2);
-}
+// What a warp left of a unit that does not lie inside its run.
+struct DecodePart {
+  int b, u;         // sequence (-1: nothing), (kv head, query block)
+  int unit0, nt;    // first tile of the unit, its number of tiles
+};
 
 template <typename T, int D, typename Tile>
-__global__ void __launch_bounds__(DecodeTile<D, static_cast<int>(sizeof(T))>::WARPS * 32, 1)
+__global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
     paged_decode_kernel(const __grid_constant__ DecodeParams p) {
-  using Cfg = DecodeTile<D, static_cast<int>(sizeof(T))>;
-  constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32, DW = Cfg::WARPS, DNT = DW * 32;
+  using Cfg = typename Tile::Cfg;
+  constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32, DW = Cfg::WARPS, DNT = DW * 32, GT = Tile::GROUP;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ long long s_start[DW];
-  __shared__ int s_valid[DW][ST];
-  __shared__ float2 s_ml[DW][8];
-  __shared__ long long s_base;
-  __shared__ int s_seq, s_last;
+  __shared__ float2 s_ml[2 * DW][GT];
+  __shared__ DecodePart s_part[2 * DW];
+  __shared__ int s_start[DW], s_seq, s_base, s_last[2];
   const tkb_kv_cache& c = p.c;
   const int w = warp_id(), lane = lane_id(), tid = threadIdx.x, units = c.Hkv * p.qblocks;
-  uint8_t* ring = smem + w * ST * 2 * Cfg::HALF;
-  float* merge = reinterpret_cast<float*>(smem + Cfg::RING);
-  uint8_t* extra = smem + Cfg::RING + Cfg::MERGE;
+  uint8_t* ring = smem + w * Cfg::RING;
+  uint8_t* extra = smem + DW * (Cfg::RING + Cfg::HEAD) + w * Cfg::EXTRA;
+  auto head_of = [&](int i) {
+    return Cfg::HEAD ? reinterpret_cast<float*>(smem + DW * Cfg::RING + i * Cfg::HEAD)
+                     : p.head + (static_cast<long long>(blockIdx.x) * DW + i) * GT * D;
+  };
 
-  // ---- this CTA's run of tiles: [t0, t1) of all `total` ones
-  long long total = 0, before = 0;
-  const int per = (c.B + DNT - 1) / DNT, s0 = min(c.B, tid * per), s1 = min(c.B, s0 + per);
-  long long mine = 0;
-  for (int b = s0; b < s1; ++b) mine += static_cast<long long>(max(1, (held_of(c, b) + TK - 1) / TK)) * units;
-  long long pre = mine;
+  // ---- this CTA's run of tiles, [t0, t1) of all `total` ones
+  const int per = (c.B + DNT - 1) / DNT, q0 = min(c.B, tid * per), q1 = min(c.B, q0 + per);
+  int mine = 0;
+  for (int b = q0; b < q1; ++b) mine += max(1, (held_of(c, b) + TK - 1) / TK) * units;
+  int pre = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, pre, d);
+    const int t = __shfl_up_sync(0xffffffffu, pre, d);
     if (lane >= d) pre += t;
   }
   if (lane == 31) s_start[w] = pre;
+  if (tid < 2 * DW) s_part[tid].b = -1;
   __syncthreads();
+  int total = 0, before = pre - mine;
 #pragma unroll
   for (int i = 0; i < DW; ++i) {
     if (i < w) before += s_start[i];
     total += s_start[i];
   }
-  before += pre - mine;
   // fewer CTAs than the grid when there is not a tile for every warp
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + DW - 1) / DW));
+  const int ctas = min(static_cast<int>(gridDim.x), (total + DW - 1) / DW);
   if (static_cast<int>(blockIdx.x) >= ctas) return;
-  const long long t0 = total * blockIdx.x / ctas, t1 = total * (blockIdx.x + 1) / ctas;
+  auto run_of = [&](int i) { return static_cast<int>(static_cast<long long>(total) * i / ctas); };
+  const int t0 = run_of(blockIdx.x), t1 = run_of(blockIdx.x + 1);
   if (before <= t0 && t0 < before + mine) {
-    long long at = before;
-    int b = s0;
+    int at = before, b = q0;
     for (;; ++b) {
-      const long long nt = static_cast<long long>(max(1, (held_of(c, b) + TK - 1) / TK)) * units;
+      const int nt = max(1, (held_of(c, b) + TK - 1) / TK) * units;
       if (t0 < at + nt) break;
       at += nt;
     }
@@ -583,27 +603,34 @@ __global__ void __launch_bounds__(DecodeTile<D, static_cast<int>(sizeof(T))>::WA
     s_base = at;
   }
   __syncthreads();
+  // this warp's run, [t, tw)
+  int t = t0 + (t1 - t0) * w / DW;
+  const int tw = t0 + (t1 - t0) * (w + 1) / DW;
   TileAt cur;
   cur.b = s_seq;
   tile_seq<TK>(c, cur);
   {
-    const long long r = t0 - s_base;
-    cur.u = static_cast<int>(r / cur.nt);
-    cur.j = static_cast<int>(r % cur.nt);
+    int r = t - s_base;
+    while (r >= cur.nt * units && cur.b < c.B) {
+      r -= cur.nt * units;
+      ++cur.b;
+      tile_seq<TK>(c, cur);
+    }
+    cur.u = r / cur.nt;
+    cur.j = r % cur.nt;
   }
 
-  // ---- loads: this warp's tiles t0 + w, t0 + w + 8, ...
+  // ---- loads
   TileAt ld = cur;
-  long long lt = t0 + w;
-  tile_advance<TK>(c, units, ld, w);
-  int lstage = 0, next_page = -1;
+  int lt = t, lstage = 0, next_page = -1, valid_ring = 0;
   // the page of the next tile is looked up while this one is computed
   auto look_up = [&]() {
-    if (lt < t1 && ld.j * TK < ld.n) next_page = __ldg(c.block_table + static_cast<long long>(ld.b) * c.max_pages + ld.j * TK / c.page_size);
+    if (lt < tw && ld.j * TK < ld.n)
+      next_page = __ldg(c.block_table + static_cast<long long>(ld.b) * c.max_pages + ld.j * TK / c.page_size);
   };
   look_up();
   auto issue = [&]() {
-    if (lt < t1) {
+    if (lt < tw) {
       const int key0 = ld.j * TK;
       int valid = min(max(ld.n - key0, 0), TK), page = next_page;
       if (valid == 0) {
@@ -628,9 +655,9 @@ __global__ void __launch_bounds__(DecodeTile<D, static_cast<int>(sizeof(T))>::WA
         cp_async16(dst + swz<Cfg::RB>(r, ch), gk + go, ok);
         cp_async16(dst + Cfg::HALF + swz<Cfg::RB>(r, ch), gv + go, ok);
       }
-      if (lane == 0) s_valid[w][lstage] = valid;
-      lt += DW;
-      tile_advance<TK>(c, units, ld, DW);
+      valid_ring = (valid_ring & ~(31 << (5 * lstage))) | (valid << (5 * lstage));
+      ++lt;
+      tile_advance<TK>(c, units, ld, 1);
       look_up();
     }
     cp_async_commit();
@@ -639,104 +666,132 @@ __global__ void __launch_bounds__(DecodeTile<D, static_cast<int>(sizeof(T))>::WA
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) issue();
 
+  // ---- this warp's units
   Tile tile;
-  long long t = t0;         // first tile of the current unit's part
-  long long mt = t0 + w;    // this warp's next tile
   int stage = 0;
   const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
-  while (t < t1) {
-    const long long unit0 = t - cur.j, end = min(t1, unit0 + cur.nt);
-    const int h = cur.u / p.qblocks, g0 = (cur.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = h * p.G + g0;
+  while (t < tw) {
+    const int unit0 = t - cur.j, unit1 = unit0 + cur.nt, end = min(tw, unit1);
+    const int g0 = (cur.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (cur.u / p.qblocks) * p.G + g0;
     tile.start(p, cur.b, h0, rows, extra);
     float* scores = p.accumulate ? p.scores + (static_cast<long long>(cur.b) * p.Hq + h0) * cap : nullptr;
-    for (; mt < end; mt += DW) {
+    const bool first = t == unit0;
+    for (; t < end; ++t) {
       cp_async_wait<ST - 2>();
       __syncwarp();
-      const int valid = s_valid[w][stage];
+      const int valid = (valid_ring >> (5 * stage)) & 31;
       const uint8_t* buf = ring + stage * 2 * Cfg::HALF;
       issue();  // into the stage that the last tile has left
-      tile.tile(p, buf, extra, valid, rows, scores ? scores + (mt - unit0) * TK : nullptr, cap);
+      tile.tile(p, buf, extra, valid, rows, scores ? scores + static_cast<long long>(t - unit0) * TK : nullptr, cap);
       __syncwarp();
       stage = stage + 1 == ST ? 0 : stage + 1;
     }
     tile.finish();
-
-    // ---- the warps' parts of this unit meet
-    const bool whole = t == unit0 && end == unit0 + cur.nt;
-    const int slot = 2 * blockIdx.x + (t == t0 ? 0 : 1);
-    for (int half = 0; half * 8 < rows; ++half) {
-      tile.put(merge + w * 8 * D, s_ml[w], half);
-      __syncthreads();
-      const int g = w + 8 * half;  // warp w joins row w
-      if (w < 8 && g < rows) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < DW; ++i) M = fmaxf(M, s_ml[i][w].x);
-        float L = 0.f, acc[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < DW; ++i) {
-          const float f = s_ml[i][w].x == M ? 1.f : ex2(s_ml[i][w].x - M);
-          L = fmaf(f, s_ml[i][w].y, L);
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(f, merge[(i * 8 + w) * D + lane * E + e], acc[e]);
-        }
-        if (whole) {
-          decode_store<T, E>(p, cur.b, h0 + g, lane, M, L, acc);
-        } else {
-          float* at = p.part + (static_cast<long long>(slot) * QT + g) * (D + 2);
-#pragma unroll
-          for (int e = 0; e < E; ++e) at[lane * E + e] = acc[e];
-          if (lane == 0) {
-            at[D] = M;
-            at[D + 1] = L;
-          }
-        }
-      }
-      __syncthreads();
+    if (first && end == unit1) {
+      tile.store(p, cur.b, h0, rows);
+    } else {
+      // a part: the unit goes on in the next run (kept in the ring, which no load will use again), or ended here
+      const int i = 2 * w + (end < unit1 ? 1 : 0);
+      if (end < unit1) cp_async_wait<0>();
+      __syncwarp();
+      tile.put(end < unit1 ? reinterpret_cast<float*>(ring) : head_of(w), s_ml[i]);
+      if (lane == 0) s_part[i] = {cur.b, cur.u, unit0, cur.nt};
     }
-    if (!whole) {
-      // ---- the CTA that ends last joins the unit's parts, in the order of the run
-      const long long last_tile = unit0 + cur.nt - 1;
-      const int c0 = static_cast<int>(((unit0 + 1) * ctas - 1) / total), c1 = static_cast<int>(((last_tile + 1) * ctas - 1) / total);
-      if (tid == 0) {
-        __threadfence();
-        const int unit = cur.b * units + cur.u;
-        const int done = atomicAdd(&p.counters[unit], 1);
-        s_last = done == c1 - c0;
-        if (s_last) p.counters[unit] = 0;  // for the next call
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        for (int g = w; g < rows; g += DW) {
-          float M = -INFINITY;
-          for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part_at<D>(p, i, total, ctas, unit0, g) + D));
-          M = warp_max(M);
-          float L = 0.f, acc[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-          for (int i = c0; i <= c1; ++i) {
-            const float* at = part_at<D>(p, i, total, ctas, unit0, g);
-            const float mi = __ldcg(at + D), li = __ldcg(at + D + 1);
-            const float f = mi == M ? 1.f : ex2(mi - M);
-            L = fmaf(f, li, L);
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = fmaf(f, __ldcg(at + lane * E + e), acc[e]);
-          }
-          decode_store<T, E>(p, cur.b, h0 + g, lane, M, L, acc);
-        }
-      }
-    }
-    // next unit
-    t = end;
     cur.j = 0;
-    if (t < t1 && ++cur.u == units) {
+    if (t < tw && ++cur.u == units) {
       cur.u = 0;
       ++cur.b;
       tile_seq<TK>(c, cur);
+    }
+  }
+  __syncthreads();
+
+  // ---- parts of the same unit meet; (unit, row) pairs are dealt to the warps
+  int pair = 0, left = 0;  // left: units this CTA leaves to a join of CTAs
+  DecodePart open[2];
+  for (int i = 0; i < 2 * DW;) {
+    const DecodePart u = s_part[i];
+    if (u.b < 0) {
+      ++i;
+      continue;
+    }
+    int j = i + 1;
+    for (; j < 2 * DW; ++j)
+      if (s_part[j].b >= 0 && s_part[j].unit0 != u.unit0) break;
+    const int g0 = (u.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (u.u / p.qblocks) * p.G + g0;
+    const bool whole = u.unit0 >= t0 && u.unit0 + u.nt <= t1;
+    for (int g = 0; g < rows; ++g, ++pair) {
+      if (pair % DW != w) continue;
+      float M = -INFINITY, L = 0.f, acc[E];
+      for (int k = i; k < j; ++k)
+        if (s_part[k].b >= 0) M = fmaxf(M, s_ml[k][g].x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int k = i; k < j; ++k) {
+        if (s_part[k].b < 0) continue;
+        const float2 ml = s_ml[k][g];
+        const float f = ml.x == M ? 1.f : ex2(ml.x - M);
+        const float* so = (k & 1 ? reinterpret_cast<const float*>(smem + (k >> 1) * Cfg::RING) : head_of(k >> 1)) + g * D + lane * E;
+        L = fmaf(f, ml.y, L);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, so[e], acc[e]);
+      }
+      if (whole) {
+        decode_store<T, E>(p, u.b, h0 + g, lane, M, L, acc);
+      } else {
+        float* at = p.part + (static_cast<long long>(2 * blockIdx.x + (t0 >= u.unit0 ? 0 : 1)) * QT + g) * (D + 2);
+#pragma unroll
+        for (int e = 0; e < E; ++e) at[lane * E + e] = acc[e];
+        if (lane == 0) {
+          at[D] = M;
+          at[D + 1] = L;
+        }
+      }
+    }
+    if (!whole && left < 2) open[left++] = u;
+    i = j;
+  }
+  if (left == 0) return;
+
+  // ---- the CTA that ends last joins the unit's parts, in the order of the runs
+  __syncthreads();
+  if (tid < left) {
+    const DecodePart u = open[tid];
+    const int c0 = static_cast<int>((static_cast<long long>(u.unit0 + 1) * ctas - 1) / total);
+    const int c1 = static_cast<int>((static_cast<long long>(u.unit0 + u.nt) * ctas - 1) / total);
+    __threadfence();
+    int* counter = &p.counters[u.b * units + u.u];
+    s_last[tid] = atomicAdd(counter, 1) == c1 - c0;
+    if (s_last[tid]) *counter = 0;  // for the next call
+    __threadfence();
+  }
+  __syncthreads();
+  for (int x = 0; x < left; ++x) {
+    if (!s_last[x]) continue;
+    const DecodePart u = open[x];
+    const int g0 = (u.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (u.u / p.qblocks) * p.G + g0;
+    const int c0 = static_cast<int>((static_cast<long long>(u.unit0 + 1) * ctas - 1) / total);
+    const int c1 = static_cast<int>((static_cast<long long>(u.unit0 + u.nt) * ctas - 1) / total);
+    for (int g = w; g < rows; g += DW) {
+      // CTA i's part is its first when its run starts inside the unit, else its second
+      auto part = [&](int i) {
+        return p.part + (static_cast<long long>(2 * i + (run_of(i) >= u.unit0 ? 0 : 1)) * QT + g) * (D + 2);
+      };
+      float M = -INFINITY, L = 0.f, acc[E];
+      for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part(i) + D));
+      M = warp_max(M);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+      for (int i = c0; i <= c1; ++i) {
+        const float* at = part(i);
+        const float mi = __ldcg(at + D), li = __ldcg(at + D + 1);
+        const float f = mi == M ? 1.f : ex2(mi - M);
+        L = fmaf(f, li, L);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, __ldcg(at + lane * E + e), acc[e]);
+      }
+      decode_store<T, E>(p, u.b, h0 + g, lane, M, L, acc);
     }
   }
 }
@@ -763,7 +818,7 @@ constexpr int kDecodeGrid = 148;  // one CTA per SM
 
 // Workspace: counters, partial results, then (accumulate) lse2 and scores.
 struct DecodeWs {
-  size_t counters, part, lse2, scores, bytes;
+  size_t counters, part, head, lse2, scores, bytes;
 };
 static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
@@ -772,7 +827,9 @@ static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
   DecodeWs w;
   w.counters = 0;
   w.part = up(units * 4);
-  w.lse2 = w.part + up(static_cast<size_t>(2) * kDecodeGrid * QT * (c.D + 2) * 4);
+  w.head = w.part + up(static_cast<size_t>(2) * kDecodeGrid * QT * (c.D + 2) * 4);
+  // the 16-row tiles (paged_decode_d) keep their first parts here
+  w.lse2 = w.head + (G > (c.dtype == TKB_F32 ? 4 : 8) ? up(static_cast<size_t>(kDecodeGrid) * 16 * QT * c.D * 4) : 0);
   w.scores = w.lse2 + (accumulate ? up(static_cast<size_t>(c.B) * Hq * 4) : 0);
   w.bytes = w.scores + (accumulate ? up(static_cast<size_t>(c.B) * Hq * c.max_pages * c.page_size * 4) : 0);
   return w;
@@ -780,13 +837,12 @@ static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
 
 template <typename T, int D, typename Tile>
 static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
-  using Cfg = DecodeTile<D, static_cast<int>(sizeof(T))>;
+  using Cfg = typename Tile::Cfg;
+  constexpr int W = Cfg::WARPS;
   auto k = paged_decode_kernel<T, D, Tile>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
   if (e != cudaSuccess) return e;
-  const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks *
-                         ((static_cast<long long>(p.c.max_pages) * p.c.page_size + Cfg::TK - 1) / Cfg::TK);
-  constexpr int W = Cfg::WARPS;
+  const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks * (p.c.max_pages * p.c.page_size / Cfg::TK);
   const int grid = static_cast<int>(most < kDecodeGrid * W ? (most + W - 1) / W : kDecodeGrid);
   k<<<grid, W * 32, Cfg::SMEM, st>>>(p);
   return cudaGetLastError();
@@ -794,10 +850,14 @@ static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
 
 template <typename T, int D>
 static cudaError_t paged_decode_d(const DecodeParams& p, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2) return paged_decode_launch<T, D, TileMma<T, D>>(p, st);
-  else if (p.G == 1) return paged_decode_launch<T, D, TileFma<D, 1>>(p, st);
-  else if (p.G <= 4) return paged_decode_launch<T, D, TileFma<D, 4>>(p, st);
-  else return paged_decode_launch<T, D, TileFma<D, 16>>(p, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.G <= 8) return paged_decode_launch<T, D, TileMma<T, D, 8>>(p, st);
+    return paged_decode_launch<T, D, TileMma<T, D, 16>>(p, st);
+  } else {
+    if (p.G == 1) return paged_decode_launch<T, D, TileFma<D, 1>>(p, st);
+    if (p.G <= 4) return paged_decode_launch<T, D, TileFma<D, 4>>(p, st);
+    return paged_decode_launch<T, D, TileFma<D, 16>>(p, st);
+  }
 }
 
 template <typename T>
