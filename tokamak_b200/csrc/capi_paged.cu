@@ -111,7 +111,10 @@ int tkb_paged_attn_decode(const tkb_kv_cache* cache, const void* q, long long q_
   if (width > 0x3FFFFFFF) return fail(TKB_ERR_ARG, "%s: row of %lld columns", who, width);
   if ((rc = rows_check(who, "q", q, q_stride, width, cache->dtype))) return rc;
   if ((rc = rows_check(who, "out", out, out_stride, width, cache->dtype))) return rc;
-  if (accumulate && !cache->weight) return fail(TKB_ERR_ARG, "%s: accumulate needs the cache's weight", who);
+  if (accumulate && (!cache->weight || !aligned16(cache->weight)))
+    return fail(TKB_ERR_ARG, "%s: accumulate needs the cache's weight, 16-byte aligned", who);
+  if (static_cast<long long>(cache->B) * cache->Hkv > 65535)
+    return fail(TKB_ERR_UNSUPPORTED, "%s: B * Hkv above 65535", who);
   if (static_cast<double>(cache->B) * Hq * cache->max_pages * cache->page_size > 8.0 * 0x3FFFFFFF)
     return fail(TKB_ERR_UNSUPPORTED, "%s: B * Hq * max_pages * page_size above 2^33", who);
   const size_t need = tkb_paged_attn_decode_workspace(cache, Hq, accumulate);

@@ -221,19 +221,6 @@ TKB_DEVFN void tile_seq(const tkb_kv_cache& c, TileAt& t) {
   t.n = t.b < c.B ? held_of(c, t.b) : 0;
   t.nt = max(1, (t.n + TK - 1) / TK);
 }
-template <int TK>
-TKB_DEVFN void tile_advance(const tkb_kv_cache& c, int units, TileAt& t, int by) {
-  t.j += by;
-  while (t.j >= t.nt && t.b < c.B) {
-    t.j -= t.nt;
-    if (++t.u == units) {
-      t.u = 0;
-      ++t.b;
-      tile_seq<TK>(c, t);
-    }
-  }
-}
-
 TKB_DEVFN void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -555,10 +542,11 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
     paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = typename Tile::Cfg;
   constexpr int TK = Cfg::TK, ST = Cfg::STAGES, E = D / 32, DW = Cfg::WARPS, DNT = DW * 32, GT = Tile::GROUP;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 s_ml[2 * DW][GT];
   __shared__ DecodePart s_part[2 * DW];
-  __shared__ int s_start[DW], s_seq, s_base, s_last[2];
+  __shared__ int3 s_at[DW];  // sequence, tokens it holds, tiles of it before the warp's first
+  __shared__ int s_start[DW], s_last[2];
   const tkb_kv_cache& c = p.c;
   const int w = warp_id(), lane = lane_id(), tid = threadIdx.x, units = c.Hkv * p.qblocks;
   uint8_t* ring = smem + w * Cfg::RING;
@@ -570,8 +558,11 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
 
   // ---- this CTA's run of tiles, [t0, t1) of all `total` ones
   const int per = (c.B + DNT - 1) / DNT, q0 = min(c.B, tid * per), q1 = min(c.B, q0 + per);
-  int mine = 0;
-  for (int b = q0; b < q1; ++b) mine += max(1, (held_of(c, b) + TK - 1) / TK) * units;
+  int mine = 0, held = 0;
+  for (int b = q0; b < q1; ++b) {
+    held = held_of(c, b);
+    mine += max(1, (held + TK - 1) / TK) * units;
+  }
   int pre = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -579,7 +570,7 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
     if (lane >= d) pre += t;
   }
   if (lane == 31) s_start[w] = pre;
-  if (tid < 2 * DW) s_part[tid].b = -1;
+  if (lane < 2) s_part[2 * w + lane].b = -1;
   __syncthreads();
   int total = 0, before = pre - mine;
 #pragma unroll
@@ -592,47 +583,56 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
   if (static_cast<int>(blockIdx.x) >= ctas) return;
   auto run_of = [&](int i) { return static_cast<int>(static_cast<long long>(total) * i / ctas); };
   const int t0 = run_of(blockIdx.x), t1 = run_of(blockIdx.x + 1);
-  if (before <= t0 && t0 < before + mine) {
-    int at = before, b = q0;
-    for (;; ++b) {
-      const int nt = max(1, (held_of(c, b) + TK - 1) / TK) * units;
-      if (t0 < at + nt) break;
-      at += nt;
-    }
-    s_seq = b;
-    s_base = at;
+  // the thread that counted a warp's first tile says so (and no more: with the
+  // divisions here too, one thread did them for all the warps in turn)
+#pragma unroll 1
+  for (int i = 0; i < DW; ++i) {
+    const int r = t0 + (t1 - t0) * i / DW - before;
+    if (r >= 0 && r < mine) s_at[i] = make_int3(q0, held, r);
   }
   __syncthreads();
   // this warp's run, [t, tw)
   int t = t0 + (t1 - t0) * w / DW;
   const int tw = t0 + (t1 - t0) * (w + 1) / DW;
   TileAt cur;
-  cur.b = s_seq;
-  tile_seq<TK>(c, cur);
-  {
-    int r = t - s_base;
-    while (r >= cur.nt * units && cur.b < c.B) {
+  cur.b = c.B;
+  if (t < tw) {
+    const int3 at = s_at[w];
+    int r = at.z;
+    cur.b = at.x;
+    cur.n = per > 1 ? held_of(c, cur.b) : at.y;
+    cur.nt = max(1, (cur.n + TK - 1) / TK);
+    while (r >= cur.nt * units) {
       r -= cur.nt * units;
       ++cur.b;
       tile_seq<TK>(c, cur);
     }
     cur.u = r / cur.nt;
-    cur.j = r % cur.nt;
+    cur.j = r - cur.u * cur.nt;
   }
 
-  // ---- loads
+  // ---- loads.  Lane i holds entry pbase + i of the sequence's page table, and
+  // the entry 32 further: both were asked for long before they are needed.
   TileAt ld = cur;
-  int lt = t, lstage = 0, next_page = -1, valid_ring = 0;
-  // the page of the next tile is looked up while this one is computed
-  auto look_up = [&]() {
-    if (lt < tw && ld.j * TK < ld.n)
-      next_page = __ldg(c.block_table + static_cast<long long>(ld.b) * c.max_pages + ld.j * TK / c.page_size);
+  int lt = t, lstage = 0, valid_ring = 0, ldb = -1, pbase = 0, pages = -1, pages_next = -1;
+  int pi = cur.j * TK / c.page_size, in_page = cur.j * TK - pi * c.page_size;
+  auto table = [&](int i) {
+    return i < c.max_pages ? __ldg(c.block_table + static_cast<long long>(ldb) * c.max_pages + i) : -1;
   };
-  look_up();
   auto issue = [&]() {
     if (lt < tw) {
-      const int key0 = ld.j * TK;
-      int valid = min(max(ld.n - key0, 0), TK), page = next_page;
+      if (ldb != ld.b || pi < pbase || pi >= pbase + 64) {
+        ldb = ld.b;
+        pbase = pi;
+        pages = table(pbase + lane);
+        pages_next = table(pbase + 32 + lane);
+      } else if (pi >= pbase + 32) {
+        pbase += 32;
+        pages = pages_next;
+        pages_next = table(pbase + 32 + lane);
+      }
+      int page = __shfl_sync(0xffffffffu, pages, pi - pbase);
+      int valid = min(max(ld.n - ld.j * TK, 0), TK);
       if (valid == 0) {
         page = -1;
       } else if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.n_pages)) {
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
         valid = 0;
       }
       const long long off =
-          page < 0 ? 0 : (page_offset(c, page, ld.u / p.qblocks) + static_cast<long long>(key0 % c.page_size) * D) *
+          page < 0 ? 0 : (page_offset(c, page, ld.u / p.qblocks) + static_cast<long long>(in_page) * D) *
                              static_cast<long long>(sizeof(T));
       const uint8_t* gk = static_cast<const uint8_t*>(c.k) + off;
       const uint8_t* gv = static_cast<const uint8_t*>(c.v) + off;
@@ -657,8 +657,19 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
       }
       valid_ring = (valid_ring & ~(31 << (5 * lstage))) | (valid << (5 * lstage));
       ++lt;
-      tile_advance<TK>(c, units, ld, 1);
-      look_up();
+      in_page += TK;
+      if (in_page == c.page_size) {
+        in_page = 0;
+        ++pi;
+      }
+      if (++ld.j == ld.nt) {
+        ld.j = pi = in_page = 0;
+        if (++ld.u == units) {
+          ld.u = 0;
+          ++ld.b;
+          tile_seq<TK>(c, ld);
+        }
+      }
     }
     cp_async_commit();
     lstage = lstage + 1 == ST ? 0 : lstage + 1;
@@ -706,40 +717,49 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
   }
   __syncthreads();
 
-  // ---- parts of the same unit meet; (unit, row) pairs are dealt to the warps
-  int pair = 0, left = 0;  // left: units this CTA leaves to a join of CTAs
-  DecodePart open[2];
-  for (int i = 0; i < 2 * DW;) {
-    const DecodePart u = s_part[i];
-    if (u.b < 0) {
-      ++i;
-      continue;
-    }
-    int j = i + 1;
-    for (; j < 2 * DW; ++j)
-      if (s_part[j].b >= 0 && s_part[j].unit0 != u.unit0) break;
-    const int g0 = (u.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (u.u / p.qblocks) * p.G + g0;
-    const bool whole = u.unit0 >= t0 && u.unit0 + u.nt <= t1;
-    for (int g = 0; g < rows; ++g, ++pair) {
-      if (pair % DW != w) continue;
-      float M = -INFINITY, L = 0.f, acc[E];
-      for (int k = i; k < j; ++k)
-        if (s_part[k].b >= 0) M = fmaxf(M, s_ml[k][g].x);
+  // ---- parts of the same unit meet.  Lane i looks at part i; a unit's parts
+  // are neighbours.  (unit, row) pairs are dealt to the warps.
+  DecodePart u;
+  u.b = -1;
+  u.unit0 = u.nt = u.u = 0;
+  if (lane < 2 * DW) u = s_part[lane];
+  const unsigned there = __ballot_sync(0xffffffffu, u.b >= 0);
+  const unsigned below = there & ((1u << lane) - 1);
+  const int prev0 = __shfl_sync(0xffffffffu, u.unit0, below ? 31 - __clz(below) : lane);
+  const unsigned leads = __ballot_sync(0xffffffffu, u.b >= 0 && (!below || prev0 != u.unit0));
+  const bool whole = u.unit0 >= t0 && u.unit0 + u.nt <= t1;
+  // units that go on in other CTAs: at most two
+  const unsigned opens = leads & __ballot_sync(0xffffffffu, !whole);
+  int turn = w;  // pairs until this warp's next
+  for (unsigned rest = leads; rest; rest &= rest - 1) {
+    const int i = __ffs(rest) - 1;
+    const unsigned after = rest & (rest - 1);
+    // this unit's parts: from its leader up to the next one
+    const unsigned group = there & ~((1u << i) - 1) & (after ? (1u << (__ffs(after) - 1)) - 1 : 0xffffffffu);
+    const int ub = __shfl_sync(0xffffffffu, u.b, i), uu = __shfl_sync(0xffffffffu, u.u, i);
+    const int unit0 = __shfl_sync(0xffffffffu, u.unit0, i);
+    const int g0 = (uu % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (uu / p.qblocks) * p.G + g0;
+    int g = turn;
+    for (; g < rows; g += DW) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (group >> lane & 1) ml = s_ml[lane][g];
+      const float M = warp_max(ml.x);
+      const float f = ml.x == M ? 1.f : ex2(ml.x - M);
+      const float L = warp_sum(f * ml.y);
+      float acc[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      for (int k = i; k < j; ++k) {
-        if (s_part[k].b < 0) continue;
-        const float2 ml = s_ml[k][g];
-        const float f = ml.x == M ? 1.f : ex2(ml.x - M);
+      for (unsigned m = group; m; m &= m - 1) {
+        const int k = __ffs(m) - 1;
+        const float fk = __shfl_sync(0xffffffffu, f, k);
         const float* so = (k & 1 ? reinterpret_cast<const float*>(smem + (k >> 1) * Cfg::RING) : head_of(k >> 1)) + g * D + lane * E;
-        L = fmaf(f, ml.y, L);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, so[e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(fk, so[e], acc[e]);
       }
-      if (whole) {
-        decode_store<T, E>(p, u.b, h0 + g, lane, M, L, acc);
+      if (!(opens >> i & 1)) {
+        decode_store<T, E>(p, ub, h0 + g, lane, M, L, acc);
       } else {
-        float* at = p.part + (static_cast<long long>(2 * blockIdx.x + (t0 >= u.unit0 ? 0 : 1)) * QT + g) * (D + 2);
+        float* at = p.part + (static_cast<long long>(2 * blockIdx.x + (t0 >= unit0 ? 0 : 1)) * QT + g) * (D + 2);
 #pragma unroll
         for (int e = 0; e < E; ++e) at[lane * E + e] = acc[e];
         if (lane == 0) {
@@ -748,70 +768,102 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
         }
       }
     }
-    if (!whole && left < 2) open[left++] = u;
-    i = j;
+    turn = g - rows;
   }
-  if (left == 0) return;
+  if (!opens) return;
 
   // ---- the CTA that ends last joins the unit's parts, in the order of the runs
   __syncthreads();
-  if (tid < left) {
-    const DecodePart u = open[tid];
-    const int c0 = static_cast<int>((static_cast<long long>(u.unit0 + 1) * ctas - 1) / total);
-    const int c1 = static_cast<int>((static_cast<long long>(u.unit0 + u.nt) * ctas - 1) / total);
+  const int left = __popc(opens), o0 = __ffs(opens) - 1, o1 = 31 - __clz(opens);
+  auto first_cta = [&](int unit0) { return static_cast<int>((static_cast<long long>(unit0 + 1) * ctas - 1) / total); };
+  if (w == 0 && (opens >> lane & 1)) {
+    const int c0 = first_cta(u.unit0), c1 = first_cta(u.unit0 + u.nt - 1);
     __threadfence();
     int* counter = &p.counters[u.b * units + u.u];
-    s_last[tid] = atomicAdd(counter, 1) == c1 - c0;
-    if (s_last[tid]) *counter = 0;  // for the next call
+    const bool last = atomicAdd(counter, 1) == c1 - c0;
+    s_last[lane == o0 ? 0 : 1] = last;
+    if (last) *counter = 0;  // for the next call
     __threadfence();
   }
   __syncthreads();
   for (int x = 0; x < left; ++x) {
     if (!s_last[x]) continue;
-    const DecodePart u = open[x];
-    const int g0 = (u.u % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (u.u / p.qblocks) * p.G + g0;
-    const int c0 = static_cast<int>((static_cast<long long>(u.unit0 + 1) * ctas - 1) / total);
-    const int c1 = static_cast<int>((static_cast<long long>(u.unit0 + u.nt) * ctas - 1) / total);
+    const int i0 = x ? o1 : o0;
+    const int ub = __shfl_sync(0xffffffffu, u.b, i0), uu = __shfl_sync(0xffffffffu, u.u, i0);
+    const int unit0 = __shfl_sync(0xffffffffu, u.unit0, i0), nt = __shfl_sync(0xffffffffu, u.nt, i0);
+    const int g0 = (uu % p.qblocks) * QT, rows = min(QT, p.G - g0), h0 = (uu / p.qblocks) * p.G + g0;
+    const int c0 = first_cta(unit0), c1 = first_cta(unit0 + nt - 1);
     for (int g = w; g < rows; g += DW) {
-      // CTA i's part is its first when its run starts inside the unit, else its second
-      auto part = [&](int i) {
-        return p.part + (static_cast<long long>(2 * i + (run_of(i) >= u.unit0 ? 0 : 1)) * QT + g) * (D + 2);
-      };
+      // CTA i's part is its first when its run starts inside the unit, else its second: only c0 may start before
+      const long long stride = 2ll * QT * (D + 2);
+      const float* part0 = p.part + (static_cast<long long>(2 * c0 + (run_of(c0) >= unit0 ? 0 : 1)) * QT + g) * (D + 2);
+      const float* part1 = p.part + (static_cast<long long>(2 * c0) * QT + g) * (D + 2);
+      auto part = [&](int i) { return i == c0 ? part0 : part1 + (i - c0) * stride; };
+      // four parts' loads at a time, none waiting for another's
       float M = -INFINITY, L = 0.f, acc[E];
-      for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part(i) + D));
-      M = warp_max(M);
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-      for (int i = c0; i <= c1; ++i) {
-        const float* at = part(i);
-        const float mi = __ldcg(at + D), li = __ldcg(at + D + 1);
-        const float f = mi == M ? 1.f : ex2(mi - M);
-        L = fmaf(f, li, L);
+      for (int i = c0; i <= c1; i += 4) {
+        float m[4], l[4], v[4][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, __ldcg(at + lane * E + e), acc[e]);
+        for (int k = 0; k < 4; ++k) {
+          m[k] = -INFINITY;
+          l[k] = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[k][e] = 0.f;
+          if (i + k <= c1) {
+            const float* at = part(i + k);
+            m[k] = __ldcg(at + D);
+            l[k] = __ldcg(at + D + 1);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[k][e] = __ldcg(at + lane * E + e);
+          }
+        }
+        const float Mn = fmaxf(fmaxf(fmaxf(M, m[0]), fmaxf(m[1], m[2])), m[3]);
+        const float f = M == Mn ? 1.f : ex2(M - Mn);
+        M = Mn;
+        L *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float fk = m[k] == M ? 1.f : ex2(m[k] - M);
+          L = fmaf(fk, l[k], L);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(fk, v[k][e], acc[e]);
+        }
       }
-      decode_store<T, E>(p, u.b, h0 + g, lane, M, L, acc);
+      decode_store<T, E>(p, ub, h0 + g, lane, M, L, acc);
     }
   }
 }
 
 // weight[slot] += sum over the group's query heads of exp(s - lse): the second
 // pass of `accumulate`, over the scores the first one kept (4 G bytes per key
-// and kv head beside the 2 D values of K and V).
+// and kv head beside the 2 D values of K and V).  A thread takes four slots:
+// pages are multiples of 16, so one page holds them.
 __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant__ DecodeParams p) {
   const tkb_kv_cache& c = p.c;
-  const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, n = held_of(c, b);
+  const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, j = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int n = held_of(c, b);
+  if (j >= n) return;
+  const int pg = j / c.page_size, page = page_of(c, b, pg);
+  if (page < 0) return;
   const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
-  const float* s = p.scores + (static_cast<long long>(b) * p.Hq + h * p.G) * cap;
+  const float* s = p.scores + (static_cast<long long>(b) * p.Hq + h * p.G) * cap + j;
   const float* lse2 = p.lse2 + static_cast<long long>(b) * p.Hq + h * p.G;
-  for (int j = blockIdx.x * 256 + threadIdx.x; j < n; j += gridDim.x * 256) {
-    const int page = page_of(c, b, j / c.page_size);
-    if (page < 0) continue;
-    float sum = 0.f;
-    for (int g = 0; g < p.G; ++g) sum += ex2(s[g * cap + j] - lse2[g]);
-    c.weight[meta_offset(c, page, h) + j % c.page_size] += sum;
+  float4* at = reinterpret_cast<float4*>(c.weight + meta_offset(c, page, h) + (j - pg * c.page_size));
+  float4 sum = *at;
+#pragma unroll 8
+  for (int g = 0; g < p.G; ++g) {
+    const float4 x = __ldcs(reinterpret_cast<const float4*>(s + g * cap));
+    const float l = lse2[g];
+    sum.x += ex2(x.x - l);
+    if (j + 1 < n) sum.y += ex2(x.y - l);
+    if (j + 2 < n) sum.z += ex2(x.z - l);
+    if (j + 3 < n) sum.w += ex2(x.w - l);
   }
+  *at = sum;
 }
 
 constexpr int kDecodeGrid = 148;  // one CTA per SM
@@ -865,8 +917,7 @@ static cudaError_t paged_decode_t(const DecodeParams& p, cudaStream_t st) {
   cudaError_t e = p.c.D == 64 ? paged_decode_d<T, 64>(p, st) : paged_decode_d<T, 128>(p, st);
   if (e == cudaSuccess && p.accumulate) {
     const long long cap = static_cast<long long>(p.c.max_pages) * p.c.page_size;
-    const int gx = static_cast<int>(cap < 64 * 256 ? (cap + 255) / 256 : 64);
-    paged_weight_kernel<<<dim3(gx, p.c.B * p.c.Hkv), 256, 0, st>>>(p);
+    paged_weight_kernel<<<dim3(static_cast<unsigned>((cap + 1023) / 1024), p.c.B * p.c.Hkv), 256, 0, st>>>(p);
     e = cudaGetLastError();
   }
   return e;
