@@ -37,7 +37,9 @@ struct SampleParams {
 };
 
 constexpr int SNT = 256, SW = SNT / 32;
+constexpr int SCTAS = 8;      // CTAs per row at most: the portable cluster size
 constexpr int SLIST = 256;    // listed elements per warp
+constexpr int SSMALL = SNT;   // listed elements of a row that are ranked directly, one per thread
 constexpr int SBINS = 512;    // bins of the guess, over the distances of non-zero weight
 constexpr float SRANGE = 22.25f;  // weights beyond this distance round to zero: 2^31 exp(-22.25) < 1/2
 
@@ -60,10 +62,17 @@ TKB_DEVFN float sample_dist(float x, float top, float inv_t) {
 TKB_DEVFN uint32_t sample_weight(float x, float top, float inv_t) {
   return __float2uint_rn(expf(-sample_dist(x, top, inv_t)) * 2147483648.f);
 }
-// The float of an order_key.
-TKB_DEVFN float key_float(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-}
+// order_key without the bits that no value of the type has: 16-bit logits need
+// half the steps of a search over keys.
+template <typename T>
+struct SampleKey {
+  static constexpr int DROP = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
+  static TKB_DEVFN uint32_t of(float x) { return order_key(x) >> DROP; }
+  static TKB_DEVFN float value(uint32_t key) {
+    const uint32_t k = key << DROP;
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~(k | ((1u << DROP) - 1)));
+  }
+};
 
 TKB_DEVFN unsigned long long warp_sum_u64(unsigned long long v) {
 #pragma unroll
@@ -74,13 +83,14 @@ TKB_DEVFN unsigned long long warp_sum_u64(unsigned long long v) {
 // 8 bytes of shared memory of CTA `rank` of the cluster.
 TKB_DEVFN unsigned long long ld_rank_u64(const void* p, int rank) {
   unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(smem_u32(p), rank)));
   return v;
 }
 
 template <typename T>
 struct Sampler {
   static constexpr int VEC = 16 / sizeof(T);
+  using Key = SampleKey<T>;
   const SampleParams& p;
   T* data;                       // the slice
   uint2* list;                   // this warp's (key, index in the row)
@@ -92,6 +102,7 @@ struct Sampler {
   bool summed = false;           // the last pass summed weights
   uint32_t list_hi = 0;
   float top, inv_t;
+  bool plain = true;             // both finite, 1/T not 0
   unsigned long long above = 0;  // this thread: weight of the elements at list_hi and above
   int n_above = 0;
 
@@ -111,73 +122,112 @@ struct Sampler {
     __syncwarp();
     cluster_sync();
   }
-  // slot i of CTA r
+  // slot i of CTA r, and of all CTAs (their loads in flight together)
   TKB_DEVFN unsigned long long read(int i, int r) const { return ld_rank_u64(&xbuf[par][i], r); }
+  TKB_DEVFN void read_all(int i, unsigned long long (&v)[SCTAS]) const {
+#pragma unroll
+    for (int r = 0; r < SCTAS; ++r) v[r] = r < p.ctas ? read(i, r) : 0;
+  }
   TKB_DEVFN void next() { par ^= 1; }
 
-  // Two sums over the whole row, known to every thread afterwards.
-  TKB_DEVFN void sum2(unsigned long long& a, unsigned long long& b) {
-    a = warp_sum_u64(a);
-    b = warp_sum_u64(b);
-    if (lane_id() == 0) {
-      buf()[2 * warp_id()] = a;
-      buf()[2 * warp_id() + 1] = b;
+  // N sums over the whole row, known to every thread afterwards.
+  template <int N>
+  TKB_DEVFN void sums(unsigned long long (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = warp_sum_u64(v[i]);
+      if (lane_id() == 0) buf()[N * warp_id() + i] = v[i];
     }
     agree();
-    a = b = 0;
-    // lane l of every warp reads slot pairs l, l + 32, ...
-    for (int i = lane_id(); i < p.ctas * SW; i += 32) {
-      a += read(2 * (i % SW), i / SW);
-      b += read(2 * (i % SW) + 1, i / SW);
+    const int j0 = lane_id(), j1 = lane_id() + 32;  // the row's warps, at most 64
+    unsigned long long a[N], b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      a[i] = j0 < p.ctas * SW ? read(N * (j0 % SW) + i, j0 / SW) : 0;
+      b[i] = j1 < p.ctas * SW ? read(N * (j1 % SW) + i, j1 / SW) : 0;
     }
-    a = warp_sum_u64(a);
-    b = warp_sum_u64(b);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a[i] + b[i];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum_u64(v[i]);
     next();
   }
 
   // One pass over the chunk: what lies at key hi and above is counted (and its
-  // weights summed, with `weights`, as are all weights), what lies in
-  // [lo, hi) is listed.
-  template <bool WEIGHTS>
-  TKB_DEVFN void pass(uint32_t lo, uint32_t hi, unsigned long long& in_list, unsigned long long& all) {
+  // weights summed, with WEIGHTS, as are all weights), what lies in [lo, hi) is
+  // listed.  `in_list`: the measure of the listed elements, of no meaning when
+  // the list spilled.  PLAIN: maximum and 1/T are finite, so that no distance
+  // needs a special case.
+  //
+  // A weight is rint(e 2^31) for e in [0, 1], without a conversion: t = e + 1
+  // rounds e to multiples of 2^-23, which are then the low bits of t; the rest,
+  // exact, becomes the low bits of rest + 1.5 2^-8 as a multiple of 2^-31.
+  // (The conversion unit also computes ex2; it would be the bound.)
+  template <bool WEIGHTS, bool PLAIN>
+  TKB_DEVFN void pass_t(uint32_t lo, uint32_t hi, unsigned long long& in_list, unsigned long long& all) {
     // thresholds as floats; hi one past the largest key means nothing is above
-    const float flo = key_float(lo), fhi = key_float(hi);
+    const float flo = Key::value(lo), fhi = Key::value(hi);
+    constexpr uint32_t ONE = 0x3F800000u, LOW = 0x3BC00000u;  // 1, 1.5 * 2^-8
+    uint32_t hi_all = 0, lo_all = 0, hi_above = 0, lo_above = 0, n = 0;
     n_list = 0;
-    n_above = 0;
     summed = WEIGHTS;
-    above = in_list = all = 0;
     for (int it = 0; it < p.per; ++it) {
       float x[VEC];
       vec(it, x);
-      bool any = false;
+      uint32_t in = 0;  // this lane's elements of the bracket
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const bool is_above = x[e] >= fhi, in = x[e] >= flo && !is_above;
-        any |= in;
-        n_above += is_above;
+        const bool is_above = x[e] >= fhi;
+        if (x[e] >= flo && !is_above) in |= 1u << e;
+        n += is_above;
         if constexpr (WEIGHTS) {
-          const uint32_t w = sample_weight(x[e], top, inv_t);
-          all += w;
-          if (is_above) above += w;
-          if (in) in_list += w;
-        } else {
-          in_list += in;
+          const float z = PLAIN ? __fmul_rn(__fsub_rn(top, x[e]), inv_t) : sample_dist(x[e], top, inv_t);
+          float ex = expf(-z);
+          if constexpr (!PLAIN) ex = ex == ex ? ex : 0.f;  // -inf logits at an infinite temperature
+          const float t = __fadd_rn(ex, 1.f);
+          const uint32_t th = __float_as_uint(t);
+          const uint32_t tl = __float_as_uint(__fadd_rn(__fsub_rn(ex, __fsub_rn(t, 1.f)), 0.005859375f));
+          hi_all += th;
+          lo_all += tl;
+          if (is_above) {
+            hi_above += th;
+            lo_above += tl;
+          }
         }
       }
-      if (__any_sync(0xffffffffu, any)) {
+      if (__any_sync(0xffffffffu, in)) {
+        const int mine = __popc(in);
+        int end = mine;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const bool in = x[e] >= flo && !(x[e] >= fhi);
-          const uint32_t m = __ballot_sync(0xffffffffu, in);
-          const int at = n_list + __popc(m & ((1u << lane_id()) - 1));
-          if (in && at < SLIST)
-            list[at] = make_uint2(order_key(x[e]), base + (it * 32 + lane_id()) * VEC + e);
-          n_list += __popc(m);
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, end, d);
+          if (lane_id() >= d) end += o;
         }
+        const int at0 = (it * 32 + lane_id()) * VEC;
+        for (int at = n_list + end - mine; in && at < SLIST; in &= in - 1, ++at) {
+          const int i = at0 + __ffs(in) - 1;
+          list[at] = make_uint2(Key::of(Elem<T>::ld(data + warp_id() * p.per * 32 * VEC + i)), base + i);
+        }
+        n_list += __shfl_sync(0xffffffffu, end, 31);
       }
     }
+    n_above = n;
+    auto joined = [](uint32_t h, uint32_t l, uint32_t count) {
+      return (static_cast<unsigned long long>(h - count * ONE) << 8) +
+             static_cast<unsigned long long>(static_cast<long long>(static_cast<int>(l - count * LOW)));
+    };
+    all = WEIGHTS ? joined(hi_all, lo_all, p.per * VEC) : 0;
+    above = WEIGHTS ? joined(hi_above, lo_above, n) : 0;
     __syncwarp();
+    in_list = 0;
+    for (int i = lane_id(); i < min(n_list, SLIST); i += 32) in_list += WEIGHTS ? weight_of(list[i].x) : 1u;
   }
+  template <bool WEIGHTS>
+  TKB_DEVFN void pass(uint32_t lo, uint32_t hi, unsigned long long& in_list, unsigned long long& all) {
+    if (!WEIGHTS || plain) pass_t<WEIGHTS, true>(lo, hi, in_list, all);
+    else pass_t<WEIGHTS, false>(lo, hi, in_list, all);
+  }
+  TKB_DEVFN uint32_t weight_of(uint32_t key) const { return sample_weight(Key::value(key), top, inv_t); }
 
   // The largest key K of [from, list_hi) such that `acc` and the listed
   // measure of the keys >= K reach `bound` (they do at `from`).  Returns K; acc
@@ -192,14 +242,21 @@ struct Sampler {
       clear();
       for (int i = lane_id(); i < n_list; i += 32) {
         const uint32_t key = list[i].x;
-        if (key >= from && (bits == 32 || (key >> bits) == (prefix >> bits)))
-          atomicAdd(&buf()[(key >> shift) & ((1u << take) - 1)],
-                    WEIGHTS ? static_cast<unsigned long long>(sample_weight(key_float(key), top, inv_t)) : 1ull);
+        if (key >= from && (bits == 32 || (key >> bits) == (prefix >> bits))) {
+          // the sum as two 32-bit ones, of the weights' lower and upper halves (at most 2048 terms each): a 64-bit
+          // add to shared memory is a loop
+          uint32_t* slot = reinterpret_cast<uint32_t*>(&buf()[(key >> shift) & ((1u << take) - 1)]);
+          const uint32_t wt = WEIGHTS ? weight_of(key) : 1u;
+          atomicAdd(slot, wt & 0xFFFFu);
+          if (WEIGHTS) atomicAdd(slot + 1, wt >> 16);
+        }
       }
       agree();
       // thread t holds digit 255 - t: a prefix sum over threads runs from the largest digit down
-      unsigned long long v = 0;
-      for (int r = 0; r < p.ctas; ++r) v += read(255 - threadIdx.x, r);
+      unsigned long long part[SCTAS], v = 0;
+      read_all(255 - threadIdx.x, part);
+#pragma unroll
+      for (int r = 0; r < SCTAS; ++r) v += (part[r] & 0xFFFFFFFFull) + ((part[r] >> 32) << 16);
       unsigned long long s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -226,66 +283,157 @@ struct Sampler {
   }
 
   // The cut of a measure (count, or weight): the largest key K of [lo, hi) such
-  // that the measure of the keys >= K reaches bound.  False when even lo's does
-  // not.  acc: the measure of the keys above the cut.  With of_all the bound
-  // comes in as a share, in 2^-32, of the sum of all weights.
+  // that the measure of the keys >= K reaches bound; acc becomes the measure of
+  // the keys above it.  With of_all the bound comes in as a share, in 2^-32, of
+  // the sum of all weights.  NONE: even lo's measure does not reach it.  FEW:
+  // no cut was looked for, since the lists hold all keys from one at or below
+  // the cut up to hi, and they are no more than SSMALL.
+  enum { NONE, CUT, FEW };
   template <bool WEIGHTS>
-  TKB_DEVFN bool search(uint32_t lo, uint32_t hi, uint32_t glo, uint32_t ghi, unsigned long long& bound, bool of_all,
-                        uint32_t& cut, unsigned long long& acc) {
+  TKB_DEVFN int search(uint32_t lo, uint32_t hi, uint32_t glo, uint32_t ghi, unsigned long long& bound, bool of_all,
+                       uint32_t& cut, unsigned long long& acc) {
+    const uint32_t end = hi;
     while (true) {
       unsigned long long in_list, all;
       pass<WEIGHTS>(glo, ghi, in_list, all);
-      unsigned long long a = WEIGHTS ? above : n_above, l = in_list;
-      const bool over = n_list > SLIST;
-      if (of_all) {
-        unsigned long long zero = 0;
-        sum2(all, zero);
-        bound = scaled_ceil(all, bound);
-        if (bound == 0) bound = 1;  // the first token always stays
-        of_all = false;
-      }
-      // the overflow flag rides on the counts' top bits
-      unsigned long long flag = over && lane_id() == 0 ? 1ull << 52 : 0ull;
-      l += flag;
-      sum2(a, l);
-      const bool spilled = l >> 52;
-      l &= (1ull << 52) - 1;
+      unsigned long long v[4] = {WEIGHTS ? above : n_above, in_list, 0, all};
+      if (lane_id() == 0) v[2] = n_list + (n_list > SLIST ? 1ull << 32 : 0ull);
+      sums(v);
+      const unsigned long long a = v[0], listed = v[2] & 0xFFFFFFFFull;
+      const bool spilled = v[2] >> 32, single = ghi - glo == 1;
+      if (of_all) bound = max(1ull, scaled_ceil(v[3], bound));  // the first token always stays
+      of_all = false;
+      // what the list measures, as far as it is known when it spilled
+      unsigned long long l = v[1];
+      if (spilled) l = !WEIGHTS ? listed : listed * weight_of(glo);
       if (a >= bound) {
         lo = ghi;
         glo = lo;
         ghi = hi;
+      } else if (spilled && WEIGHTS && !single) {
+        hi = ghi;
+        ghi = glo + (ghi - glo) / 2;
       } else if (a + l < bound) {
-        if (glo == lo) return false;
+        if (glo == lo) return NONE;
         hi = glo;
         glo = lo;
         ghi = hi;
       } else if (!spilled) {
         list_ok = true;
         list_hi = ghi;
+        if (ghi == end && listed <= SSMALL) return FEW;
         acc = a;
         cut = radix<WEIGHTS>(glo, acc, bound);
-        return true;
+        return CUT;
+      } else if (single) {  // one key, more equal logits than the lists hold
+        list_ok = false;
+        acc = a;
+        cut = glo;
+        return CUT;
       } else {
         lo = glo;
         hi = ghi;
-        if (hi - lo == 1) {  // one key, more equal logits than the lists hold
-          list_ok = false;
-          acc = a;
-          cut = lo;
-          return true;
-        }
         glo = lo + (hi - lo) / 2;
       }
     }
   }
+
+  // The whole row decided from no more than SSMALL listed elements, the row's
+  // largest: they are brought to CTA 0, each of whose threads compares one of
+  // them with all the others.
+  // bound: what top-p leaves (0: its share of the first k's weight).
+  TKB_DEVFN void few(int row, int k, bool nucleus, float tp, unsigned long long bound, uint32_t least, uint2* s_few) {
+    const int lane = lane_id(), tid = threadIdx.x;
+    if (lane == 0) buf()[warp_id()] = n_list;
+    agree();
+    int c[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int i = 2 * lane + j;
+      if (i < p.ctas * SW) c[j] = static_cast<int>(read(i % SW, i / SW));
+    }
+    int end = c[0] + c[1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end += t;
+    }
+    const int n = __shfl_sync(0xffffffffu, end, 31), mine = rank * SW + warp_id();
+    const int at = __shfl_sync(0xffffffffu, end - c[0] - c[1], mine / 2) +
+                   (mine & 1 ? __shfl_sync(0xffffffffu, c[0], mine / 2) : 0);
+    const uint32_t dst = mapa_shared(smem_u32(s_few), 0);
+    for (int i = lane; i < n_list; i += 32)
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst + 8 * (at + i)), "r"(list[i].x), "r"(list[i].y)
+                   : "memory");
+    next();
+    agree();
+    if (rank != 0) return;
+    uint32_t* s_w = reinterpret_cast<uint32_t*>(xbuf[0]);
+    unsigned long long* s_kept = xbuf[1];
+    const uint2 e = tid < n ? s_few[tid] : make_uint2(0u, 0u);
+    const uint32_t wt = tid < n ? weight_of(e.x) : 0u;
+    s_w[tid] = wt;
+    __syncthreads();
+    // tokens before this one in the order of the truncations, and their weight
+    int rank_of = 0;
+    unsigned long long before = 0;
+    for (int j = 0; j < n; ++j) {
+      const uint2 o = s_few[j];
+      if (o.x > e.x || (o.x == e.x && o.y < e.y)) {
+        ++rank_of;
+        before += s_w[j];
+      }
+    }
+    bool keep = tid < n && (k == 0 || rank_of < k);
+    if (nucleus) {
+      const unsigned long long total = block_sum(keep ? wt : 0ull);
+      if (bound == 0) bound = max(1ull, scaled_ceil(total, fixed32(tp)));
+      keep = keep && before < bound;
+    }
+    keep = keep && wt >= least;
+    s_kept[tid] = keep ? wt : 0ull;
+    const unsigned long long total = block_sum(keep ? wt : 0ull);  // (its barriers publish s_kept)
+    const unsigned long long kept = block_sum(keep ? 1ull : 0ull);
+    const unsigned long long target = scaled_floor(total, fixed32(p.u[row]));
+    unsigned long long run = 0;
+    for (int j = 0; j < n; ++j)
+      if (s_few[j].y < e.y) run += s_kept[j];
+    if (keep && run <= target && target < run + wt) finish(row, e.y, Key::value(e.x), total, static_cast<int>(kept));
+  }
+  TKB_DEVFN unsigned long long block_sum(unsigned long long v) {
+    v = warp_sum_u64(v);
+    __syncthreads();
+    if (lane_id() == 0) s_tmp[warp_id()] = v;
+    __syncthreads();
+    unsigned long long s = 0;
+#pragma unroll
+    for (int i = 0; i < SW; ++i) s += s_tmp[i];
+    return s;
+  }
+  TKB_DEVFN void finish(int row, int token, float x, unsigned long long total, int kept) {
+    p.token[row] = token;
+    if (p.kept) p.kept[row] = kept;
+    if (p.logprob)
+      p.logprob[row] = -sample_dist(x, top, inv_t) - logf(static_cast<float>(total) * 4.656612873077393e-10f);
+  }
 };
+
+// Larger of two packed pairs, NaN if either is.
+template <typename T>
+TKB_DEVFN uint32_t max_nan2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ SampleParams p) {
   constexpr int VEC = Sampler<T>::VEC;
+  using Key = SampleKey<T>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned long long s_x[2][256], s_tmp[16];
-  __shared__ uint2 s_list[SW][SLIST];
+  __shared__ uint2 s_list[SW][SLIST], s_few[SSMALL];
   Sampler<T> s(p);
   const int row = blockIdx.x / p.ctas, tid = threadIdx.x, lane = lane_id(), w = warp_id(), V = p.V;
   s.rank = blockIdx.x % p.ctas;
@@ -316,33 +464,48 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
 
   // ---- maximum; NaN becomes -inf for all that follows
   float tmax = -INFINITY;
-  for (int it = 0; it < p.per; ++it) {
-    float v[VEC];
-    s.vec(it, v);
-    bool nan = false;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      nan |= v[e] != v[e];
-      tmax = fmaxf(tmax, v[e]);
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
+    for (int it = 0; it < p.per; ++it) {
+      const uint4 q = *reinterpret_cast<const uint4*>(s.data + (w * p.per + it) * 32 * VEC + lane * VEC);
+      m = max_nan2<T>(max_nan2<T>(m, max_nan2<T>(q.x, q.y)), max_nan2<T>(q.z, q.w));
     }
-    if (nan) {
+    const float2 f = unpack2<std::is_same<T, __nv_bfloat16>::value>(m);
+    tmax = f.x != f.x || f.y != f.y ? NAN : fmaxf(f.x, f.y);
+  } else {
+    for (int it = 0; it < p.per; ++it) {
+      float v[VEC];
+      s.vec(it, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = v[e] != v[e] ? -INFINITY : v[e];
+      for (int e = 0; e < VEC; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(tmax) : "f"(tmax), "f"(v[e]));
+    }
+  }
+  if (tmax != tmax) {
+    tmax = -INFINITY;
+    for (int it = 0; it < p.per; ++it) {
+      float v[VEC];
+      s.vec(it, v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[e] = v[e] != v[e] ? -INFINITY : v[e];
+        tmax = fmaxf(tmax, v[e]);
+      }
       stv<T, VEC>(s.data + (w * p.per + it) * 32 * VEC + lane * VEC, v);
     }
   }
   float top = warp_max(tmax);
-  if (lane == 0) s.buf()[w] = order_key(top);
+  if (lane == 0) s.buf()[w] = Key::of(top);
   s.agree();
   uint32_t tk = 0;
   for (int i = lane; i < p.ctas * SW; i += 32) tk = max(tk, static_cast<uint32_t>(s.read(i % SW, i / SW)));
   tk = __reduce_max_sync(0xffffffffu, tk);
   s.next();
-  top = key_float(tk);
+  top = Key::value(tk);
   s.top = top;
   const float temp = p.temperature ? p.temperature[row] : 1.f;
   const bool greedy = !(temp > 0.f);
   s.inv_t = greedy ? 1.f : __frcp_rn(temp);
+  s.plain = top < INFINITY && s.inv_t < INFINITY && s.inv_t > 0.f;
 
   if (top == -INFINITY || greedy) {
     // the lowest index of the maximum
@@ -381,14 +544,14 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
   // keys of non-zero weight lie in [low, high)
   const uint32_t high = tk + 1;
   const float reach = top - (SRANGE + 1.f) / s.inv_t;
-  const uint32_t low = reach == reach ? min(order_key(reach), tk) : order_key(-INFINITY);
+  const uint32_t low = reach == reach ? min(Key::of(reach), tk) : Key::of(-INFINITY);
 
   uint32_t cut = 0;  // kept: keys above `cut`, and the first `ties` tokens of exactly that key
   long long ties = 0;
   if (k || nucleus) {
     uint32_t glo = low, ghi = high;
     if (p.per * 32 * VEC > SLIST) {
-      // ---- the guess.  Thread maxima enter one by one, a quarter of the other elements stands for the rest.
+      // ---- the guess.  Thread maxima enter one by one, an eighth of the other elements stands for the rest.
       uint32_t* hist = reinterpret_cast<uint32_t*>(s.buf());
       s.clear();
       const float to_bin = SBINS / SRANGE;
@@ -397,7 +560,7 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
       if (zmax < SRANGE) atomicAdd(&hist[min(SBINS - 1, static_cast<int>(zmax * to_bin))],
                                    k ? 1u : static_cast<uint32_t>(__expf(-zmax) * 131072.f));
       if (!by_max) {
-        const int ns = max(1, p.per / 4);
+        const int ns = max(1, p.per / 8);
         const float f = static_cast<float>(p.per) / ns;
         for (int it = 0; it < ns; ++it) {
           float v[VEC];
@@ -413,11 +576,12 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
       }
       s.agree();
       // thread t: bins 2t and 2t + 1 of the whole row, and what the bins up to them hold
-      unsigned long long h0 = 0, h1 = 0;
-      for (int r = 0; r < p.ctas; ++r) {
-        const unsigned long long v = s.read(tid, r);
-        h0 += v & 0xFFFFFFFFull;
-        h1 += v >> 32;
+      unsigned long long part[SCTAS], h0 = 0, h1 = 0;
+      s.read_all(tid, part);
+#pragma unroll
+      for (int r = 0; r < SCTAS; ++r) {
+        h0 += part[r] & 0xFFFFFFFFull;
+        h1 += part[r] >> 32;
       }
       unsigned long long c = h0 + h1;
 #pragma unroll
@@ -456,68 +620,84 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
       __syncthreads();
       s.next();
       if (blo < SBINS) {
-        const float e = top - (blo + 1) / to_bin / s.inv_t;
-        if (e == e) glo = max(low, min(order_key(e), tk));
+        const float e = top - (blo + (by_max ? 1 : 2)) / to_bin / s.inv_t;  // (a bin to spare)
+        if (e == e) glo = max(low, min(Key::of(e), tk));
       }
       if (want_hi > 0 && bhi < SBINS && bhi > 0) {
-        const float e = top - bhi / to_bin / s.inv_t;
-        if (e == e) ghi = min(high, max(order_key(e), glo + 1));
+        const float e = top - (bhi - 1) / to_bin / s.inv_t;
+        if (e == e) ghi = min(high, max(Key::of(e), glo + 1));
       }
     }
 
-    auto weight = [&](uint32_t key) -> unsigned long long { return sample_weight(key_float(key), top, s.inv_t); };
     // tokens of key `cut` that stay when the weight above it is acc
     auto ties_of = [&](unsigned long long bound, unsigned long long acc) -> long long {
-      const unsigned long long wt = weight(cut);
+      const unsigned long long wt = s.weight_of(cut);
       return wt ? static_cast<long long>((bound - acc + wt - 1) / wt) : V;
     };
     unsigned long long bound = k, acc = 0;
-    bool limited = false;
+    int found = Sampler<T>::NONE;
+    bool whole_row = false;
     if (k) {
-      limited = s.template search<false>(low, high, glo, high, bound, false, cut, acc);
-      if (limited) ties = k - static_cast<long long>(acc);
+      found = s.template search<false>(low, high, glo, high, bound, false, cut, acc);
+      if (found == Sampler<T>::CUT) ties = k - static_cast<long long>(acc);
     }
-    if (nucleus && !limited) {
+    if (nucleus && found == Sampler<T>::NONE) {
       // of the whole row (or of fewer than k tokens of any weight)
+      whole_row = true;
       bound = fixed32(tp);
-      if (s.template search<true>(low, high, k ? low : glo, k ? high : ghi, bound, true, cut, acc)) ties = ties_of(bound, acc);
-    } else if (nucleus) {
+      found = s.template search<true>(low, high, k ? low : glo, k ? high : ghi, bound, true, cut, acc);
+      if (found == Sampler<T>::CUT) ties = ties_of(bound, acc);
+    } else if (nucleus && found == Sampler<T>::CUT) {
       // of the first k: their weight above the cut first
-      unsigned long long sum = 0, zero = 0;
+      unsigned long long v[1] = {0};
       const bool listed = s.list_ok && s.list_hi == high;
       if (listed) {
         for (int i = lane; i < s.n_list; i += 32)
-          if (s.list[i].x > cut) sum += weight(s.list[i].x);
+          if (s.list[i].x > cut) v[0] += s.weight_of(s.list[i].x);
       } else {
-        unsigned long long in_list;
-        s.template pass<true>(cut, cut + 1, in_list, zero);
-        sum = s.above;
-        zero = 0;
+        unsigned long long in_list, all;
+        s.template pass<true>(cut, cut + 1, in_list, all);
+        v[0] = s.above;
         s.list_ok = false;
       }
-      s.sum2(sum, zero);
-      bound = scaled_ceil(sum + ties * weight(cut), fixed32(tp));
-      if (bound == 0) bound = 1;
+      s.sums(v);
+      const unsigned long long sum = v[0];
+      bound = max(1ull, scaled_ceil(sum + ties * s.weight_of(cut), fixed32(tp)));
       if (bound > sum) {
         ties = min(ties, ties_of(bound, sum));
       } else {
         acc = 0;
-        if (listed) cut = s.template radix<true>(cut + 1, acc, bound);
-        else s.template search<true>(cut + 1, high, cut + 1, high, bound, false, cut, acc);
-        ties = ties_of(bound, acc);
+        if (listed) {
+          cut = s.template radix<true>(cut + 1, acc, bound);
+          ties = ties_of(bound, acc);
+        } else {
+          found = s.template search<true>(cut + 1, high, cut + 1, high, bound, false, cut, acc);
+          if (found == Sampler<T>::CUT) ties = ties_of(bound, acc);
+        }
       }
+      if (found == Sampler<T>::FEW) {
+        // every token of the bracket is in the lists and the bound is known: the cut from them
+        acc = 0;
+        cut = s.template radix<true>(cut + 1, acc, bound);
+        ties = ties_of(bound, acc);
+        found = Sampler<T>::CUT;
+      }
+    }
+    if (found == Sampler<T>::FEW) {
+      s.few(row, k, nucleus, tp, whole_row ? bound : 0, least, s_few);
+      return;
     }
   }
 
   // ---- every warp's kept weight, number kept, and tokens of the cut's own key
-  const float fcut = cut ? key_float(cut) : -INFINITY;
+  const float fcut = cut ? Key::value(cut) : -INFINITY;
   const uint32_t wt = cut ? sample_weight(fcut, top, s.inv_t) : 0u;
   if (wt < least) ties = 0;
   unsigned long long sum = 0;
   unsigned int n_kept = 0, n_tie = 0;
   // the list holds them all, or all that the last pass did not sum already
   const bool listed = s.list_ok && (s.list_hi == high ||
-                                    (s.summed && sample_weight(key_float(s.list_hi), top, s.inv_t) >= least));
+                                    (s.summed && sample_weight(Key::value(s.list_hi), top, s.inv_t) >= least));
   if (listed) {
     if (s.list_hi != high) {
       sum = s.above;
@@ -525,7 +705,7 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
     }
     for (int i = lane; i < s.n_list; i += 32) {
       const uint32_t key = s.list[i].x;
-      const uint32_t wi = sample_weight(key_float(key), top, s.inv_t);
+      const uint32_t wi = sample_weight(Key::value(key), top, s.inv_t);
       if (key > cut && wi >= least) {
         sum += wi;
         ++n_kept;
@@ -596,63 +776,78 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
   unsigned long long run = __shfl_sync(0xffffffffu, in1 ? before + cs[0] : before, owner);
   long long tie_run = __shfl_sync(0xffffffffu, in1 ? tie_pre + ct[0] : tie_pre, owner);
 
-  // ---- the warp whose chunk it is finds the token
-  if (chunk == s.rank * SW + w) {
-    for (int it = 0; it < p.per; ++it) {
-      float v[VEC];
-      s.vec(it, v);
-      int nt = 0;
+  s.next();
+  s.agree();  // nobody reads this CTA's buffers any more
+  // ---- the CTA whose chunk it is finds the token: warp i takes the chunk's i-th 256 (or 128) elements of every eight
+  if (chunk / SW != s.rank) return;
+  const T* part = s.data + (chunk % SW) * p.per * 32 * VEC;
+  for (int it0 = 0; it0 < p.per; it0 += SW) {
+    const int it = it0 + w;
+    float v[VEC];
+    if (it < p.per) {
+      ldv<T, VEC>(part + it * 32 * VEC + lane * VEC, v);
+    } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) nt += v[e] == fcut;
-      int pre = nt;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, pre, d);
-        if (lane >= d) pre += t;
-      }
-      const int all_ties = __shfl_sync(0xffffffffu, pre, 31);
-      long long rank = tie_run + pre - nt;
-      uint32_t we[VEC];
-      unsigned long long mine = 0;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const bool tie = v[e] == fcut;
-        const uint32_t wi = sample_weight(v[e], top, s.inv_t);
-        we[e] = wi >= least && (v[e] > fcut || (tie && rank < ties)) ? wi : 0u;
-        rank += tie;
-        mine += we[e];
-      }
-      unsigned long long end = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long t = __shfl_up_sync(0xffffffffu, end, d);
-        if (lane >= d) end += t;
-      }
-      end += run;
-      if (end > target && end - mine <= target) {
-        unsigned long long at = end - mine;
-        int e = 0;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          at += we[i];
-          if (at <= target) e = i + 1;
-        }
-        const int token = s.base + (it * 32 + lane) * VEC + e;
-        float xe = v[0];
-#pragma unroll
-        for (int i = 1; i < VEC; ++i)
-          if (i == e) xe = v[i];
-        p.token[row] = token;
-        if (p.kept) p.kept[row] = static_cast<int32_t>(kept_all);
-        if (p.logprob)
-          p.logprob[row] = -sample_dist(xe, top, s.inv_t) - logf(static_cast<float>(total) * 4.656612873077393e-10f);
-      }
-      run = __shfl_sync(0xffffffffu, end, 31);
-      tie_run += all_ties;
-      if (run > target) break;
+      for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
     }
+    int nt = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) nt += v[e] == fcut;
+    int pre = nt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, pre, d);
+      if (lane >= d) pre += t;
+    }
+    __syncthreads();
+    if (lane == 31) s_tmp[w] = pre;
+    __syncthreads();
+    long long rank = tie_run + pre - nt;
+    for (int i = 0; i < SW; ++i) {
+      const long long n = static_cast<long long>(s_tmp[i]);
+      if (i < w) rank += n;
+      tie_run += n;
+    }
+    uint32_t we[VEC];
+    unsigned long long mine = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const bool tie = v[e] == fcut;
+      const uint32_t wi = sample_weight(v[e], top, s.inv_t);
+      we[e] = wi >= least && (v[e] > fcut || (tie && rank < ties)) ? wi : 0u;
+      rank += tie;
+      mine += we[e];
+    }
+    unsigned long long end = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long t = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end += t;
+    }
+    if (lane == 31) s_tmp[SW + w] = end;
+    __syncthreads();
+    end += run;
+    for (int i = 0; i < SW; ++i) {
+      const unsigned long long n = s_tmp[SW + i];
+      if (i < w) end += n;
+      run += n;
+    }
+    if (end > target && end - mine <= target) {
+      unsigned long long at = end - mine;
+      int e = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        at += we[i];
+        if (at <= target) e = i + 1;
+      }
+      float xe = v[0];
+#pragma unroll
+      for (int i = 1; i < VEC; ++i)
+        if (i == e) xe = v[i];
+      s.finish(row, (chunk * p.per + it) * 32 * VEC + lane * VEC + e, xe, total, static_cast<int>(kept_all));
+    }
+    if (run > target) break;  // the same in every warp
   }
-  s.agree();  // the others may still read this CTA's buffer
 }
 
 constexpr int kSampleMaxV = 1 << 18;
@@ -664,7 +859,7 @@ constexpr int kSampleMaxV = 1 << 18;
 static void sample_shape(int rows, int V, int esize, int& ctas, int& per) {
   const int vec = 16 / esize, chunk = SW * 32 * vec;  // elements per CTA and vector
   ctas = 1;
-  while (ctas < 8 && (static_cast<long long>(V) * esize > static_cast<long long>(ctas) * 32768 ||
+  while (ctas < SCTAS && (static_cast<long long>(V) * esize > static_cast<long long>(ctas) * 32768 ||
                       (static_cast<long long>(rows) * ctas * 2 <= 296 && V > ctas * chunk)))
     ctas *= 2;
   per = (V + ctas * chunk - 1) / (ctas * chunk);
