@@ -256,7 +256,8 @@ int tkb_lmhead_ce(const void *X, long long ldx, const void *W, long long ldw, co
  *   pos          [n_pages][Hkv][page_size] position of the token a slot
  *                holds, or NULL (needed by tkb_kv_evict).
  *   weight       [n_pages][Hkv][page_size] accumulated attention weight of a
- *                slot, or NULL (needed by tkb_kv_evict).
+ *                slot, or NULL (needed by tkb_kv_evict).  pos and weight
+ *                16-byte aligned.
  *   block_table  [B][max_pages]; slot j of sequence b lies in page
  *                block_table[b][j / page_size].  Only the entries that the
  *                lengths reach are read.

@@ -158,6 +158,8 @@ int tkb_kv_evict(const tkb_kv_cache* cache, const int32_t* seen, int budget, int
   if (rc) return rc;
   if (!seen || !cache->pos || !cache->weight)
     return fail(TKB_ERR_ARG, "%s: seen and the cache's pos and weight are needed", who);
+  if (!aligned16(cache->pos) || !aligned16(cache->weight))
+    return fail(TKB_ERR_ARG, "%s: pos and weight must be 16-byte aligned", who);
   if (budget <= 0 || recent < 0 || sinks < 0 || static_cast<long long>(recent) + sinks > budget)
     return fail(TKB_ERR_ARG, "%s: budget must be positive and hold recent + sinks tokens", who);
   const size_t need = tkb_kv_evict_workspace(cache);

@@ -1,9 +1,26 @@
 // paged.cu -- the paged key-value cache: new tokens enter it, one new token
 // per sequence attends over it, tokens leave it by accumulated weight.
+#include <atomic>
+
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
 namespace tkb {
+
+// Raises a kernel's limit of dynamic shared memory, once per device (the call
+// costs as much host time as a launch).
+template <auto Kernel>
+static cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Element offset of slot 0 of (page, kv head) in k and v.
 TKB_DEVFN long long page_offset(const tkb_kv_cache& c, int page, int h) {
@@ -42,8 +59,11 @@ __global__ void kv_lens_kernel(int32_t* __restrict__ lens, int32_t* __restrict__
 
 // ============================================================ append
 // qkv_prep_fwd_kernel (rows.cu) with each row's own position, its K and V
-// columns stored to the row's slot.  One block per row; the row's D/2 cosines
-// and sines are computed once, in shared memory, for all its heads.
+// columns stored to the row's slot.  A block takes R rows: their cosines and
+// sines (D/2 each, for all heads) are computed once, in shared memory, and a
+// thread walks the R rows of a column, so that bias and gain are read once for
+// them and R loads are in flight.  R is 4 for prompts, 1 when the rows would
+// not fill the GPU.
 struct AppendParams {
   tkb_kv_cache c;
   const void* qkv;
@@ -58,110 +78,123 @@ struct AppendParams {
   RopeTable tab;
 };
 
-template <typename T>
+template <typename T, int R>
 __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ float s_cs[64], s_sn[64];
-  __shared__ long long s_kv, s_meta;  // element offset of the row's slot of kv head 0; its pos / weight index
-  __shared__ int s_pos;
+  __shared__ float s_cs[R][64], s_sn[R][64];
+  __shared__ long long s_kv[R], s_meta[R];  // element offset of the row's slot of kv head 0; its pos / weight index
+  __shared__ int s_pos[R];
   const tkb_kv_cache& c = p.c;
   const int Hq = p.Hq, Hkv = c.Hkv, D = c.D, C = (Hq + 2 * Hkv) * D, nqk = Hq + Hkv, nvec = C / 8, grp = D / 8;
   const T* in = static_cast<const T*>(p.qkv);
   T* out = static_cast<T*>(p.out);
-  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    __syncthreads();  // the previous row's shared values have been read
-    if (threadIdx.x < D / 2) {
-      // the row's sequence: the last b with row_start[b] <= row
-      int b = row, back = 1;
-      bool has = true;
-      if (p.row_start) {
-        int lo = 0, hi = c.B;
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (p.row_start[mid] <= row) lo = mid; else hi = mid;
-        }
-        b = lo;
-        back = p.row_start[b + 1] - row;
-        has = back > 0 && p.row_start[b] <= row;
-      }
-      const int slot = c.seq_lens[b] - back;
-      const int pos = (p.seen ? p.seen[b] : c.seq_lens[b]) - back;
-      if (p.rope) {
-        float sn, cs;
-        rope_cs(pos, p.tab.inv_freq[threadIdx.x], sn, cs);
-        s_cs[threadIdx.x] = cs;
-        s_sn[threadIdx.x] = sn;
-      }
-      if (threadIdx.x == 0) {
-        int page = -1;
-        if (has && slot >= 0 && slot < c.max_pages * c.page_size) page = page_of(c, b, slot / c.page_size);
-        else atomicOr(&g_device_error, ERR_BAD_INDEX);
-        const int in_page = slot % c.page_size;
-        s_kv = page < 0 ? -1 : page_offset(c, page, 0) + static_cast<long long>(in_page) * D;
-        s_meta = page < 0 ? -1 : meta_offset(c, page, 0) + in_page;
-        s_pos = pos;
-      }
+  const int row0 = blockIdx.x * R, tid = threadIdx.x;
+  // ---- where the rows go: the sequence is the last b with row_start[b] <= row
+  int b0 = row0;
+  if (p.row_start) {
+    int upto = 0;
+    for (int b = 0; b < c.B; b += NT) upto += __syncthreads_count(b + tid < c.B && p.row_start[b + tid] <= row0);
+    b0 = upto - 1;
+  }
+  if (tid < R && row0 + tid < p.rows) {
+    const int row = row0 + tid;
+    int b = p.row_start ? b0 : row, back = 1;
+    bool has = true;
+    if (p.row_start) {
+      while (b + 1 < c.B && p.row_start[b + 1] <= row) ++b;
+      has = b >= 0 && p.row_start[b] <= row && row < p.row_start[b + 1];
+      b = max(b, 0);
+      back = p.row_start[b + 1] - row;
+    }
+    const int held = c.seq_lens[b], slot = held - back;
+    int page = -1;
+    if (has && slot >= 0 && slot < c.max_pages * c.page_size) page = page_of(c, b, slot / c.page_size);
+    else atomicOr(&g_device_error, ERR_BAD_INDEX);
+    const int in_page = slot % c.page_size;
+    s_kv[tid] = page < 0 ? -1 : page_offset(c, page, 0) + static_cast<long long>(in_page) * D;
+    s_meta[tid] = page < 0 ? -1 : meta_offset(c, page, 0) + in_page;
+    s_pos[tid] = (p.seen ? p.seen[b] : held) - back;
+  }
+  __syncthreads();
+  if (p.rope) {
+    for (int i = tid; i < R * (D / 2); i += NT) {
+      const int r = i / (D / 2), d = i % (D / 2);
+      float sn = 0.f, cs = 1.f;
+      if (row0 + r < p.rows) rope_cs(s_pos[r], p.tab.inv_freq[d], sn, cs);
+      s_cs[r][d] = cs;
+      s_sn[r][d] = sn;
     }
     __syncthreads();
-    const long long base = static_cast<long long>(row) * p.qkv_stride;
-    for (int v0 = 0; v0 < nvec; v0 += NT) {
-      const int vi = v0 + threadIdx.x;
-      const bool act = vi < nvec;
-      const int col = vi * 8, hd = col / D, d = col % D;
-      float v[8];
-      if (act) {
-        ldv<T, 8>(in + base + col, v);
-        if (p.bias) {
-          float bb[8];
-          ldf<8>(p.bias + col, bb);
+  }
+  for (int v0 = 0; v0 < nvec; v0 += NT) {
+    const int vi = v0 + tid;
+    const bool act = vi < nvec;
+    const int col = vi * 8, hd = col / D, d = col % D;
+    float v[R][8], bb[8], gg[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += bb[e];
-        }
-      } else {
+    for (int r = 0; r < R; ++r) {
+      if (act && row0 + r < p.rows) ldv<T, 8>(in + static_cast<long long>(row0 + r) * p.qkv_stride + col, v[r]);
+      else
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      }
-      if (p.qknorm) {
+        for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
+    }
+    if (p.bias && act) {
+      ldf<8>(p.bias + col, bb);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[r][e] += bb[e];
+    }
+    const bool turned = act && hd < nqk;
+    if (p.qknorm) {
+      if (p.gain && turned) ldf<8>(p.gain + col, gg);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
         float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[r][e], v[r][e], ss);
         for (int m = grp >> 1; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        if (act && hd < nqk) {
+        if (turned) {
           const float is = 1.0f / sqrtf(ss / static_cast<float>(D) + 1e-5f);
-          float gg[8];
-          if (p.gain) ldf<8>(p.gain + col, gg);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = v[e] * is * (p.gain ? gg[e] : 1.0f);
+          for (int e = 0; e < 8; ++e) v[r][e] = v[r][e] * is * (p.gain ? gg[e] : 1.0f);
         }
-      }
-      if (!act) continue;
-      if (p.rope && hd < nqk) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float sn = s_sn[d / 2 + e], cs = s_cs[d / 2 + e];
-          const float x0 = v[2 * e], x1 = v[2 * e + 1];
-          v[2 * e] = x0 * cs - x1 * sn;
-          v[2 * e + 1] = x0 * sn + x1 * cs;
-        }
-      }
-      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + static_cast<long long>(row) * p.out_stride + col, v);
-      if (hd >= Hq && s_kv >= 0) {
-        const int h = hd < nqk ? hd - Hq : hd - nqk;
-        T* pool = static_cast<T*>(hd < nqk ? c.k : c.v);
-        stv<T, 8>(pool + s_kv + static_cast<long long>(h) * c.page_size * D + d, v);
       }
     }
-    if (s_meta >= 0)
-      for (int h = threadIdx.x; h < Hkv; h += NT) {
-        const long long at = s_meta + static_cast<long long>(h) * c.page_size;
-        if (c.pos) c.pos[at] = s_pos;
-        if (c.weight) c.weight[at] = 0.f;
+    if (!act) continue;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= p.rows) break;
+      if (p.rope && turned) {
+        const float4 cs = *reinterpret_cast<const float4*>(&s_cs[r][d / 2]), sn = *reinterpret_cast<const float4*>(&s_sn[r][d / 2]);
+        const float c4[4] = {cs.x, cs.y, cs.z, cs.w}, s4[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = v[r][2 * e], x1 = v[r][2 * e + 1];
+          v[r][2 * e] = x0 * c4[e] - x1 * s4[e];
+          v[r][2 * e + 1] = x0 * s4[e] + x1 * c4[e];
+        }
       }
+      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + static_cast<long long>(row0 + r) * p.out_stride + col, v[r]);
+      if (hd >= Hq && s_kv[r] >= 0) {
+        const int h = hd < nqk ? hd - Hq : hd - nqk;
+        T* pool = static_cast<T*>(hd < nqk ? c.k : c.v);
+        stv<T, 8>(pool + s_kv[r] + static_cast<long long>(h) * c.page_size * D + d, v[r]);
+      }
+    }
+  }
+  for (int i = tid; i < R * Hkv; i += NT) {
+    const int r = i % R, h = i / R;
+    if (row0 + r >= p.rows || s_meta[r] < 0) continue;
+    const long long at = s_meta[r] + static_cast<long long>(h) * c.page_size;
+    if (c.pos) c.pos[at] = s_pos[r];
+    if (c.weight) c.weight[at] = 0.f;
   }
 }
 
 template <typename T>
 static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
-  kv_append_kernel<T><<<row_grid(p.rows, 8), NT, 0, st>>>(p);
+  if (p.rows >= 148 * 8) kv_append_kernel<T, 4><<<(p.rows + 3) / 4, NT, 0, st>>>(p);
+  else kv_append_kernel<T, 1><<<p.rows, NT, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -892,7 +925,7 @@ static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
   using Cfg = typename Tile::Cfg;
   constexpr int W = Cfg::WARPS;
   auto k = paged_decode_kernel<T, D, Tile>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+  cudaError_t e = allow_smem<paged_decode_kernel<T, D, Tile>>(Cfg::SMEM);
   if (e != cudaSuccess) return e;
   const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks * (p.c.max_pages * p.c.page_size / Cfg::TK);
   const int grid = static_cast<int>(most < kDecodeGrid * W ? (most + W - 1) / W : kDecodeGrid);
@@ -924,8 +957,8 @@ static cudaError_t paged_decode_t(const DecodeParams& p, cudaStream_t st) {
 }
 
 // ============================================================ eviction
-// Per (sequence, kv head): the budget-th largest key by bisection on counts,
-// then the freed slots below the budget and the kept tokens above it, both in
+// Per (sequence, kv head): the budget-th largest key by a radix search over
+// counts (11, 11 and 10 bits), then the freed slots below the budget and the kept tokens above it, both in
 // ascending order, then the moves.  Reads 8 bytes per slot; the moves (read
 // and written once) are what HBM is busy with, so several CTAs share a unit
 // when there are few units.  They form a cluster: each finds the same cut from
@@ -949,15 +982,6 @@ TKB_DEVFN uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the block of a warp-uniform count; `sh` holds two sums used in turn.
-template <int THREADS>
-TKB_DEVFN int evict_count(int v, int* sh, int turn) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  if (lane_id() == 0) sh[turn * (THREADS / 32) + warp_id()] = v;
-  __syncthreads();
-  int s = lane_id() < THREADS / 32 ? sh[turn * (THREADS / 32) + lane_id()] : 0;
-  return __reduce_add_sync(0xffffffffu, s);
-}
 // Exclusive prefix over the warps of a warp-uniform count.
 template <int THREADS>
 TKB_DEVFN int evict_prefix(int v, int* sh, int turn, int& total) {
@@ -972,7 +996,7 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant__ EvictParams p) {
   constexpr int W = THREADS / 32;
   extern __shared__ __align__(16) uint32_t s_keys[];
-  __shared__ int sh[2 * W];
+  __shared__ int sh[2 * W], hist[2048], s_cut[3];
   const tkb_kv_cache& c = p.c;
   const int unit = blockIdx.x / p.split, rank = blockIdx.x % p.split;
   const int b = unit / c.Hkv, h = unit % c.Hkv, tid = threadIdx.x, w = warp_id(), lane = lane_id();
@@ -984,58 +1008,94 @@ __global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant
   const int newest = p.seen[b] - p.recent;
   const bool by_pos = p.recent > 0 || p.sinks > 0;
   const int32_t* table = c.block_table + static_cast<long long>(b) * c.max_pages;
+  // four slots a thread: pages are multiples of 16, so one page holds them
 #pragma unroll 4
-  for (int j = tid; j < n; j += THREADS) {
+  for (int j = 4 * tid; j < n; j += 4 * THREADS) {
     const int pg = j / ps, page = __ldg(table + pg);
-    uint32_t k = 0u;
+    uint4 k = make_uint4(0u, 0u, 0u, 0u);
     if (static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages)) {
       const long long at = meta_offset(c, page, h) + (j - pg * ps);
-      k = order_key(c.weight[at]);
+      const float4 x = *reinterpret_cast<const float4*>(c.weight + at);
+      k = make_uint4(order_key(x.x), order_key(x.y), order_key(x.z), order_key(x.w));
       if (by_pos) {
-        const int pos = c.pos[at];
-        if (pos >= newest || pos < p.sinks) k = 0xFFFFFFFFu;
+        const int4 pos = *reinterpret_cast<const int4*>(c.pos + at);
+        if (pos.x >= newest || pos.x < p.sinks) k.x = 0xFFFFFFFFu;
+        if (pos.y >= newest || pos.y < p.sinks) k.y = 0xFFFFFFFFu;
+        if (pos.z >= newest || pos.z < p.sinks) k.z = 0xFFFFFFFFu;
+        if (pos.w >= newest || pos.w < p.sinks) k.w = 0xFFFFFFFFu;
       }
     } else {
       atomicOr(&g_device_error, ERR_BAD_INDEX);
     }
-    keys[j] = k;
+    *reinterpret_cast<uint4*>(keys + j) = k;  // the key area holds whole pages
   }
-  __syncthreads();
 
-  // ---- the cut: the largest key that at least `budget` tokens reach
-  uint32_t lo = 0, hi = 0xFFFFFFFFu;  // reached by budget tokens at lo; hi: the largest candidate
-  int turn = 0, reach = n;            // tokens with key >= lo
-  while (lo < hi && reach != p.budget) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    int cnt = 0;
-    for (int j = tid; j < n; j += THREADS) cnt += keys[j] >= mid;
-    cnt = evict_count<THREADS>(cnt, sh, turn);
-    turn ^= 1;
-    if (cnt >= p.budget) {
-      lo = mid;
-      reach = cnt;
-    } else {
-      hi = mid - 1;
+  // ---- the cut: the largest key that at least `budget` tokens reach.  Weights
+  // differ in their first 11 bits (sign, exponent, two bits) enough to spread
+  // the first histogram; a warp whose keys agree adds once.
+  uint32_t lo = 0;
+  int need = p.budget;  // of the tokens that share lo's bits so far
+  int in_bin = 0;
+#pragma unroll 1
+  for (int level = 0; level < 3; ++level) {
+    const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11, bins = 1 << bits;
+    for (int i = tid; i < bins; i += THREADS) hist[i] = 0;
+    __syncthreads();
+    for (int j0 = 0; j0 < n; j0 += THREADS) {
+      const int j = j0 + tid;
+      const uint32_t k = j < n ? keys[j] : 0u;
+      const bool in = j < n && (level == 0 || (k >> (shift + bits)) == (lo >> (shift + bits)));
+      const int bin = static_cast<int>((k >> shift) & (bins - 1));
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      if (!m) continue;
+      const int lead = __ffs(m) - 1, first = __shfl_sync(0xffffffffu, bin, lead);
+      if (__all_sync(0xffffffffu, !in || bin == first)) {
+        if (lane == lead) atomicAdd(&hist[first], __popc(m));
+      } else if (in) {
+        atomicAdd(&hist[bin], 1);
+      }
     }
+    __syncthreads();
+    // thread t: the bins from the top, `run` at a time
+    const int run = bins / THREADS;
+    int sum = 0;
+    for (int i = 0; i < run; ++i) sum += hist[bins - 1 - tid * run - i];
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 31) sh[w] = upto;
+    __syncthreads();
+    const int x = lane < W ? sh[lane] : 0;
+    upto += __reduce_add_sync(0xffffffffu, lane < w ? x : 0);
+    if (upto >= need && upto - sum < need) {
+      int above = upto - sum, bin = bins - 1 - tid * run;
+      while (above + hist[bin] < need) above += hist[bin--];
+      s_cut[0] = bin;
+      s_cut[1] = need - above;
+      s_cut[2] = hist[bin];
+    }
+    __syncthreads();
+    lo |= static_cast<uint32_t>(s_cut[0]) << shift;
+    need = s_cut[1];
+    in_bin = s_cut[2];
   }
-  // kept: every key >= lo when just the budget reaches it, else the keys above it and the first `need` equal to it
+  // kept: the keys above lo, and of those equal to it the first `need`
   const int chunk = (n + THREADS - 1) / THREADS * 32, j0 = min(n, w * chunk), j1 = min(n, j0 + chunk);
-  int need = n, tie_base = 0;
-  __syncthreads();
-  if (reach != p.budget) {
-    int above = 0, ties = 0, total;
-    for (int j = j0 + lane; j < j1; j += 32) {
-      above += keys[j] > lo;
-      ties += keys[j] == lo;
-    }
-    above = evict_count<THREADS>(above, sh, 0);
-    need = p.budget - above;
+  int tie_base = 0;
+  if (need < in_bin) {  // not all of them: their order counts
+    int ties = 0, total;
+    for (int j = j0 + lane; j < j1; j += 32) ties += keys[j] == lo;
+    __syncthreads();
     tie_base = evict_prefix<THREADS>(__reduce_add_sync(0xffffffffu, ties), sh, 1, total);
     __syncthreads();
   }
   // `f(j, kept)` for the warp's slots in order, 32 at a time
   auto walk = [&](auto f) {
     int rank_base = tie_base;
+#pragma unroll 2
     for (int j = j0; j < j1; j += 32) {
       const bool in = j + lane < j1;
       const uint32_t k = in ? keys[j + lane] : 0u;
@@ -1133,7 +1193,7 @@ static cudaError_t kv_evict_launch(EvictParams p, cudaStream_t st) {
   p.split = evict_split(p.c);
   const size_t smem = p.keys ? 0 : static_cast<size_t>(slots) * 4;
   auto k = kv_evict_kernel<T, THREADS>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSmemKeys * 4);
+  cudaError_t e = allow_smem<kv_evict_kernel<T, THREADS>>(kEvictSmemKeys * 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.c.B) * p.c.Hkv * p.split);

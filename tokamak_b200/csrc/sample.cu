@@ -870,7 +870,8 @@ static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
   sample_shape(p.rows, p.V, sizeof(T), p.ctas, p.per);
   const size_t smem = static_cast<size_t>(p.per) * SNT * 16;
   auto k = sample_kernel<T>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // the widest slice: kSampleMaxV fp32 logits over SCTAS CTAs
+  cudaError_t e = allow_smem<sample_kernel<T>>(kSampleMaxV / SCTAS * 4);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.ctas);

@@ -227,8 +227,12 @@ class _KVCacheStruct(ctypes.Structure):
                 ("dtype", ctypes.c_int)]
 
 
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
 def _expect(t, name, shape, dtype):
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous()):
+    if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous()):
         raise TkbError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, "
                        f"got {t.dtype} {tuple(t.shape)}")
 
@@ -268,7 +272,7 @@ class KVCache:
 
 def kv_lens(seq_lens, limit, seen=None, add=0, row_start=None):
     """seq_lens = min(seq_lens + n, limit) and seen += n, on the device (n = add, or row_start's differences)."""
-    check(lib().tkb_kv_lens(_p(seq_lens), _p(seen), _p(row_start), int(add), int(limit), seq_lens.numel(), _raw_stream(seq_lens)),
+    check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add), int(limit), seq_lens.numel(), _raw_stream(seq_lens)),
           "tkb_kv_lens")
 
 
@@ -281,8 +285,8 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
     rows = qkv.shape[0]
     if out is None:
         out = torch.empty(rows, (Hq + 2 * cache.Hkv if full else Hq) * cache.D, dtype=qkv.dtype, device=qkv.device)
-    check(lib().tkb_kv_append(cache.ref, _p(qkv), qkv.stride(0), _p(bias), _p(qk_gain), _p(out), out.stride(0),
-                              int(full), _p(row_start), _p(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
+    check(lib().tkb_kv_append(cache.ref, _ptr(qkv), qkv.stride(0), _ptr(bias), _ptr(qk_gain), _ptr(out), out.stride(0),
+                              int(full), _ptr(row_start), _ptr(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
                               low, high, octx, _raw_stream(qkv)), "tkb_kv_append")
     return out
 
@@ -307,8 +311,8 @@ def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=
         lse = torch.empty(cache.B, Hq, dtype=torch.float32, device=q.device)
     if workspace is None:
         workspace = paged_attn_workspace(cache, Hq, accumulate)
-    check(lib().tkb_paged_attn_decode(cache.ref, _p(q), q.stride(0), _p(out), out.stride(0), _p(lse), Hq,
-                                      cache.D ** -0.5 if scale is None else scale, int(accumulate), _p(workspace),
+    check(lib().tkb_paged_attn_decode(cache.ref, _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(lse), Hq,
+                                      cache.D ** -0.5 if scale is None else scale, int(accumulate), _ptr(workspace),
                                       workspace.numel(), _raw_stream(q)), "tkb_paged_attn_decode")
     return out, lse
 
@@ -325,7 +329,7 @@ def kv_evict(cache, budget, seen, recent=0, sinks=0, workspace=None):
     kv_lens(cache.seq_lens, budget) after the last layer."""
     if workspace is None:
         workspace = kv_evict_workspace(cache)
-    check(lib().tkb_kv_evict(cache.ref, _p(seen), int(budget), int(recent), int(sinks), _p(workspace),
+    check(lib().tkb_kv_evict(cache.ref, _ptr(seen), int(budget), int(recent), int(sinks), _ptr(workspace),
                              workspace.numel(), _raw_stream(seen)), "tkb_kv_evict")
 
 
@@ -338,10 +342,10 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
                         (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
         _expect(t, name, (rows,), dt)
-    token = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    kept = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    check(lib().tkb_sample_logits(_p(logits), logits.stride(0) if rows > 1 else V, _p(u), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
-                                  _p(token), _p(logprob), _p(kept), rows, V, dtype_code(logits), _raw_stream(logits)),
+    logprob = torch.empty_like(u)
+    token = torch.empty_like(u, dtype=torch.int32)
+    kept = torch.empty_like(token)
+    check(lib().tkb_sample_logits(_ptr(logits), logits.stride(0) if rows > 1 else V, _ptr(u), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+                                  _ptr(token), _ptr(logprob), _ptr(kept), rows, V, dtype_code(logits), _raw_stream(logits)),
           "tkb_sample_logits")
     return token, logprob, kept
