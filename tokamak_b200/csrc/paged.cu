@@ -78,16 +78,56 @@ struct AppendParams {
   RopeTable tab;
 };
 
-template <typename T, int R>
+// Eight elements as loaded, and as floats.
+template <typename T>
+struct Raw8 {
+  uint4 q[sizeof(T) / 2];
+  TKB_DEVFN void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) q[i] = ld_stream_v4(reinterpret_cast<const uint4*>(p) + i);
+  }
+  TKB_DEVFN void floats(float (&f)[8]) const {
+    const uint32_t u[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t v[4] = {q[1].x, q[1].y, q[1].z, q[1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = __uint_as_float(u[i]);
+        f[4 + i] = __uint_as_float(v[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = unpack2<std::is_same<T, __nv_bfloat16>::value>(u[i]);
+        f[2 * i] = x.x;
+        f[2 * i + 1] = x.y;
+      }
+    }
+  }
+};
+
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float s_cs[R][64], s_sn[R][64];
   __shared__ long long s_kv[R], s_meta[R];  // element offset of the row's slot of kv head 0; its pos / weight index
   __shared__ int s_pos[R];
   const tkb_kv_cache& c = p.c;
-  const int Hq = p.Hq, Hkv = c.Hkv, D = c.D, C = (Hq + 2 * Hkv) * D, nqk = Hq + Hkv, nvec = C / 8, grp = D / 8;
+  const int Hq = p.Hq, Hkv = c.Hkv, C = (Hq + 2 * Hkv) * D, nqk = Hq + Hkv, nvec = C / 8;
+  constexpr int grp = D / 8;
   const T* in = static_cast<const T*>(p.qkv);
   T* out = static_cast<T*>(p.out);
-  const int row0 = blockIdx.x * R, tid = threadIdx.x;
+  const int row0 = blockIdx.x * R, tid = threadIdx.x, rows = min(R, p.rows - row0);
+  in += static_cast<long long>(row0) * p.qkv_stride;
+  if (out) out += static_cast<long long>(row0) * p.out_stride;
+  // the next column's loads are under way while one is worked on, the first one's during what comes before
+  Raw8<T> raw[R];
+  auto fetch = [&](int vi) {
+    if (vi < nvec)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < rows) raw[r].load(in + r * p.qkv_stride + vi * 8);
+  };
+  fetch(tid);
   // ---- where the rows go: the sequence is the last b with row_start[b] <= row
   int b0 = row0;
   if (p.row_start) {
@@ -119,7 +159,7 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     for (int i = tid; i < R * (D / 2); i += NT) {
       const int r = i / (D / 2), d = i % (D / 2);
       float sn = 0.f, cs = 1.f;
-      if (row0 + r < p.rows) rope_cs(s_pos[r], p.tab.inv_freq[d], sn, cs);
+      if (r < rows) rope_cs(s_pos[r], p.tab.inv_freq[d], sn, cs);
       s_cs[r][d] = cs;
       s_sn[r][d] = sn;
     }
@@ -132,11 +172,12 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     float v[R][8], bb[8], gg[8];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (act && row0 + r < p.rows) ldv<T, 8>(in + static_cast<long long>(row0 + r) * p.qkv_stride + col, v[r]);
+      if (act && r < rows) raw[r].floats(v[r]);
       else
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
     }
+    fetch(vi + NT);
     if (p.bias && act) {
       ldf<8>(p.bias + col, bb);
 #pragma unroll
@@ -146,24 +187,29 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     }
     const bool turned = act && hd < nqk;
     if (p.qknorm) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gg[e] = 1.0f;
       if (p.gain && turned) ldf<8>(p.gain + col, gg);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(v[r][e], v[r][e], ss);
+#pragma unroll
         for (int m = grp >> 1; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
         if (turned) {
-          const float is = 1.0f / sqrtf(ss / static_cast<float>(D) + 1e-5f);
+          const float is = rsqrtf(fmaf(ss, 1.0f / D, 1e-5f));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[r][e] = v[r][e] * is * (p.gain ? gg[e] : 1.0f);
+          for (int e = 0; e < 8; ++e) v[r][e] *= is * gg[e];
         }
       }
     }
     if (!act) continue;
+    // the column's place in a slot's K or V, for the columns that have one
+    T* pool = static_cast<T*>(turned ? c.k : c.v) + static_cast<long long>(turned ? hd - Hq : hd - nqk) * c.page_size * D + d;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (row0 + r >= p.rows) break;
+      if (r >= rows) break;
       if (p.rope && turned) {
         const float4 cs = *reinterpret_cast<const float4*>(&s_cs[r][d / 2]), sn = *reinterpret_cast<const float4*>(&s_sn[r][d / 2]);
         const float c4[4] = {cs.x, cs.y, cs.z, cs.w}, s4[4] = {sn.x, sn.y, sn.z, sn.w};
@@ -174,28 +220,29 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
           v[r][2 * e + 1] = x0 * s4[e] + x1 * c4[e];
         }
       }
-      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + static_cast<long long>(row0 + r) * p.out_stride + col, v[r]);
-      if (hd >= Hq && s_kv[r] >= 0) {
-        const int h = hd < nqk ? hd - Hq : hd - nqk;
-        T* pool = static_cast<T*>(hd < nqk ? c.k : c.v);
-        stv<T, 8>(pool + s_kv[r] + static_cast<long long>(h) * c.page_size * D + d, v[r]);
-      }
+      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + r * p.out_stride + col, v[r]);
+      if (hd >= Hq && s_kv[r] >= 0) stv<T, 8>(pool + s_kv[r], v[r]);
     }
   }
   for (int i = tid; i < R * Hkv; i += NT) {
     const int r = i % R, h = i / R;
-    if (row0 + r >= p.rows || s_meta[r] < 0) continue;
+    if (r >= rows || s_meta[r] < 0) continue;
     const long long at = s_meta[r] + static_cast<long long>(h) * c.page_size;
     if (c.pos) c.pos[at] = s_pos[r];
     if (c.weight) c.weight[at] = 0.f;
   }
 }
 
+template <typename T, int D>
+static cudaError_t kv_append_d(const AppendParams& p, cudaStream_t st) {
+  if (p.rows >= 148 * 8) kv_append_kernel<T, D, 4><<<(p.rows + 3) / 4, NT, 0, st>>>(p);
+  else kv_append_kernel<T, D, 1><<<p.rows, NT, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
 template <typename T>
 static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
-  if (p.rows >= 148 * 8) kv_append_kernel<T, 4><<<(p.rows + 3) / 4, NT, 0, st>>>(p);
-  else kv_append_kernel<T, 1><<<p.rows, NT, 0, st>>>(p);
-  return cudaGetLastError();
+  return p.c.D == 64 ? kv_append_d<T, 64>(p, st) : kv_append_d<T, 128>(p, st);
 }
 
 // ============================================================ attention of one token
