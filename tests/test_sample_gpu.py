@@ -79,6 +79,32 @@ def test_sample(dtype, rows, V, mode):
     check_rows(logits, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,ld", [(40000, 40000), (40001, 40003), (70000, 70016)])
+def test_many_wide_rows(dtype, V, ld):
+    """More rows than the GPU has SMs: one CTA per row, every truncation and odd value among them."""
+    rng = np.random.default_rng(V)
+    rows = 160
+    x = 2 * rng.standard_normal((rows, ld)).astype(np.float32)
+    x[3, :] = -np.inf
+    x[4, 5:] = np.nan
+    x[5, 100:30000] = -np.inf
+    x[6, 30000:] = np.nan
+    x[7, 39999] = np.inf
+    x[8, :] = 1.0
+    x[9] *= 10
+    x[10] *= 0.01
+    logits = dev(x, dtype)[:, :V]
+    t = rng.uniform(0.3, 2.0, rows)
+    t[11], t[12], t[13], t[14] = 0.0, 1e-30, 1e30, 50.0
+    k = np.where(rng.random(rows) < 0.5, 0, rng.integers(1, 3000, rows))
+    p = np.where(rng.random(rows) < 0.3, 1.0, rng.uniform(0.05, 0.999, rows))
+    m = np.where(rng.random(rows) < 0.5, 0.0, rng.uniform(0.001, 0.3, rows))
+    check_rows(logits, rng.random(rows), t, k, p, m)
+    check_rows(logits, rng.random(rows), t, None, np.full(rows, 0.9), None)
+    check_rows(logits, rng.random(rows), t, None, None, None)
+
+
 def test_defaults_strides_and_whole_ranges():
     """No parameters at all; rows inside wider rows; parameters at their ends."""
     rng = np.random.default_rng(1)

@@ -12,6 +12,10 @@
 // (HBM is read once) and each warp a contiguous chunk of it.  The CTAs agree
 // by writing their part into a buffer of their own, one cluster barrier, and
 // reading everybody's: every CTA then decides the same from the same numbers.
+// When there are rows enough to fill the GPU with one CTA each, a row has one
+// CTA of 512 threads (STREAM) that reads it again from L2 in every pass
+// instead: no cluster to wait for, and a row's fixed work is done by 16 warps
+// instead of 64.
 // The cut of top-k or top-p is found without sorting: a guess brackets it,
 // one pass sums what lies above the bracket exactly and lists what lies
 // inside, and a radix search over the list gives the cut.  A wrong or too wide
@@ -36,10 +40,8 @@ struct SampleParams {
   int ctas;         // CTAs per row
 };
 
-constexpr int SNT = 256, SW = SNT / 32;
 constexpr int SCTAS = 8;      // CTAs per row at most: the portable cluster size
-constexpr int SLIST = 256;    // listed elements per warp
-constexpr int SSMALL = SNT;   // listed elements of a row that are ranked directly, one per thread
+constexpr int SSMALL = 256;   // listed elements of a row that are ranked directly, one per thread
 constexpr int SBINS = 512;    // bins of the guess, over the distances of non-zero weight
 constexpr float SRANGE = 22.25f;  // weights beyond this distance round to zero: 2^31 exp(-22.25) < 1/2
 
@@ -87,12 +89,16 @@ TKB_DEVFN unsigned long long ld_rank_u64(const void* p, int rank) {
   return v;
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 struct Sampler {
   static constexpr int VEC = 16 / sizeof(T);
+  static constexpr int NTH = STREAM ? 512 : 256, SW = NTH / 32;
+  static constexpr int CTAS = STREAM ? 1 : SCTAS;   // at most
+  static constexpr int SLIST = STREAM ? 768 : 256;  // listed elements per warp
   using Key = SampleKey<T>;
   const SampleParams& p;
-  T* data;                       // the slice
+  T* data;                       // the slice (STREAM: the row)
+  bool aligned = true, dirty = false;  // STREAM: 16-byte loads are possible; the row has NaN
   uint2* list;                   // this warp's (key, index in the row)
   unsigned long long (*xbuf)[256];  // two exchange buffers
   unsigned long long* s_tmp;     // 16 values of the block
@@ -109,24 +115,46 @@ struct Sampler {
   TKB_DEVFN Sampler(const SampleParams& q) : p(q) {}
 
   TKB_DEVFN void vec(int it, float (&x)[VEC]) const {
-    ldv<T, VEC>(data + (warp_id() * p.per + it) * 32 * VEC + lane_id() * VEC, x);
+    at(warp_id(), it, x);
+  }
+  // this lane's elements of vector `it` of warp w
+  TKB_DEVFN void at(int w, int it, float (&x)[VEC]) const {
+    const int i = ((w * p.per + it) * 32 + lane_id()) * VEC;
+    if constexpr (!STREAM) {
+      ldv<T, VEC>(data + i, x);
+    } else {
+      if (aligned && i + VEC <= p.V) {
+        const uint4 q = ld_stream_v4(reinterpret_cast<const uint4*>(data + i));
+        ldv<T, VEC>(reinterpret_cast<const T*>(&q), x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = i + e < p.V ? Elem<T>::ld(data + i + e) : -INFINITY;
+      }
+      if (dirty)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = x[e] != x[e] ? -INFINITY : x[e];
+    }
   }
 
   // ---- agreement: fill buf() (after clear() where it is summed into), then agree(), then read()
   TKB_DEVFN unsigned long long* buf() { return xbuf[par]; }
   TKB_DEVFN void clear() {
-    xbuf[par][threadIdx.x] = 0;
+    if (threadIdx.x < 256) xbuf[par][threadIdx.x] = 0;
     __syncthreads();
   }
   TKB_DEVFN void agree() {
     __syncwarp();
-    cluster_sync();
+    if constexpr (STREAM) __syncthreads();
+    else cluster_sync();
   }
   // slot i of CTA r, and of all CTAs (their loads in flight together)
-  TKB_DEVFN unsigned long long read(int i, int r) const { return ld_rank_u64(&xbuf[par][i], r); }
-  TKB_DEVFN void read_all(int i, unsigned long long (&v)[SCTAS]) const {
+  TKB_DEVFN unsigned long long read(int i, int r) const {
+    if constexpr (STREAM) return xbuf[par][i];
+    else return ld_rank_u64(&xbuf[par][i], r);
+  }
+  TKB_DEVFN void read_all(int i, unsigned long long (&v)[CTAS]) const {
 #pragma unroll
-    for (int r = 0; r < SCTAS; ++r) v[r] = r < p.ctas ? read(i, r) : 0;
+    for (int r = 0; r < CTAS; ++r) v[r] = r < p.ctas && i >= 0 && i < 256 ? read(i, r) : 0;
   }
   TKB_DEVFN void next() { par ^= 1; }
 
@@ -206,7 +234,8 @@ struct Sampler {
         const int at0 = (it * 32 + lane_id()) * VEC;
         for (int at = n_list + end - mine; in && at < SLIST; in &= in - 1, ++at) {
           const int i = at0 + __ffs(in) - 1;
-          list[at] = make_uint2(Key::of(Elem<T>::ld(data + warp_id() * p.per * 32 * VEC + i)), base + i);
+          const float v = STREAM && base + i >= p.V ? -INFINITY : Elem<T>::ld(data + warp_id() * p.per * 32 * VEC + i);
+          list[at] = make_uint2(Key::of(v), base + i);
         }
         n_list += __shfl_sync(0xffffffffu, end, 31);
       }
@@ -253,10 +282,10 @@ struct Sampler {
       }
       agree();
       // thread t holds digit 255 - t: a prefix sum over threads runs from the largest digit down
-      unsigned long long part[SCTAS], v = 0;
-      read_all(255 - threadIdx.x, part);
+      unsigned long long part[CTAS], v = 0;
+      read_all(255 - static_cast<int>(threadIdx.x), part);
 #pragma unroll
-      for (int r = 0; r < SCTAS; ++r) v += (part[r] & 0xFFFFFFFFull) + ((part[r] >> 32) << 16);
+      for (int r = 0; r < CTAS; ++r) v += (part[r] & 0xFFFFFFFFull) + ((part[r] >> 32) << 16);
       unsigned long long s = v;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -269,12 +298,12 @@ struct Sampler {
       for (int i = 0; i < warp_id(); ++i) pre += s_tmp[i];
       s += pre;
       if (s >= bound && s - v < bound) {
-        s_tmp[8] = 255 - threadIdx.x;
-        s_tmp[9] = s - v;
+        s_tmp[2 * SW] = 255 - threadIdx.x;
+        s_tmp[2 * SW + 1] = s - v;
       }
       __syncthreads();
-      prefix |= static_cast<uint32_t>(s_tmp[8]) << shift;
-      acc = s_tmp[9];
+      prefix |= static_cast<uint32_t>(s_tmp[2 * SW]) << shift;
+      acc = s_tmp[2 * SW + 1];
       __syncthreads();
       next();
       bits = shift;
@@ -306,17 +335,23 @@ struct Sampler {
       // what the list measures, as far as it is known when it spilled
       unsigned long long l = v[1];
       if (spilled) l = !WEIGHTS ? listed : listed * weight_of(glo);
+      // a guess that missed is followed by its neighbour, as wide as what is missing (or too much) would be at the
+      // listed measure per key, and half as much again
+      const double miss = (a >= bound ? a - bound : bound - a - l) / (static_cast<double>(l) + 1.0);
+      const uint32_t wide = 1 + static_cast<uint32_t>(fmin((ghi - glo) * (1.5 * miss + 0.25), 1e9));
       if (a >= bound) {
         lo = ghi;
         glo = lo;
-        ghi = hi;
+        ghi = hi - lo > wide ? lo + wide : hi;
       } else if (spilled && WEIGHTS && !single) {
+        // of the bracket, the upper part that the lists should hold
+        const double part = fmin(0.5, 0.4 * p.ctas * SW * SLIST / static_cast<double>(listed));
         hi = ghi;
-        ghi = glo + (ghi - glo) / 2;
+        glo = ghi - max(1u, static_cast<uint32_t>((ghi - glo) * part));
       } else if (a + l < bound) {
         if (glo == lo) return NONE;
         hi = glo;
-        glo = lo;
+        glo = hi - lo > wide ? hi - wide : lo;
         ghi = hi;
       } else if (!spilled) {
         list_ok = true;
@@ -363,7 +398,8 @@ struct Sampler {
                    (mine & 1 ? __shfl_sync(0xffffffffu, c[0], mine / 2) : 0);
     const uint32_t dst = mapa_shared(smem_u32(s_few), 0);
     for (int i = lane; i < n_list; i += 32)
-      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst + 8 * (at + i)), "r"(list[i].x), "r"(list[i].y)
+      if (STREAM) s_few[at + i] = list[i];
+      else asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst + 8 * (at + i)), "r"(list[i].x), "r"(list[i].y)
                    : "memory");
     next();
     agree();
@@ -372,7 +408,7 @@ struct Sampler {
     unsigned long long* s_kept = xbuf[1];
     const uint2 e = tid < n ? s_few[tid] : make_uint2(0u, 0u);
     const uint32_t wt = tid < n ? weight_of(e.x) : 0u;
-    s_w[tid] = wt;
+    if (tid < SSMALL) s_w[tid] = wt;
     __syncthreads();
     // tokens before this one in the order of the truncations, and their weight
     int rank_of = 0;
@@ -391,7 +427,7 @@ struct Sampler {
       keep = keep && before < bound;
     }
     keep = keep && wt >= least;
-    s_kept[tid] = keep ? wt : 0ull;
+    if (tid < SSMALL) s_kept[tid] = keep ? wt : 0ull;
     const unsigned long long total = block_sum(keep ? wt : 0ull);  // (its barriers publish s_kept)
     const unsigned long long kept = block_sum(keep ? 1ull : 0ull);
     const unsigned long long target = scaled_floor(total, fixed32(p.u[row]));
@@ -427,59 +463,70 @@ TKB_DEVFN uint32_t max_nan2(uint32_t a, uint32_t b) {
   return r;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ SampleParams p) {
-  constexpr int VEC = Sampler<T>::VEC;
+template <typename T, bool STREAM>
+__global__ void __launch_bounds__(Sampler<T, STREAM>::NTH) sample_kernel(const __grid_constant__ SampleParams p) {
+  using S = Sampler<T, STREAM>;
+  constexpr int VEC = S::VEC, SW = S::SW, SLIST = S::SLIST, CTAS = S::CTAS;
   using Key = SampleKey<T>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ unsigned long long s_x[2][256], s_tmp[16];
-  __shared__ uint2 s_list[SW][SLIST], s_few[SSMALL];
-  Sampler<T> s(p);
+  extern __shared__ __align__(16) uint8_t smem[];  // the lists, then the slice
+  __shared__ unsigned long long s_x[2][256], s_tmp[2 * SW + 8];
+  __shared__ uint2 s_few[SSMALL];
+  S s(p);
   const int row = blockIdx.x / p.ctas, tid = threadIdx.x, lane = lane_id(), w = warp_id(), V = p.V;
   s.rank = blockIdx.x % p.ctas;
-  s.data = reinterpret_cast<T*>(smem);
-  s.list = s_list[w];
+  s.list = reinterpret_cast<uint2*>(smem) + w * SLIST;
   s.xbuf = s_x;
   s.s_tmp = s_tmp;
   s.base = (s.rank * SW + w) * p.per * 32 * VEC;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
-
-  // ---- the slice into shared memory: each lane the vectors it will read
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  for (int it = 0; it < p.per; ++it) {
-    const int i = s.base + (it * 32 + lane) * VEC;
-    T* dst = s.data + (w * p.per + it) * 32 * VEC + lane * VEC;
-    if (aligned && i + VEC <= V) {
-      cp_async16(smem_u32(dst), x + i, 16);
-    } else {
+  s.aligned = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  if constexpr (STREAM) {
+    s.data = const_cast<T*>(x);
+  } else {
+    // ---- the slice into shared memory: each lane the vectors it will read
+    s.data = reinterpret_cast<T*>(smem + SW * SLIST * sizeof(uint2));
+    for (int it = 0; it < p.per; ++it) {
+      const int i = s.base + (it * 32 + lane) * VEC;
+      T* dst = s.data + (w * p.per + it) * 32 * VEC + lane * VEC;
+      if (s.aligned && i + VEC <= V) {
+        cp_async16(smem_u32(dst), x + i, 16);
+      } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (i + e < V) dst[e] = x[i + e];
-        else Elem<T>::st(dst + e, -INFINITY);
+        for (int e = 0; e < VEC; ++e) {
+          if (i + e < V) dst[e] = x[i + e];
+          else Elem<T>::st(dst + e, -INFINITY);
+        }
       }
     }
+    cp_async_commit();
+    cp_async_wait<0>();
   }
-  cp_async_commit();
-  cp_async_wait<0>();
 
   // ---- maximum; NaN becomes -inf for all that follows
   float tmax = -INFINITY;
-  if constexpr (sizeof(T) == 2) {
-    uint32_t m = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
+  {
+    uint32_t m = sizeof(T) == 4 ? 0u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;  // -inf
+#pragma unroll(STREAM ? 8 : 1)
     for (int it = 0; it < p.per; ++it) {
-      const uint4 q = *reinterpret_cast<const uint4*>(s.data + (w * p.per + it) * 32 * VEC + lane * VEC);
-      m = max_nan2<T>(max_nan2<T>(m, max_nan2<T>(q.x, q.y)), max_nan2<T>(q.z, q.w));
-    }
-    const float2 f = unpack2<std::is_same<T, __nv_bfloat16>::value>(m);
-    tmax = f.x != f.x || f.y != f.y ? NAN : fmaxf(f.x, f.y);
-  } else {
-    for (int it = 0; it < p.per; ++it) {
-      float v[VEC];
-      s.vec(it, v);
+      const int i = ((w * p.per + it) * 32 + lane) * VEC;
+      if (sizeof(T) == 2 && (!STREAM || (s.aligned && i + VEC <= V))) {
+        const uint4* at = reinterpret_cast<const uint4*>(s.data + i);
+        const uint4 q = STREAM ? ld_stream_v4(at) : *at;
+        m = max_nan2<T>(max_nan2<T>(m, max_nan2<T>(q.x, q.y)), max_nan2<T>(q.z, q.w));
+      } else {
+        float v[VEC];
+        s.vec(it, v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(tmax) : "f"(tmax), "f"(v[e]));
+        for (int e = 0; e < VEC; ++e) asm("max.NaN.f32 %0, %1, %2;" : "=f"(tmax) : "f"(tmax), "f"(v[e]));
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = unpack2<std::is_same<T, __nv_bfloat16>::value>(m);
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(tmax) : "f"(tmax), "f"(f.x));
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(tmax) : "f"(tmax), "f"(f.y));
     }
   }
+  if constexpr (STREAM) s.dirty = __syncthreads_or(tmax != tmax);
   if (tmax != tmax) {
     tmax = -INFINITY;
     for (int it = 0; it < p.per; ++it) {
@@ -490,7 +537,7 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
         v[e] = v[e] != v[e] ? -INFINITY : v[e];
         tmax = fmaxf(tmax, v[e]);
       }
-      stv<T, VEC>(s.data + (w * p.per + it) * 32 * VEC + lane * VEC, v);
+      if constexpr (!STREAM) stv<T, VEC>(s.data + (w * p.per + it) * 32 * VEC + lane * VEC, v);
     }
   }
   float top = warp_max(tmax);
@@ -556,9 +603,10 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
       s.clear();
       const float to_bin = SBINS / SRANGE;
       const float zmax = sample_dist(tmax, top, s.inv_t);
-      const bool by_max = k && k <= p.ctas * SNT / 2;  // enough maxima to bound the k-th largest from below
+      const bool by_max = k && k <= p.ctas * S::NTH / 2;  // enough maxima to bound the k-th largest from below
       if (zmax < SRANGE) atomicAdd(&hist[min(SBINS - 1, static_cast<int>(zmax * to_bin))],
                                    k ? 1u : static_cast<uint32_t>(__expf(-zmax) * 131072.f));
+      float spread = 0.f;  // the estimate's variance
       if (!by_max) {
         const int ns = max(1, p.per / 8);
         const float f = static_cast<float>(p.per) / ns;
@@ -568,18 +616,21 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const float z = sample_dist(v[e], top, s.inv_t);
-            if (v[e] < tmax && z < SRANGE)
+            if (v[e] < tmax && z < SRANGE) {
+              const float ez = f * __expf(-z);
+              spread = fmaf(ez, ez, spread);
               atomicAdd(&hist[min(SBINS - 1, static_cast<int>(z * to_bin))],
-                        k ? static_cast<uint32_t>(f + 0.5f) : static_cast<uint32_t>(f * __expf(-z) * 131072.f + 0.5f));
+                        static_cast<uint32_t>(k ? f + 0.5f : ez * 131072.f + 0.5f));
+            }
           }
         }
       }
       s.agree();
       // thread t: bins 2t and 2t + 1 of the whole row, and what the bins up to them hold
-      unsigned long long part[SCTAS], h0 = 0, h1 = 0;
+      unsigned long long part[CTAS], h0 = 0, h1 = 0;
       s.read_all(tid, part);
 #pragma unroll
-      for (int r = 0; r < SCTAS; ++r) {
+      for (int r = 0; r < CTAS; ++r) {
         h0 += part[r] & 0xFFFFFFFFull;
         h1 += part[r] >> 32;
       }
@@ -590,7 +641,11 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
         if (lane >= d) c += t;
       }
       if (lane == 31) s_tmp[w] = c;
-      if (tid == 0) s_tmp[10] = s_tmp[11] = SBINS;
+      if (STREAM) {
+        spread = warp_sum(spread);
+        if (lane == 0) s_tmp[SW + w] = __float_as_uint(spread);
+      }
+      if (tid == 0) s_tmp[2 * SW + 2] = s_tmp[2 * SW + 3] = SBINS;
       __syncthreads();
       unsigned long long total = 0;
       for (int i = 0; i < SW; ++i) {
@@ -606,17 +661,25 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
         want_lo = 1.2 * k + 8.0 * sqrt(static_cast<double>(k));
         want_hi = -1.0;
       } else {
-        // the tail below the cut is sampled well: an error of the sum moves the cut by its share of 1 - p
-        const double q = fmax(static_cast<double>(tp), 0.0), room = 0.05 * (1.0 - q) + 1e-4;
+        // the tail below the cut is sampled well: an error of the sum moves the cut by its share of 1 - p.
+        // With 2048 thread maxima 0.05 was enough; with 512 the sampled terms tell their own spread.
+        double room = 0.05;
+        if (STREAM) {
+          spread = 0.f;
+          for (int i = 0; i < SW; ++i) spread += __uint_as_float(static_cast<uint32_t>(s_tmp[SW + i]));
+          room = 0.02 + 3.0 * sqrtf(spread) * 131072.0 / (static_cast<double>(total) + 1.0);
+        }
+        const double q = fmax(static_cast<double>(tp), 0.0);
+        room = room * (1.0 - q) + 1e-4;
         want_lo = (q + room) * total;
         want_hi = (q - room) * total;
       }
-      if (c0 >= want_lo && b0 < want_lo) s_tmp[10] = 2 * tid;
-      else if (c >= want_lo && c0 < want_lo) s_tmp[10] = 2 * tid + 1;
-      if (b0 <= want_hi && c0 > want_hi) s_tmp[11] = 2 * tid;
-      else if (c0 <= want_hi && c > want_hi) s_tmp[11] = 2 * tid + 1;
+      if (c0 >= want_lo && b0 < want_lo) s_tmp[2 * SW + 2] = 2 * tid;
+      else if (c >= want_lo && c0 < want_lo) s_tmp[2 * SW + 2] = 2 * tid + 1;
+      if (b0 <= want_hi && c0 > want_hi) s_tmp[2 * SW + 3] = 2 * tid;
+      else if (c0 <= want_hi && c > want_hi) s_tmp[2 * SW + 3] = 2 * tid + 1;
       __syncthreads();
-      const int blo = static_cast<int>(s_tmp[10]), bhi = static_cast<int>(s_tmp[11]);
+      const int blo = static_cast<int>(s_tmp[2 * SW + 2]), bhi = static_cast<int>(s_tmp[2 * SW + 3]);
       __syncthreads();
       s.next();
       if (blo < SBINS) {
@@ -635,19 +698,19 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
       return wt ? static_cast<long long>((bound - acc + wt - 1) / wt) : V;
     };
     unsigned long long bound = k, acc = 0;
-    int found = Sampler<T>::NONE;
+    int found = S::NONE;
     bool whole_row = false;
     if (k) {
       found = s.template search<false>(low, high, glo, high, bound, false, cut, acc);
-      if (found == Sampler<T>::CUT) ties = k - static_cast<long long>(acc);
+      if (found == S::CUT) ties = k - static_cast<long long>(acc);
     }
-    if (nucleus && found == Sampler<T>::NONE) {
+    if (nucleus && found == S::NONE) {
       // of the whole row (or of fewer than k tokens of any weight)
       whole_row = true;
       bound = fixed32(tp);
       found = s.template search<true>(low, high, k ? low : glo, k ? high : ghi, bound, true, cut, acc);
-      if (found == Sampler<T>::CUT) ties = ties_of(bound, acc);
-    } else if (nucleus && found == Sampler<T>::CUT) {
+      if (found == S::CUT) ties = ties_of(bound, acc);
+    } else if (nucleus && found == S::CUT) {
       // of the first k: their weight above the cut first
       unsigned long long v[1] = {0};
       const bool listed = s.list_ok && s.list_hi == high;
@@ -672,18 +735,18 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
           ties = ties_of(bound, acc);
         } else {
           found = s.template search<true>(cut + 1, high, cut + 1, high, bound, false, cut, acc);
-          if (found == Sampler<T>::CUT) ties = ties_of(bound, acc);
+          if (found == S::CUT) ties = ties_of(bound, acc);
         }
       }
-      if (found == Sampler<T>::FEW) {
+      if (found == S::FEW) {
         // every token of the bracket is in the lists and the bound is known: the cut from them
         acc = 0;
         cut = s.template radix<true>(cut + 1, acc, bound);
         ties = ties_of(bound, acc);
-        found = Sampler<T>::CUT;
+        found = S::CUT;
       }
     }
-    if (found == Sampler<T>::FEW) {
+    if (found == S::FEW) {
       s.few(row, k, nucleus, tp, whole_row ? bound : 0, least, s_few);
       return;
     }
@@ -780,12 +843,11 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
   s.agree();  // nobody reads this CTA's buffers any more
   // ---- the CTA whose chunk it is finds the token: warp i takes the chunk's i-th 256 (or 128) elements of every eight
   if (chunk / SW != s.rank) return;
-  const T* part = s.data + (chunk % SW) * p.per * 32 * VEC;
   for (int it0 = 0; it0 < p.per; it0 += SW) {
     const int it = it0 + w;
     float v[VEC];
     if (it < p.per) {
-      ldv<T, VEC>(part + it * 32 * VEC + lane * VEC, v);
+      s.at(chunk % SW, it, v);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] = -INFINITY;
@@ -851,32 +913,32 @@ __global__ void __launch_bounds__(SNT) sample_kernel(const __grid_constant__ Sam
 }
 
 constexpr int kSampleMaxV = 1 << 18;
+constexpr int kSampleStreamRows = 148;
 
 // CTAs per row and vectors per lane.  Slices of 32 KB leave room for four CTAs
 // per SM, whose barriers and passes overlap; few rows are cut finer, down to
 // one vector per lane, until there are two CTAs per SM.  Eight CTAs is the
 // portable cluster size.
 static void sample_shape(int rows, int V, int esize, int& ctas, int& per) {
-  const int vec = 16 / esize, chunk = SW * 32 * vec;  // elements per CTA and vector
+  const int vec = 16 / esize, chunk = 256 * vec;  // elements per CTA and vector
   ctas = 1;
   while (ctas < SCTAS && (static_cast<long long>(V) * esize > static_cast<long long>(ctas) * 32768 ||
-                      (static_cast<long long>(rows) * ctas * 2 <= 296 && V > ctas * chunk)))
+                          (static_cast<long long>(rows) * ctas * 2 <= 296 && V > ctas * chunk)))
     ctas *= 2;
   per = (V + ctas * chunk - 1) / (ctas * chunk);
 }
 
-template <typename T>
-static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
-  sample_shape(p.rows, p.V, sizeof(T), p.ctas, p.per);
-  const size_t smem = static_cast<size_t>(p.per) * SNT * 16;
-  auto k = sample_kernel<T>;
+template <typename T, bool STREAM>
+static cudaError_t sample_launch(const SampleParams& p, cudaStream_t st) {
+  using S = Sampler<T, STREAM>;
   // the widest slice: kSampleMaxV fp32 logits over SCTAS CTAs
-  cudaError_t e = allow_smem<sample_kernel<T>>(kSampleMaxV / SCTAS * 4);
+  constexpr int lists = S::SW * S::SLIST * static_cast<int>(sizeof(uint2));
+  cudaError_t e = allow_smem<sample_kernel<T, STREAM>>(lists + (STREAM ? 0 : kSampleMaxV / SCTAS * 4));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.ctas);
-  cfg.blockDim = dim3(SNT);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(S::NTH);
+  cfg.dynamicSmemBytes = lists + (STREAM ? 0 : static_cast<size_t>(p.per) * S::NTH * 16);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -884,7 +946,19 @@ static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, p);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, STREAM>, p);
+}
+
+template <typename T>
+static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
+  sample_shape(p.rows, p.V, sizeof(T), p.ctas, p.per);
+  if (p.ctas > 1 && p.rows >= kSampleStreamRows) {
+    constexpr int chunk = Sampler<T, true>::NTH * Sampler<T, true>::VEC;
+    p.ctas = 1;
+    p.per = (p.V + chunk - 1) / chunk;
+    return sample_launch<T, true>(p, st);
+  }
+  return sample_launch<T, false>(p, st);
 }
 
 }  // namespace tkb
