@@ -1088,18 +1088,22 @@ __global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant
     const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11, bins = 1 << bits;
     for (int i = tid; i < bins; i += THREADS) hist[i] = 0;
     __syncthreads();
-    for (int j0 = 0; j0 < n; j0 += THREADS) {
-      const int j = j0 + tid;
-      const uint32_t k = j < n ? keys[j] : 0u;
-      const bool in = j < n && (level == 0 || (k >> (shift + bits)) == (lo >> (shift + bits)));
-      const int bin = static_cast<int>((k >> shift) & (bins - 1));
-      const unsigned m = __ballot_sync(0xffffffffu, in);
-      if (!m) continue;
-      const int lead = __ffs(m) - 1, first = __shfl_sync(0xffffffffu, bin, lead);
-      if (__all_sync(0xffffffffu, !in || bin == first)) {
-        if (lane == lead) atomicAdd(&hist[first], __popc(m));
-      } else if (in) {
-        atomicAdd(&hist[bin], 1);
+    for (int j0 = 0; j0 < n; j0 += 4 * THREADS) {
+      const int j = j0 + 4 * tid;
+      const uint4 q = j < n ? *reinterpret_cast<const uint4*>(keys + j) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t k4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = j + e < n && (level == 0 || ((k4[e] ^ lo) >> (shift + bits)) == 0);
+        const int bin = static_cast<int>((k4[e] >> shift) & (bins - 1));
+        const unsigned m = __ballot_sync(0xffffffffu, in);
+        if (!m) continue;
+        const int lead = __ffs(m) - 1, first = __shfl_sync(0xffffffffu, bin, lead);
+        if (__all_sync(0xffffffffu, !in || bin == first)) {
+          if (lane == lead) atomicAdd(&hist[first], __popc(m));
+        } else if (in) {
+          atomicAdd(&hist[bin], 1);
+        }
       }
     }
     __syncthreads();
@@ -1130,50 +1134,88 @@ __global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant
     in_bin = s_cut[2];
   }
   // kept: the keys above lo, and of those equal to it the first `need`
-  const int chunk = (n + THREADS - 1) / THREADS * 32, j0 = min(n, w * chunk), j1 = min(n, j0 + chunk);
+  const int chunk = (n + 4 * THREADS - 1) / (4 * THREADS) * 128, j0 = min(n, w * chunk), j1 = min(n, j0 + chunk);
+  const bool some = need < in_bin;  // not all tokens of key lo stay: their order counts
   int tie_base = 0;
-  if (need < in_bin) {  // not all of them: their order counts
+  if (some) {
     int ties = 0, total;
     for (int j = j0 + lane; j < j1; j += 32) ties += keys[j] == lo;
     __syncthreads();
     tie_base = evict_prefix<THREADS>(__reduce_add_sync(0xffffffffu, ties), sh, 1, total);
     __syncthreads();
   }
-  // `f(j, kept)` for the warp's slots in order, 32 at a time
+  // `f(j, hole, mover)` for the warp's slots in order, four a lane: bit e of
+  // the masks stands for slot j + e
   auto walk = [&](auto f) {
     int rank_base = tie_base;
-#pragma unroll 2
-    for (int j = j0; j < j1; j += 32) {
-      const bool in = j + lane < j1;
-      const uint32_t k = in ? keys[j + lane] : 0u;
-      const unsigned m = __ballot_sync(0xffffffffu, in && k == lo);
-      const bool kept = in && (k > lo || (k == lo && rank_base + __popc(m & ((1u << lane) - 1)) < need));
-      rank_base += __popc(m);
-      f(j + lane, in, kept);
+    for (int jj = j0; jj < j1; jj += 128) {
+      const int j = jj + 4 * lane;
+      const uint4 q = j < j1 ? *reinterpret_cast<const uint4*>(keys + j) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t k4[4] = {q.x, q.y, q.z, q.w};
+      unsigned in = 0, kept = 0, tie = 0, low = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (j + e < j1) in |= 1u << e;
+        if (j + e < p.budget) low |= 1u << e;
+        if (k4[e] > lo) kept |= 1u << e;
+        if (k4[e] == lo) tie |= 1u << e;
+      }
+      kept &= in;
+      tie &= in;
+      if (some) {
+        int upto = __popc(tie);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        int rank = rank_base + upto - __popc(tie);
+        rank_base += __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tie >> e & 1) {
+            if (rank >= need) tie &= ~(1u << e);
+            ++rank;
+          }
+      }
+      kept |= tie;
+      f(j, in & ~kept & low, kept & ~low);
     }
   };
   int holes = 0, movers = 0, total;
-  walk([&](int j, bool in, bool kept) {
-    holes += __popc(__ballot_sync(0xffffffffu, in && !kept && j < p.budget));
-    movers += __popc(__ballot_sync(0xffffffffu, kept && j >= p.budget));
+  walk([&](int, unsigned hole, unsigned mover) {
+    holes += __popc(hole);
+    movers += __popc(mover);
   });
-  int hole_at = evict_prefix<THREADS>(holes, sh, 0, total);
-  int mover_at = evict_prefix<THREADS>(movers, sh, 1, total);  // as many movers as holes
+  int hole_at = evict_prefix<THREADS>(__reduce_add_sync(0xffffffffu, holes), sh, 0, total);
+  int mover_at = evict_prefix<THREADS>(__reduce_add_sync(0xffffffffu, movers), sh, 1, total);  // as many as holes
   // this CTA's share of the moves
   const int m0 = static_cast<int>(static_cast<long long>(total) * rank / p.split);
   const int m1 = static_cast<int>(static_cast<long long>(total) * (rank + 1) / p.split);
   uint2* to = p.lists + static_cast<long long>(unit) * 2 * p.cap;
   uint2* from = to + p.cap;
-  walk([&](int j, bool in, bool kept) {
-    const bool hole = in && !kept && j < p.budget, mover = kept && j >= p.budget;
-    const unsigned mh = __ballot_sync(0xffffffffu, hole), mm = __ballot_sync(0xffffffffu, mover);
-    const int at = hole ? hole_at + __popc(mh & ((1u << lane) - 1)) : mover_at + __popc(mm & ((1u << lane) - 1));
-    if ((hole || mover) && at >= m0 && at < m1) {
-      const int pg = j / ps;
-      (hole ? to : from)[at] = make_uint2(__ldg(table + pg), j - pg * ps);
+  walk([&](int j, unsigned hole, unsigned mover) {
+    const int mine = __popc(hole) | __popc(mover) << 16;
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += o;
     }
-    hole_at += __popc(mh);
-    mover_at += __popc(mm);
+    const int all = __shfl_sync(0xffffffffu, upto, 31);
+    upto -= mine;
+    if (mine) {
+      const int pg = j / ps;  // one page holds the four slots
+      const uint32_t page = __ldg(table + pg);
+      int at = hole_at + (upto & 0xFFFF);
+      for (; hole; hole &= hole - 1, ++at)
+        if (at >= m0 && at < m1) to[at] = make_uint2(page, j + __ffs(hole) - 1 - pg * ps);
+      at = mover_at + (upto >> 16);
+      for (; mover; mover &= mover - 1, ++at)
+        if (at >= m0 && at < m1) from[at] = make_uint2(page, j + __ffs(mover) - 1 - pg * ps);
+    }
+    hole_at += all & 0xFFFF;
+    mover_at += all >> 16;
   });
   __syncthreads();
   if (p.split > 1) cluster_sync();  // every CTA of the unit has read its keys

@@ -913,7 +913,6 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH) sample_kernel(const _
 }
 
 constexpr int kSampleMaxV = 1 << 18;
-constexpr int kSampleStreamRows = 148;
 
 // CTAs per row and vectors per lane.  Slices of 32 KB leave room for four CTAs
 // per SM, whose barriers and passes overlap; few rows are cut finer, down to
@@ -949,10 +948,15 @@ static cudaError_t sample_launch(const SampleParams& p, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, sample_kernel<T, STREAM>, p);
 }
 
+// One CTA per row pays when rows are wide and enough (us, cluster / one CTA,
+// nucleus 0.9): 64 KB rows 40 / 46 at 296 rows, 63 / 77 at 512; 128 KB rows
+// 52 / 50 at 200, 66 / 56 at 296; 256 KB rows 119 / 128 at 200, 166 / 142 at
+// 296, 271 / 215 at 512; 512 KB rows 147 / 122 at 148, 468 / 298 at 512.
 template <typename T>
 static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
   sample_shape(p.rows, p.V, sizeof(T), p.ctas, p.per);
-  if (p.ctas > 1 && p.rows >= kSampleStreamRows) {
+  const long long bytes = static_cast<long long>(p.V) * sizeof(T);
+  if ((bytes > 65536 && p.rows >= 224) || (bytes > 262144 && p.rows >= 148)) {
     constexpr int chunk = Sampler<T, true>::NTH * Sampler<T, true>::VEC;
     p.ctas = 1;
     p.per = (p.V + chunk - 1) / chunk;
