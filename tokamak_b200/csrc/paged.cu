@@ -22,6 +22,31 @@ static cudaError_t allow_smem(int bytes) {
   return e;
 }
 
+// Launches of this file and sample.cu let the kernel come up while the one
+// before it in the stream ends (programmatic dependent launch): the kernel's
+// first act is grid_wait(), which returns when everything launched before has
+// completed and is visible, so nothing else changes.
+TKB_DEVFN void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename P>
+static cudaError_t launch_early(void (*kernel)(P), dim3 grid, int block, size_t smem, cudaStream_t st, const P& p,
+                                int cluster = 0) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 // Element offset of slot 0 of (page, kv head) in k and v.
 TKB_DEVFN long long page_offset(const tkb_kv_cache& c, int page, int h) {
   return static_cast<long long>(page) * c.page_stride + static_cast<long long>(h) * c.page_size * c.D;
@@ -120,6 +145,7 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
   in += static_cast<long long>(row0) * p.qkv_stride;
   if (out) out += static_cast<long long>(row0) * p.out_stride;
   // the next column's loads are under way while one is worked on, the first one's during what comes before
+  grid_wait();
   Raw8<T> raw[R];
   auto fetch = [&](int vi) {
     if (vi < nvec)
@@ -235,9 +261,8 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
 
 template <typename T, int D>
 static cudaError_t kv_append_d(const AppendParams& p, cudaStream_t st) {
-  if (p.rows >= 148 * 8) kv_append_kernel<T, D, 4><<<(p.rows + 3) / 4, NT, 0, st>>>(p);
-  else kv_append_kernel<T, D, 1><<<p.rows, NT, 0, st>>>(p);
-  return cudaGetLastError();
+  if (p.rows >= 148 * 8) return launch_early(kv_append_kernel<T, D, 4>, dim3((p.rows + 3) / 4), NT, 0, st, p);
+  return launch_early(kv_append_kernel<T, D, 1>, dim3(p.rows), NT, 0, st, p);
 }
 
 template <typename T>
@@ -636,6 +661,7 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
                      : p.head + (static_cast<long long>(blockIdx.x) * DW + i) * GT * D;
   };
 
+  grid_wait();
   // ---- this CTA's run of tiles, [t0, t1) of all `total` ones
   const int per = (c.B + DNT - 1) / DNT, q0 = min(c.B, tid * per), q1 = min(c.B, q0 + per);
   int mine = 0, held = 0;
@@ -925,6 +951,7 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
 __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant__ DecodeParams p) {
   const tkb_kv_cache& c = p.c;
   const int b = blockIdx.y / c.Hkv, h = blockIdx.y % c.Hkv, j = (blockIdx.x * 256 + threadIdx.x) * 4;
+  grid_wait();
   const int n = held_of(c, b);
   if (j >= n) return;
   const int pg = j / c.page_size, page = page_of(c, b, pg);
@@ -976,8 +1003,7 @@ static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const long long most = static_cast<long long>(p.c.B) * p.c.Hkv * p.qblocks * (p.c.max_pages * p.c.page_size / Cfg::TK);
   const int grid = static_cast<int>(most < kDecodeGrid * W ? (most + W - 1) / W : kDecodeGrid);
-  k<<<grid, W * 32, Cfg::SMEM, st>>>(p);
-  return cudaGetLastError();
+  return launch_early(k, dim3(grid), W * 32, Cfg::SMEM, st, p);
 }
 
 template <typename T, int D>
@@ -997,8 +1023,7 @@ static cudaError_t paged_decode_t(const DecodeParams& p, cudaStream_t st) {
   cudaError_t e = p.c.D == 64 ? paged_decode_d<T, 64>(p, st) : paged_decode_d<T, 128>(p, st);
   if (e == cudaSuccess && p.accumulate) {
     const long long cap = static_cast<long long>(p.c.max_pages) * p.c.page_size;
-    paged_weight_kernel<<<dim3(static_cast<unsigned>((cap + 1023) / 1024), p.c.B * p.c.Hkv), 256, 0, st>>>(p);
-    e = cudaGetLastError();
+    e = launch_early(paged_weight_kernel, dim3(static_cast<unsigned>((cap + 1023) / 1024), p.c.B * p.c.Hkv), 256, 0, st, p);
   }
   return e;
 }
@@ -1047,6 +1072,7 @@ __global__ void __launch_bounds__(THREADS) kv_evict_kernel(const __grid_constant
   const tkb_kv_cache& c = p.c;
   const int unit = blockIdx.x / p.split, rank = blockIdx.x % p.split;
   const int b = unit / c.Hkv, h = unit % c.Hkv, tid = threadIdx.x, w = warp_id(), lane = lane_id();
+  grid_wait();
   const int n = held_of(c, b), ps = c.page_size;
   if (n <= p.budget) return;  // the whole cluster
   uint32_t* keys = p.keys ? p.keys + static_cast<long long>(blockIdx.x) * c.max_pages * ps : s_keys;
@@ -1281,21 +1307,10 @@ static cudaError_t kv_evict_launch(EvictParams p, cudaStream_t st) {
   const long long slots = static_cast<long long>(p.c.max_pages) * p.c.page_size;
   p.split = evict_split(p.c);
   const size_t smem = p.keys ? 0 : static_cast<size_t>(slots) * 4;
-  auto k = kv_evict_kernel<T, THREADS>;
   cudaError_t e = allow_smem<kv_evict_kernel<T, THREADS>>(kEvictSmemKeys * 4);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.c.B) * p.c.Hkv * p.split);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, p);
+  return launch_early(kv_evict_kernel<T, THREADS>, dim3(static_cast<unsigned>(p.c.B) * p.c.Hkv * p.split), THREADS, smem,
+                      st, p, p.split);
 }
 
 template <typename T>

@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH) sample_kernel(const _
   extern __shared__ __align__(16) uint8_t smem[];  // the lists, then the slice
   __shared__ unsigned long long s_x[2][256], s_tmp[2 * SW + 8];
   __shared__ uint2 s_few[SSMALL];
+  grid_wait();
   S s(p);
   const int row = blockIdx.x / p.ctas, tid = threadIdx.x, lane = lane_id(), w = warp_id(), V = p.V;
   s.rank = blockIdx.x % p.ctas;
@@ -934,18 +935,8 @@ static cudaError_t sample_launch(const SampleParams& p, cudaStream_t st) {
   constexpr int lists = S::SW * S::SLIST * static_cast<int>(sizeof(uint2));
   cudaError_t e = allow_smem<sample_kernel<T, STREAM>>(lists + (STREAM ? 0 : kSampleMaxV / SCTAS * 4));
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * p.ctas);
-  cfg.blockDim = dim3(S::NTH);
-  cfg.dynamicSmemBytes = lists + (STREAM ? 0 : static_cast<size_t>(p.per) * S::NTH * 16);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T, STREAM>, p);
+  return launch_early(sample_kernel<T, STREAM>, dim3(static_cast<unsigned>(p.rows) * p.ctas), S::NTH,
+                      lists + (STREAM ? 0 : static_cast<size_t>(p.per) * S::NTH * 16), st, p, p.ctas);
 }
 
 // One CTA per row pays when rows are wide and enough (us, cluster / one CTA,
