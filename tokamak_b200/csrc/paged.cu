@@ -84,11 +84,14 @@ __global__ void kv_lens_kernel(int32_t* __restrict__ lens, int32_t* __restrict__
 
 // ============================================================ append
 // qkv_prep_fwd_kernel (rows.cu) with each row's own position, its K and V
-// columns stored to the row's slot.  A block takes R rows: their cosines and
-// sines (D/2 each, for all heads) are computed once, in shared memory, and a
-// thread walks the R rows of a column, so that bias and gain are read once for
-// them and R loads are in flight.  R is 4 for prompts, 1 when the rows would
-// not fill the GPU.
+// columns stored to the row's slot.  HBM bounds it for prompts.  A block takes
+// R * GROUPS rows: where they go and their cosines and sines (D/2 each, for
+// all heads) are found once, in shared memory, while the first columns load;
+// then a thread walks R rows of a column at a time, so that bias and gain are
+// read once for them, with the next R loads in flight.  At 12.5 k rows of 10240
+// f16 columns (563 MB): 2 x 2 rows 115 us (0.75 of HBM), 2 x 1 119, 4 x 1 124,
+// 1 x 4 125, 2 x 4 127, 4 x 2 149 (fewer, larger blocks leave a ragged last
+// wave).  One row a block when the rows would not fill the GPU.
 struct AppendParams {
   tkb_kv_cache c;
   const void* qkv;
@@ -131,29 +134,30 @@ struct Raw8 {
   }
 };
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, int GROUPS>
 __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ float s_cs[R][64], s_sn[R][64];
-  __shared__ long long s_kv[R], s_meta[R];  // element offset of the row's slot of kv head 0; its pos / weight index
-  __shared__ int s_pos[R];
+  constexpr int RB = R * GROUPS;  // rows of the block
+  __shared__ float s_cs[RB][64], s_sn[RB][64];
+  __shared__ long long s_kv[RB], s_meta[RB];  // element offset of the row's slot of kv head 0; its pos / weight index
+  __shared__ int s_pos[RB];
   const tkb_kv_cache& c = p.c;
   const int Hq = p.Hq, Hkv = c.Hkv, C = (Hq + 2 * Hkv) * D, nqk = Hq + Hkv, nvec = C / 8;
   constexpr int grp = D / 8;
   const T* in = static_cast<const T*>(p.qkv);
   T* out = static_cast<T*>(p.out);
-  const int row0 = blockIdx.x * R, tid = threadIdx.x, rows = min(R, p.rows - row0);
+  const int row0 = blockIdx.x * RB, tid = threadIdx.x, rows = min(RB, p.rows - row0);
   in += static_cast<long long>(row0) * p.qkv_stride;
   if (out) out += static_cast<long long>(row0) * p.out_stride;
   // the next column's loads are under way while one is worked on, the first one's during what comes before
   grid_wait();
   Raw8<T> raw[R];
-  auto fetch = [&](int vi) {
+  auto fetch = [&](int g, int vi) {
     if (vi < nvec)
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (r < rows) raw[r].load(in + r * p.qkv_stride + vi * 8);
+        if (g + r < rows) raw[r].load(in + (g + r) * p.qkv_stride + vi * 8);
   };
-  fetch(tid);
+  fetch(0, tid);
   // ---- where the rows go: the sequence is the last b with row_start[b] <= row
   int b0 = row0;
   if (p.row_start) {
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     for (int b = 0; b < c.B; b += NT) upto += __syncthreads_count(b + tid < c.B && p.row_start[b + tid] <= row0);
     b0 = upto - 1;
   }
-  if (tid < R && row0 + tid < p.rows) {
+  if (tid < rows) {
     const int row = row0 + tid;
     int b = p.row_start ? b0 : row, back = 1;
     bool has = true;
@@ -182,7 +186,7 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
   }
   __syncthreads();
   if (p.rope) {
-    for (int i = tid; i < R * (D / 2); i += NT) {
+    for (int i = tid; i < RB * (D / 2); i += NT) {
       const int r = i / (D / 2), d = i % (D / 2);
       float sn = 0.f, cs = 1.f;
       if (r < rows) rope_cs(s_pos[r], p.tab.inv_freq[d], sn, cs);
@@ -191,6 +195,9 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     }
     __syncthreads();
   }
+#pragma unroll 1
+  for (int g = 0; g < rows; g += R)
+#pragma unroll 1
   for (int v0 = 0; v0 < nvec; v0 += NT) {
     const int vi = v0 + tid;
     const bool act = vi < nvec;
@@ -198,12 +205,13 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     float v[R][8], bb[8], gg[8];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (act && r < rows) raw[r].floats(v[r]);
+      if (act && g + r < rows) raw[r].floats(v[r]);
       else
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
     }
-    fetch(vi + NT);
+    if (v0 + NT < nvec) fetch(g, vi + NT);
+    else if (g + R < rows) fetch(g + R, tid);
     if (p.bias && act) {
       ldf<8>(p.bias + col, bb);
 #pragma unroll
@@ -235,9 +243,10 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     T* pool = static_cast<T*>(turned ? c.k : c.v) + static_cast<long long>(turned ? hd - Hq : hd - nqk) * c.page_size * D + d;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (r >= rows) break;
+      if (g + r >= rows) break;
       if (p.rope && turned) {
-        const float4 cs = *reinterpret_cast<const float4*>(&s_cs[r][d / 2]), sn = *reinterpret_cast<const float4*>(&s_sn[r][d / 2]);
+        const float4 cs = *reinterpret_cast<const float4*>(&s_cs[g + r][d / 2]),
+                     sn = *reinterpret_cast<const float4*>(&s_sn[g + r][d / 2]);
         const float c4[4] = {cs.x, cs.y, cs.z, cs.w}, s4[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -246,12 +255,12 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
           v[r][2 * e + 1] = x0 * s4[e] + x1 * c4[e];
         }
       }
-      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + r * p.out_stride + col, v[r]);
-      if (hd >= Hq && s_kv[r] >= 0) stv<T, 8>(pool + s_kv[r], v[r]);
+      if (out && (hd < Hq || p.out_full)) stv<T, 8>(out + (g + r) * p.out_stride + col, v[r]);
+      if (hd >= Hq && s_kv[g + r] >= 0) stv<T, 8>(pool + s_kv[g + r], v[r]);
     }
   }
-  for (int i = tid; i < R * Hkv; i += NT) {
-    const int r = i % R, h = i / R;
+  for (int i = tid; i < RB * Hkv; i += NT) {
+    const int r = i % RB, h = i / RB;
     if (r >= rows || s_meta[r] < 0) continue;
     const long long at = s_meta[r] + static_cast<long long>(h) * c.page_size;
     if (c.pos) c.pos[at] = s_pos[r];
@@ -261,8 +270,8 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
 
 template <typename T, int D>
 static cudaError_t kv_append_d(const AppendParams& p, cudaStream_t st) {
-  if (p.rows >= 148 * 8) return launch_early(kv_append_kernel<T, D, 4>, dim3((p.rows + 3) / 4), NT, 0, st, p);
-  return launch_early(kv_append_kernel<T, D, 1>, dim3(p.rows), NT, 0, st, p);
+  if (p.rows >= 148 * 8) return launch_early(kv_append_kernel<T, D, 2, 2>, dim3((p.rows + 3) / 4), NT, 0, st, p);
+  return launch_early(kv_append_kernel<T, D, 1, 1>, dim3(p.rows), NT, 0, st, p);
 }
 
 template <typename T>

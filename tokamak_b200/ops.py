@@ -283,6 +283,8 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
     if qkv.dtype != cache.k.dtype:
         raise TkbError(f"kv_append: rows are {qkv.dtype}, the cache is {cache.k.dtype}")
     rows = qkv.shape[0]
+    if qkv.shape[1] != (Hq + 2 * cache.Hkv) * cache.D:
+        raise TkbError(f"kv_append: rows of {qkv.shape[1]} columns, not {(Hq + 2 * cache.Hkv) * cache.D}")
     if out is None:
         out = torch.empty(rows, (Hq + 2 * cache.Hkv if full else Hq) * cache.D, dtype=qkv.dtype, device=qkv.device)
     check(lib().tkb_kv_append(cache.ref, _ptr(qkv), qkv.stride(0), _ptr(bias), _ptr(qk_gain), _ptr(out), out.stride(0),
@@ -303,10 +305,10 @@ def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=
     """Attention of one token per sequence over its cache: q [B, Hq*D] -> (out [B, Hq*D], lse [B, Hq] fp32)."""
     if q.dtype != cache.k.dtype:
         raise TkbError(f"paged_attn_decode: q is {q.dtype}, the cache is {cache.k.dtype}")
-    if q.shape[0] != cache.B:
-        raise TkbError(f"paged_attn_decode: {q.shape[0]} query rows for {cache.B} sequences")
+    if q.shape != (cache.B, Hq * cache.D):
+        raise TkbError(f"paged_attn_decode: q is {tuple(q.shape)}, not {(cache.B, Hq * cache.D)}")
     if out is None:
-        out = torch.empty(cache.B, Hq * cache.D, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if lse is None:
         lse = torch.empty(cache.B, Hq, dtype=torch.float32, device=q.device)
     if workspace is None:
