@@ -196,48 +196,88 @@ struct Sampler {
     // thresholds as floats; hi one past the largest key means nothing is above
     const float flo = Key::value(lo), fhi = Key::value(hi);
     constexpr uint32_t ONE = 0x3F800000u, LOW = 0x3BC00000u;  // 1, 1.5 * 2^-8
-    uint32_t hi_all = 0, lo_all = 0, hi_above = 0, lo_above = 0, n = 0;
-    n_list = 0;
+    uint32_t hi_all = 0, lo_all = 0, hi_above = 0, lo_above = 0, n = 0, n_in = 0;
+    // the vectors with listed elements, as (vector << 8 | mask), from the end of the list's memory downwards
+    uint32_t* marks = reinterpret_cast<uint32_t*>(list + SLIST) - 1;
+    int n_marks = 0;
     summed = WEIGHTS;
+    const uint64_t top2 = f2(top, top), inv2 = f2(inv_t, inv_t), one2 = f2(1.f, 1.f), low2 = f2(0.005859375f, 0.005859375f);
     for (int it = 0; it < p.per; ++it) {
       float x[VEC];
       vec(it, x);
       uint32_t in = 0;  // this lane's elements of the bracket
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const bool is_above = x[e] >= fhi;
-        if (x[e] >= flo && !is_above) in |= 1u << e;
-        n += is_above;
+      for (int e = 0; e < VEC; e += 2) {
+        const bool above0 = x[e] >= fhi, above1 = x[e + 1] >= fhi;
+        if (x[e] >= flo && !above0) in |= 1u << e;
+        if (x[e + 1] >= flo && !above1) in |= 2u << e;
+        n += above0;
+        n += above1;
         if constexpr (WEIGHTS) {
-          const float z = PLAIN ? __fmul_rn(__fsub_rn(top, x[e]), inv_t) : sample_dist(x[e], top, inv_t);
-          float ex = expf(-z);
-          if constexpr (!PLAIN) ex = ex == ex ? ex : 0.f;  // -inf logits at an infinite temperature
-          const float t = __fadd_rn(ex, 1.f);
-          const uint32_t th = __float_as_uint(t);
-          const uint32_t tl = __float_as_uint(__fadd_rn(__fsub_rn(ex, __fsub_rn(t, 1.f)), 0.005859375f));
-          hi_all += th;
-          lo_all += tl;
-          if (is_above) {
-            hi_above += th;
-            lo_above += tl;
+          float z0, z1;
+          if constexpr (PLAIN) {
+            f2_split(mul_f2(sub_f2(top2, f2(x[e], x[e + 1])), inv2), z0, z1);
+          } else {
+            z0 = sample_dist(x[e], top, inv_t);
+            z1 = sample_dist(x[e + 1], top, inv_t);
+          }
+          float e0 = expf(-z0), e1 = expf(-z1);
+          if constexpr (!PLAIN) {  // -inf logits at an infinite temperature
+            e0 = e0 == e0 ? e0 : 0.f;
+            e1 = e1 == e1 ? e1 : 0.f;
+          }
+          const uint64_t ex = f2(e0, e1), t = add_f2(ex, one2);
+          const uint64_t l = add_f2(sub_f2(ex, sub_f2(t, one2)), low2);
+          float t0, t1, l0, l1;
+          f2_split(t, t0, t1);
+          f2_split(l, l0, l1);
+          hi_all += __float_as_uint(t0) + __float_as_uint(t1);
+          lo_all += __float_as_uint(l0) + __float_as_uint(l1);
+          if (above0) {
+            hi_above += __float_as_uint(t0);
+            lo_above += __float_as_uint(l0);
+          }
+          if (above1) {
+            hi_above += __float_as_uint(t1);
+            lo_above += __float_as_uint(l1);
           }
         }
       }
-      if (__any_sync(0xffffffffu, in)) {
-        const int mine = __popc(in);
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      if (m) {
+        const int at = n_marks + __popc(m & ((1u << lane_id()) - 1));
+        if (in && at < 2 * SLIST) *(marks - at) = static_cast<uint32_t>(it * 32 + lane_id()) << 8 | in;
+        n_marks += __popc(m);
+        n_in += __popc(in);
+      }
+    }
+    n_list = __reduce_add_sync(0xffffffffu, n_in);
+    __syncwarp();
+    // From marks to elements, in place, the lowest mark (the last one) first:
+    // every mark still unread stands for one element at least, so what is
+    // written (8 bytes an element, from the front) ends before the unread marks
+    // (4 bytes each, up to the end) begin.
+    if (n_list <= SLIST) {
+      int done = 0;
+      for (int i = 0; i < n_marks; i += 32) {
+        uint32_t mark = i + lane_id() < n_marks ? *(marks - (n_marks - 1 - i - lane_id())) : 0u;
+        const int mine = __popc(mark & 0xFFu);
         int end = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const int o = __shfl_up_sync(0xffffffffu, end, d);
           if (lane_id() >= d) end += o;
         }
-        const int at0 = (it * 32 + lane_id()) * VEC;
-        for (int at = n_list + end - mine; in && at < SLIST; in &= in - 1, ++at) {
-          const int i = at0 + __ffs(in) - 1;
-          const float v = STREAM && base + i >= p.V ? -INFINITY : Elem<T>::ld(data + warp_id() * p.per * 32 * VEC + i);
-          list[at] = make_uint2(Key::of(v), base + i);
+        const int first = static_cast<int>(mark >> 8) * VEC;
+        int at = done + end - mine;
+        __syncwarp();
+        for (mark &= 0xFFu; mark && at < SLIST; mark &= mark - 1, ++at) {
+          const int j = base + first + __ffs(mark) - 1;
+          const float v = STREAM && j >= p.V ? -INFINITY : Elem<T>::ld(data + (STREAM ? j : j - rank * SW * p.per * 32 * VEC));
+          list[at] = make_uint2(Key::of(v), j);
         }
-        n_list += __shfl_sync(0xffffffffu, end, 31);
+        done += __shfl_sync(0xffffffffu, end, 31);
+        __syncwarp();
       }
     }
     n_above = n;
@@ -464,7 +504,7 @@ TKB_DEVFN uint32_t max_nan2(uint32_t a, uint32_t b) {
 }
 
 template <typename T, bool STREAM>
-__global__ void __launch_bounds__(Sampler<T, STREAM>::NTH) sample_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(Sampler<T, STREAM>::NTH, 1024 / Sampler<T, STREAM>::NTH) sample_kernel(const __grid_constant__ SampleParams p) {
   using S = Sampler<T, STREAM>;
   constexpr int VEC = S::VEC, SW = S::SW, SLIST = S::SLIST, CTAS = S::CTAS;
   using Key = SampleKey<T>;
