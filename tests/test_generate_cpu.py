@@ -118,3 +118,21 @@ def test_python_checks():
         ops.sample_logits(torch.zeros(2, 8), torch.zeros(3))
     with pytest.raises(TkbError):
         ops.sample_logits(torch.zeros(2, 8), torch.zeros(2), top_k=torch.zeros(2))
+    q2 = torch.zeros(2, 4 * 64)
+    with pytest.raises(TkbError):
+        ops.paged_attn_decode(c, q2, 4, out=torch.zeros(2, 64))
+    with pytest.raises(TkbError):
+        ops.paged_attn_decode(c, q2, 4, lse=torch.zeros(2, 3))
+    rows = torch.zeros(2, 8 * 64)
+    for bad in (dict(bias=torch.zeros(7)), dict(qk_gain=torch.zeros(8 * 64)), dict(seen=lens.long()),
+                dict(row_start=lens), dict(out=torch.zeros(2, 64))):
+        with pytest.raises(TkbError):
+            ops.kv_append(c, rows, 4, **bad)
+    with pytest.raises(TkbError):
+        ops.kv_append(c, rows[:, :64], 4)
+    with pytest.raises(TkbError):
+        ops.kv_evict(c, 8, lens[:1])
+    with pytest.raises(TkbError):
+        ops.kv_lens(lens.long(), 4)
+    with pytest.raises(TkbError):
+        ops.kv_lens(lens, 4, row_start=lens)

@@ -426,3 +426,42 @@ def test_evict_then_attend():
         for h in range(2):
             kept = set(c.pos[c.table[b, :4].long(), h].flatten().tolist())
             assert set(range(lens[b] - 16, lens[b])) | {0, 1} <= kept and len(kept) == 64
+
+
+# ------------------------------------------------------------------ many sequences, long caches
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decode_more_sequences_than_threads(dtype):
+    """Each thread counts several sequences' tiles, empty ones among them."""
+    rng = np.random.default_rng(3)
+    lens = rng.integers(0, 40, 1100).tolist()
+    lens[700] = 900
+    c = Cache(dtype, lens, 1, 64, 16)
+    g = c.g
+    c.k.copy_(torch.randn(c.k.shape, generator=g, device="cuda"))
+    c.v.copy_(torch.randn(c.v.shape, generator=g, device="cuda"))
+    q = c.randn(len(lens), 2 * 64, dtype=dtype)
+    out, lse = ops().paged_attn_decode(c.handle, q, 2)
+    check_attention(c, q, 2, lens, out, lse, dtype)
+    assert device_error() == 0
+
+
+def test_append_many_prompts():
+    rng = np.random.default_rng(4)
+    fresh = rng.integers(0, 12, 700).tolist()
+    total = sum(fresh)
+    c = Cache(torch.float32, fresh, 1, 64, 16)
+    start = torch.from_numpy(np.concatenate(([0], np.cumsum(fresh))).astype(np.int32)).cuda()
+    rows = c.randn(total, 3 * 64)
+    out = ops().kv_append(c.handle, rows, 1, row_start=start, rope=False)
+    assert torch.equal(out, rows[:, :64])
+    seq = np.repeat(np.arange(700), fresh)
+    slot = np.concatenate([np.arange(n) for n in fresh]).astype(np.int64)
+    pages = c.table[torch.from_numpy(seq).cuda(), 0].long()
+    at = torch.from_numpy(slot).cuda()
+    assert torch.equal(c.k[pages, 0, at], rows[:, 64:128]) and torch.equal(c.v[pages, 0, at], rows[:, 128:])
+    assert int((c.pos != -7).sum()) == total and device_error() == 0
+
+
+def test_evict_from_caches_too_long_for_shared_memory():
+    """Above 49152 slots a sequence's keys are kept in the workspace."""
+    assert evict_case(torch.bfloat16, [60000, 100], 1, 64, 1024, 500, 50, 4, shuffle=False) > 400

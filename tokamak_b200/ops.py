@@ -237,6 +237,12 @@ def _expect(t, name, shape, dtype):
                        f"got {t.dtype} {tuple(t.shape)}")
 
 
+def _vec(t, name, n, dtype):
+    """t, if given, holds n contiguous values of dtype."""
+    if t is not None and (t.numel() != n or t.dtype != dtype or not t.is_contiguous()):
+        raise TkbError(f"{name}: expected {n} contiguous {dtype}, got {t.dtype} {tuple(t.shape)}")
+
+
 class KVCache:
     """One attention layer's paged key-value cache (tkb_kv_cache): tensors
     k, v [n_pages, Hkv, page_size, D] (any page stride, the rest contiguous),
@@ -272,7 +278,11 @@ class KVCache:
 
 def kv_lens(seq_lens, limit, seen=None, add=0, row_start=None):
     """seq_lens = min(seq_lens + n, limit) and seen += n, on the device (n = add, or row_start's differences)."""
-    check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add), int(limit), seq_lens.numel(), _raw_stream(seq_lens)),
+    B = seq_lens.numel()
+    _vec(seq_lens, "seq_lens", B, torch.int32)
+    _vec(seen, "seen", B, torch.int32)
+    _vec(row_start, "row_start", B + 1, torch.int32)
+    check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add), int(limit), B, _raw_stream(seq_lens)),
           "tkb_kv_lens")
 
 
@@ -283,10 +293,18 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
     if qkv.dtype != cache.k.dtype:
         raise TkbError(f"kv_append: rows are {qkv.dtype}, the cache is {cache.k.dtype}")
     rows = qkv.shape[0]
-    if qkv.shape[1] != (Hq + 2 * cache.Hkv) * cache.D:
-        raise TkbError(f"kv_append: rows of {qkv.shape[1]} columns, not {(Hq + 2 * cache.Hkv) * cache.D}")
+    C = (Hq + 2 * cache.Hkv) * cache.D
+    width = C if full else Hq * cache.D
+    if qkv.shape != (rows, C) or qkv.stride(1) != 1:
+        raise TkbError(f"kv_append: qkv is {tuple(qkv.shape)}, not rows of {C} contiguous columns")
+    _vec(seen, "seen", cache.B, torch.int32)
+    _vec(row_start, "row_start", cache.B + 1, torch.int32)
+    _vec(bias, "bias", C, torch.float32)
+    _vec(qk_gain, "qk_gain", (Hq + cache.Hkv) * cache.D, torch.float32)
     if out is None:
-        out = torch.empty(rows, (Hq + 2 * cache.Hkv if full else Hq) * cache.D, dtype=qkv.dtype, device=qkv.device)
+        out = torch.empty(rows, width, dtype=qkv.dtype, device=qkv.device)
+    elif out.shape != (rows, width) or out.dtype != qkv.dtype or out.stride(1) != 1:
+        raise TkbError(f"kv_append: out is {out.dtype} {tuple(out.shape)}, not {qkv.dtype} {(rows, width)}")
     check(lib().tkb_kv_append(cache.ref, _ptr(qkv), qkv.stride(0), _ptr(bias), _ptr(qk_gain), _ptr(out), out.stride(0),
                               int(full), _ptr(row_start), _ptr(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
                               low, high, octx, _raw_stream(qkv)), "tkb_kv_append")
@@ -309,8 +327,14 @@ def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=
         raise TkbError(f"paged_attn_decode: q is {tuple(q.shape)}, not {(cache.B, Hq * cache.D)}")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise TkbError(f"paged_attn_decode: out is {out.dtype} {tuple(out.shape)}, not as q")
+    if q.stride(1) != 1 or out.stride(1) != 1:
+        raise TkbError("paged_attn_decode: columns of q and out must be contiguous")
     if lse is None:
         lse = torch.empty(cache.B, Hq, dtype=torch.float32, device=q.device)
+    else:
+        _vec(lse, "lse", cache.B * Hq, torch.float32)
     if workspace is None:
         workspace = paged_attn_workspace(cache, Hq, accumulate)
     check(lib().tkb_paged_attn_decode(cache.ref, _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(lse), Hq,
@@ -329,6 +353,7 @@ def kv_evict_workspace(cache):
 def kv_evict(cache, budget, seen, recent=0, sinks=0, workspace=None):
     """Keep `budget` tokens of every (sequence, kv head) that holds more, by accumulated weight (tkb_kv_evict);
     kv_lens(cache.seq_lens, budget) after the last layer."""
+    _vec(seen, "seen", cache.B, torch.int32)
     if workspace is None:
         workspace = kv_evict_workspace(cache)
     check(lib().tkb_kv_evict(cache.ref, _ptr(seen), int(budget), int(recent), int(sinks), _ptr(workspace),
@@ -347,7 +372,7 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     logprob = torch.empty_like(u)
     token = torch.empty_like(u, dtype=torch.int32)
     kept = torch.empty_like(token)
-    check(lib().tkb_sample_logits(_ptr(logits), logits.stride(0) if rows > 1 else V, _ptr(u), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
-                                  _ptr(token), _ptr(logprob), _ptr(kept), rows, V, dtype_code(logits), _raw_stream(logits)),
-          "tkb_sample_logits")
+    check(lib().tkb_sample_logits(_ptr(logits), logits.stride(0) if rows > 1 else V, _ptr(u), _ptr(temperature),
+                                  _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(logprob), _ptr(kept), rows, V,
+                                  dtype_code(logits), _raw_stream(logits)), "tkb_sample_logits")
     return token, logprob, kept
