@@ -2,11 +2,10 @@
 tkb_kv_evict, tkb_kv_lens) against the float64 oracle.
 
 Tolerances, in relative L2.  Storing a value in a type of m mantissa bits is
-off by up to 2^-(m+1), 0.58 of that in the root mean square; the attention
-rounds its probabilities to the same type before the product with V, another
-such error in every term.  Twice the larger bound of one rounding, 2^-m,
-covers both: 2^-8 for bf16 stores, 2^-7 for bf16 attention; 2^-11 and 2^-10
-for f16.  fp32: sums of D (128) products of unit values are off by some
+off by up to 2^-(m+1), 0.58 of that in the root mean square: 2^-m for stores
+(2^-8 for bf16, 2^-11 for f16).  The attention may round its probabilities to
+the same type before the product with V, another such error in every term:
+twice that bound, 2^-7 and 2^-10.  fp32: sums of D (128) products of unit values are off by some
 1e-6, exponentials of the scores by as much, so 1e-5; log-sum-exps and
 accumulated weights are fp32 in every type: 2e-5.
 """

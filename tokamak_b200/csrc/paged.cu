@@ -482,15 +482,21 @@ struct TileMma {
       m[1] = mn[1];
     }
     const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-    uint32_t a[4];
+    uint32_t a[4], b[4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const float p0 = ex2(s[t][0] - m0), p1 = ex2(s[t][1] - m0), p2 = ex2(s[t][2] - m1), p3 = ex2(s[t][3] - m1);
       l[0] += p0 + p1;
       l[1] += p2 + p3;
-      // P in 16 bits: the tensor cores take P and V in one type; the sum keeps 32
+      // The tensor cores take P and V in one 16-bit type: P goes in as its
+      // rounding and what that left over (two products), so that only the
+      // output itself is rounded to 16 bits.  One rounded P cost 1.4 times the
+      // output's own rounding error; the second product is hidden behind HBM.
       a[2 * t] = pack2<BF16>(p0, p1);
       a[2 * t + 1] = pack2<BF16>(p2, p3);
+      const float2 h0 = unpack2<BF16>(a[2 * t]), h1 = unpack2<BF16>(a[2 * t + 1]);
+      b[2 * t] = pack2<BF16>(p0 - h0.x, p1 - h0.y);
+      b[2 * t + 1] = pack2<BF16>(p2 - h1.x, p3 - h1.y);
     }
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
@@ -498,6 +504,8 @@ struct TileMma {
       ldsm4_t(vb + swz<Cfg::RB>((mi & 1) * 8 + ri, d * 2 + (mi >> 1)), f);
       mma16816<BF16>(o[2 * d], a, f[0], f[1]);
       mma16816<BF16>(o[2 * d + 1], a, f[2], f[3]);
+      mma16816<BF16>(o[2 * d], b, f[0], f[1]);
+      mma16816<BF16>(o[2 * d + 1], b, f[2], f[3]);
     }
   }
 
