@@ -417,7 +417,7 @@ struct Sampler {
   // largest: they are brought to CTA 0, each of whose threads compares one of
   // them with all the others.
   // bound: what top-p leaves (0: its share of the first k's weight).
-  TKB_DEVFN void few(int row, int k, bool nucleus, float tp, unsigned long long bound, uint32_t least, uint2* s_few) {
+  TKB_DEVFN void few(int row, int k, bool nucleus, float tp, unsigned long long bound, uint32_t least, uint4* s_few) {
     const int lane = lane_id(), tid = threadIdx.x;
     if (lane == 0) buf()[warp_id()] = n_list;
     agree();
@@ -436,28 +436,31 @@ struct Sampler {
     const int n = __shfl_sync(0xffffffffu, end, 31), mine = rank * SW + warp_id();
     const int at = __shfl_sync(0xffffffffu, end - c[0] - c[1], mine / 2) +
                    (mine & 1 ? __shfl_sync(0xffffffffu, c[0], mine / 2) : 0);
+    // (key, index, weight, kept weight) of each
     const uint32_t dst = mapa_shared(smem_u32(s_few), 0);
     for (int i = lane; i < n_list; i += 32)
-      if (STREAM) s_few[at + i] = list[i];
-      else asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst + 8 * (at + i)), "r"(list[i].x), "r"(list[i].y)
-                   : "memory");
+      if (STREAM) s_few[at + i] = make_uint4(list[i].x, list[i].y, 0u, 0u);
+      else asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(dst + 16 * (at + i)), "r"(list[i].x), "r"(list[i].y)
+                        : "memory");
     next();
     agree();
     if (rank != 0) return;
-    uint32_t* s_w = reinterpret_cast<uint32_t*>(xbuf[0]);
-    unsigned long long* s_kept = xbuf[1];
-    const uint2 e = tid < n ? s_few[tid] : make_uint2(0u, 0u);
+    const bool mine_in = warp_id() * 32 < n;  // warps past the list only take part in the sums
+    const uint4 e = tid < n ? s_few[tid] : make_uint4(0u, 0u, 0u, 0u);
     const uint32_t wt = tid < n ? weight_of(e.x) : 0u;
-    if (tid < SSMALL) s_w[tid] = wt;
+    if (tid < n) s_few[tid].z = wt;
     __syncthreads();
     // tokens before this one in the order of the truncations, and their weight
     int rank_of = 0;
     unsigned long long before = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint2 o = s_few[j];
-      if (o.x > e.x || (o.x == e.x && o.y < e.y)) {
-        ++rank_of;
-        before += s_w[j];
+    if (mine_in) {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const uint4 o = s_few[j];
+        if (o.x > e.x || (o.x == e.x && o.y < e.y)) {
+          ++rank_of;
+          before += o.z;
+        }
       }
     }
     bool keep = tid < n && (k == 0 || rank_of < k);
@@ -467,14 +470,18 @@ struct Sampler {
       keep = keep && before < bound;
     }
     keep = keep && wt >= least;
-    if (tid < SSMALL) s_kept[tid] = keep ? wt : 0ull;
-    const unsigned long long total = block_sum(keep ? wt : 0ull);  // (its barriers publish s_kept)
-    const unsigned long long kept = block_sum(keep ? 1ull : 0ull);
+    if (tid < n) s_few[tid].w = keep ? wt : 0u;
+    // weights in the lower 52 bits, the number kept above them (its barriers publish s_few)
+    const unsigned long long sum = block_sum(keep ? wt | 1ull << 52 : 0ull), total = sum & ((1ull << 52) - 1);
     const unsigned long long target = scaled_floor(total, fixed32(p.u[row]));
+    if (!mine_in) return;
     unsigned long long run = 0;
-    for (int j = 0; j < n; ++j)
-      if (s_few[j].y < e.y) run += s_kept[j];
-    if (keep && run <= target && target < run + wt) finish(row, e.y, Key::value(e.x), total, static_cast<int>(kept));
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const uint4 o = s_few[j];
+      if (o.y < e.y) run += o.w;
+    }
+    if (keep && run <= target && target < run + wt) finish(row, e.y, Key::value(e.x), total, static_cast<int>(sum >> 52));
   }
   TKB_DEVFN unsigned long long block_sum(unsigned long long v) {
     v = warp_sum_u64(v);
@@ -508,9 +515,8 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH, 1024 / Sampler<T, STR
   using S = Sampler<T, STREAM>;
   constexpr int VEC = S::VEC, SW = S::SW, SLIST = S::SLIST, CTAS = S::CTAS;
   using Key = SampleKey<T>;
-  extern __shared__ __align__(16) uint8_t smem[];  // the lists, then the slice
+  extern __shared__ __align__(16) uint8_t smem[];  // the lists, then the slice (STREAM: what few() gathers)
   __shared__ unsigned long long s_x[2][256], s_tmp[2 * SW + 8];
-  __shared__ uint2 s_few[SSMALL];
   grid_wait();
   S s(p);
   const int row = blockIdx.x / p.ctas, tid = threadIdx.x, lane = lane_id(), w = warp_id(), V = p.V;
@@ -788,7 +794,9 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH, 1024 / Sampler<T, STR
       }
     }
     if (found == S::FEW) {
-      s.few(row, k, nucleus, tp, whole_row ? bound : 0, least, s_few);
+      // gathered over CTA 0's slice: every pass over it has ended
+      s.few(row, k, nucleus, tp, whole_row ? bound : 0, least,
+            reinterpret_cast<uint4*>(smem + SW * SLIST * sizeof(uint2)));
       return;
     }
   }
@@ -973,10 +981,11 @@ static cudaError_t sample_launch(const SampleParams& p, cudaStream_t st) {
   using S = Sampler<T, STREAM>;
   // the widest slice: kSampleMaxV fp32 logits over SCTAS CTAs
   constexpr int lists = S::SW * S::SLIST * static_cast<int>(sizeof(uint2));
-  cudaError_t e = allow_smem<sample_kernel<T, STREAM>>(lists + (STREAM ? 0 : kSampleMaxV / SCTAS * 4));
+  cudaError_t e = allow_smem<sample_kernel<T, STREAM>>(lists + (STREAM ? SSMALL * 16 : kSampleMaxV / SCTAS * 4));
   if (e != cudaSuccess) return e;
   return launch_early(sample_kernel<T, STREAM>, dim3(static_cast<unsigned>(p.rows) * p.ctas), S::NTH,
-                      lists + (STREAM ? 0 : static_cast<size_t>(p.per) * S::NTH * 16), st, p, p.ctas);
+                      lists + (STREAM ? SSMALL * sizeof(uint4) : static_cast<size_t>(p.per) * S::NTH * 16), st, p,
+                      p.ctas);
 }
 
 // One CTA per row pays when rows are wide and enough (us, cluster / one CTA,
