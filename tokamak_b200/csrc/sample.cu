@@ -988,15 +988,16 @@ static cudaError_t sample_launch(const SampleParams& p, cudaStream_t st) {
                       p.ctas);
 }
 
-// One CTA per row pays when rows are wide and enough (us, cluster / one CTA,
-// nucleus 0.9): 64 KB rows 40 / 46 at 296 rows, 63 / 77 at 512; 128 KB rows
-// 52 / 50 at 200, 66 / 56 at 296; 256 KB rows 119 / 128 at 200, 166 / 142 at
-// 296, 271 / 215 at 512; 512 KB rows 147 / 122 at 148, 468 / 298 at 512.
+// One CTA per row pays when rows are wide and there is one for every SM (us,
+// cluster / one CTA, nucleus 0.9 and top-k 50): 64 KB rows 25 / 29 and 15 / 17 at
+// 148 rows, 57 / 70 and 33 / 39 at 512; 128 KB rows 34 / 32 and 21 / 18 at 148,
+// 100 / 88 and 56 / 43 at 512; 256 KB rows 83 / 84 and 52 / 40 at 148, 253 / 197
+// and 158 / 95 at 512; 512 KB rows 136 / 107 and 76 / 56 at 148, 435 / 262 and
+// 231 / 135 at 512.
 template <typename T>
 static cudaError_t sample_t(SampleParams p, cudaStream_t st) {
   sample_shape(p.rows, p.V, sizeof(T), p.ctas, p.per);
-  const long long bytes = static_cast<long long>(p.V) * sizeof(T);
-  if ((bytes > 65536 && p.rows >= 224) || (bytes > 262144 && p.rows >= 148)) {
+  if (static_cast<long long>(p.V) * sizeof(T) > 65536 && p.rows >= 148) {
     constexpr int chunk = Sampler<T, true>::NTH * Sampler<T, true>::VEC;
     p.ctas = 1;
     p.per = (p.V + chunk - 1) / chunk;
