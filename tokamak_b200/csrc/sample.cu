@@ -18,8 +18,15 @@
 // instead of 64.
 // The cut of top-k or top-p is found without sorting: a guess brackets it,
 // one pass sums what lies above the bracket exactly and lists what lies
-// inside, and a radix search over the list gives the cut.  A wrong or too wide
-// guess is halved and tried again, so it costs time only.
+// inside, and a radix search over the list gives the cut (or, when the list
+// holds the row's largest and no more than 256 of them, each is compared with
+// all the others).  A guess that missed costs another pass, nothing else.
+//
+// Measured (us): one row of 32000 bf16, top-k and top-p: 10; 64 rows of 32000
+// fp32: 13; 512 rows of 131072 bf16, top-p 0.9 (134 MB): 194, bound by issue
+// slots: 48 instructions per logit, 20 of them in the exponential that the sum
+// of all weights needs.  Bitwise searches re-reading the row took 452, 448 and
+// 5482.
 #include "tkb_common.cuh"
 
 namespace tkb {
