@@ -324,7 +324,7 @@ struct DecodeTile {
   static constexpr int TK = RB <= 256 ? 16 : 8;     // keys per tile
   static constexpr int HALF = TK * RB;              // bytes of the K (or V) part
   static constexpr int WARPS = D * ES == 128 ? 16 : 8;
-  static constexpr int STAGES = ES == 4 && GT > 8 ? 2 : 3;
+  static constexpr int STAGES = ES == 4 && GT > 4 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * HALF;    // per warp
   static constexpr int HEAD = GT <= 8 ? GT * D * 4 : 0;                  // per warp: its first part (else in the workspace)
   static constexpr int EXTRA = ES == 4 ? GT * D * 4 + GT * TK * 4 : 0;   // per warp: q, p
@@ -564,7 +564,7 @@ struct TileFma {
     float* sq = reinterpret_cast<float*>(extra);
     const float* src = static_cast<const float*>(p.q) + b * p.q_stride + static_cast<long long>(h0) * D;
     __syncwarp();
-    for (int i = lane_id(); i < rows * D; i += 32) sq[i] = __ldg(src + i) * p.scale_log2;
+    for (int i = lane_id(); i < GT * D; i += 32) sq[i] = i < rows * D ? __ldg(src + i) * p.scale_log2 : 0.f;
     __syncwarp();
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
@@ -587,34 +587,48 @@ struct TileFma {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
       k[i] = *reinterpret_cast<const float4*>(buf + swz<Cfg::RB>(key, part + PART * i));
+    // all GT heads without branches, so that their chains overlap (heads past `rows` have q = 0)
+    float s[GT];
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
-      if (g < rows) {
-        float s = 0.f;
+      s[g] = 0.f;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const float4 q = *reinterpret_cast<const float4*>(sq + g * D + (part + PART * i) * 4);
-          s = fmaf(q.x, k[i].x, s);
-          s = fmaf(q.y, k[i].y, s);
-          s = fmaf(q.z, k[i].z, s);
-          s = fmaf(q.w, k[i].w, s);
-        }
-#pragma unroll
-        for (int d = 1; d < PART; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (key >= valid) s = -INFINITY;
-        if (scores && part == 0) scores[g * score_stride + key] = s;
-        float x = s;
-#pragma unroll
-        for (int d = PART; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-        const float mn = fmaxf(m[g], x);
-        const float keep = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn), pr = mn == -INFINITY ? 0.f : ex2(s - mn);
-        m[g] = mn;
-        // every lane adds its own key's share: the lanes of a key carry it PART times
-        l[g] = l[g] * keep + pr;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[g][e] *= keep;
-        if (part == 0) sp[g * TK + key] = pr;
+      for (int i = 0; i < CH; ++i) {
+        const float4 q = *reinterpret_cast<const float4*>(sq + g * D + (part + PART * i) * 4);
+        s[g] = fmaf(q.x, k[i].x, s[g]);
+        s[g] = fmaf(q.y, k[i].y, s[g]);
+        s[g] = fmaf(q.z, k[i].z, s[g]);
+        s[g] = fmaf(q.w, k[i].w, s[g]);
       }
+    }
+#pragma unroll
+    for (int d = 1; d < PART; d <<= 1)
+#pragma unroll
+      for (int g = 0; g < GT; ++g) s[g] += __shfl_xor_sync(0xffffffffu, s[g], d);
+    float x[GT];
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+      if (key >= valid) s[g] = -INFINITY;
+      x[g] = s[g];
+    }
+    if (scores && part == 0)
+#pragma unroll
+      for (int g = 0; g < GT; ++g)
+        if (g < rows) scores[g * score_stride + key] = s[g];
+#pragma unroll
+    for (int d = PART; d < 32; d <<= 1)
+#pragma unroll
+      for (int g = 0; g < GT; ++g) x[g] = fmaxf(x[g], __shfl_xor_sync(0xffffffffu, x[g], d));
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+      const float mn = fmaxf(m[g], x[g]);
+      const float keep = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn), pr = mn == -INFINITY ? 0.f : ex2(s[g] - mn);
+      m[g] = mn;
+      // every lane adds its own key's share: the lanes of a key carry it PART times
+      l[g] = l[g] * keep + pr;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[g][e] *= keep;
+      if (part == 0) sp[g * TK + key] = pr;
     }
     __syncwarp();
     const uint8_t* vb = buf + Cfg::HALF;
@@ -630,12 +644,11 @@ struct TileFma {
         v[0] = t.x; v[1] = t.y;
       }
 #pragma unroll
-      for (int g = 0; g < GT; ++g)
-        if (g < rows) {
-          const float pr = sp[g * TK + j];
+      for (int g = 0; g < GT; ++g) {
+        const float pr = sp[g * TK + j];
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[g][e] = fmaf(pr, v[e], o[g][e]);
-        }
+        for (int e = 0; e < E; ++e) o[g][e] = fmaf(pr, v[e], o[g][e]);
+      }
     }
     __syncwarp();
   }
@@ -1011,7 +1024,7 @@ static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
   w.part = up(units * 4);
   w.head = w.part + up(static_cast<size_t>(2) * kDecodeGrid * QT * (c.D + 2) * 4);
   // the 16-row tiles (paged_decode_d) keep their first parts here
-  w.lse2 = w.head + (G > (c.dtype == TKB_F32 ? 4 : 8) ? up(static_cast<size_t>(kDecodeGrid) * 16 * QT * c.D * 4) : 0);
+  w.lse2 = w.head + (G > 8 ? up(static_cast<size_t>(kDecodeGrid) * 16 * QT * c.D * 4) : 0);
   w.scores = w.lse2 + (accumulate ? up(static_cast<size_t>(c.B) * Hq * 4) : 0);
   w.bytes = w.scores + (accumulate ? up(static_cast<size_t>(c.B) * Hq * c.max_pages * c.page_size * 4) : 0);
   return w;
@@ -1029,6 +1042,12 @@ static cudaError_t paged_decode_launch(const DecodeParams& p, cudaStream_t st) {
   return launch_early(k, dim3(grid), W * 32, Cfg::SMEM, st, p);
 }
 
+// Rows of a tile by the query heads per kv head.  16-bit: 8 or 16, since parts
+// of 16 rows have no room in shared memory beside three stages of loads.
+// fp32: the registers and shared memory of q grow with them, and heads that are
+// not there cost as much as those that are; 8 sequences of 3-4 k tokens, 4 kv
+// heads of 128 (floor 18 us): 1 head 32 us, 4 heads 35 (with one branch per
+// head, 41), 8 heads 52 (in the 16-row tile, with branches, 81), 16 heads 91.
 template <typename T, int D>
 static cudaError_t paged_decode_d(const DecodeParams& p, cudaStream_t st) {
   if constexpr (sizeof(T) == 2) {
@@ -1037,6 +1056,7 @@ static cudaError_t paged_decode_d(const DecodeParams& p, cudaStream_t st) {
   } else {
     if (p.G == 1) return paged_decode_launch<T, D, TileFma<D, 1>>(p, st);
     if (p.G <= 4) return paged_decode_launch<T, D, TileFma<D, 4>>(p, st);
+    if (p.G <= 8) return paged_decode_launch<T, D, TileFma<D, 8>>(p, st);
     return paged_decode_launch<T, D, TileFma<D, 16>>(p, st);
   }
 }
