@@ -315,8 +315,9 @@ int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stri
  * the sum over its query heads of softmax(s)_slot.  The work is cut over the
  * cached lengths and joined in a fixed order: equal inputs give equal bits.
  * workspace: tkb_paged_attn_decode_workspace bytes, 256-byte aligned, zeroed
- * before its first use; every call leaves it fit for the next one.  Calls
- * that may overlap need workspaces of their own. */
+ * before its first use; every call leaves it fit for the next one, of any
+ * cache and shape that it is large enough for.  Calls that may overlap need
+ * workspaces of their own. */
 size_t tkb_paged_attn_decode_workspace(const tkb_kv_cache *cache, int Hq, int accumulate);
 int tkb_paged_attn_decode(const tkb_kv_cache *cache, const void *q, long long q_stride, void *out,
                           long long out_stride, float *lse, int Hq, float scale, int accumulate,

@@ -464,3 +464,36 @@ def test_append_many_prompts():
 def test_evict_from_caches_too_long_for_shared_memory():
     """Above 49152 slots a sequence's keys are kept in the workspace."""
     assert evict_case(torch.bfloat16, [60000, 100], 1, 64, 1024, 500, 50, 4, shuffle=False) > 400
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_workspace_serves_every_shape(dtype):
+    """One workspace, zeroed once, for caches of other batches, head counts and head widths in turn, and with
+    accumulated weights between them: the bits of a workspace of each cache's own, and the oracle's values."""
+    rng = np.random.default_rng(11)
+    shapes = [([3000], 8, 4, 128, False), (rng.integers(0, 2000, 32).tolist(), 8, 2, 64, False),
+              (rng.integers(500, 900, 20).tolist(), 2, 20, 64, True), ([1500, 0, 700], 1, 1, 128, True)]
+    caches = []
+    for lens, Hkv, G, D, acc in shapes:
+        c = Cache(dtype, lens, Hkv, D, 16)
+        for t in (c.k, c.v):
+            t.copy_(torch.randn(t.shape, generator=c.g, device="cuda"))
+        caches.append((c, c.randn(len(lens), Hkv * G * D, dtype=dtype)))
+    need = [ops().paged_attn_workspace(c.handle, Hkv * G, acc).numel()
+            for (c, _), (_, Hkv, G, _, acc) in zip(caches, shapes)]
+    ws = torch.zeros(max(need), dtype=torch.uint8, device="cuda")
+    fresh = {}
+    for i in (0, 1, 0, 1, 2, 1, 3, 0, 2, 3, 1):
+        (c, q), (lens, Hkv, G, D, acc) = caches[i], shapes[i]
+
+        def call(workspace):
+            c.weight.zero_()
+            out, lse = torch.full_like(q, 7.0), torch.full((len(lens), Hkv * G), 7.0, device="cuda")
+            ops().paged_attn_decode(c.handle, q, Hkv * G, accumulate=acc, out=out, lse=lse, workspace=workspace)
+            return out, lse, c.weight.clone()
+
+        if i not in fresh:
+            fresh[i] = call(None)
+            check_attention(c, q, Hkv * G, lens, fresh[i][0], fresh[i][1], dtype)
+        for got, want in zip(call(ws), fresh[i]):
+            assert torch.equal(got, want), i

@@ -293,7 +293,9 @@ static cudaError_t kv_append_t(const AppendParams& p, cudaStream_t st) {
 // written by that warp at once; the others are parts, at most two per warp,
 // which meet once, at the CTA's end, and where a unit spans CTAs, in the CTA
 // that finishes last (a counter in the workspace), in the order of the run, so
-// the result does not depend on who that is.
+// the result does not depend on who that is.  The counter is that of the CTA
+// the unit starts in, of which it is the last unit: one per CTA, in one place
+// whatever the cache's shape, so that a workspace serves them all in turn.
 //
 // Measured: 16 sequences of 15-16 k tokens, 64/8 heads of 128, bf16 (1.05 GB):
 // 183 us, 5.7 TB/s, 0.88 of HBM, and 17 us for the weights of `accumulate`; 32
@@ -311,7 +313,7 @@ struct DecodeParams {
   float* lse;
   int Hq, G, qblocks, accumulate;
   float scale_log2;
-  int* counters;                      // per unit, 0 between calls
+  int* counters;                      // per CTA, for the unit that goes on from it; 0 between calls
   float* part;                        // [2 * grid][QT][D + 2]: O, then m, l of each row
   float* head;                        // [grid * 16 warps][QT][D]: first parts, when they are not in shared memory
   float* lse2;                        // accumulate: [B][Hq], in powers of 2
@@ -921,7 +923,7 @@ __global__ void __launch_bounds__(Tile::Cfg::WARPS * 32, 1)
   if (w == 0 && (opens >> lane & 1)) {
     const int c0 = first_cta(u.unit0), c1 = first_cta(u.unit0 + u.nt - 1);
     __threadfence();
-    int* counter = &p.counters[u.b * units + u.u];
+    int* counter = &p.counters[c0];
     const bool last = atomicAdd(counter, 1) == c1 - c0;
     s_last[lane == o0 ? 0 : 1] = last;
     if (last) *counter = 0;  // for the next call
@@ -1011,17 +1013,18 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant
 
 constexpr int kDecodeGrid = 148;  // one CTA per SM
 
-// Workspace: counters, partial results, then (accumulate) lse2 and scores.
+// Workspace: counters, partial results, then (accumulate) lse2 and scores.  The
+// counters alone keep a state between calls; they lie first and are as many for
+// every shape, since one call's data over another's counters would lose joins.
 struct DecodeWs {
   size_t counters, part, head, lse2, scores, bytes;
 };
 static DecodeWs decode_ws(const tkb_kv_cache& c, int Hq, int accumulate) {
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const int G = Hq / c.Hkv;
-  const size_t units = static_cast<size_t>(c.B) * c.Hkv * ((G + QT - 1) / QT);
   DecodeWs w;
   w.counters = 0;
-  w.part = up(units * 4);
+  w.part = up(kDecodeGrid * 4);
   w.head = w.part + up(static_cast<size_t>(2) * kDecodeGrid * QT * (c.D + 2) * 4);
   // the 16-row tiles (paged_decode_d) keep their first parts here
   w.lse2 = w.head + (G > 8 ? up(static_cast<size_t>(kDecodeGrid) * 16 * QT * c.D * 4) : 0);

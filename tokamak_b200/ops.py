@@ -312,7 +312,7 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
 
 
 def paged_attn_workspace(cache, Hq, accumulate=False):
-    """Zeroed workspace of paged_attn_decode; one per stream that calls it."""
+    """Zeroed workspace of paged_attn_decode; one per stream that calls it, the largest of its caches' serving all."""
     n = lib().tkb_paged_attn_decode_workspace(cache.ref, Hq, int(accumulate))
     if n == 0:
         check(-1, "tkb_paged_attn_decode_workspace")
