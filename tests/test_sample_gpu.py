@@ -205,3 +205,51 @@ def test_frequencies():
     want /= want.sum()
     got = np.bincount(token.cpu().numpy(), minlength=V) / n
     assert np.abs(got - want).max() < 1.01 / n + 1e-6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,V,ld", [(160, 262144, 262144), (149, 262143, 262151), (148, 260100, 260100),
+                                       (3, 262144, 262144)])
+def test_equal_weights_in_the_widest_rows(dtype, rows, V, ld):
+    """Up to 2^18 tokens of the largest weight: equal logits, all +inf, a temperature that makes every exponential 1,
+    and equal ones among masked ones.  Every count and token is known exactly."""
+    rng = np.random.default_rng(V + rows)
+    x = np.full((rows, ld), 1.5, np.float32)
+    kind = np.arange(rows) % 4
+    x[kind == 1] = np.inf
+    spread = dev(2 * rng.standard_normal(ld).astype(np.float32), dtype)
+    x[kind == 2] = spread.float().cpu().numpy()
+    half = rng.random(ld) < 0.5
+    half[0] = True
+    x[kind == 3] = np.where(half, 1.5, -np.inf)
+    logits = dev(x, dtype)[:, :V]
+    t = np.where(kind == 2, 1e30, 1.0)
+    p = np.float32(rng.integers(1, 2 ** 16, rows) / 2 ** 16)
+    p[rows // 2] = 1.0
+    p[:3] = np.float32([0.9, 0.5, 0.999])
+    u = np.float32(rng.integers(0, 2 ** 24, rows) / 2 ** 24)
+    token, logprob, kept = (a.cpu().numpy() for a in ops().sample_logits(logits, dev(u), temperature=dev(t),
+                                                                         top_p=dev(p)))
+    falling = np.lexsort((np.arange(V), -spread.float().cpu().numpy()[:V].astype(np.float64)))
+    for r in range(rows):
+        idx = falling if kind[r] == 2 else np.flatnonzero(half[:V]) if kind[r] == 3 else np.arange(V)
+        if p[r] < 1:
+            idx = np.sort(idx[:math.ceil(math.floor(float(p[r]) * 2 ** 32) * len(idx) / 2 ** 32)])
+        assert kept[r] == len(idx), r
+        at = math.floor(float(u[r]) * 2 ** 32) * len(idx) // 2 ** 32
+        assert token[r] == np.sort(idx)[at], r
+        assert abs(logprob[r] + math.log(len(idx))) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_widest_rows_with_every_truncation(dtype):
+    """The largest vocabulary, one CTA per row, on ordinary logits."""
+    rng = np.random.default_rng(18)
+    rows, V = 148, 262144
+    logits = dev(2 * rng.standard_normal((rows, V)), dtype)
+    t = rng.uniform(0.3, 2.0, rows)
+    t[5], t[6] = 0.0, 50.0
+    k = np.where(rng.random(rows) < 0.5, 0, rng.integers(1, 3000, rows))
+    p = np.where(rng.random(rows) < 0.3, 1.0, rng.uniform(0.05, 0.999, rows))
+    m = np.where(rng.random(rows) < 0.5, 0.0, rng.uniform(0.001, 0.3, rows))
+    check_rows(logits, rng.random(rows), t, k, p, m)

@@ -50,6 +50,7 @@ struct SampleParams {
 constexpr int SCTAS = 8;      // CTAs per row at most: the portable cluster size
 constexpr int SSMALL = 256;   // listed elements of a row that are ranked directly, one per thread
 constexpr int SBINS = 512;    // bins of the guess, over the distances of non-zero weight
+constexpr int kSampleMaxV = 1 << 18;
 constexpr float SRANGE = 22.25f;  // weights beyond this distance round to zero: 2^31 exp(-22.25) < 1/2
 
 // floor(total * part / 2^32) with part < 2^32
@@ -198,6 +199,12 @@ struct Sampler {
   // rounds e to multiples of 2^-23, which are then the low bits of t; the rest,
   // exact, becomes the low bits of rest + 1.5 2^-8 as a multiple of 2^-31.
   // (The conversion unit also computes ex2; it would be the bound.)
+  //
+  // A lane's upper parts add up to 2^23 for each weight near 2^31, in 32 bits:
+  // 512 of them, all that a lane can have (one CTA per row, V near 2^18), make
+  // 2^32, which is 0 again.  No other sum of 512 is, but that of weights below
+  // 2^7 alone, so one of the lane's elements tells the two apart.  (Adding to 64
+  // bits every 256 elements inside the loop cost 4 % of the pass.)
   template <bool WEIGHTS, bool PLAIN>
   TKB_DEVFN void pass_t(uint32_t lo, uint32_t hi, unsigned long long& in_list, unsigned long long& all) {
     // thresholds as floats; hi one past the largest key means nothing is above
@@ -294,6 +301,16 @@ struct Sampler {
     };
     all = WEIGHTS ? joined(hi_all, lo_all, p.per * VEC) : 0;
     above = WEIGHTS ? joined(hi_above, lo_above, n) : 0;
+    if constexpr (WEIGHTS && STREAM) {
+      constexpr uint32_t MOST = kSampleMaxV / NTH;  // elements per lane
+      static_assert((1ull << 23) * MOST <= 1ull << 32, "a lane's sum wraps at its end at most");
+      if (p.per * VEC == MOST) {
+        float x[VEC];
+        vec(0, x);
+        if (hi_all == MOST * ONE && sample_weight(x[0], top, inv_t) >> 30) all += 1ull << 40;
+        if (n == MOST) above = all;
+      }
+    }
     __syncwarp();
     in_list = 0;
     for (int i = lane_id(); i < min(n_list, SLIST); i += 32) in_list += WEIGHTS ? weight_of(list[i].x) : 1u;
@@ -967,8 +984,6 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH, 1024 / Sampler<T, STR
     if (run > target) break;  // the same in every warp
   }
 }
-
-constexpr int kSampleMaxV = 1 << 18;
 
 // CTAs per row and vectors per lane.  Slices of 32 KB leave room for four CTAs
 // per SM, whose barriers and passes overlap; few rows are cut finer, down to
