@@ -497,3 +497,27 @@ def test_decode_workspace_serves_every_shape(dtype):
             check_attention(c, q, Hkv * G, lens, fresh[i][0], fresh[i][1], dtype)
         for got, want in zip(call(ws), fresh[i]):
             assert torch.equal(got, want), i
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_nan_is_not_an_empty_cache(dtype):
+    """NaN in a query, in every key of a kv head and in one key reaches the heads that use it, and no others; a
+    sequence that holds nothing still gives 0 and -inf."""
+    lens, Hkv, G, D, page = [40, 0, 600, 40, 3], 2, 4, 64, 16
+    c = Cache(dtype, lens, Hkv, D, page).fill(lens)
+    Hq = Hkv * G
+    q = c.randn(5, Hq * D, dtype=dtype)
+    good = [t.clone() for t in ops().paged_attn_decode(c.handle, q, Hq)]
+    q.view(5, Hq, D)[0, 3, 5] = float("nan")
+    c.k[c.table[2].long(), 1, :, 7] = float("nan")
+    c.k[c.table[3, 1].long(), 0, 2, 0] = float("nan")
+    bad = torch.zeros(5, Hq, dtype=torch.bool, device="cuda")
+    bad[0, 3] = bad[2, G:] = bad[3, :G] = True
+    for acc in (False, True):
+        c.weight.zero_()
+        out, lse = ops().paged_attn_decode(c.handle, q, Hq, accumulate=acc)
+        assert torch.equal(out.view(5, Hq, D).isnan(), bad.unsqueeze(-1).expand(5, Hq, D))
+        assert torch.equal(lse.isnan(), bad)
+        for got, want in zip((out.view(5, Hq, D), lse), (good[0].view(5, Hq, D), good[1])):
+            assert torch.equal(got[~bad], want[~bad])
+        assert (out[1] == 0).all() and torch.isneginf(lse[1]).all()

@@ -624,7 +624,8 @@ struct TileFma {
 #pragma unroll
     for (int g = 0; g < GT; ++g) {
       const float mn = fmaxf(m[g], x[g]);
-      const float keep = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn), pr = mn == -INFINITY ? 0.f : ex2(s[g] - mn);
+      // the maximum passes over NaN: where it is still -inf, nothing but masked keys (ex2 gives 0) or NaN (and it stays NaN)
+      const float keep = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn), pr = ex2(s[g] - (mn == -INFINITY ? 0.f : mn));
       m[g] = mn;
       // every lane adds its own key's share: the lanes of a key carry it PART times
       l[g] = l[g] * keep + pr;
