@@ -283,9 +283,13 @@ typedef struct {
 /* Lengths on the device: seq_lens[b] = min(seq_lens[b] + n_b, limit) and
  * seen[b] += n_b (seen, the tokens a sequence has had so far, may be NULL),
  * with n_b = row_start[b + 1] - row_start[b], or `add` when row_start is
- * NULL.  Before a step: add 1 with limit max_pages * page_size (a sequence
- * that would pass the limit sets bit 2 of the device error word); after an
- * eviction: add 0 with limit `budget`. */
+ * NULL.  Before rows are appended: limit INT32_MAX.  A sequence may then count
+ * more tokens than its pages hold: the append leaves out the rows that have no
+ * slot, the attention reads the full cache, each sets bit 2 of the device
+ * error word, and an eviction brings the length back.  (A limit that cuts
+ * the new rows off, which sets the bit here, moves them onto the last slots
+ * below it, which hold tokens: tkb_kv_append counts back from seq_lens.)  After
+ * an eviction: add 0 with limit `budget`. */
 int tkb_kv_lens(int32_t *seq_lens, int32_t *seen, const int32_t *row_start, int add, int limit, int B, void *stream);
 
 /* New tokens enter the cache.  Packed rows qkv [rows][(Hq + 2*Hkv)*D]
@@ -299,7 +303,8 @@ int tkb_kv_lens(int32_t *seq_lens, int32_t *seen, const int32_t *row_start, int 
  * (where present).  out (may be NULL) gets the prepared row: its Hq*D query
  * columns, or with out_full the whole packed row, as tkb_gqa_attn_fwd and
  * tkb_paged_attn_decode take it.  Rows that have no slot (n_b > seq_lens[b],
- * a bad page) set bit 2 of the device error word; their out is written. */
+ * a slot past max_pages * page_size, a bad page) are not stored and set bit 2
+ * of the device error word; their out is written. */
 int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stride, const float *bias,
                   const float *qk_gain, void *out, long long out_stride, int out_full, const int32_t *row_start,
                   const int32_t *seen, int rows, int Hq, int has_qknorm, int has_rope, float theta,

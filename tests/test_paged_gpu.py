@@ -521,3 +521,54 @@ def test_decode_nan_is_not_an_empty_cache(dtype):
         for got, want in zip((out.view(5, Hq, D), lse), (good[0].view(5, Hq, D), good[1])):
             assert torch.equal(got[~bad], want[~bad])
         assert (out[1] == 0).all() and torch.isneginf(lse[1]).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float32)])
+def test_rows_past_the_capacity_are_left_out(D, dtype):
+    """Sequences that grow past their last page: what is held stays, the rows that fit are written, the others set
+    bit 2; the attention then sees the full cache."""
+    Hq, Hkv, page = 4, 2, 16
+    held, fresh = [30, 32, 31, 5, 30, 32], [5, 1, 1, 2, 50, 40]
+    c = Cache(dtype, held, Hkv, D, page).fill(held)
+    cap = c.handle.capacity
+    assert cap == 32
+    k0, v0, pos0, w0 = num(c.k), num(c.v), c.pos.cpu().numpy().copy(), num(c.weight)
+    seen = torch.tensor([h + 1000 for h in held], dtype=torch.int32, device="cuda")
+    start = torch.tensor(np.concatenate(([0], np.cumsum(fresh))), dtype=torch.int32, device="cuda")
+    C = (Hq + 2 * Hkv) * D
+    rows = c.randn(sum(fresh), C, dtype=dtype)
+    ops().kv_lens(c.lens, seen=seen, row_start=start)
+    out = ops().kv_append(c.handle, rows, Hq, seen=seen, row_start=start, rope=False)
+    assert device_error() == 4
+    assert torch.equal(out, rows[:, :Hq * D])
+    table, x = c.table.cpu().numpy(), num(rows).reshape(-1, Hq + 2 * Hkv, D)
+    for b in range(len(held)):
+        for i in range(fresh[b]):
+            j = held[b] + i
+            if j < cap:
+                at = table[b, j // page], slice(None), j % page
+                k0[at], v0[at] = x[int(start[b]) + i, Hq:Hq + Hkv], x[int(start[b]) + i, Hq + Hkv:]
+                pos0[at], w0[at] = j + 1000, 0
+    for got, want in ((num(c.k), k0), (num(c.v), v0), (num(c.weight), w0)):
+        assert np.array_equal(got, want, equal_nan=True)
+    assert np.array_equal(c.pos.cpu().numpy(), pos0)
+    # and one token more for every sequence, of which one still has room
+    before = [t.clone() for t in (c.k, c.v, c.pos)]
+    ops().kv_lens(c.lens, seen=seen, add=1)
+    one = c.randn(len(held), C, dtype=dtype)
+    ops().kv_append(c.handle, one, Hq, seen=seen, rope=False)
+    assert device_error() == 4
+    at = int(c.table[3, 0]), slice(None), 7
+    for t, was, part in ((c.k, before[0], one[3, Hq * D:(Hq + Hkv) * D]), (c.v, before[1], one[3, (Hq + Hkv) * D:])):
+        was[at] = part.view(Hkv, D)
+        assert torch.equal(t.isnan(), was.isnan()) and torch.equal(t.nan_to_num(), was.nan_to_num())
+    before[2][at] = 1007
+    assert torch.equal(c.pos, before[2])
+    q = c.randn(len(held), Hq * D, dtype=dtype)
+    out, lse = ops().paged_attn_decode(c.handle, q, Hq)
+    assert device_error() == 4
+    check_attention(c, q, Hq, [cap, cap, cap, 8, cap, cap], out, lse, dtype)
+    # an eviction brings the lengths back below the budget
+    ops().kv_evict(c.handle, 16, seen, recent=4)
+    ops().kv_lens(c.lens, 16)
+    assert device_error() == 4 and c.lens.tolist() == [16, 16, 16, 8, 16, 16]

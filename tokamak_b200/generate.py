@@ -126,7 +126,7 @@ class Generator:
         tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.int64, device=dev)
         self.lens.zero_()
         self.seen.zero_()
-        ops.kv_lens(self.lens, self.caches[0].capacity, seen=self.seen, row_start=row_start)
+        ops.kv_lens(self.lens, seen=self.seen, row_start=row_start)
         self.held = list(n)
 
         def attend(i, qkv):
@@ -143,7 +143,7 @@ class Generator:
 
     def decode(self):
         """One step: the tokens in self.token enter the caches; returns the next logits [batch, vocab]."""
-        ops.kv_lens(self.lens, self.caches[0].capacity, seen=self.seen, add=1)
+        ops.kv_lens(self.lens, seen=self.seen, add=1)
 
         def attend(i, qkv):
             q = self._append(i, qkv)

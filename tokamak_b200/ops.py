@@ -276,13 +276,15 @@ class KVCache:
         return self.max_pages * self.page_size
 
 
-def kv_lens(seq_lens, limit, seen=None, add=0, row_start=None):
-    """seq_lens = min(seq_lens + n, limit) and seen += n, on the device (n = add, or row_start's differences)."""
+def kv_lens(seq_lens, limit=None, seen=None, add=0, row_start=None):
+    """seq_lens = min(seq_lens + n, limit) and seen += n, on the device (n = add, or row_start's differences).
+    No limit before rows are appended (kv_append leaves out those past the capacity); the budget after an eviction."""
     B = seq_lens.numel()
     _vec(seq_lens, "seq_lens", B, torch.int32)
     _vec(seen, "seen", B, torch.int32)
     _vec(row_start, "row_start", B + 1, torch.int32)
-    check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add), int(limit), B, _raw_stream(seq_lens)),
+    check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add),
+                            0x7FFFFFFF if limit is None else int(limit), B, _raw_stream(seq_lens)),
           "tkb_kv_lens")
 
 
