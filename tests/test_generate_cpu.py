@@ -136,3 +136,41 @@ def test_python_checks():
         ops.kv_lens(lens.long(), 4)
     with pytest.raises(TkbError):
         ops.kv_lens(lens, 4, row_start=lens)
+
+
+def test_tensors_of_the_host_are_refused():
+    """Right in shape and type, but on the host: an error here instead of a kernel that reads host addresses."""
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, ops
+    k = torch.zeros(4, 2, 16, 64)
+    meta = dict(pos=torch.zeros(4, 2, 16, dtype=torch.int32), weight=torch.zeros(4, 2, 16))
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    c = ops.KVCache(k, k.clone(), table, lens, **meta)
+    calls = [lambda: ops.kv_lens(lens, add=1), lambda: ops.kv_append(c, torch.zeros(2, 8 * 64), 4, seen=lens),
+             lambda: ops.paged_attn_decode(c, torch.zeros(2, 4 * 64), 4), lambda: ops.kv_evict(c, 8, lens),
+             lambda: ops.sample_logits(torch.zeros(2, 8), torch.zeros(2))]
+    for call in calls:
+        with pytest.raises(TkbError, match="CUDA device"):
+            call()
+    with pytest.raises(TkbError, match="expected all tensors on cpu"):
+        ops.KVCache(k, k.clone(), table, lens.to("meta"), **meta)
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    """One tensor on another device than the first, or all on another than the current one."""
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, ops
+
+    class On:
+        def __init__(self, i):
+            self.i, self.device = i, f"cuda:{i}" if i >= 0 else "cpu"
+
+        def get_device(self):
+            return self.i
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 70 + dev, raising=False)
+    assert ops._launch_stream("call", On(1), None, On(1)) == 71
+    for tensors in ((On(0), On(0)), (On(1), On(0)), (On(1), None, On(-1)), (On(-1), On(1))):
+        with pytest.raises(TkbError, match="call"):
+            ops._launch_stream("call", *tensors)

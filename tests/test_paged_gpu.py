@@ -572,3 +572,28 @@ def test_rows_past_the_capacity_are_left_out(D, dtype):
     ops().kv_evict(c.handle, 16, seen, recent=4)
     ops().kv_lens(c.lens, 16)
     assert device_error() == 4 and c.lens.tolist() == [16, 16, 16, 8, 16, 16]
+
+
+def test_a_host_tensor_among_device_tensors_is_refused():
+    from tokamak_b200 import TkbError
+    c = Cache(torch.bfloat16, [5, 9], 2, 64, 16).fill([5, 9])
+    q, rows = c.randn(2, 4 * 64, dtype=torch.bfloat16), c.randn(2, 8 * 64, dtype=torch.bfloat16)
+    seen = c.lens.clone()
+    o = ops()
+    ws, ews = o.paged_attn_workspace(c.handle, 4), o.kv_evict_workspace(c.handle)
+    for call in (lambda: o.kv_lens(c.lens, seen=seen.cpu(), add=1), lambda: o.kv_append(c.handle, rows.cpu(), 4),
+                 lambda: o.kv_append(c.handle, rows, 4, seen=seen.cpu()),
+                 lambda: o.kv_append(c.handle, rows, 4, bias=torch.zeros(8 * 64)),
+                 lambda: o.kv_append(c.handle, rows, 4, row_start=torch.tensor([0, 1, 2], dtype=torch.int32)),
+                 lambda: o.kv_append(c.handle, rows, 4, out=q.cpu()),
+                 lambda: o.paged_attn_decode(c.handle, q.cpu(), 4, out=q.clone()),
+                 lambda: o.paged_attn_decode(c.handle, q, 4, lse=torch.zeros(2, 4)),
+                 lambda: o.paged_attn_decode(c.handle, q, 4, workspace=ws.cpu()),
+                 lambda: o.kv_evict(c.handle, 4, seen.cpu()), lambda: o.kv_evict(c.handle, 4, seen, workspace=ews.cpu()),
+                 lambda: o.sample_logits(q, torch.zeros(2)),
+                 lambda: o.sample_logits(q, torch.zeros(2, device="cuda"), top_p=torch.ones(2)),
+                 lambda: o.KVCache(c.k, c.v, c.table, c.lens.cpu())):
+        with pytest.raises(TkbError, match="expected"):
+            call()
+    out, lse = o.paged_attn_decode(c.handle, q, 4, workspace=ws)
+    check_attention(c, q, 4, [5, 9], out, lse, torch.bfloat16)

@@ -28,11 +28,6 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _raw_stream(t):
-    """The current stream of t's device as an integer (0.2 us; the Stream object of _stream costs 3.4)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index) if t.is_cuda else 0
-
-
 def _ws(nbytes, device):
     if nbytes == 0:
         return None, 0
@@ -243,6 +238,18 @@ def _vec(t, name, n, dtype):
         raise TkbError(f"{name}: expected {n} contiguous {dtype}, got {t.dtype} {tuple(t.shape)}")
 
 
+def _launch_stream(who, first, *others):
+    """The current stream as an integer (0.2 us; the Stream object of _stream costs 3.4), once all tensors given are
+    found on the current CUDA device: a kernel would take any other address for its own memory."""
+    dev = first.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise TkbError(f"{who}: expected tensors on the current CUDA device, got one on {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise TkbError(f"{who}: expected all tensors on {first.device}, got one on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 class KVCache:
     """One attention layer's paged key-value cache (tkb_kv_cache): tensors
     k, v [n_pages, Hkv, page_size, D] (any page stride, the rest contiguous),
@@ -261,6 +268,9 @@ class KVCache:
         _expect(seq_lens, "seq_lens", (B,), torch.int32)
         _expect(pos, "pos", (n_pages, Hkv, page), torch.int32)
         _expect(weight, "weight", (n_pages, Hkv, page), torch.float32)
+        for t in (v, block_table, seq_lens, pos, weight):
+            if t is not None and t.device != k.device:
+                raise TkbError(f"KVCache: expected all tensors on {k.device}, got one on {t.device}")
         self.k, self.v, self.block_table, self.seq_lens, self.pos, self.weight = k, v, block_table, seq_lens, pos, weight
         self.B, self.Hkv, self.D, self.page_size, self.max_pages = B, Hkv, D, page, max_pages
         # a single page has no stride of its own
@@ -283,8 +293,9 @@ def kv_lens(seq_lens, limit=None, seen=None, add=0, row_start=None):
     _vec(seq_lens, "seq_lens", B, torch.int32)
     _vec(seen, "seen", B, torch.int32)
     _vec(row_start, "row_start", B + 1, torch.int32)
+    stream = _launch_stream("kv_lens", seq_lens, seen, row_start)
     check(lib().tkb_kv_lens(seq_lens.data_ptr(), _ptr(seen), _ptr(row_start), int(add),
-                            0x7FFFFFFF if limit is None else int(limit), B, _raw_stream(seq_lens)),
+                            0x7FFFFFFF if limit is None else int(limit), B, stream),
           "tkb_kv_lens")
 
 
@@ -307,9 +318,10 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
         out = torch.empty(rows, width, dtype=qkv.dtype, device=qkv.device)
     elif out.shape != (rows, width) or out.dtype != qkv.dtype or out.stride(1) != 1:
         raise TkbError(f"kv_append: out is {out.dtype} {tuple(out.shape)}, not {qkv.dtype} {(rows, width)}")
+    stream = _launch_stream("kv_append", cache.k, qkv, bias, qk_gain, out, row_start, seen)
     check(lib().tkb_kv_append(cache.ref, _ptr(qkv), qkv.stride(0), _ptr(bias), _ptr(qk_gain), _ptr(out), out.stride(0),
                               int(full), _ptr(row_start), _ptr(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
-                              low, high, octx, _raw_stream(qkv)), "tkb_kv_append")
+                              low, high, octx, stream), "tkb_kv_append")
     return out
 
 
@@ -339,9 +351,10 @@ def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=
         _vec(lse, "lse", cache.B * Hq, torch.float32)
     if workspace is None:
         workspace = paged_attn_workspace(cache, Hq, accumulate)
+    stream = _launch_stream("paged_attn_decode", cache.k, q, out, lse, workspace)
     check(lib().tkb_paged_attn_decode(cache.ref, _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(lse), Hq,
                                       cache.D ** -0.5 if scale is None else scale, int(accumulate), _ptr(workspace),
-                                      workspace.numel(), _raw_stream(q)), "tkb_paged_attn_decode")
+                                      workspace.numel(), stream), "tkb_paged_attn_decode")
     return out, lse
 
 
@@ -358,8 +371,9 @@ def kv_evict(cache, budget, seen, recent=0, sinks=0, workspace=None):
     _vec(seen, "seen", cache.B, torch.int32)
     if workspace is None:
         workspace = kv_evict_workspace(cache)
+    stream = _launch_stream("kv_evict", cache.k, seen, workspace)
     check(lib().tkb_kv_evict(cache.ref, _ptr(seen), int(budget), int(recent), int(sinks), _ptr(workspace),
-                             workspace.numel(), _raw_stream(seen)), "tkb_kv_evict")
+                             workspace.numel(), stream), "tkb_kv_evict")
 
 
 def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
@@ -371,10 +385,11 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
                         (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
         _expect(t, name, (rows,), dt)
+    stream = _launch_stream("sample_logits", logits, u, temperature, top_k, top_p, min_p)
     logprob = torch.empty_like(u)
     token = torch.empty_like(u, dtype=torch.int32)
     kept = torch.empty_like(token)
     check(lib().tkb_sample_logits(_ptr(logits), logits.stride(0) if rows > 1 else V, _ptr(u), _ptr(temperature),
                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(logprob), _ptr(kept), rows, V,
-                                  dtype_code(logits), _raw_stream(logits)), "tkb_sample_logits")
+                                  dtype_code(logits), stream), "tkb_sample_logits")
     return token, logprob, kept
