@@ -102,3 +102,59 @@ def test_refusals():
         gen.prefill([[]])
     with pytest.raises(TkbError):
         gen.generate([[1] * 60], 10)
+
+
+@pytest.mark.parametrize("prompts", [(90, 40), (64, 90), (90, 3)])
+def test_a_long_prompt_is_cut_by_its_own_attention(prompts):
+    """A prompt longer than the budget is weighed by the attention of its last `window` tokens, each over the tokens up
+    to itself, and the first cut keeps the heaviest wherever they lie."""
+    from oracle import paged_oracle as ref
+    from tokamak_b200 import generate
+    cfg = make(gqa=True)
+    rng = np.random.default_rng(6)
+    embed = rng.standard_normal((cfg["vocab"], cfg["d_model"])).astype(np.float32)
+    budget, recent, sinks, window, page = 48, 10, 2, 7, 16
+    gen = generate.Generator(cfg, weights(cfg), embed, 2, 96, page_size=page, budget=budget, slack=16, recent=recent,
+                             sinks=sinks, window=window)
+    seen_rows = []
+    append = gen._append
+
+    def record(i, qkv, **more):
+        out = append(i, qkv, **more)
+        seen_rows.append(out.double().cpu().numpy())
+        return out
+
+    gen._append = record
+    tokens = [rng.integers(0, cfg["vocab"], n).tolist() for n in prompts]
+    gen.prefill(tokens)
+    Hq, Hkv, D = cfg["q_heads"], cfg["kv_heads"], cfg["head_dim"]
+    G, start = Hq // Hkv, np.concatenate(([0], np.cumsum(prompts)))
+    want = {}
+    for layer, rows in enumerate(seen_rows):
+        table = gen.table.cpu().numpy()
+        got = gen.caches[layer].weight.double().cpu().numpy()
+        pos = gen.caches[layer].pos.cpu().numpy()
+        for b, n in enumerate(prompts):
+            x = rows[start[b]:start[b + 1]].reshape(n, Hq + 2 * Hkv, D)
+            for h in range(Hkv):
+                w = np.zeros(n)
+                for i in range(max(0, n - window), n):
+                    for g in range(G):
+                        s = x[:i + 1, Hq + h] @ x[i, h * G + g] * D ** -0.5
+                        e = np.exp(s - s.max())
+                        w[:i + 1] += e / e.sum()
+                have = np.array([got[table[b, j // page], h, j % page] for j in range(n)])
+                # fp32 softmax of bf16 rows that both sides share: the bound of the decode attention's weights
+                assert rel_l2(have, w) < 2e-5
+                at = [pos[table[b, j // page], h, j % page] for j in range(n)]
+                moves = ref.evict_moves(have, at, n, budget, n, recent, sinks)
+                kept = set(range(min(n, budget))) - {m[0] for m in moves} | {m[1] for m in moves}
+                want[layer, b, h] = {at[j] for j in kept}
+    gen.evict()
+    for (layer, b, h), kept in want.items():
+        c = gen.caches[layer]
+        n = min(prompts[b], budget)
+        pos = c.pos[c.block_table[b].long(), h].flatten()[:n].tolist()
+        assert set(pos) == kept
+        if prompts[b] > budget:  # not merely the first ones and the newest
+            assert kept != set(range(budget - recent)) | set(range(prompts[b] - recent, prompts[b]))
