@@ -174,3 +174,26 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     for tensors in ((On(0), On(0)), (On(1), On(0)), (On(1), None, On(-1)), (On(-1), On(1))):
         with pytest.raises(TkbError, match="call"):
             ops._launch_stream("call", *tensors)
+
+
+def small_generator(**more):
+    """A generator whose tensors stay on the host: for what it refuses before it computes anything."""
+    pytest.importorskip("torch")
+    import numpy as np
+    from tokamak_b200 import configs, generate
+    cfg = dict(configs.C1, layers=1)
+    embed = more.pop("embed", np.zeros((cfg["vocab"], cfg["d_model"]), np.float32))
+    return cfg, generate.Generator(cfg, generate.random_checkpoint(cfg), embed, 2, 64, device="cpu", **more)
+
+
+def test_generator_refuses_token_ids_outside_the_vocabulary():
+    """Before the look-up, which would be an assertion on the device."""
+    import numpy as np
+    from tokamak_b200 import TkbError
+    cfg, gen = small_generator()
+    for bad in (cfg["vocab"], -1, 1 << 40):
+        with pytest.raises(TkbError, match="token ids"):
+            gen.prefill([[1, 2], [3, bad]])
+    for shape in ((cfg["vocab"] - 1, cfg["d_model"]), (cfg["vocab"], cfg["d_model"] + 1), (cfg["vocab"] * cfg["d_model"],)):
+        with pytest.raises(TkbError, match="embed"):
+            small_generator(embed=np.zeros(shape, np.float32))
