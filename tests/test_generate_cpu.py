@@ -197,3 +197,11 @@ def test_generator_refuses_token_ids_outside_the_vocabulary():
     for shape in ((cfg["vocab"] - 1, cfg["d_model"]), (cfg["vocab"], cfg["d_model"] + 1), (cfg["vocab"] * cfg["d_model"],)):
         with pytest.raises(TkbError, match="embed"):
             small_generator(embed=np.zeros(shape, np.float32))
+
+
+def test_generator_refuses_a_budget_without_room_at_once():
+    """recent + sinks above the budget: known before the first token, not at the first cut."""
+    from tokamak_b200 import TkbError
+    _, gen = small_generator(budget=8, slack=8, recent=6, sinks=4)
+    with pytest.raises(TkbError, match="recent"):
+        gen.generate([[1] * 10, [2]], 8)   # 16 tokens are held before the eighth

@@ -158,3 +158,10 @@ def test_a_long_prompt_is_cut_by_its_own_attention(prompts):
         assert set(pos) == kept
         if prompts[b] > budget:  # not merely the first ones and the newest
             assert kept != set(range(budget - recent)) | set(range(prompts[b] - recent, prompts[b]))
+
+
+@pytest.mark.parametrize("budget", [1, 16, 40])
+def test_command_with_a_small_budget(budget):
+    """The command goes past its first cut whatever the budget."""
+    from tokamak_b200 import generate
+    generate.main(["--steps", "90", "--batch", "2", "--prompt", "20", "--budget", str(budget)])

@@ -200,6 +200,9 @@ class Generator:
             raise TkbError("generate: more tokens than max_tokens and no budget")
         if self.budget and self.budget + self.slack > self.max_tokens:
             raise TkbError("generate: max_tokens must hold budget + slack tokens")
+        if self.budget and self.recent + self.sinks > self.budget and \
+                max(len(p) for p in prompts) + steps - 2 >= self.budget + self.slack:
+            raise TkbError("generate: the budget must hold recent + sinks tokens")
         full = lambda v, dt: torch.full((B,), v, dtype=dt, device=dev)  # noqa: E731
         sampling = dict(temperature=full(temperature, torch.float32), top_k=full(top_k, torch.int32) if top_k else None,
                         top_p=full(top_p, torch.float32) if top_p < 1 else None,
@@ -256,7 +259,9 @@ def main(argv=None):
     rng = np.random.default_rng(a.seed)
     embed = rng.standard_normal((cfg["vocab"], cfg["d_model"]), dtype=np.float32)
     most = max(a.prompt, a.budget + 64) if a.budget else a.prompt + a.steps
-    gen = Generator(cfg, weights, embed, a.batch, most, budget=a.budget)
+    # protected tokens that a small budget has room for
+    recent = 32 if a.budget >= 36 else a.budget // 2
+    gen = Generator(cfg, weights, embed, a.batch, most, budget=a.budget, recent=recent, sinks=min(4, a.budget - recent))
     prompts = [rng.integers(0, cfg["vocab"], a.prompt).tolist() for _ in range(a.batch)]
     options = dict(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p)
     gen.generate(prompts, min(4, a.steps), **options)  # warm-up
