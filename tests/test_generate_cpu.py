@@ -205,3 +205,15 @@ def test_generator_refuses_a_budget_without_room_at_once():
     _, gen = small_generator(budget=8, slack=8, recent=6, sinks=4)
     with pytest.raises(TkbError, match="recent"):
         gen.generate([[1] * 10, [2]], 8)   # 16 tokens are held before the eighth
+
+
+def test_prompts_of_the_command(tmp_path):
+    pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, generate
+    path = tmp_path / "prompts.txt"
+    path.write_text("1 2 3\n\n  7\n")
+    assert generate.read_prompts(path) == [[1, 2, 3], [7]]
+    for bad in ("1 two\n", "\n"):
+        path.write_text(bad)
+        with pytest.raises(TkbError):
+            generate.read_prompts(path)

@@ -165,3 +165,20 @@ def test_command_with_a_small_budget(budget):
     """The command goes past its first cut whatever the budget."""
     from tokamak_b200 import generate
     generate.main(["--steps", "90", "--batch", "2", "--prompt", "20", "--budget", str(budget)])
+
+
+def test_command_runs_a_given_model(tmp_path, capsys):
+    """Checkpoint, embedding and prompts from files: the tokens of a Generator on the same."""
+    from tokamak_b200 import configs, generate, runtime
+    cfg = configs.C1
+    ckpt = weights(cfg)
+    embed = np.random.default_rng(8).standard_normal((cfg["vocab"], cfg["d_model"])).astype(np.float32)
+    prompts = [[5, 6, 7, 8], [9], list(range(40))]
+    (tmp_path / "model.tkmw").write_bytes(runtime.tkm1_pack(ckpt))
+    np.save(tmp_path / "table.npy", embed)
+    (tmp_path / "prompts.txt").write_text("\n".join(" ".join(map(str, p)) for p in prompts))
+    generate.main(["--checkpoint", str(tmp_path / "model.tkmw"), "--embedding", str(tmp_path / "table.npy"), "--tokens",
+                   str(tmp_path / "prompts.txt"), "--steps", "10", "--temperature", "0"])
+    lines = [[int(t) for t in row.split()] for row in capsys.readouterr().out.splitlines()[-3:]]
+    want = generate.Generator(cfg, ckpt, embed, 3, 64).generate(prompts, 10, temperature=0.0)
+    assert lines == want.tolist()

@@ -2,12 +2,14 @@
 key-value cache: prompts in one pass, then one token per sequence and step,
 the step captured as a CUDA graph.
 
-    python -m tokamak_b200.generate [--config C1|C4] [--checkpoint model.tkmw]
-        [--batch 8] [--prompt 100] [--steps 64] [--budget 0] [--top-k 50] [--top-p 0.95] [--temperature 0.8]
+    python -m tokamak_b200.generate [--config C1|C4] [--checkpoint model.tkmw] [--embedding table.npy]
+        [--tokens prompts.txt | --batch 8 --prompt 100] [--steps 64] [--budget 0] [--top-k 50] [--top-p 0.95]
+        [--temperature 0.8]
 
 Weights come from a TKM1 checkpoint that the engine trained on the same
-configuration (random ones without it); the embedding table, which the engine
-takes as its input rows, from the caller.  Kernels: tkb_add_rmsnorm_fwd,
+configuration; the embedding table [vocab, d_model], which the engine takes as
+its input rows, from the caller; prompts as token ids, one prompt a line.
+Each is random where it is not given.  Kernels: tkb_add_rmsnorm_fwd,
 tkb_gemm, tkb_gemm_swiglu, tkb_gqa_attn_fwd (prompts), tkb_kv_append,
 tkb_paged_attn_decode, tkb_kv_evict, tkb_sample_logits.  torch only holds the
 tensors and looks embeddings up.
@@ -232,6 +234,18 @@ class Generator:
         return out.t()
 
 
+def read_prompts(path):
+    """Lists of token ids from a text file, one prompt a line, empty lines left out."""
+    with open(path) as f:
+        try:
+            prompts = [[int(t) for t in line.split()] for line in f if line.strip()]
+        except ValueError as e:
+            raise TkbError(f"{path}: {e}")
+    if not prompts:
+        raise TkbError(f"{path}: no prompts")
+    return prompts
+
+
 def main(argv=None):
     import argparse
     import time
@@ -240,6 +254,8 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description="Generate tokens with a decoder of tokamak_b200.configs.")
     ap.add_argument("--config", default="C1", choices=("C1", "C4"))
     ap.add_argument("--checkpoint", help="TKM1 file of that configuration (default: random weights)")
+    ap.add_argument("--embedding", help=".npy file of the embedding table [vocab, d_model] (default: a random one)")
+    ap.add_argument("--tokens", help="text file of prompts, token ids, one prompt a line (default: random ones)")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--prompt", type=int, default=100, help="tokens per (random) prompt")
     ap.add_argument("--steps", type=int, default=64)
@@ -257,12 +273,19 @@ def main(argv=None):
     else:
         weights = random_checkpoint(cfg, a.seed)
     rng = np.random.default_rng(a.seed)
-    embed = rng.standard_normal((cfg["vocab"], cfg["d_model"]), dtype=np.float32)
-    most = max(a.prompt, a.budget + 64) if a.budget else a.prompt + a.steps
+    if a.embedding:
+        embed = np.load(a.embedding)
+    else:
+        embed = rng.standard_normal((cfg["vocab"], cfg["d_model"]), dtype=np.float32)
+    if a.tokens:
+        prompts = read_prompts(a.tokens)
+    else:
+        prompts = [rng.integers(0, cfg["vocab"], a.prompt).tolist() for _ in range(a.batch)]
+    batch, longest = len(prompts), max(map(len, prompts))
+    most = max(longest, a.budget + 64) if a.budget else longest + a.steps
     # protected tokens that a small budget has room for
     recent = 32 if a.budget >= 36 else a.budget // 2
-    gen = Generator(cfg, weights, embed, a.batch, most, budget=a.budget, recent=recent, sinks=min(4, a.budget - recent))
-    prompts = [rng.integers(0, cfg["vocab"], a.prompt).tolist() for _ in range(a.batch)]
+    gen = Generator(cfg, weights, embed, batch, most, budget=a.budget, recent=recent, sinks=min(4, a.budget - recent))
     options = dict(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p)
     gen.generate(prompts, min(4, a.steps), **options)  # warm-up
     g = torch.Generator(device="cuda").manual_seed(a.seed)
@@ -270,8 +293,12 @@ def main(argv=None):
     t = time.perf_counter()
     tokens = gen.generate(prompts, a.steps, generator=g, **options).cpu()
     t = time.perf_counter() - t
-    print(f"{a.config}: {a.batch} x {a.steps} tokens in {t * 1e3:.1f} ms ({a.batch * a.steps / t:.0f} tokens/s, prompts included)")
-    print("first sequence:", tokens[0].tolist())
+    print(f"{a.config}: {batch} x {a.steps} tokens in {t * 1e3:.1f} ms ({batch * a.steps / t:.0f} tokens/s, prompts included)")
+    if a.tokens:  # one line for each prompt's
+        for row in tokens.tolist():
+            print(*row)
+    else:
+        print("first sequence:", tokens[0].tolist())
 
 
 if __name__ == "__main__":
