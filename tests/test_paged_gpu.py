@@ -597,3 +597,29 @@ def test_a_host_tensor_among_device_tensors_is_refused():
             call()
     out, lse = o.paged_attn_decode(c.handle, q, 4, workspace=ws)
     check_attention(c, q, 4, [5, 9], out, lse, torch.bfloat16)
+
+
+def test_strides_of_single_rows_heads_and_pages_mean_nothing():
+    """torch gives a dimension of size one any stride: one sequence's rows, one kv head, one page, one token's logits."""
+    lens, D, page = [11], 64, 16
+    c = Cache(torch.bfloat16, lens, 1, D, page, extra=0).fill(lens)
+    odd = [torch.empty(page * D + 8, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, page, D), s)
+           for s in ((24, 3, D, 1), (7, 5, D, 1))]
+    for t, src in zip(odd, (c.k, c.v)):
+        t.copy_(src)
+    cache = ops().KVCache(*odd, c.table, c.lens, pos=c.pos, weight=c.weight)
+    rows = c.randn(1, 4 * D, dtype=torch.bfloat16)
+    same = rows.as_strided(rows.shape, (1, 1))
+    want = ops().kv_append(c.handle, rows, 2)
+    room = torch.empty_like(want)
+    got = ops().kv_append(cache, same, 2, out=room.as_strided(room.shape, (3, 1)))
+    assert torch.equal(want, room) and torch.equal(got, room)
+    for t, src in zip(odd, (c.k, c.v)):  # the slots past the length are NaN in both
+        assert np.array_equal(num(t), num(src), equal_nan=True)
+    want, lse = ops().paged_attn_decode(c.handle, room, 2)
+    out = torch.empty_like(want)
+    _, lse2 = ops().paged_attn_decode(cache, got, 2, out=out.as_strided(out.shape, (1, 1)))
+    assert torch.equal(out, want) and torch.equal(lse, lse2)
+    token, _, kept = ops().sample_logits(torch.zeros(6, 2, device="cuda")[:, ::2].as_strided((3, 1), (2, 9)),
+                                         torch.zeros(3, device="cuda"))
+    assert token.tolist() == [0, 0, 0] and kept.tolist() == [1, 1, 1] and device_error() == 0

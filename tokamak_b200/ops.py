@@ -238,6 +238,11 @@ def _vec(t, name, n, dtype):
         raise TkbError(f"{name}: expected {n} contiguous {dtype}, got {t.dtype} {tuple(t.shape)}")
 
 
+def _row_stride(t, width):
+    """Elements from row to row of [rows, width]; a single row's stride means nothing."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
 def _launch_stream(who, first, *others):
     """The current stream as an integer (0.2 us; the Stream object of _stream costs 3.4), once all tensors given are
     found on the current CUDA device: a kernel would take any other address for its own memory."""
@@ -261,7 +266,8 @@ class KVCache:
         B, max_pages = block_table.shape
         for t, name in ((k, "k"), (v, "v")):
             if tuple(t.shape) != (n_pages, Hkv, page, D) or t.dtype != k.dtype or \
-                    t.stride()[1:] != (page * D, D, 1) or t.stride(0) != k.stride(0):
+                    t.stride()[2:] != (D, 1) or (Hkv > 1 and t.stride(1) != page * D) or \
+                    (n_pages > 1 and t.stride(0) != k.stride(0)):
                 raise TkbError(f"{name}: expected {k.dtype} [n_pages, Hkv, page_size, D], contiguous within a page, "
                                "k and v with the same page stride")
         _expect(block_table, "block_table", (B, max_pages), torch.int32)
@@ -319,9 +325,9 @@ def kv_append(cache, qkv, Hq, seen=None, row_start=None, bias=None, qk_gain=None
     elif out.shape != (rows, width) or out.dtype != qkv.dtype or out.stride(1) != 1:
         raise TkbError(f"kv_append: out is {out.dtype} {tuple(out.shape)}, not {qkv.dtype} {(rows, width)}")
     stream = _launch_stream("kv_append", cache.k, qkv, bias, qk_gain, out, row_start, seen)
-    check(lib().tkb_kv_append(cache.ref, _ptr(qkv), qkv.stride(0), _ptr(bias), _ptr(qk_gain), _ptr(out), out.stride(0),
-                              int(full), _ptr(row_start), _ptr(seen), rows, Hq, int(qknorm), int(rope), theta, rope_scale,
-                              low, high, octx, stream), "tkb_kv_append")
+    check(lib().tkb_kv_append(cache.ref, _ptr(qkv), _row_stride(qkv, C), _ptr(bias), _ptr(qk_gain), _ptr(out),
+                              _row_stride(out, width), int(full), _ptr(row_start), _ptr(seen), rows, Hq, int(qknorm),
+                              int(rope), theta, rope_scale, low, high, octx, stream), "tkb_kv_append")
     return out
 
 
@@ -352,9 +358,10 @@ def paged_attn_decode(cache, q, Hq, scale=None, accumulate=False, out=None, lse=
     if workspace is None:
         workspace = paged_attn_workspace(cache, Hq, accumulate)
     stream = _launch_stream("paged_attn_decode", cache.k, q, out, lse, workspace)
-    check(lib().tkb_paged_attn_decode(cache.ref, _ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(lse), Hq,
-                                      cache.D ** -0.5 if scale is None else scale, int(accumulate), _ptr(workspace),
-                                      workspace.numel(), stream), "tkb_paged_attn_decode")
+    width = Hq * cache.D
+    check(lib().tkb_paged_attn_decode(cache.ref, _ptr(q), _row_stride(q, width), _ptr(out), _row_stride(out, width),
+                                      _ptr(lse), Hq, cache.D ** -0.5 if scale is None else scale, int(accumulate),
+                                      _ptr(workspace), workspace.numel(), stream), "tkb_paged_attn_decode")
     return out, lse
 
 
@@ -380,7 +387,7 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     """(token int32, logprob fp32, kept int32) per row of logits [rows, V] from uniform numbers u [rows]
     (tkb_sample_logits); the parameters are per-row tensors (top_k int32, the others fp32) or None."""
     rows, V = logits.shape
-    if logits.stride(1) != 1:
+    if V > 1 and logits.stride(1) != 1:
         raise TkbError("sample_logits: a row's logits must be contiguous")
     for t, name, dt in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
                         (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32), (min_p, "min_p", torch.float32)):
@@ -389,7 +396,7 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
     logprob = torch.empty_like(u)
     token = torch.empty_like(u, dtype=torch.int32)
     kept = torch.empty_like(token)
-    check(lib().tkb_sample_logits(_ptr(logits), logits.stride(0) if rows > 1 else V, _ptr(u), _ptr(temperature),
+    check(lib().tkb_sample_logits(_ptr(logits), _row_stride(logits, V), _ptr(u), _ptr(temperature),
                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(logprob), _ptr(kept), rows, V,
                                   dtype_code(logits), stream), "tkb_sample_logits")
     return token, logprob, kept
