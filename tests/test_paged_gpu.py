@@ -623,3 +623,40 @@ def test_strides_of_single_rows_heads_and_pages_mean_nothing():
     token, _, kept = ops().sample_logits(torch.zeros(6, 2, device="cuda")[:, ::2].as_strided((3, 1), (2, 9)),
                                          torch.zeros(3, device="cuda"))
     assert token.tolist() == [0, 0, 0] and kept.tolist() == [1, 1, 1] and device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,G", [(64, 8), (128, 8), (64, 16), (128, 4)])
+def test_decode_rounds_only_the_output(dtype, D, G):
+    """The probabilities are not rounded to the type: the error is the output's own rounding r.  P goes in with 16
+    significant bits or more, so it adds at most 2^-16 of the result's size, and the fp32 sums 1e-5: against r (1.7e-3
+    for bf16, 2.1e-4 for f16) that is sqrt(1 + (2.5e-5 / r)^2) < 1.01.  One rounding of P would add an error of the
+    size of r itself (a factor of about 1.2 to 1.4)."""
+    lens = [1500, 700, 64, 333]
+    c = Cache(dtype, lens, 2, D, 16).fill(lens)
+    q = c.randn(4, 2 * G * D, dtype=dtype)
+    out, _ = ops().paged_attn_decode(c.handle, q, 2 * G)
+    k, v, table = num(c.k), num(c.v), c.table.cpu().numpy()
+    want = np.array([ref.attend(k, v, table[b], n, num(q)[b].reshape(2 * G, D), D ** -0.5)[0].ravel()
+                     for b, n in enumerate(lens)])
+    r = rel_l2(num(torch.from_numpy(want).to(dtype)), want)
+    assert rel_l2(num(out), want) < 1.01 * r
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_decode_of_the_same_inputs_gives_the_same_bits(dtype):
+    """Twice on one workspace and on a fresh one, with calls of other lengths between; nothing is filled again."""
+    lens = [3000, 17, 900, 1]
+    c = Cache(dtype, lens, 2, 128, 16)
+    for t in (c.k, c.v):
+        t.copy_(torch.randn(t.shape, generator=c.g, device="cuda"))
+    q = c.randn(4, 8 * 128, dtype=dtype)
+    ws = ops().paged_attn_workspace(c.handle, 8)
+    first = ops().paged_attn_decode(c.handle, q, 8, workspace=ws)
+    for other in ([1, 1, 1, 1], [0, 0, 0, 0], [3000, 2000, 900, 600]):
+        c.lens.copy_(torch.tensor(other))
+        ops().paged_attn_decode(c.handle, q, 8, workspace=ws)
+    c.lens.copy_(torch.tensor(lens))
+    check_attention(c, q, 8, lens, *first, dtype)
+    for again in (ops().paged_attn_decode(c.handle, q, 8, workspace=ws), ops().paged_attn_decode(c.handle, q, 8)):
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
