@@ -126,8 +126,14 @@ int tkb_swiglu_bwd(const void *dh, const void *gu, const float *bg, const float 
  * 43-70; rule src/tkm_registry.c:688-770).  Row layout as the packed qkv
  * above; position = row % S.  Bias add on every column; QKNorm (per-head
  * RMS over D, eps 1e-5, gain qk_gain[(Hq+Hkv)*D]) and RoPE on the Q and K
- * heads.  RoPE rotates pair i of a head by pos * theta^(-i/D), with the
- * reference's frequency adjustment when rope_scale > 1.
+ * heads.  RoPE rotates pair i of a head by pos * f, f = theta^(-i/D), with the
+ * reference's frequency adjustment when rope_scale > 1: with w = 2 pi / f, f is
+ * divided by rope_scale where w > octx/low_freq_factor, and multiplied by
+ * 1 - t (1 - 1/rope_scale), t = (octx/w - low) / (high - low), where
+ * octx/high_freq_factor <= w <= octx/low.  This ramp runs from the whole
+ * division at octx/high to none at octx/low, the other way round than
+ * Llama 3's published rule, and jumps at both ends: models trained here and
+ * run here agree, weights trained elsewhere with that rule do not.
  * save_istd [rows][Hq+Hkv] (needed with QKNorm). */
 int tkb_qkv_prep_fwd(const void *in, const float *bias, const float *qk_gain, void *out,
                      float *save_istd, int rows, int S, int Hq, int Hkv, int D,
@@ -294,7 +300,8 @@ int tkb_kv_lens(int32_t *seq_lens, int32_t *seen, const int32_t *row_start, int 
 
 /* New tokens enter the cache.  Packed rows qkv [rows][(Hq + 2*Hkv)*D]
  * (qkv_stride elements apart) get tkb_qkv_prep_fwd's bias, QKNorm and RoPE
- * (same parameters), except that the position is the token's own:
+ * (same parameters, its frequency adjustment among them), except that the
+ * position is the token's own:
  * row_start [B + 1] gives the rows of each sequence (NULL: row b belongs to
  * sequence b and rows == B); with n_b rows, row i of sequence b goes to slot
  * seq_lens[b] - n_b + i and stands at position seen[b] - n_b + i (seen NULL:
@@ -317,8 +324,10 @@ int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stri
  * [B] rows of Hq*D (q_stride, out_stride elements apart, 16-byte aligned),
  * lse [B][Hq] fp32 (may be NULL).  A sequence that holds nothing gets out 0
  * and lse -inf.  With `accumulate`, weight[slot] of each kv head also grows by
- * the sum over its query heads of softmax(s)_slot.  The work is cut over the
- * cached lengths and joined in a fixed order: equal inputs give equal bits.
+ * the sum over its query heads of softmax(s)_slot.  NaN in q, k or v reaches
+ * the heads that use it; an infinite v makes their out infinite or NaN.  The
+ * work is cut over the cached lengths and joined in a fixed order: equal
+ * inputs give equal bits.
  * workspace: tkb_paged_attn_decode_workspace bytes, 256-byte aligned, zeroed
  * before its first use; every call leaves it fit for the next one, of any
  * cache and shape that it is large enough for.  Calls that may overlap need

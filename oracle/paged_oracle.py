@@ -10,8 +10,11 @@ import numpy as np
 
 
 def rope_frequencies(D, theta, scale=1.0, low=1.0, high=4.0, octx=8192.0):
-    """Angle per position of each pair of a head, with the wavelengths above
-    octx/low divided by `scale` and those down to octx/high blended."""
+    """Angle per position of each pair of a head.  With scale > 1 the frequencies
+    of wavelengths above octx/low are divided by it, and those of wavelengths
+    from octx/high to octx/low by a ramp from the whole of it (at octx/high) to
+    nothing (at octx/low): the engine's rule, which Llama 3's published one
+    runs the other way round."""
     f = theta ** (-np.arange(D // 2) / D)
     if scale > 1.0:
         for i in range(D // 2):

@@ -23,10 +23,12 @@
 // all the others).  A guess that missed costs another pass, nothing else.
 //
 // Measured (us): one row of 32000 bf16, top-k and top-p: 10; 64 rows of 32000
-// fp32: 13; 512 rows of 131072 bf16, top-p 0.9 (134 MB): 194, bound by issue
-// slots: 48 instructions per logit, 20 of them in the exponential that the sum
-// of all weights needs.  Bitwise searches re-reading the row took 452, 448 and
-// 5482.
+// fp32: 13; 512 rows of 131072 bf16, top-p 0.9 (134 MB): 194.  The last has 48
+// instructions per logit, 20 of them in the exponential that the sum of all
+// weights needs, which issue in 0.61 of the cycles (87 us of them at full
+// rate); most of the rest waits for the vector that a pass has just asked for,
+// and for SMs that have four rows where others have three.  Bitwise searches
+// re-reading the row took 452, 448 and 5482.
 #include "tkb_common.cuh"
 
 namespace tkb {
@@ -336,7 +338,7 @@ struct Sampler {
       for (int i = lane_id(); i < n_list; i += 32) {
         const uint32_t key = list[i].x;
         if (key >= from && (bits == 32 || (key >> bits) == (prefix >> bits))) {
-          // the sum as two 32-bit ones, of the weights' lower and upper halves (at most 2048 terms each): a 64-bit
+          // the sum as two 32-bit ones, of the weights' lower and upper halves (at most SW * SLIST terms each): a 64-bit
           // add to shared memory is a loop
           uint32_t* slot = reinterpret_cast<uint32_t*>(&buf()[(key >> shift) & ((1u << take) - 1)]);
           const uint32_t wt = WEIGHTS ? weight_of(key) : 1u;
@@ -873,7 +875,7 @@ __global__ void __launch_bounds__(Sampler<T, STREAM>::NTH, 1024 / Sampler<T, STR
     s.buf()[SW + w] = (static_cast<unsigned long long>(n_kept) << 32) | n_tie;
   }
   s.agree();
-  // lane l: chunks 2l and 2l + 1 of the row's ctas * 8
+  // lane l: chunks 2l and 2l + 1 of the row's ctas * SW
   unsigned long long cs[2] = {0, 0};
   long long ct[2] = {0, 0}, ck[2] = {0, 0};
 #pragma unroll
