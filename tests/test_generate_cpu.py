@@ -217,3 +217,14 @@ def test_prompts_of_the_command(tmp_path):
         path.write_text(bad)
         with pytest.raises(TkbError):
             generate.read_prompts(path)
+
+
+def test_generator_takes_an_embedding_with_more_rows_than_the_vocabulary():
+    import numpy as np
+    from tokamak_b200 import TkbError, configs
+    V, d = configs.C1["vocab"], configs.C1["d_model"]
+    _, gen = small_generator(embed=np.zeros((V + 8, d), np.float32))
+    with pytest.raises(TkbError, match=f"0 to {V + 7}"):
+        gen.prefill([[V + 8], [0]])
+    with pytest.raises(TkbError, match="CUDA device"):  # the ids pass; the tensors are on the host
+        gen.prefill([[V + 7], [0]])

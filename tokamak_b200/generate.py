@@ -86,7 +86,8 @@ class Generator:
                             bg=put(w["bg"]), bu=put(w["bu"]), wd=put(w["wd"], d), bd=put(w["bd"])) for w in layers]
         self.head = dict(norm=put(head["norm"]), w=put(head["w"], V), b=put(head["b"]))
         self.embed = torch.as_tensor(embed, dtype=torch.bfloat16, device=device)
-        if self.embed.shape != (V, d):  # a look-up past its end would be a device assert
+        # a look-up past its end would be a device assert; rows past the vocabulary may hold prompt-only tokens
+        if self.embed.dim() != 2 or self.embed.shape[0] < V or self.embed.shape[1] != d:
             raise TkbError(f"Generator: embed is {tuple(self.embed.shape)}, not {(V, d)}")
         pages = -(-max_tokens // page_size)
         self.table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
@@ -141,8 +142,8 @@ class Generator:
         n = [len(p) for p in prompts]
         if len(n) != self.batch or min(n) < 1 or max(n) > self.max_tokens:
             raise TkbError("prefill: one prompt of 1 to max_tokens tokens per sequence")
-        if min(map(min, prompts)) < 0 or max(map(max, prompts)) >= self.cfg["vocab"]:
-            raise TkbError(f"prefill: token ids are 0 to {self.cfg['vocab'] - 1}")
+        if min(map(min, prompts)) < 0 or max(map(max, prompts)) >= self.embed.shape[0]:
+            raise TkbError(f"prefill: token ids are 0 to {self.embed.shape[0] - 1}")
         dev = self.token.device
         start = np.concatenate(([0], np.cumsum(n))).astype(np.int32)
         row_start = torch.from_numpy(start).to(dev)
@@ -171,7 +172,7 @@ class Generator:
         return ops.gemm(last, self.head["w"], bias=self.head["b"], out_dtype=torch.float32)
 
     def decode(self):
-        """One step: the tokens in self.token (0 to vocab - 1) enter the caches; returns the next logits [batch, vocab]."""
+        """One step: the tokens in self.token (rows of embed) enter the caches; returns the next logits [batch, vocab]."""
         ops.kv_lens(self.lens, seen=self.seen, add=1)
 
         def attend(i, qkv):
