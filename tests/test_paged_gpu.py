@@ -660,3 +660,26 @@ def test_decode_of_the_same_inputs_gives_the_same_bits(dtype):
     check_attention(c, q, 8, lens, *first, dtype)
     for again in (ops().paged_attn_decode(c.handle, q, 8, workspace=ws), ops().paged_attn_decode(c.handle, q, 8)):
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Hkv,G,D,lens", [(2, 4, 64, [700, 33, 5]), (1, 12, 128, [2000, 16, 1])])
+def test_decode_infinite_values_stay_infinite(dtype, Hkv, G, D, lens):
+    """An infinity in v is the sum's, in its column and for the heads that use it; two of both signs make NaN; slots
+    past the length do not count."""
+    c = Cache(dtype, lens, Hkv, D, 16).fill(lens)
+    B, Hq = len(lens), Hkv * G
+    q = c.randn(B, Hq * D, dtype=dtype)
+    good = ops().paged_attn_decode(c.handle, q, Hq)[0].clone().view(B, Hkv, G, D)
+    inf = float("inf")
+    want = good.clone()
+    for b, n in enumerate(lens):
+        for j, col, x in ((0, 3, inf), (n // 2, 10, -inf), (n - 1, 40, inf)):
+            c.v[c.table[b, j // 16].long(), 0, j % 16, col] = x
+            want[b, 0, :, col] = x
+    c.v[c.table[0, 20].long(), 0, 4, 3] = -inf   # the other sign in the same column of another key
+    want[0, 0, :, 3] = float("nan")
+    out, lse = ops().paged_attn_decode(c.handle, q, Hq)
+    out = out.view(B, Hkv, G, D)
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(), want.nan_to_num())
+    assert torch.isfinite(lse).all()
