@@ -325,9 +325,9 @@ int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stri
  * lse [B][Hq] fp32 (may be NULL).  A sequence that holds nothing gets out 0
  * and lse -inf.  With `accumulate`, weight[slot] of each kv head also grows by
  * the sum over its query heads of softmax(s)_slot.  NaN in q, k or v reaches
- * the heads that use it, as does an infinite v, whatever its probability but
- * for what fp32 cannot hold.  The work is cut over the cached lengths and
- * joined in a fixed order: equal inputs give equal bits.
+ * the heads that use it, and so does an infinite v (NaN where its probability
+ * is below the fp32 range).  The work is cut over the cached lengths and joined
+ * in a fixed order: equal inputs give equal bits.
  * workspace: tkb_paged_attn_decode_workspace bytes, 256-byte aligned, zeroed
  * before its first use; every call leaves it fit for the next one, of any
  * cache and shape that it is large enough for.  Calls that may overlap need
