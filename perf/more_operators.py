@@ -196,8 +196,6 @@ def prepare(case, seed):
         s.meta0 = s.meta.clone()
         rows = [max(0, n - m) for m, n in zip(before, after)]
         s.row_start, s.rows = starts(rows), max(1, sum(rows))
-        if own:
-            s.workspace = ops.kv_pages_workspace(B)
     else:
         dt = DTYPES[case["dtype"]]
         rows = lengths(case)
@@ -256,7 +254,7 @@ def run_pages(s):
     s.meta.copy_(s.meta0)
     if own:
         granted, slots = s.ops.kv_pages(s.table, s.held, s.lens, s.free, s.n_free, page, row_start=s.row_start,
-                                        rows=s.rows, workspace=s.workspace)
+                                        rows=s.rows)
         return [s.table, s.held, s.free, s.n_free, granted, slots]
     want = torch.clamp(-(-s.lens // page), max=most)
     entry = torch.arange(most, device=DEV)
