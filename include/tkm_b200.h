@@ -352,6 +352,79 @@ size_t tkb_kv_evict_workspace(const tkb_kv_cache *cache);
 int tkb_kv_evict(const tkb_kv_cache *cache, const int32_t *seen, int budget, int recent, int sinks,
                  void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------ many requests at once
+ * Attention of a chunk of new tokens per sequence over its cached tokens:
+ * pieces of prompts after earlier pieces, whole prompts, drafted tokens, or
+ * single tokens, each sequence with its own number of rows.  row_start
+ * [B + 1] gives the rows of each sequence (NULL: row b belongs to sequence b
+ * and rows == B); they are the last n_b of its seq_lens[b] tokens and already
+ * in the cache (tkb_kv_lens, tkb_kv_append): row i of sequence b attends over
+ * slots 0 .. seq_lens[b] - n_b + i, in whatever order the older ones lie (after
+ * an eviction).  For query head h (kv head h / (Hq/Hkv)): s_j = scale * q . k_j,
+ * out = sum_j softmax(s)_j v_j, lse = ln sum_j exp(s_j).  q and out [rows] of
+ * Hq*D (q_stride, out_stride elements apart, 16-byte aligned, not
+ * overlapping), lse [rows][Hq] fp32 (may be NULL).  scale is positive.
+ * bf16/f16 run on tcgen05 tensor cores with the probabilities rounded to the
+ * type and sums in fp32; f32 runs fp32 FMA.  NaN or an infinity in q, k or v
+ * reaches the rows that see it and no others.  A row that sees no slot (its
+ * sequence counts fewer tokens than rows, or its pages are bad) gets out 0
+ * and lse -inf.  A row_start that does not ascend inside [0, rows], a length
+ * or page that does not exist sets bit 2 of the device error word; rows of no
+ * sequence keep their out and lse.  Equal inputs give equal bits.
+ * workspace: tkb_paged_attn_chunk_workspace bytes, 256-byte aligned; no state
+ * is kept in it.  Calls that may overlap need workspaces of their own. */
+size_t tkb_paged_attn_chunk_workspace(const tkb_kv_cache *cache, int rows, int Hq);
+int tkb_paged_attn_chunk(const tkb_kv_cache *cache, const void *q, long long q_stride, void *out,
+                         long long out_stride, float *lse, const int32_t *row_start, int rows, int Hq,
+                         float scale, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Block tables from the lengths of the requests.  The pages of a pool are
+ * owned by the sequences (block_table [B][max_pages], of which the first
+ * held[b] entries of row b are in use) or free: free_pages [n_pages] is a
+ * stack of *n_free page numbers.  Sequence b needs ceil(lens[b] / page_size)
+ * pages, at most max_pages.  First the sequences that hold more give the
+ * surplus back: their last entries, by sequence and then by entry, are pushed
+ * in that order, and become -1.  Then those that hold fewer are served from the
+ * top of the stack, in the order of the sequences and of their entries, each
+ * whole or not at all: up to the first whose need, with the needs of all before
+ * it, exceeds the stack; it and those after it that need pages get none.
+ * Written: block_table, held, free_pages, n_free, and granted[b] (may be
+ * NULL): 1 when sequence b's pages hold all its tokens.  Entries of
+ * free_pages above *n_free keep what they held.
+ * slots (may be NULL) gets, for each of `rows` rows, the place of its token in
+ * the pool, page * page_size + slot in the page, for callers that move tokens
+ * themselves: row_start as for tkb_kv_append, lens counting the new rows; -1
+ * for a row without a place.  One call for a cache serves all layers that
+ * share the table.  Lengths below 0, counts outside their range and pages
+ * above n_pages set bit 2 of the device error word and are cut to the range.
+ * B at most 4096, B * max_pages below 2^30, page_size 1 to 1024. */
+int tkb_kv_pages(int32_t *block_table, int32_t *held, const int32_t *lens, int32_t *free_pages, int32_t *n_free,
+                 int32_t *granted, int64_t *slots, const int32_t *row_start, int rows, int B, int max_pages,
+                 int page_size, int n_pages, void *stream);
+
+/* Low-rank adapters of many requests beside a shared projection: for every
+ * row r of a sequence with adapter i = adapter[b] >= 0
+ *   out_r = y_r + scale[i] * (x_r A_i) B_i
+ * with x [rows][K], y (the shared projection's output) and out [rows][N] (out
+ * may be y, at the same stride), A [n_adapters][K][R] and B [n_adapters][R][N],
+ * all of one dtype, rows x_stride, y_stride, out_stride elements apart; scale
+ * [n_adapters] fp32 (NULL: 1).  Products and sums are fp32, the result is
+ * rounded once.  adapter[b] = -1: out_r = y_r.  Rows of no sequence are left
+ * as they were.  An adapter that does not exist counts as -1 and sets bit 2 of
+ * the device error word.  K, N and the strides: multiples of 16 bytes, the
+ * pointers 16-byte aligned; R a multiple of 8 up to 128.
+ * The plan sorts the rows by adapter: tkb_lora_plan writes it from adapter [B]
+ * and row_start (as for tkb_kv_append), once for all projections that take
+ * the same rows, and tkb_lora_add reads it.  plan: tkb_lora_plan_bytes,
+ * workspace: tkb_lora_workspace bytes, both 256-byte aligned. */
+size_t tkb_lora_plan_bytes(int B, int rows, int n_adapters);
+int tkb_lora_plan(const int32_t *adapter, const int32_t *row_start, int B, int rows, int n_adapters, void *plan,
+                  size_t plan_bytes, void *stream);
+size_t tkb_lora_workspace(int rows, int R);
+int tkb_lora_add(const void *plan, const void *x, long long x_stride, const void *A, const void *B_, const float *scale,
+                 const void *y, long long y_stride, void *out, long long out_stride, int B, int rows, int n_adapters,
+                 int K, int N, int R, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------ sampling
  * One token per row of logits [rows][V] (ld elements apart) from given
  * uniform numbers u[rows] in [0, 1); temperature, top_k, top_p, min_p are per

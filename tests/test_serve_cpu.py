@@ -1,0 +1,164 @@
+"""Refusals of the entry points that serve many requests at once: bad arguments
+are turned down with a message before any CUDA call."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import tokamak_b200
+from oracle import serve_oracle as ref
+from tests.test_generate_cpu import cache, message
+
+vp = ctypes.c_void_p
+
+
+def chunk(c, rows=2, Hq=4, q=256, out=512, stride=256, out_stride=256, start=256, scale=0.1, ws=256, n=1 << 40):
+    L = tokamak_b200.lib()
+    return L.tkb_paged_attn_chunk(ctypes.byref(c) if c else None, vp(q), stride, vp(out), out_stride, None, vp(start),
+                                  rows, Hq, scale, vp(ws), n, None)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(k=0), -1), (dict(seq_lens=0), -1), (dict(block_table=0), -1), (dict(k=264), -1), (dict(dtype=7), -1),
+    (dict(B=0), -1), (dict(B=5000), -3), (dict(D=96), -3), (dict(page_size=24), -1), (dict(page_size=2048), -1),
+    (dict(page_stride=2 * 16 * 64 - 8), -1), (dict(max_pages=1 << 28), -1), (dict(n_pages=0), -1), (dict(Hkv=0), -1)])
+def test_chunk_bad_caches(over, code):
+    c = cache(**over)
+    assert chunk(c) == code and message()
+    assert tokamak_b200.lib().tkb_paged_attn_chunk_workspace(ctypes.byref(c), 2, 4) == 0
+
+
+def test_chunk_refusals():
+    c = cache()
+    assert chunk(None) == -1
+    assert chunk(c, Hq=3) == -1 and "multiple" in message()
+    assert chunk(c, Hq=0) == -1 and chunk(c, rows=0) == -1 and chunk(c, rows=(1 << 26) + 1) == -3
+    assert chunk(c, rows=3, start=0) == -1 and "row_start" in message()
+    assert chunk(c, q=0) == -1 and chunk(c, out=0) == -1
+    assert chunk(c, q=264) == -1 and chunk(c, stride=128) == -1 and chunk(c, out_stride=260) == -1
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert chunk(c, scale=scale) == -1 and "scale" in message()
+    assert chunk(c, ws=0) == -4 and chunk(c, n=8) == -4 and chunk(c, ws=272) == -4
+    L = tokamak_b200.lib()
+    assert L.tkb_paged_attn_chunk_workspace(ctypes.byref(c), 0, 4) == 0
+    assert L.tkb_paged_attn_chunk_workspace(ctypes.byref(c), 2, 3) == 0
+    small, large = (L.tkb_paged_attn_chunk_workspace(ctypes.byref(c), n, 4) for n in (2, 4096))
+    assert 0 < small <= large
+
+
+def test_pages_refusals():
+    def call(table=256, held=256, lens=256, free=256, n_free=256, slots=0, start=0, rows=0, B=2, most=4, page=16, n=8):
+        return tokamak_b200.lib().tkb_kv_pages(vp(table), vp(held), vp(lens), vp(free), vp(n_free), None, vp(slots),
+                                               vp(start), rows, B, most, page, n, None)
+    for name in ("table", "held", "lens", "free", "n_free"):
+        assert call(**{name: 0}) == -1 and "null" in message()
+    assert call(B=0) == -1 and call(B=5000) == -3 and call(most=0) == -1 and call(n=0) == -1
+    assert call(page=0) == -1 and call(page=1025) == -1 and call(most=1 << 29, B=2) == -3
+    assert call(slots=256, rows=0) == -1 and call(slots=256, rows=3) == -1 and "row_start" in message()
+    assert call(slots=260, rows=2) == -1 and "aligned" in message()
+
+
+def test_lora_refusals():
+    L = tokamak_b200.lib()
+
+    def plan(adapter=256, start=256, B=2, rows=9, n=3, at=256, size=1 << 30):
+        return L.tkb_lora_plan(vp(adapter), vp(start), B, rows, n, vp(at), size, None)
+    assert plan(adapter=0) == -1 and plan(B=0) == -1 and plan(rows=0) == -1 and plan(n=0) == -1 and plan(B=5000) == -3
+    assert plan(start=0) == -1 and "row_start" in message()
+    assert plan(at=0) == -4 and plan(size=8) == -4 and plan(at=264) == -4
+    assert L.tkb_lora_plan_bytes(0, 1, 1) == 0 and L.tkb_lora_plan_bytes(1, 1, 0) == 0
+    assert L.tkb_lora_workspace(0, 8) == 0 and L.tkb_lora_workspace(8, 0) == 0
+
+    def add(p=256, x=256, xs=64, a=256, b=256, y=256, ys=64, out=512, os=64, B=2, rows=9, n=3, K=64, N=64, R=8, dt=1,
+            ws=256, size=1 << 30):
+        return L.tkb_lora_add(vp(p), vp(x), xs, vp(a), vp(b), None, vp(y), ys, vp(out), os, B, rows, n, K, N, R, dt,
+                              vp(ws), size, None)
+    for name in ("p", "x", "a", "b", "y", "out"):
+        assert add(**{name: 0}) == -1, name
+    assert add(R=0) == -3 and add(R=12) == -3 and add(R=136) == -3
+    assert add(K=60) == -1 and add(N=4) == -1 and add(K=0) == -1 and add(n=0) == -1 and add(dt=5) == -1
+    assert add(xs=56) == -1 and add(ys=68) == -1 and add(os=0) == -1 and add(x=264) == -1 and add(a=264) == -1
+    assert add(out=256, y=256, os=128) == -1 and "stride" in message()
+    assert add(ws=0) == -4 and add(size=16) == -4 and add(ws=264) == -4
+
+
+def test_python_checks():
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, ops
+    k = torch.zeros(4, 2, 16, 64)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    c = ops.KVCache(k, k.clone(), table, lens)
+    q, start = torch.zeros(7, 4 * 64), torch.tensor([0, 3, 7], dtype=torch.int32)
+    for args, more in (((q[:, :64], 4), {}), ((q.bfloat16(), 4), {}), ((q.view(-1), 4), {}), ((q, 4), dict(row_start=lens)),
+                       ((q, 4), dict(row_start=start.long())), ((q, 4), dict(row_start=start, out=q[:3])),
+                       ((q, 4), dict(row_start=start, lse=torch.zeros(7, 3))), ((q, 3), dict(row_start=start)),
+                       ((q.t().contiguous().t(), 4), dict(row_start=start))):
+        with pytest.raises(TkbError):
+            ops.paged_attn_chunk(c, *args, **more)
+    one = torch.zeros(1, dtype=torch.int32)
+    free = torch.zeros(9, dtype=torch.int32)
+    for bad in (dict(held=one), dict(lens=lens.long()), dict(n_free=lens), dict(block_table=table.t()),
+                dict(row_start=lens, rows=4), dict(free_pages=free[::2])):
+        with pytest.raises(TkbError):
+            ops.kv_pages(**{**dict(block_table=table, held=lens, lens=lens, free_pages=free, n_free=one, page_size=16),
+                            **bad})
+    with pytest.raises(TkbError):
+        ops.lora_plan(lens.long(), 2, 7, row_start=start)
+    with pytest.raises(TkbError):
+        ops.lora_plan(lens, 2, 7, row_start=lens)
+    plan = ops.LoraPlan(torch.zeros(256, dtype=torch.uint8), 2, 7, 3)
+    good = dict(x=torch.zeros(7, 64), A=torch.zeros(3, 64, 8), B=torch.zeros(3, 8, 32), y=torch.zeros(7, 32))
+    for bad in (dict(x=torch.zeros(6, 64)), dict(x=torch.zeros(7, 64).half()), dict(A=torch.zeros(2, 64, 8)),
+                dict(B=torch.zeros(3, 16, 32)), dict(y=torch.zeros(7, 40)), dict(out=torch.zeros(7, 31)),
+                dict(scale=torch.zeros(2)), dict(x=torch.zeros(64, 7).t()), dict(A=torch.zeros(3, 8, 64).transpose(1, 2))):
+        with pytest.raises(TkbError):
+            ops.lora_add(plan, **{**good, **bad})
+
+
+def test_tensors_of_the_host_are_refused():
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, ops
+    k = torch.zeros(4, 2, 16, 64)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    c = ops.KVCache(k, k.clone(), table, lens)
+    start = torch.tensor([0, 3, 7], dtype=torch.int32)
+    plan = ops.LoraPlan(torch.zeros(256, dtype=torch.uint8), 2, 7, 3)
+    calls = [lambda: ops.paged_attn_chunk(c, torch.zeros(7, 4 * 64), 4, row_start=start),
+             lambda: ops.kv_pages(table, lens, lens.clone(), torch.zeros(9, dtype=torch.int32), lens[:1], 16),
+             lambda: ops.lora_plan(lens, 3, 7, row_start=start),
+             lambda: ops.lora_add(plan, torch.zeros(7, 64), torch.zeros(3, 64, 8), torch.zeros(3, 8, 32),
+                                  torch.zeros(7, 32))]
+    for call in calls:
+        with pytest.raises(TkbError, match="CUDA device"):
+            call()
+
+
+def test_oracle_of_the_chunk_against_differences_and_single_tokens():
+    """The oracle itself: rows of a chunk are single tokens over ever more slots, and d lse / d score is the weight of
+    its key, by differences."""
+    from oracle import paged_oracle
+    rng = np.random.default_rng(0)
+    k, v = rng.standard_normal((2, 3, 2, 16, 8))
+    pages, q = np.array([2, 0]), rng.standard_normal((5, 4, 8))
+    out, lse = ref.chunk(k, v, pages, 20, q, 0.3)
+    for i in range(5):
+        o, l, p = paged_oracle.attend(k, v, pages, 16 + i, q[i], 0.3)
+        assert np.allclose(out[i], o) and np.allclose(lse[i], l)
+    # moving key 3 along the query by eps moves its score by eps |q|^2 scale
+    eps, h = 1e-6, 0
+    _, _, p = paged_oracle.attend(k, v, pages, 20, q[4], 0.3)
+    moved = k.copy()
+    moved[2, h, 3] += eps * q[4, 0]
+    _, more = ref.chunk(moved, v, pages, 20, q, 0.3)
+    assert abs((more[4, 0] - lse[4, 0]) / (eps * (q[4, 0] ** 2).sum() * 0.3) - p[0, 3]) < 1e-5
+
+
+def test_oracle_of_the_pages_keeps_every_page_once():
+    rng = np.random.default_rng(1)
+    table, held, stack = np.full((6, 5), -1), np.zeros(6, int), list(range(17))
+    for _ in range(50):
+        lens = rng.integers(0, 81, 6)
+        table, held, stack, granted = ref.pages(table, held, lens, stack, 16)
+        used = [int(p) for b in range(6) for p in table[b, :held[b]]]
+        assert sorted(used + stack) == list(range(17)) and (table[np.arange(5) >= held[:, None]] == -1).all()
+        assert all(bool(g) == (h * 16 >= n) for g, h, n in zip(granted, held, lens))

@@ -63,6 +63,13 @@ _SIGS = {
     "tkb_kv_evict_workspace": ([_vp], _sz),
     "tkb_kv_evict": ([_vp, _vp, _i, _i, _i, _vp, _sz, _vp], _i),
     "tkb_sample_logits": ([_vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp], _i),
+    "tkb_paged_attn_chunk_workspace": ([_vp, _i, _i], _sz),
+    "tkb_paged_attn_chunk": ([_vp, _vp, _ll, _vp, _ll, _vp, _vp, _i, _i, _f, _vp, _sz, _vp], _i),
+    "tkb_kv_pages": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp], _i),
+    "tkb_lora_plan_bytes": ([_i, _i, _i], _sz),
+    "tkb_lora_plan": ([_vp, _vp, _i, _i, _i, _vp, _sz, _vp], _i),
+    "tkb_lora_workspace": ([_i, _i], _sz),
+    "tkb_lora_add": ([_vp, _vp, _ll, _vp, _vp, _vp, _vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp], _i),
     "tkb_gemm_swiglu": ([_vp, _ll, _vp, _ll, _i, _vp, _vp, _vp, _ll, _vp, _ll, _i, _i, _vp], _i),
 }
 

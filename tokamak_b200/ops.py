@@ -400,3 +400,115 @@ def sample_logits(logits, u, temperature=None, top_k=None, top_p=None, min_p=Non
                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(token), _ptr(logprob), _ptr(kept), rows, V,
                                   dtype_code(logits), stream), "tkb_sample_logits")
     return token, logprob, kept
+
+
+def paged_attn_chunk_workspace(cache, rows, Hq):
+    """Workspace of paged_attn_chunk for up to `rows` rows; one per stream that calls it."""
+    n = lib().tkb_paged_attn_chunk_workspace(cache.ref, rows, Hq)
+    if n == 0:
+        check(-1, "tkb_paged_attn_chunk_workspace")
+    return torch.empty(n, dtype=torch.uint8, device=cache.k.device)
+
+
+def paged_attn_chunk(cache, q, Hq, row_start=None, scale=None, out=None, lse=None, workspace=None):
+    """Attention of the newest tokens of every sequence over its cache (tkb_paged_attn_chunk): q [rows, Hq*D], rows of
+    sequence b from row_start[b] to row_start[b + 1] (None: one each) -> (out [rows, Hq*D], lse [rows, Hq] fp32).
+    Rows of no sequence are not written."""
+    if q.dtype != cache.k.dtype:
+        raise TkbError(f"paged_attn_chunk: q is {q.dtype}, the cache is {cache.k.dtype}")
+    width = Hq * cache.D
+    if q.dim() != 2 or q.shape[1] != width:
+        raise TkbError(f"paged_attn_chunk: q is {tuple(q.shape)}, not rows of {width} columns")
+    rows = q.shape[0]
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise TkbError(f"paged_attn_chunk: out is {out.dtype} {tuple(out.shape)}, not as q")
+    if q.stride(1) != 1 or out.stride(1) != 1:
+        raise TkbError("paged_attn_chunk: columns of q and out must be contiguous")
+    if lse is None:
+        lse = torch.empty(rows, Hq, dtype=torch.float32, device=q.device)
+    else:
+        _vec(lse, "lse", rows * Hq, torch.float32)
+    _vec(row_start, "row_start", cache.B + 1, torch.int32)
+    if workspace is None:
+        workspace = paged_attn_chunk_workspace(cache, rows, Hq)
+    stream = _launch_stream("paged_attn_chunk", cache.k, q, out, lse, row_start, workspace)
+    check(lib().tkb_paged_attn_chunk(cache.ref, _ptr(q), _row_stride(q, width), _ptr(out), _row_stride(out, width),
+                                     _ptr(lse), _ptr(row_start), rows, Hq, cache.D ** -0.5 if scale is None else scale,
+                                     _ptr(workspace), workspace.numel(), stream), "tkb_paged_attn_chunk")
+    return out, lse
+
+
+def kv_pages(block_table, held, lens, free_pages, n_free, page_size, row_start=None, rows=None):
+    """Pages for sequences of `lens` tokens (tkb_kv_pages): block_table [B, max_pages], held [B], the stack free_pages
+    [n_pages] and its height n_free [1] are brought up to date, all int32.  Returns (granted [B] int32, slots): with
+    `rows`, slots [rows] int64 is each new row's place in the pool (row_start as in kv_append), else None."""
+    B, max_pages = block_table.shape
+    _expect(block_table, "block_table", (B, max_pages), torch.int32)
+    _vec(held, "held", B, torch.int32)
+    _vec(lens, "lens", B, torch.int32)
+    _vec(free_pages, "free_pages", free_pages.numel(), torch.int32)
+    _vec(n_free, "n_free", 1, torch.int32)
+    _vec(row_start, "row_start", B + 1, torch.int32)
+    stream = _launch_stream("kv_pages", block_table, held, lens, free_pages, n_free, row_start)
+    granted = torch.empty_like(held)
+    slots = None if rows is None else torch.empty(rows, dtype=torch.int64, device=held.device)
+    check(lib().tkb_kv_pages(_ptr(block_table), _ptr(held), _ptr(lens), _ptr(free_pages), _ptr(n_free), _ptr(granted),
+                             _ptr(slots), _ptr(row_start), 0 if rows is None else rows, B, max_pages, page_size,
+                             free_pages.numel(), stream), "tkb_kv_pages")
+    return granted, slots
+
+
+class LoraPlan:
+    """Rows sorted by adapter, for every lora_add that takes the same rows (tkb_lora_plan)."""
+
+    def __init__(self, buffer, B, rows, n_adapters):
+        self.buffer, self.B, self.rows, self.n_adapters = buffer, B, rows, n_adapters
+
+
+def lora_plan(adapter, n_adapters, rows, row_start=None):
+    """The plan of `rows` rows whose sequences use adapter [B] (int32, -1: none); row_start as in kv_append."""
+    B = adapter.numel()
+    _vec(adapter, "adapter", B, torch.int32)
+    _vec(row_start, "row_start", B + 1, torch.int32)
+    stream = _launch_stream("lora_plan", adapter, row_start)
+    n = lib().tkb_lora_plan_bytes(B, rows, n_adapters)
+    if n == 0:
+        check(-1, "tkb_lora_plan_bytes")
+    buffer = torch.empty(n, dtype=torch.uint8, device=adapter.device)
+    check(lib().tkb_lora_plan(_ptr(adapter), _ptr(row_start), B, rows, n_adapters, _ptr(buffer), n, stream),
+          "tkb_lora_plan")
+    return LoraPlan(buffer, B, rows, n_adapters)
+
+
+def lora_workspace(rows, R, device="cuda"):
+    """Workspace of lora_add for up to `rows` rows and ranks up to R; one per stream that calls it."""
+    n = lib().tkb_lora_workspace(rows, R)
+    if n == 0:
+        check(-1, "tkb_lora_workspace")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def lora_add(plan, x, A, B, y, scale=None, out=None, workspace=None):
+    """out = y + scale * (x A) B with each row's own adapter (tkb_lora_add): x [rows, K], A [n_adapters, K, R],
+    B [n_adapters, R, N], y [rows, N], scale [n_adapters] fp32 or None; y itself where no out is given.  Returns out."""
+    out = y if out is None else out
+    n, K, R = A.shape
+    N = B.shape[2]
+    if n != plan.n_adapters:
+        raise TkbError(f"lora_add: {n} adapters, the plan is for {plan.n_adapters}")
+    _expect(A, "A", (n, K, R), x.dtype)
+    _expect(B, "B", (n, R, N), x.dtype)
+    _vec(scale, "scale", n, torch.float32)
+    for t, name, width in ((x, "x", K), (y, "y", N), (out, "out", N)):
+        if t.shape != (plan.rows, width) or t.dtype != x.dtype or (width > 1 and t.stride(1) != 1):
+            raise TkbError(f"lora_add: {name} is {t.dtype} {tuple(t.shape)}, not {x.dtype} {(plan.rows, width)} with "
+                           "contiguous columns")
+    if workspace is None:
+        workspace = lora_workspace(plan.rows, R, x.device)
+    stream = _launch_stream("lora_add", x, A, B, y, out, scale, plan.buffer, workspace)
+    check(lib().tkb_lora_add(_ptr(plan.buffer), _ptr(x), _row_stride(x, K), _ptr(A), _ptr(B), _ptr(scale), _ptr(y),
+                             _row_stride(y, N), _ptr(out), _row_stride(out, N), plan.B, plan.rows, n, K, N, R,
+                             dtype_code(x), _ptr(workspace), workspace.numel(), stream), "tkb_lora_add")
+    return out
