@@ -28,7 +28,7 @@ extern "C" {
 
 size_t tkb_paged_attn_chunk_workspace(const tkb_kv_cache* cache, int rows, int Hq) {
   if (chunk_check("tkb_paged_attn_chunk_workspace", cache, rows, Hq)) return 0;
-  return 256;
+  return round256(chunk_ws(*cache).bytes);
 }
 
 int tkb_paged_attn_chunk(const tkb_kv_cache* cache, const void* q, long long q_stride, void* out,
@@ -41,6 +41,9 @@ int tkb_paged_attn_chunk(const tkb_kv_cache* cache, const void* q, long long q_s
   if (!q || !out) return fail(TKB_ERR_ARG, "%s: null pointer", who);
   if (!(scale > 0.f) || std::isinf(scale)) return fail(TKB_ERR_ARG, "%s: scale must be positive", who);
   const long long width = static_cast<long long>(Hq) * cache->D;
+  // the units' costs are summed in 64 bits
+  if (static_cast<double>(rows) * Hq * cache->max_pages * cache->page_size > 9e15)
+    return fail(TKB_ERR_UNSUPPORTED, "%s: rows * Hq * max_pages * page_size above 9e15", who);
   if ((rc = rows_check(who, "q", q, q_stride, width, cache->dtype))) return rc;
   if ((rc = rows_check(who, "out", out, out_stride, width, cache->dtype))) return rc;
   const size_t need = tkb_paged_attn_chunk_workspace(cache, rows, Hq);
@@ -60,9 +63,11 @@ int tkb_paged_attn_chunk(const tkb_kv_cache* cache, const void* q, long long q_s
   p.G = Hq / cache->Hkv;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CALL(T) paged_chunk_t<T>(p, st)
-  return cuda_status(TKB_BY_DTYPE(cache->dtype, CALL), who, 1);
+  unsigned kernels = 0;
+#define CALL(T) paged_chunk_t<T>(p, workspace, st, kernels)
+  const cudaError_t e = TKB_BY_DTYPE(cache->dtype, CALL);
 #undef CALL
+  return cuda_status(e, who, kernels);
 }
 
 int tkb_kv_pages(int32_t* block_table, int32_t* held, const int32_t* lens, int32_t* free_pages, int32_t* n_free,

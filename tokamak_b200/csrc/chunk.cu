@@ -1,11 +1,31 @@
 // chunk.cu -- attention of a chunk of new tokens over the paged key-value
 // cache: pieces of prompts, whole prompts, drafted tokens, single tokens.
+//
+// out_i = softmax(scale q_i K^T) V over the slots row i sees, one pass over K
+// and V with the running maximum and sum of each row.  4 D FLOP a (query, head,
+// slot) against 4 D bytes a (kv head, slot) in 16 bits: the tensor cores bound
+// it from some 250 packed query rows a kv head on, HBM below that.
+//
+// 16-bit types.  The query heads of a kv head share its K and V, so their rows
+// are packed: a tile of 128 rows holds 128 / G tokens x G heads.  A unit
+// (sequence, kv head, up to two tiles of tokens) streams the slots that its last
+// token sees in blocks of 128.  All units' blocks, in order, are dealt out as
+// equal runs, whatever the lengths, to one CTA per SM; a unit that spans CTAs
+// leaves unnormalised parts in the workspace, which a second kernel joins in
+// the order of the run.  Inside a CTA the roles are those of the prompt's own
+// attention (attn_fwd.cu): one warp issues TMA, one the tcgen05 products, two
+// warpgroups hold a query row a thread and do the softmax.  A unit of two tiles
+// gives each warpgroup one of them; a unit of one gives them its blocks in
+// turn, and their two results meet in shared memory at its end.
+// TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [256+D,256+2D),
+// P as 16-bit pairs over the first half of S.
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
 namespace tkb {
 
-struct ChunkParams {
+struct alignas(64) ChunkParams {
+  CUtensorMap tmQ, tmK, tmV;  // 16-bit types
   tkb_kv_cache c;
   const void* q;
   void* out;
@@ -13,7 +33,13 @@ struct ChunkParams {
   const int32_t* row_start;
   long long q_stride, out_stride;
   int rows, Hq, G;
+  int gb, hb;          // query heads per tile, blocks of them per kv head (G <= hb * gb)
+  int tt;              // tokens per tile: 128 / gb
+  int gran;            // slots per TMA box: what divides both a page and a block of 128
   float scale_log2;
+  float4* part;        // [2 * grid][2 tiles][D / 4][128 rows] unnormalised parts
+  float2* part_ml;     // [2 * grid][2][128] their maxima (in powers of 2) and sums
+  int4* span;          // [grid] what the CTA left: ChunkSpan bits, sequence, head group, unit
 };
 
 // The rows of sequence b: first row and number, inside [0, rows).
@@ -33,6 +59,878 @@ TKB_DEVFN void chunk_rows(const int32_t* row_start, int rows, int b, int& first,
   n = hi - lo;
 }
 
+// ============================================================ the deal
+// sum over i < n of floor((a i + b) / m); a, b >= 0
+TKB_DEVFN long long floor_sum(long long n, unsigned m, unsigned a, long long b) {
+  long long sum = 0;
+  while (true) {
+    if (a >= m) {
+      sum += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const long long y = static_cast<long long>(a) * n + b;
+    if (y < m) return sum;
+    n = y / m;
+    b = y % m;
+    const unsigned was = m;
+    m = a;
+    a = was;
+  }
+}
+
+constexpr int kChunkGrid = 148;   // one CTA per SM
+constexpr int kChunkBlock = 128;  // slots per block
+// What a block costs beside a block of a single tile: with two tiles twice the
+// products; and what a unit costs on top (its queries' load, its rows' output).
+constexpr int kCostPair = 2, kCostUnit = 2;
+constexpr int kCostLeast = 6;     // a CTA's run at least: shorter ones cost more to join than they save
+
+// A sequence: its rows, how many slots its first row sees less one (may be
+// negative), what it holds, and its units.
+struct ChunkSeq {
+  int first, n, base, held;
+  int units;
+  long long cost;  // of one head group
+};
+TKB_DEVFN int chunk_blocks(int base, int upto) {  // blocks for a row that sees base + upto slots; at least one
+  return 1 + (max(base, 0) + upto - 1) / kChunkBlock;
+}
+TKB_DEVFN long long chunk_cost_before(const ChunkParams& p, const ChunkSeq& s, int u) {  // of the first u (full) units
+  const int per = 2 * p.tt;
+  return static_cast<long long>(u) * (kCostUnit + kCostPair) +
+         kCostPair * floor_sum(u, kChunkBlock, per, static_cast<long long>(max(s.base, 0)) + per - 1);
+}
+TKB_DEVFN long long chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
+  const int t0 = u * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
+  return kCostUnit + static_cast<long long>(tokens > p.tt ? kCostPair : 1) * chunk_blocks(s.base, t0 + tokens);
+}
+TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
+  ChunkSeq s;
+  chunk_rows(p.row_start, p.rows, b, s.first, s.n);
+  const int most = p.c.max_pages * p.c.page_size, held = max(p.c.seq_lens[b], -(1 << 30));
+  // rows without a slot see none, rows past the table all of it
+  if (held < s.n || held > most) {
+    if (s.n) atomicOr(&g_device_error, ERR_BAD_INDEX);
+  }
+  s.held = min(max(held, 0), most);
+  s.base = min(held, most + s.n) - s.n;
+  s.units = (s.n + 2 * p.tt - 1) / (2 * p.tt);
+  s.cost = s.n ? chunk_cost_before(p, s, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
+  return s;
+}
+
+// One unit's share of a CTA's run.
+struct ChunkItem {
+  int b, hg, u;            // sequence, head group (kv head, block of query heads), unit of the sequence
+  int t0, tokens;          // its tokens among the sequence's rows
+  int nb[2];               // blocks of its tiles (the second's are all the unit's)
+  int jb, je;              // the run's blocks
+  bool pair;               // two tiles
+  TKB_DEVFN bool whole() const { return jb == 0 && je == nb[1]; }
+};
+// Walks the items of a run; every role of the CTA walks for itself.
+struct ChunkWalk {
+  ChunkSeq s;
+  int b, hg, u;
+  long long at, x0, x1;    // cost where the unit starts, where the run does and ends
+  TKB_DEVFN bool next(const ChunkParams& p, ChunkItem& it) {
+    while (at < x1) {
+      if (u == s.units) {
+        u = 0;
+        if (++hg == p.c.Hkv * p.hb) {
+          hg = 0;
+          do {
+            if (++b >= p.c.B) return false;
+            s = chunk_seq(p, b);
+          } while (s.n == 0);
+        }
+      }
+      const long long cost = chunk_cost(p, s, u);
+      it.b = b;
+      it.hg = hg;
+      it.u = u;
+      it.t0 = u * 2 * p.tt;
+      it.tokens = min(2 * p.tt, s.n - it.t0);
+      it.pair = it.tokens > p.tt;
+      it.nb[0] = chunk_blocks(s.base, it.t0 + min(it.tokens, p.tt));
+      it.nb[1] = chunk_blocks(s.base, it.t0 + it.tokens);
+      const int w = it.pair ? kCostPair : 1;
+      auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later
+        return x <= kCostUnit ? 0 : static_cast<int>((x - kCostUnit + w - 1) / w);
+      };
+      it.jb = block_at(x0 - at);
+      it.je = x1 - at >= cost ? it.nb[1] : min(it.nb[1], block_at(x1 - at));
+      at += cost;
+      ++u;
+      if (it.jb < it.je) return true;
+    }
+    return false;
+  }
+};
+
+// The run of this CTA; false when it has none.  All threads of the block (NT_ of them) call it.
+template <int NT_>
+TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
+  __shared__ long long s_sum[NT_ / 32], s_x[3];
+  __shared__ int s_at[3];
+  const int tid = threadIdx.x, lane = lane_id(), wid = warp_id();
+  const int per = (p.c.B + NT_ - 1) / NT_, b0 = min(tid * per, p.c.B), b1 = min(b0 + per, p.c.B);
+  const int groups = p.c.Hkv * p.hb;
+  long long mine = 0;
+  ChunkSeq s;
+  for (int b = b0; b < b1; ++b) {
+    s = chunk_seq(p, b);
+    mine += s.cost * groups;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += y;
+  }
+  if (lane == 31) s_sum[wid] = upto;
+  __syncthreads();
+  long long total = 0;
+  for (int i = 0; i < NT_ / 32; ++i) {
+    if (i == wid) upto += total;
+    total += s_sum[i];
+  }
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + kCostLeast - 1) / kCostLeast));
+  const int c = blockIdx.x;
+  if (c >= ctas) return false;
+  const long long x0 = total * c / ctas, x1 = total * (c + 1) / ctas;
+  long long at = upto - mine;
+  if (at <= x0 && x0 < upto) {  // the run starts in one of this thread's sequences
+    for (int b = b0; b < b1; ++b) {
+      s = chunk_seq(p, b);
+      if (x0 < at + s.cost * groups) {
+        const int hg = static_cast<int>((x0 - at) / s.cost);
+        at += s.cost * hg;
+        int lo = 0, hi = s.units - 1;  // last unit that starts at x0 or before
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (at + chunk_cost_before(p, s, mid) <= x0) lo = mid;
+          else hi = mid - 1;
+        }
+        s_at[0] = b;
+        s_at[1] = hg;
+        s_at[2] = lo;
+        s_x[0] = at + chunk_cost_before(p, s, lo);
+        break;
+      }
+      at += s.cost * groups;
+    }
+  }
+  __syncthreads();
+  w.b = s_at[0];
+  w.hg = s_at[1];
+  w.u = s_at[2];
+  w.at = s_x[0];
+  w.x0 = x0;
+  w.x1 = x1;
+  w.s = chunk_seq(p, w.b);
+  return true;
+}
+
+// What a CTA left in the workspace: a part of a unit that earlier CTAs began, whether it is the unit's last, and the
+// first part of a unit that goes on in later ones.
+enum ChunkSpan : int { SPAN_GOES_ON = 1, SPAN_ENDS = 2, SPAN_BEGINS = 4 };
+
+// The (sequence row, query head) of row r of tile w of a unit; false where there is none.
+TKB_DEVFN bool chunk_row(const ChunkParams& p, const ChunkSeq& s, int hg, int t0, int tokens, int w, int r, int& tok,
+                         int& hq) {
+  const int t = r / p.gb, g = (hg % p.hb) * p.gb + r % p.gb;
+  tok = t0 + w * p.tt + t;
+  hq = (hg / p.hb) * p.G + g;
+  return t < p.tt && w * p.tt + t < tokens && g < p.G;
+}
+
+// ============================================================ 16-bit types: tcgen05
+template <int D>
+struct ChunkCfg {
+  static constexpr int TILE = 128 * D * 2;  // bytes of one 128-row x D tile
+  static constexpr int SLAB = 128 * 128;    // bytes of one 64-column swizzle slab
+  static constexpr int NST = D == 64 ? 4 : 2;  // stages of the K ring and of the V ring
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_V = OFF_K + NST * TILE;
+  static constexpr int OFF_X = OFF_V + NST * TILE;       // half of the second warpgroup's O, [D / 8][128] float4
+  static constexpr int OFF_XML = OFF_X + 128 * (D / 2) * 4;
+  static constexpr int OFF_BAR = OFF_XML + 128 * 8;
+  // q_full, q_empty, k_full[NST], k_empty[NST], v_full[NST], v_empty[NST], s_full[2], p_ready[2][2], o_done[2],
+  // x_full, x_empty, drain
+  static constexpr int NBAR = 2 + 4 * NST + 8 + 3;
+  static constexpr int NMASK = 16;                       // page marks of the newest blocks (more than are in flight)
+  static constexpr int OFF_MASK = OFF_BAR + NBAR * 8;
+  static constexpr int OFF_MISC = OFF_MASK + NMASK * 4;
+  static constexpr int SMEM = OFF_MISC + 16 + 1024;      // + slack for 1024-byte alignment
+  static_assert(SMEM <= 232448, "tiles exceed 227 KB of shared memory");
+  static constexpr uint32_t TM_S0 = 0, TM_S1 = 128, TM_O0 = 256, TM_O1 = 256 + D;
+};
+
+// One block of the online softmax for this thread's query row: S from TMEM,
+// slots from `lim` on and those of bad pages (bits of `there`, 16 slots each) masked, the
+// running maximum raised when this block's exceeds it by more than 8
+// (rescaling O in TMEM), P written over S in two halves, release(h) once half
+// h is in TMEM.  P is rounded to the type (half a step; the row sum is that of
+// the unrounded values).
+template <int D, bool BF16, typename Release>
+TKB_DEVFN void chunk_softmax(uint32_t tS, uint32_t tO, float sl2, bool first, bool cut, int lim, unsigned there,
+                             float& m_used, float& l, Release&& release) {
+  uint32_t r0[32], r1[32], r2[32], r3[32];
+  tmem_ld32(tS + 0, r0);
+  tmem_ld32(tS + 32, r1);
+  tmem_ld32(tS + 64, r2);
+  tmem_ld32(tS + 96, r3);
+  wait_ld_dep(r0);
+  wait_ld_dep(r1);
+  wait_ld_dep(r2);
+  wait_ld_dep(r3);
+  float sv[128];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    sv[i] = __uint_as_float(r0[i]);
+    sv[32 + i] = __uint_as_float(r1[i]);
+    sv[64 + i] = __uint_as_float(r2[i]);
+    sv[96 + i] = __uint_as_float(r3[i]);
+  }
+  if (cut) {
+#pragma unroll
+    for (int c = 0; c < 128; ++c)
+      if (c >= lim || !(there >> (c >> 4) & 1)) sv[c] = -INFINITY;
+  }
+  float mx0 = sv[0], mx1 = sv[1], mx2 = sv[2], mx3 = sv[3];
+#pragma unroll
+  for (int c = 4; c < 124; c += 8) {
+    mx0 = fmax3(mx0, sv[c], sv[c + 1]);
+    mx1 = fmax3(mx1, sv[c + 2], sv[c + 3]);
+    mx2 = fmax3(mx2, sv[c + 4], sv[c + 5]);
+    mx3 = fmax3(mx3, sv[c + 6], sv[c + 7]);
+  }
+  mx0 = fmax3(mx0, sv[124], sv[125]);
+  mx1 = fmax3(mx1, sv[126], sv[127]);
+  const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;
+  float resc = 1.f;
+  bool raised = false;
+  if (first) {
+    m_used = mx;
+  } else if (mx > m_used + 8.0f) {  // from -inf too: the O so far is then a sum of zeros
+    resc = ex2(m_used - mx);
+    l *= resc;
+    m_used = mx;
+    raised = true;
+  }
+  const float base = m_used == -INFINITY ? 0.f : -m_used;
+  const uint64_t sl2x2 = f2(sl2, sl2), nmx2 = f2(base, base);
+  uint32_t pk0[32], pk1[32];
+  uint64_t ls0 = f2(0.f, 0.f), ls1 = f2(0.f, 0.f);
+  auto exp_pair = [&](int from, int i, uint32_t& pk, uint64_t& ls) {
+    float x0, x1, a, c;
+    f2_split(fma_f2(f2(sv[from + 2 * i], sv[from + 2 * i + 1]), sl2x2, nmx2), x0, x1);
+    a = ex2(x0);
+    c = ex2(x1);
+    ls = add_f2(ls, f2(a, c));
+    pk = pack2_int<BF16>(a, c);
+  };
+#pragma unroll
+  for (int i = 0; i < 32; ++i) exp_pair(0, i, pk0[i], (i & 1) ? ls1 : ls0);
+  if (__any_sync(0xffffffffu, raised)) {  // warp-collective, as the prompt's own attention does it
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tO + c * 32, o);
+      wait_ld_dep(o);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * resc);
+      tmem_st32(tO + c * 32, o);
+    }
+  }
+  tmem_st32(tS + 0, pk0);
+  tmem_wait_st();
+  tc_fence_before();
+  release(0);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) exp_pair(64, i, pk1[i], (i & 1) ? ls1 : ls0);
+  {
+    float a0, a1, b0, b1;
+    f2_split(ls0, a0, a1);
+    f2_split(ls1, b0, b1);
+    l += (a0 + b0) + (a1 + b1);
+  }
+  tmem_st32(tS + 32, pk1);
+  tmem_wait_st();
+  tc_fence_before();
+  release(1);
+}
+
+// Where a finished row of an item goes: out, or a part in the workspace.
+struct ChunkSink {
+  bool part;
+  long long slot;  // part: index of (CTA, which, tile) * 128 + row
+  float inv;       // out: 1 / l, 0 for a row that sees nothing
+  uint16_t* out;   // out: column 0 of the row's head
+};
+template <int D, bool BF16>
+TKB_DEVFN void chunk_put4(const ChunkParams& p, const ChunkSink& k, int col4, float a, float b, float c, float d) {
+  if (k.part) {
+    // [tile][D / 4][128]: the rows of a warp side by side
+    p.part[(k.slot >> 7) * (D / 4) * 128 + col4 * 128 + (k.slot & 127)] = make_float4(a, b, c, d);
+  } else {
+    uint2 v = make_uint2(0u, 0u);
+    if (k.inv != 0.f) v = make_uint2(pack2<BF16>(a * k.inv, b * k.inv), pack2<BF16>(c * k.inv, d * k.inv));
+    *reinterpret_cast<uint2*>(k.out + col4 * 4) = v;
+  }
+}
+
+// A value of V that is not finite, in a slot that some rows of a tile see and
+// others do not, spoils the products of those others too (0 * inf).  So rows
+// whose O is not finite look whether such a slot lies behind their last one;
+// if one does, their O is computed again from the slots they see alone.  Whole
+// warps call it, `bad` marks the lanes with such a row.
+template <int D, bool BF16>
+__noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int jb, int end, bool bad, int lim, int row,
+                                         int hq, float m, const ChunkSink& sink) {
+  constexpr int E = D / 32;
+  const tkb_kv_cache& c = p.c;
+  const int lane = lane_id();
+  using U = typename std::conditional<E == 4, uint2, uint32_t>::type;
+  auto load = [&](const void* pool, int page, int in, float (&f)[E]) {
+    const U u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(pool) + page_offset(c, page, h) +
+                                            static_cast<long long>(in) * D + lane * E);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      const float2 x = unpack2<BF16>(w[e]);
+      f[2 * e] = x.x;
+      f[2 * e + 1] = x.y;
+    }
+  };
+  auto page_at = [&](int j) {
+    const int pg = c.block_table[static_cast<long long>(b) * c.max_pages + j / c.page_size];
+    return static_cast<unsigned>(pg) < static_cast<unsigned>(c.n_pages) ? pg : -1;
+  };
+  const int from = __reduce_min_sync(0xffffffffu, bad ? max(lim, jb * kChunkBlock) : end);
+  int last = -1;  // the last slot with a value of V that is not finite
+  for (int j = from; j < end; ++j) {
+    const int page = page_at(j);
+    if (page < 0) continue;
+    float v[E];
+    load(c.v, page, j % c.page_size, v);
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) odd |= !(fabsf(v[e]) < INFINITY);
+    if (__any_sync(0xffffffffu, odd)) last = j;
+  }
+  unsigned todo = __ballot_sync(0xffffffffu, bad && last >= lim);
+  for (; todo; todo &= todo - 1) {
+    const int src = __ffs(todo) - 1;
+    const int rl = __shfl_sync(0xffffffffu, lim, src), rr = __shfl_sync(0xffffffffu, row, src),
+              rh = __shfl_sync(0xffffffffu, hq, src);
+    const float rm = __shfl_sync(0xffffffffu, m, src);
+    const float base = rm == -INFINITY ? 0.f : rm;
+    float q[E], o[E];
+    const U u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(p.q) + rr * p.q_stride +
+                                            static_cast<long long>(rh) * D + lane * E);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      const float2 x = unpack2<BF16>(w[e]);
+      q[2 * e] = x.x;
+      q[2 * e + 1] = x.y;
+      o[2 * e] = o[2 * e + 1] = 0.f;
+    }
+    for (int j = jb * kChunkBlock; j < min(rl, end); ++j) {
+      const int page = page_at(j);
+      if (page < 0) continue;
+      float k[E], v[E], s = 0.f;
+      load(c.k, page, j % c.page_size, k);
+      load(c.v, page, j % c.page_size, v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
+      const float pr = ex2(fmaf(warp_sum(s), p.scale_log2, -base));
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(pr, v[e], o[e]);
+    }
+    ChunkSink to;
+    to.part = sink.part;
+    to.slot = __shfl_sync(0xffffffffu, sink.slot, src);
+    to.inv = __shfl_sync(0xffffffffu, sink.inv, src);
+    to.out = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(sink.out), src));
+    __syncwarp();
+    if constexpr (E == 4) {
+      chunk_put4<D, BF16>(p, to, lane, o[0], o[1], o[2], o[3]);
+    } else {
+      const float a = __shfl_down_sync(0xffffffffu, o[0], 1), d = __shfl_down_sync(0xffffffffu, o[1], 1);
+      if (!(lane & 1)) chunk_put4<D, BF16>(p, to, lane >> 1, o[0], o[1], a, d);
+    }
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant__ ChunkParams p) {
+  using C = ChunkCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;
+  uint64_t* k_empty = k_full + C::NST;
+  uint64_t* v_full = k_empty + C::NST;
+  uint64_t* v_empty = v_full + C::NST;
+  uint64_t* s_full = v_empty + C::NST;
+  uint64_t* p_ready = s_full + 2;  // [w][half]
+  uint64_t* o_done = p_ready + 4;
+  uint64_t* x_full = o_done + 2;
+  uint64_t* x_empty = x_full + 1;
+  uint64_t* mma_drain = x_empty + 1;
+  uint32_t* marks = reinterpret_cast<uint32_t*>(smem + C::OFF_MASK);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+  const int warp = warp_id(), lane = lane_id();
+
+  if (threadIdx.x == 0) {
+    for (uint64_t* x : {q_full, q_empty, mma_drain}) mbar_init(x, 1);
+    for (int s = 0; s < C::NST; ++s)
+      for (uint64_t* x : {k_full, k_empty, v_full, v_empty}) mbar_init(x + s, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_ready[2 * w], 128);
+      mbar_init(&p_ready[2 * w + 1], 128);
+      mbar_init(&o_done[w], 1);
+    }
+    mbar_init(x_full, 128);
+    mbar_init(x_empty, 128);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&p.tmQ);
+    prefetch_tmap(&p.tmK);
+    prefetch_tmap(&p.tmV);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  grid_wait();
+  ChunkWalk walk;
+  const bool any = chunk_deal<320>(p, walk);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ChunkItem it;
+
+  if (!any) {
+    if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(0, 0, 0, 0);
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    // A lane issues one box: `gran` slots of one 64-column slab of K or V.
+    const int boxes = kChunkBlock / p.gran, nl = boxes * (D / 64);
+    const int gi = lane % boxes, hh = lane / boxes;
+    const int box_rows = p.gran;
+    const uint32_t q_bytes = static_cast<uint32_t>(p.gb) * p.tt * D * 2;
+    int nq = 0, nk = 0, nv = 0;  // loads issued
+    bool ok = true;
+    while (ok && walk.next(p, it)) {
+      const int h = it.hg / p.hb, hq0 = h * p.G + (it.hg % p.hb) * p.gb;
+      const ChunkSeq& s = walk.s;
+      // read once by a unit alone, or by the units that follow too
+      const uint64_t pol_q = policy_evict_first(), pol_kv = s.units > 1 ? policy_evict_last() : policy_evict_first();
+      const int32_t* table = p.c.block_table + static_cast<long long>(it.b) * p.c.max_pages;
+      // this lane's page in block j: beyond the pool (the box is then zeros) where there is none
+      auto page_in = [&](int j, bool& bad) {
+        const int slot = j * kChunkBlock + gi * box_rows;
+        bad = false;
+        if (lane >= nl || slot >= s.held) return p.c.n_pages;
+        const int pg = __ldg(table + slot / p.c.page_size);
+        bad = static_cast<unsigned>(pg) >= static_cast<unsigned>(p.c.n_pages);
+        return bad ? p.c.n_pages : pg;
+      };
+      bool bad;
+      int page = page_in(it.jb, bad);
+      if (!(ok = mbar_wait_warp(q_empty, (nq & 1) ^ 1, abort_flag))) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full, (it.pair ? 2 : 1) * q_bytes);
+        for (int w = 0; w < (it.pair ? 2 : 1); ++w)
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x)
+            tma_load_3d(smem + C::OFF_Q + w * C::TILE + x * C::SLAB, &p.tmQ, q_full, x * 64, hq0,
+                        s.first + it.t0 + w * p.tt, pol_q);
+      }
+      ++nq;
+      for (int j = it.jb; j < it.je; ++j) {
+        bool bad_next = false;
+        int next = 0;
+        if (j + 1 < it.je) next = page_in(j + 1, bad_next);
+        const int in_head = (j * kChunkBlock + gi * box_rows) % p.c.page_size + h * p.c.page_size;
+        // bits of the 16-slot groups that lie in bad pages
+        const unsigned lost = __reduce_or_sync(0xffffffffu, bad ? ((1u << (box_rows / 16)) - 1) << (gi * box_rows / 16) : 0u);
+        if (lost && lane == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
+        const int sk = nk % C::NST;
+        if (!(ok = mbar_wait_warp(&k_empty[sk], ((nk / C::NST) & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          marks[nk % C::NMASK] = ~lost;
+          mbar_arrive_expect_tx(&k_full[sk], C::TILE);
+        }
+        __syncwarp();
+        if (lane < nl)
+          tma_load_3d(smem + C::OFF_K + sk * C::TILE + hh * C::SLAB + gi * box_rows * 128, &p.tmK, &k_full[sk], hh * 64,
+                      in_head, page, pol_kv);
+        ++nk;
+        const int sv = nv % C::NST;
+        if (!(ok = mbar_wait_warp(&v_empty[sv], ((nv / C::NST) & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&v_full[sv], C::TILE);
+        __syncwarp();
+        if (lane < nl)
+          tma_load_3d(smem + C::OFF_V + sv * C::TILE + hh * C::SLAB + gi * box_rows * 128, &p.tmV, &v_full[sv], hh * 64,
+                      in_head, page, pol_kv);
+        ++nv;
+        page = next;
+        bad = bad_next;
+      }
+    }
+    if (*abort_flag) {
+      // Let every copy this CTA started land before the CTA exits.
+      volatile int never = 0;
+      if (nq) mbar_wait(q_full, (nq - 1) & 1, &never);
+      for (int i = max(0, nk - C::NST); i < nk; ++i) mbar_wait(&k_full[i % C::NST], (i / C::NST) & 1, &never);
+      for (int i = max(0, nv - C::NST); i < nv; ++i) mbar_wait(&v_full[i % C::NST], (i / C::NST) & 1, &never);
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_f16kind(128, 128, BF16, false, false);
+      constexpr uint32_t idO = idesc_f16kind(128, D, BF16, false, true);
+      const uint32_t sQ = sbase + C::OFF_Q, sK = sbase + C::OFF_K, sV = sbase + C::OFF_V;
+      auto issue_S = [&](int w, int tile, int stage) {  // S of warpgroup w: its tile's queries, the stage's keys
+        const uint32_t qa = sQ + tile * C::TILE, ka = sK + stage * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * C::SLAB + (kk & 3) * 32;
+          umma_ss(tmem + (w ? C::TM_S1 : C::TM_S0), sdesc_sw128(qa + off, 16, 1024),
+                  sdesc_sw128(ka + off, 16, 1024), idS, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+      };
+      auto issue_PV = [&](int w, int stage, int half, bool acc) {
+        const uint32_t va = sV + stage * C::TILE;
+        const uint32_t tP = tmem + (w ? C::TM_S1 : C::TM_S0);
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int kk = half * 4 + k4;
+          umma_ts(tmem + (w ? C::TM_O1 : C::TM_O0), tP + kk * 8, sdesc_sw128(va + kk * 2048, C::SLAB, 1024), idO,
+                  (acc || kk > 0) ? 1u : 0u);
+        }
+      };
+      int nq = 0, nk = 0, nv = 0;  // Q tiles, K and V blocks met so far
+      int np[2] = {0, 0};          // blocks of each warpgroup whose P has been used
+      bool ok = true;
+      auto wait_k = [&]() {
+        if (!(ok = mbar_wait(&k_full[nk % C::NST], (nk / C::NST) & 1, abort_flag))) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto half_PV = [&](int w, int half, bool acc) {
+        if (!(ok = mbar_wait(&p_ready[2 * w + half], np[w] & 1, abort_flag))) return false;
+        tc_fence_after();
+        issue_PV(w, nv % C::NST, half, acc);
+        return true;
+      };
+      while (ok && walk.next(p, it)) {
+        if (!(ok = mbar_wait(q_full, nq & 1, abort_flag))) break;
+        ++nq;
+        tc_fence_after();
+        const int jb = it.jb, je = it.je;
+        if (it.pair) {
+          // both warpgroups meet the same blocks, each with its own tile; the first tile's may end earlier
+          const int end[2] = {min(je, it.nb[0]), je};
+          if (!wait_k()) break;
+          for (int w = 0; w < 2; ++w)
+            if (jb < end[w]) issue_S(w, w, nk % C::NST);
+          umma_commit(&k_empty[nk % C::NST]);
+          ++nk;
+          if (jb + 1 == je) umma_commit(q_empty);
+          for (int j = jb; ok && j < je; ++j) {
+            if (!(ok = mbar_wait(&v_full[nv % C::NST], (nv / C::NST) & 1, abort_flag))) break;
+            bool k_next = false;
+            for (int w = 0; w < 2 && ok; ++w) {
+              if (j >= end[w]) continue;
+              if (!half_PV(w, 0, j > jb) || !half_PV(w, 1, true)) break;
+              ++np[w];
+              if (j + 1 == end[w]) umma_commit(&o_done[w]);
+              if (j + 1 < end[w]) {
+                if (!k_next && !wait_k()) break;
+                k_next = true;
+                issue_S(w, w, nk % C::NST);
+              }
+            }
+            if (!ok) break;
+            umma_commit(&v_empty[nv % C::NST]);
+            ++nv;
+            if (k_next) {
+              umma_commit(&k_empty[nk % C::NST]);
+              ++nk;
+              if (j + 2 == je) umma_commit(q_empty);
+            }
+          }
+        } else {
+          // the warpgroups take the blocks of the one tile in turn
+          const int n = je - jb;
+          for (int i = 0; i < min(n, 2); ++i) {
+            if (!wait_k()) break;
+            issue_S(i, 0, nk % C::NST);
+            umma_commit(&k_empty[nk % C::NST]);
+            ++nk;
+          }
+          if (ok && n <= 2) umma_commit(q_empty);
+          for (int i = 0; ok && i < n; ++i) {
+            const int w = i & 1;
+            if (!(ok = mbar_wait(&v_full[nv % C::NST], (nv / C::NST) & 1, abort_flag))) break;
+            if (!half_PV(w, 0, i > 1) || !half_PV(w, 1, true)) break;
+            ++np[w];
+            umma_commit(&v_empty[nv % C::NST]);
+            ++nv;
+            if (i + 2 >= n) umma_commit(&o_done[w]);
+            if (i + 2 < n) {
+              if (!wait_k()) break;
+              issue_S(w, 0, nk % C::NST);
+              umma_commit(&k_empty[nk % C::NST]);
+              ++nk;
+              if (i + 3 == n) umma_commit(q_empty);
+            }
+          }
+        }
+      }
+      if (!ok) {
+        // Make sure no MMA is still running when TMEM is released.
+        volatile int never = 0;
+        umma_commit(mma_drain);
+        mbar_wait(mma_drain, 0, &never);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax warpgroups
+    const int w = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_off + (w ? C::TM_S1 : C::TM_S0);
+    const uint32_t tO = tmem + lane_off + (w ? C::TM_O1 : C::TM_O0);
+    float4* xo = reinterpret_cast<float4*>(smem + C::OFF_X);
+    float2* xml = reinterpret_cast<float2*>(smem + C::OFF_XML);
+    const float sl2 = p.scale_log2;
+    int ns = 0, no = 0, nb = 0, nx = 0;  // blocks of this warpgroup, items with blocks of it, blocks of the CTA, exchanges
+    int flags = 0, span_b = 0, span_hg = 0, span_u = 0;
+    bool ok = true;
+    while (ok && walk.next(p, it)) {
+      const ChunkSeq& s = walk.s;
+      const int tile = it.pair ? w : 0;
+      int tok, hq;
+      const bool valid = chunk_row(p, s, it.hg, it.t0, it.tokens, tile, r, tok, hq);
+      const int lim = valid ? min(max(s.base + tok + 1, 0), s.held) : 0;
+      const bool busy = __any_sync(0xffffffffu, valid);  // a warp without rows leaves its P as it is: nobody reads its O
+      const int tile_lim = min(max(s.base + it.t0 + tile * p.tt + 1, 0), s.held);  // what the tile's first row sees
+      const int step = it.pair ? 1 : 2, j0 = it.jb + (it.pair ? 0 : w), end = it.pair ? min(it.je, it.nb[w]) : it.je;
+      float m = -INFINITY, l = 0.f;
+      for (int j = j0; j < end; j += step) {
+        const int at = j * kChunkBlock, nth = nb + j - it.jb;
+        if (!(ok = mbar_wait_warp(&s_full[w], ns & 1, abort_flag))) break;
+        tc_fence_after();
+        if (at + kChunkBlock > s.held) {
+          // slots of the last page behind the sequence's end may hold anything, and 0 * NaN is NaN: V there becomes 0
+          const int stage = nth % C::NST;
+          if (!(ok = mbar_wait_warp(&v_full[stage], (nth / C::NST) & 1, abort_flag))) break;
+          const int from = max(s.held - at, 0);
+          for (int i = from * 8 + r; i < kChunkBlock * 8; i += 128)
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x)
+              *reinterpret_cast<uint4*>(smem + C::OFF_V + stage * C::TILE + x * C::SLAB + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        const unsigned there = *reinterpret_cast<volatile uint32_t*>(&marks[nth % C::NMASK]);
+        auto release = [&](int half) { mbar_arrive(&p_ready[2 * w + half]); };
+        if (busy) {
+          chunk_softmax<D, BF16>(tS, tO, sl2, j == j0, at + kChunkBlock > tile_lim || there != ~0u, lim - at, there, m, l,
+                                 release);
+        } else {
+          release(0);
+          release(1);
+        }
+        ++ns;
+      }
+      if (!ok) break;
+      nb += it.je - it.jb;
+      const bool has = j0 < end;
+      if (has) {
+        if (!(ok = mbar_wait_warp(&o_done[w], no & 1, abort_flag))) break;
+        ++no;
+        tc_fence_after();
+      }
+      // ---- the warpgroups' halves of a single tile meet: the second hands over its m, l and O, half of the columns at a time
+      const bool meet = !it.pair && it.je - it.jb > 1;
+      float f0 = 1.f, f1 = 0.f;
+      bool sees0 = true, sees1 = false;  // a half that saw nothing has an O of masked values alone
+      if (!it.pair && w == 1) {
+        if (meet) {
+          xml[r] = make_float2(m, l);
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = mbar_wait_warp(x_empty, (nx & 1) ^ 1, abort_flag))) break;
+#pragma unroll 1
+            for (int c = 0; c < D / 64; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + half * (D / 2) + c * 32, o);
+              wait_ld_dep(o);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                xo[(c * 8 + i) * 128 + r] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            }
+            mbar_arrive(x_full);
+            ++nx;
+          }
+          if (!ok) break;
+        }
+        continue;
+      }
+      // ---- the tile's rows go out
+      ChunkSink sink;
+      sink.part = !it.whole();
+      const int which = it.jb > 0 ? 0 : 1;
+      sink.slot = ((2ll * blockIdx.x + which) * 2 + tile) * 128 + r;
+      if (sink.part) {
+        flags |= which ? SPAN_BEGINS : SPAN_GOES_ON | (it.je == it.nb[1] ? SPAN_ENDS : 0);
+        if (which) {
+          span_b = it.b;
+          span_hg = it.hg;
+          span_u = it.u;
+        }
+      }
+      const int row = s.first + tok;
+      sink.out = static_cast<uint16_t*>(p.out) + (valid ? row * p.out_stride + static_cast<long long>(hq) * D : 0);
+      bool odd = false;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        if (meet && c % (D / 64) == 0) {  // the next half of the other's columns
+          if (!(ok = mbar_wait_warp(x_full, nx & 1, abort_flag))) break;
+          if (c == 0) {
+            const float2 ml = xml[r];
+            const float mm = fmaxf(m, ml.x);
+            sees0 = m != -INFINITY;
+            sees1 = ml.x != -INFINITY;
+            f0 = sees0 ? ex2(m - mm) : 0.f;
+            f1 = sees1 ? ex2(ml.x - mm) : 0.f;
+            l = f0 * l + f1 * ml.y;
+            m = m != m ? m : mm;
+          }
+        }
+        if (c == 0) {
+          sink.inv = l == 0.f ? 0.f : 1.f / l;
+          if (valid) {
+            if (sink.part) p.part_ml[sink.slot] = make_float2(m, l);
+            else if (p.lse) p.lse[static_cast<long long>(row) * p.Hq + hq] = (m + lg2(l)) * 0.69314718055994531f;
+          }
+        }
+        if (has) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          wait_ld_dep(o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = __uint_as_float(o[4 * i + e]);
+            if (meet) {
+              const float4 x = xo[(c % (D / 64) * 8 + i) * 128 + r];
+              const float b[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) a[e] = (sees0 ? f0 * a[e] : 0.f) + (sees1 ? f1 * b[e] : 0.f);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= !(fabsf(a[e]) < INFINITY);
+            if (valid) chunk_put4<D, BF16>(p, sink, c * 8 + i, a[0], a[1], a[2], a[3]);
+          }
+        }
+        if (meet && (c + 1) % (D / 64) == 0) {
+          mbar_arrive(x_empty);
+          ++nx;
+        }
+      }
+      if (!ok) break;
+      // O that is not finite though l is: look behind the row's last slot
+      const int last = min(end * kChunkBlock, s.held);
+      const bool bad = has && odd && valid && l > 0.f && lim < last;
+      if (__any_sync(0xffffffffu, bad))
+        chunk_again<D, BF16>(p, it.b, it.hg / p.hb, it.jb, last, bad, lim, row, hq, m, sink);
+    }
+    if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(ok ? flags : 0, span_b, span_hg, span_u);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of units that span CTAs: the block of CTA c takes the unit
+// that begins there and goes on behind it, with the parts of the CTAs that
+// follow up to the one that ends it, in their order.  A thread has one row and
+// 32 columns; blockIdx.y is tile and column group.
+template <int D, typename T>
+__global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+  grid_wait();
+  const int c = blockIdx.x, w = blockIdx.y / (D / 32), cg = blockIdx.y % (D / 32), r = threadIdx.x;
+  const int4 span = p.span[c];
+  if (!(span.x & SPAN_BEGINS)) return;
+  const ChunkSeq s = chunk_seq(p, span.y);
+  const int t0 = span.w * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
+  int tok, hq;
+  if (!chunk_row(p, s, span.z, t0, tokens, w, r, tok, hq)) return;
+  // CTA c's second part, then the first parts of those that follow
+  float m = -INFINITY, l = 0.f, o[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) o[i] = 0.f;
+  int flags = 0;
+  for (int x = c; x < gridDim.x && !(flags & SPAN_ENDS); ++x) {
+    if (x > c) {
+      flags = p.span[x].x;
+      if (!(flags & SPAN_GOES_ON)) continue;  // a run too short to hold a block
+    }
+    const long long slot = ((2ll * x + (x == c ? 1 : 0)) * 2 + w) * 128;
+    const float2 ml = p.part_ml[slot + r];
+    if (ml.x == -INFINITY) continue;  // it saw nothing
+    const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : ex2(m - mm), f1 = ex2(ml.x - mm);
+    l = f0 * l + f1 * ml.y;
+    m = mm;
+    const float4* part = p.part + slot / 128 * (D / 4) * 128 + cg * 8 * 128 + r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = part[i * 128];
+      o[4 * i] = fmaf(f1, v.x, f0 * o[4 * i]);
+      o[4 * i + 1] = fmaf(f1, v.y, f0 * o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(f1, v.z, f0 * o[4 * i + 2]);
+      o[4 * i + 3] = fmaf(f1, v.w, f0 * o[4 * i + 3]);
+    }
+  }
+  const long long row = s.first + tok;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(p.out) + row * p.out_stride + static_cast<long long>(hq) * D + cg * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = l == 0.f ? 0.f : o[i + e] * inv;
+    stv<T, 8>(out + i, v);
+  }
+  if (p.lse && cg == 0) p.lse[row * p.Hq + hq] = (m + lg2(l)) * 0.69314718055994531f;
+}
+
+// ============================================================ fp32
 template <typename T, int E>
 TKB_DEVFN void lane_values(const T* p, float (&f)[E]) {
 #pragma unroll
@@ -98,10 +996,72 @@ __global__ void __launch_bounds__(256) chunk_simple_kernel(const __grid_constant
   }
 }
 
+template <int D, typename T>
+static cudaError_t chunk_tc(const ChunkParams& p, cudaStream_t st) {
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  cudaError_t e = allow_smem<chunk_tc_kernel<D, BF16>>(ChunkCfg<D>::SMEM);
+  if (e == cudaSuccess) e = launch_early(chunk_tc_kernel<D, BF16>, dim3(kChunkGrid), 320, ChunkCfg<D>::SMEM, st, p);
+  if (e == cudaSuccess) e = launch_early(chunk_join_kernel<D, T>, dim3(kChunkGrid, 2 * D / 32), 128, 0, st, p);
+  return e;
+}
+
+// A 3-D map over 16-bit elements; the first dimension is contiguous, strides in elements.
+static cudaError_t chunk_tmap(CUtensorMap* m, const void* base, bool bf16, const long long (&dims)[3],
+                              const long long (&strides)[2], int box1, int box2) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const cuuint64_t d[3] = {static_cast<cuuint64_t>(dims[0]), static_cast<cuuint64_t>(dims[1]),
+                           static_cast<cuuint64_t>(dims[2])};
+  const cuuint64_t s[2] = {static_cast<cuuint64_t>(strides[0] * 2), static_cast<cuuint64_t>(strides[1] * 2)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box1), static_cast<cuuint32_t>(box2)}, one[3] = {1, 1, 1};
+  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// Layout of the workspace.
+struct ChunkWs {
+  size_t ml, span, bytes;
+};
+static ChunkWs chunk_ws(const tkb_kv_cache& c) {
+  ChunkWs w;
+  const size_t tiles = 2 * kChunkGrid * 2;
+  w.ml = tiles * 128 * c.D * 4;
+  w.span = w.ml + tiles * 128 * sizeof(float2);
+  w.bytes = w.span + kChunkGrid * sizeof(int4);
+  return w;
+}
+
+// Launches, and how many kernels they were.
 template <typename T>
-static cudaError_t paged_chunk_t(const ChunkParams& p, cudaStream_t st) {
-  if (p.c.D == 64) return launch_early(chunk_simple_kernel<T, 64>, dim3(p.rows), 256, 0, st, p);
-  return launch_early(chunk_simple_kernel<T, 128>, dim3(p.rows), 256, 0, st, p);
+static cudaError_t paged_chunk_t(ChunkParams& p, void* workspace, cudaStream_t st, unsigned& kernels) {
+  const int D = p.c.D;
+  if constexpr (sizeof(T) == 4) {
+    kernels = 1;
+    return D == 64 ? launch_early(chunk_simple_kernel<T, 64>, dim3(p.rows), 256, 0, st, p)
+                   : launch_early(chunk_simple_kernel<T, 128>, dim3(p.rows), 256, 0, st, p);
+  } else {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    const ChunkWs w = chunk_ws(p.c);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.part = reinterpret_cast<float4*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+    p.span = reinterpret_cast<int4*>(ws + w.span);
+    p.hb = (p.G + 127) / 128;
+    p.gb = (p.G + p.hb - 1) / p.hb;
+    p.tt = 128 / p.gb;
+    p.gran = kChunkBlock;
+    while (p.c.page_size % p.gran) p.gran /= 2;
+    cudaError_t e = chunk_tmap(&p.tmQ, p.q, BF16, {D, p.Hq, p.rows}, {D, p.q_stride}, p.gb, p.tt);
+    const long long heads = static_cast<long long>(p.c.Hkv) * p.c.page_size;
+    if (e == cudaSuccess) e = chunk_tmap(&p.tmK, p.c.k, BF16, {D, heads, p.c.n_pages}, {D, p.c.page_stride}, p.gran, 1);
+    if (e == cudaSuccess) e = chunk_tmap(&p.tmV, p.c.v, BF16, {D, heads, p.c.n_pages}, {D, p.c.page_stride}, p.gran, 1);
+    kernels = 2;
+    if (e != cudaSuccess) return e;
+    return D == 64 ? chunk_tc<64, T>(p, st) : chunk_tc<128, T>(p, st);
+  }
 }
 
 }  // namespace tkb
