@@ -94,7 +94,6 @@ constexpr int kCostLeast = 6;     // a CTA's run at least: shorter ones cost mor
 struct ChunkSeq {
   int first, n, base, held;
   int units;
-  long long cost;  // of one head group
 };
 TKB_DEVFN int chunk_blocks(int base, int upto) {  // blocks for a row that sees base + upto slots; at least one
   return 1 + (max(base, 0) + upto - 1) / kChunkBlock;
@@ -104,9 +103,9 @@ TKB_DEVFN long long chunk_cost_before(const ChunkParams& p, const ChunkSeq& s, i
   return static_cast<long long>(u) * (kCostUnit + kCostPair) +
          kCostPair * floor_sum(u, kChunkBlock, per, static_cast<long long>(max(s.base, 0)) + per - 1);
 }
-TKB_DEVFN long long chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
+TKB_DEVFN int chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
   const int t0 = u * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
-  return kCostUnit + static_cast<long long>(tokens > p.tt ? kCostPair : 1) * chunk_blocks(s.base, t0 + tokens);
+  return kCostUnit + (tokens > p.tt ? kCostPair : 1) * chunk_blocks(s.base, t0 + tokens);
 }
 TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   ChunkSeq s;
@@ -119,8 +118,10 @@ TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   s.held = min(max(held, 0), most);
   s.base = min(held, most + s.n) - s.n;
   s.units = (s.n + 2 * p.tt - 1) / (2 * p.tt);
-  s.cost = s.n ? chunk_cost_before(p, s, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
   return s;
+}
+TKB_DEVFN long long chunk_seq_cost(const ChunkParams& p, const ChunkSeq& s) {  // of one head group
+  return s.n ? chunk_cost_before(p, s, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
 }
 
 // One unit's share of a CTA's run.
@@ -132,12 +133,21 @@ struct ChunkItem {
   bool pair;               // two tiles
   TKB_DEVFN bool whole() const { return jb == 0 && je == nb[1]; }
 };
-// Walks the items of a run; every role of the CTA walks for itself.
+// Walks the items of a run.  Every warp walks for itself, its state in shared
+// memory: a lane steps it, and the registers are the softmax's.
 struct ChunkWalk {
   ChunkSeq s;
+  ChunkItem it;
   int b, hg, u;
+  int more;
   long long at, x0, x1;    // cost where the unit starts, where the run does and ends
-  TKB_DEVFN bool next(const ChunkParams& p, ChunkItem& it) {
+  TKB_DEVFN bool next(const ChunkParams& p) {
+    __syncwarp();
+    if (lane_id() == 0) more = step(p);
+    __syncwarp();
+    return more;
+  }
+  TKB_DEVFN bool step(const ChunkParams& p) {
     while (at < x1) {
       if (u == s.units) {
         u = 0;
@@ -149,7 +159,7 @@ struct ChunkWalk {
           } while (s.n == 0);
         }
       }
-      const long long cost = chunk_cost(p, s, u);
+      const int cost = chunk_cost(p, s, u);
       it.b = b;
       it.hg = hg;
       it.u = u;
@@ -158,12 +168,12 @@ struct ChunkWalk {
       it.pair = it.tokens > p.tt;
       it.nb[0] = chunk_blocks(s.base, it.t0 + min(it.tokens, p.tt));
       it.nb[1] = chunk_blocks(s.base, it.t0 + it.tokens);
-      const int w = it.pair ? kCostPair : 1;
-      auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later
-        return x <= kCostUnit ? 0 : static_cast<int>((x - kCostUnit + w - 1) / w);
+      auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later, x below its cost
+        const int y = static_cast<int>(x) - kCostUnit;
+        return it.pair ? (y + kCostPair - 1) / kCostPair : y;
       };
-      it.jb = block_at(x0 - at);
-      it.je = x1 - at >= cost ? it.nb[1] : min(it.nb[1], block_at(x1 - at));
+      it.jb = x0 <= at + kCostUnit ? 0 : x0 - at >= cost ? it.nb[1] : block_at(x0 - at);
+      it.je = x1 <= at + kCostUnit ? 0 : x1 - at >= cost ? it.nb[1] : block_at(x1 - at);
       at += cost;
       ++u;
       if (it.jb < it.je) return true;
@@ -172,7 +182,7 @@ struct ChunkWalk {
   }
 };
 
-// The run of this CTA; false when it has none.  All threads of the block (NT_ of them) call it.
+// The run of this CTA, into each warp's walk; false when it has none.  All threads of the block (NT_ of them) call it.
 template <int NT_>
 TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
   __shared__ long long s_sum[NT_ / 32], s_x[3];
@@ -184,7 +194,7 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
   ChunkSeq s;
   for (int b = b0; b < b1; ++b) {
     s = chunk_seq(p, b);
-    mine += s.cost * groups;
+    mine += chunk_seq_cost(p, s) * groups;
   }
   long long upto = mine;
 #pragma unroll
@@ -207,9 +217,10 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
   if (at <= x0 && x0 < upto) {  // the run starts in one of this thread's sequences
     for (int b = b0; b < b1; ++b) {
       s = chunk_seq(p, b);
-      if (x0 < at + s.cost * groups) {
-        const int hg = static_cast<int>((x0 - at) / s.cost);
-        at += s.cost * hg;
+      const long long cost = chunk_seq_cost(p, s);
+      if (x0 < at + cost * groups) {
+        const int hg = static_cast<int>((x0 - at) / cost);
+        at += cost * hg;
         int lo = 0, hi = s.units - 1;  // last unit that starts at x0 or before
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
@@ -222,17 +233,19 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
         s_x[0] = at + chunk_cost_before(p, s, lo);
         break;
       }
-      at += s.cost * groups;
+      at += cost * groups;
     }
   }
   __syncthreads();
-  w.b = s_at[0];
-  w.hg = s_at[1];
-  w.u = s_at[2];
-  w.at = s_x[0];
-  w.x0 = x0;
-  w.x1 = x1;
-  w.s = chunk_seq(p, w.b);
+  if (lane == 0) {
+    w.b = s_at[0];
+    w.hg = s_at[1];
+    w.u = s_at[2];
+    w.at = s_x[0];
+    w.x0 = x0;
+    w.x1 = x1;
+    w.s = chunk_seq(p, w.b);
+  }
   return true;
 }
 
@@ -258,15 +271,16 @@ struct ChunkCfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + NST * TILE;
-  static constexpr int OFF_X = OFF_V + NST * TILE;       // half of the second warpgroup's O, [D / 8][128] float4
-  static constexpr int OFF_XML = OFF_X + 128 * (D / 2) * 4;
+  static constexpr int OFF_X = OFF_V + NST * TILE;       // 32 columns of the second warpgroup's O, [8][128] float4
+  static constexpr int OFF_XML = OFF_X + 128 * 32 * 4;
   static constexpr int OFF_BAR = OFF_XML + 128 * 8;
   // q_full, q_empty, k_full[NST], k_empty[NST], v_full[NST], v_empty[NST], s_full[2], p_ready[2][2], o_done[2],
   // x_full, x_empty, drain
   static constexpr int NBAR = 2 + 4 * NST + 8 + 3;
   static constexpr int NMASK = 16;                       // page marks of the newest blocks (more than are in flight)
   static constexpr int OFF_MASK = OFF_BAR + NBAR * 8;
-  static constexpr int OFF_MISC = OFF_MASK + NMASK * 4;
+  static constexpr int OFF_WALK = (OFF_MASK + NMASK * 4 + 7) / 8 * 8;
+  static constexpr int OFF_MISC = OFF_WALK + 10 * sizeof(ChunkWalk);
   static constexpr int SMEM = OFF_MISC + 16 + 1024;      // + slack for 1024-byte alignment
   static_assert(SMEM <= 232448, "tiles exceed 227 KB of shared memory");
   static constexpr uint32_t TM_S0 = 0, TM_S1 = 128, TM_O0 = 256, TM_O1 = 256 + D;
@@ -353,8 +367,13 @@ TKB_DEVFN void chunk_softmax(uint32_t tS, uint32_t tO, float sl2, bool first, bo
   tmem_wait_st();
   tc_fence_before();
   release(0);
+  if (cut && __all_sync(0xffffffffu, lim <= 64)) {  // nothing of the second half is seen
 #pragma unroll
-  for (int i = 0; i < 32; ++i) exp_pair(64, i, pk1[i], (i & 1) ? ls1 : ls0);
+    for (int i = 0; i < 32; ++i) pk1[i] = 0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) exp_pair(64, i, pk1[i], (i & 1) ? ls1 : ls0);
+  }
   {
     float a0, a1, b0, b1;
     f2_split(ls0, a0, a1);
@@ -384,6 +403,28 @@ TKB_DEVFN void chunk_put4(const ChunkParams& p, const ChunkSink& k, int col4, fl
     if (k.inv != 0.f) v = make_uint2(pack2<BF16>(a * k.inv, b * k.inv), pack2<BF16>(c * k.inv, d * k.inv));
     *reinterpret_cast<uint2*>(k.out + col4 * 4) = v;
   }
+}
+
+// Lane i of four holds row i's chunks 0..3; after it, chunk i of rows 0..3.
+TKB_DEVFN void quad_transpose(uint4 (&v)[4]) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(v);
+  const bool odd = lane_id() & 1, high = lane_id() & 2;
+#pragma unroll
+  for (int k = 0; k < 4; k += 2)  // chunks k, k + 1 with the neighbour
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[4 * k + e] : w[4 * k + 4 + e], 1);
+      w[4 * k + e] = odd ? got : w[4 * k + e];
+      w[4 * k + 4 + e] = odd ? w[4 * k + 4 + e] : got;
+    }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)  // chunks k, k + 2 with the lane two on
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? w[4 * k + e] : w[4 * k + 8 + e], 2);
+      w[4 * k + e] = high ? got : w[4 * k + e];
+      w[4 * k + 8 + e] = high ? w[4 * k + 8 + e] : got;
+    }
 }
 
 // A value of V that is not finite, in a slot that some rows of a tile see and
@@ -517,13 +558,13 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     tmem_relinquish();
   }
   grid_wait();
-  ChunkWalk walk;
+  ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * static_cast<int>(sizeof(ChunkWalk)));
+  const ChunkItem& it = walk.it;
   const bool any = chunk_deal<320>(p, walk);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  ChunkItem it;
 
   if (!any) {
     if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -536,7 +577,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     const uint32_t q_bytes = static_cast<uint32_t>(p.gb) * p.tt * D * 2;
     int nq = 0, nk = 0, nv = 0;  // loads issued
     bool ok = true;
-    while (ok && walk.next(p, it)) {
+    while (ok && walk.next(p)) {
       const int h = it.hg / p.hb, hq0 = h * p.G + (it.hg % p.hb) * p.gb;
       const ChunkSeq& s = walk.s;
       // read once by a unit alone, or by the units that follow too
@@ -603,7 +644,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    if (lane == 0) {  // steps its walk alone
       constexpr uint32_t idS = idesc_f16kind(128, 128, BF16, false, false);
       constexpr uint32_t idO = idesc_f16kind(128, D, BF16, false, true);
       const uint32_t sQ = sbase + C::OFF_Q, sK = sbase + C::OFF_K, sV = sbase + C::OFF_V;
@@ -641,7 +682,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         issue_PV(w, nv % C::NST, half, acc);
         return true;
       };
-      while (ok && walk.next(p, it)) {
+      while (ok && walk.step(p)) {
         if (!(ok = mbar_wait(q_full, nq & 1, abort_flag))) break;
         ++nq;
         tc_fence_after();
@@ -725,7 +766,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     int ns = 0, no = 0, nb = 0, nx = 0;  // blocks of this warpgroup, items with blocks of it, blocks of the CTA, exchanges
     int flags = 0, span_b = 0, span_hg = 0, span_u = 0;
     bool ok = true;
-    while (ok && walk.next(p, it)) {
+    while (ok && walk.next(p)) {
       const ChunkSeq& s = walk.s;
       const int tile = it.pair ? w : 0;
       int tok, hq;
@@ -769,7 +810,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         ++no;
         tc_fence_after();
       }
-      // ---- the warpgroups' halves of a single tile meet: the second hands over its m, l and O, half of the columns at a time
+      // ---- the warpgroups' halves of a single tile meet: the second hands over its m, l and O, 32 columns at a time
       const bool meet = !it.pair && it.je - it.jb > 1;
       float f0 = 1.f, f1 = 0.f;
       bool sees0 = true, sees1 = false;  // a half that saw nothing has an O of masked values alone
@@ -777,22 +818,18 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         if (meet) {
           xml[r] = make_float2(m, l);
 #pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
+          for (int c = 0; c < D / 32; ++c) {
             if (!(ok = mbar_wait_warp(x_empty, (nx & 1) ^ 1, abort_flag))) break;
-#pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + half * (D / 2) + c * 32, o);
-              wait_ld_dep(o);
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            wait_ld_dep(o);
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                xo[(c * 8 + i) * 128 + r] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-            }
+            for (int i = 0; i < 8; ++i)
+              xo[i * 128 + r] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                            __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
             mbar_arrive(x_full);
             ++nx;
           }
-          if (!ok) break;
         }
         continue;
       }
@@ -812,9 +849,19 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       const int row = s.first + tok;
       sink.out = static_cast<uint16_t*>(p.out) + (valid ? row * p.out_stride + static_cast<long long>(hq) * D : 0);
       bool odd = false;
+      // four lanes write one row's 64 bytes: where the rows of this lane's quad go (16 bytes a lane), null for none
+      uint16_t* rows4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        rows4[i] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(valid ? sink.out : nullptr),
+                                                           (lane & ~3) + i));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (rows4[i]) rows4[i] += (lane & 3) * 8;
+      float4* part = p.part + (sink.slot >> 7) * (D / 4) * 128 + r;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
-        if (meet && c % (D / 64) == 0) {  // the next half of the other's columns
+        if (meet) {  // the other's columns
           if (!(ok = mbar_wait_warp(x_full, nx & 1, abort_flag))) break;
           if (c == 0) {
             const float2 ml = xml[r];
@@ -838,23 +885,38 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
           wait_ld_dep(o);
+          if (meet) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float a[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] = __uint_as_float(o[4 * i + e]);
-            if (meet) {
-              const float4 x = xo[(c % (D / 64) * 8 + i) * 128 + r];
+            for (int i = 0; i < 8; ++i) {
+              const float4 x = xo[i * 128 + r];
               const float b[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) a[e] = (sees0 ? f0 * a[e] : 0.f) + (sees1 ? f1 * b[e] : 0.f);
+              for (int e = 0; e < 4; ++e)
+                o[4 * i + e] = __float_as_uint((sees0 ? f0 * __uint_as_float(o[4 * i + e]) : 0.f) + (sees1 ? f1 * b[e] : 0.f));
             }
+          }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= !(fabsf(a[e]) < INFINITY);
-            if (valid) chunk_put4<D, BF16>(p, sink, c * 8 + i, a[0], a[1], a[2], a[3]);
+          for (int i = 0; i < 32; ++i) odd |= !(fabsf(__uint_as_float(o[i])) < INFINITY);
+          if (sink.part) {
+            if (valid) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                part[(c * 8 + i) * 128] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                      __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+            }
+          } else {
+            uint4 v[4];
+            uint32_t* vw = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              vw[i] = sink.inv == 0.f ? 0u : pack2<BF16>(__uint_as_float(o[2 * i]) * sink.inv, __uint_as_float(o[2 * i + 1]) * sink.inv);
+            quad_transpose(v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (rows4[i]) *reinterpret_cast<uint4*>(rows4[i] + c * 32) = v[i];
           }
         }
-        if (meet && (c + 1) % (D / 64) == 0) {
+        if (meet) {
           mbar_arrive(x_empty);
           ++nx;
         }
