@@ -98,10 +98,9 @@ struct ChunkSeq {
 TKB_DEVFN int chunk_blocks(int base, int upto) {  // blocks for a row that sees base + upto slots; at least one
   return 1 + (max(base, 0) + upto - 1) / kChunkBlock;
 }
-TKB_DEVFN long long chunk_cost_before(const ChunkParams& p, const ChunkSeq& s, int u) {  // of the first u (full) units
-  const int per = 2 * p.tt;
+__noinline__ __device__ long long chunk_cost_before(int per, int base, int u) {  // of the first u (full) units
   return static_cast<long long>(u) * (kCostUnit + kCostPair) +
-         kCostPair * floor_sum(u, kChunkBlock, per, static_cast<long long>(max(s.base, 0)) + per - 1);
+         kCostPair * floor_sum(u, kChunkBlock, per, static_cast<long long>(max(base, 0)) + per - 1);
 }
 TKB_DEVFN int chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
   const int t0 = u * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
@@ -121,7 +120,7 @@ TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   return s;
 }
 TKB_DEVFN long long chunk_seq_cost(const ChunkParams& p, const ChunkSeq& s) {  // of one head group
-  return s.n ? chunk_cost_before(p, s, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
+  return s.n ? chunk_cost_before(2 * p.tt, s.base, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
 }
 
 // One unit's share of a CTA's run.
@@ -185,66 +184,77 @@ struct ChunkWalk {
 // The run of this CTA, into each warp's walk; false when it has none.  All threads of the block (NT_ of them) call it.
 template <int NT_>
 TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
-  __shared__ long long s_sum[NT_ / 32], s_x[3];
+  __shared__ long long s_sum[NT_ / 32], s_x;
   __shared__ int s_at[3];
+  __shared__ ChunkSeq s_seq;
   const int tid = threadIdx.x, lane = lane_id(), wid = warp_id();
   const int per = (p.c.B + NT_ - 1) / NT_, b0 = min(tid * per, p.c.B), b1 = min(b0 + per, p.c.B);
   const int groups = p.c.Hkv * p.hb;
-  long long mine = 0;
-  ChunkSeq s;
-  for (int b = b0; b < b1; ++b) {
-    s = chunk_seq(p, b);
-    mine += chunk_seq_cost(p, s) * groups;
-  }
-  long long upto = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += y;
-  }
-  if (lane == 31) s_sum[wid] = upto;
-  __syncthreads();
-  long long total = 0;
-  for (int i = 0; i < NT_ / 32; ++i) {
-    if (i == wid) upto += total;
-    total += s_sum[i];
-  }
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + kCostLeast - 1) / kCostLeast));
-  const int c = blockIdx.x;
-  if (c >= ctas) return false;
-  const long long x0 = total * c / ctas, x1 = total * (c + 1) / ctas;
-  long long at = upto - mine;
-  if (at <= x0 && x0 < upto) {  // the run starts in one of this thread's sequences
+  long long at = 0, x0 = 0, x1 = 0;
+  // first the costs of this thread's sequences, then, with the sums over all, the one the run starts in
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    long long upto = at;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-      s = chunk_seq(p, b);
+      const ChunkSeq s = chunk_seq(p, b);
       const long long cost = chunk_seq_cost(p, s);
-      if (x0 < at + cost * groups) {
-        const int hg = static_cast<int>((x0 - at) / cost);
-        at += cost * hg;
+      if (pass && upto <= x0 && x0 < upto + cost * groups) {
+        int hg = 0;
+        while (x0 >= upto + cost) {
+          upto += cost;
+          ++hg;
+        }
         int lo = 0, hi = s.units - 1;  // last unit that starts at x0 or before
+#pragma unroll 1
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
-          if (at + chunk_cost_before(p, s, mid) <= x0) lo = mid;
+          if (upto + chunk_cost_before(2 * p.tt, s.base, mid) <= x0) lo = mid;
           else hi = mid - 1;
         }
         s_at[0] = b;
         s_at[1] = hg;
         s_at[2] = lo;
-        s_x[0] = at + chunk_cost_before(p, s, lo);
+        s_x = upto + chunk_cost_before(2 * p.tt, s.base, lo);
+        s_seq = s;
         break;
       }
-      at += cost * groups;
+      upto += cost * groups;
     }
+    if (pass) break;
+    const long long mine = upto;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    if (lane == 31) s_sum[wid] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll 1
+    for (int i = 0; i < NT_ / 32; ++i) {
+      if (i == wid) upto += total;
+      total += s_sum[i];
+    }
+    const int ctas = total < static_cast<long long>(gridDim.x) * kCostLeast
+                         ? (static_cast<int>(total) + kCostLeast - 1) / kCostLeast : gridDim.x;
+    const int c = blockIdx.x;
+    if (c >= ctas) return false;
+    // total * c / ctas
+    const long long each = total / ctas, rest = total - each * ctas;
+    x0 = each * c + static_cast<int>(rest) * c / ctas;
+    x1 = each * (c + 1) + static_cast<int>(rest) * (c + 1) / ctas;
+    at = upto - mine;
   }
   __syncthreads();
   if (lane == 0) {
     w.b = s_at[0];
     w.hg = s_at[1];
     w.u = s_at[2];
-    w.at = s_x[0];
+    w.at = s_x;
     w.x0 = x0;
     w.x1 = x1;
-    w.s = chunk_seq(p, w.b);
+    w.s = s_seq;
   }
   return true;
 }
@@ -285,6 +295,14 @@ struct ChunkCfg {
   static_assert(SMEM <= 232448, "tiles exceed 227 KB of shared memory");
   static constexpr uint32_t TM_S0 = 0, TM_S1 = 128, TM_O0 = 256, TM_O1 = 256 + D;
 };
+
+TKB_DEVFN void wait_ld16_dep(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 
 // One block of the online softmax for this thread's query row: S from TMEM,
 // slots from `lim` on and those of bad pages (bits of `there`, 16 slots each) masked, the
@@ -405,36 +423,14 @@ TKB_DEVFN void chunk_put4(const ChunkParams& p, const ChunkSink& k, int col4, fl
   }
 }
 
-// Lane i of four holds row i's chunks 0..3; after it, chunk i of rows 0..3.
-TKB_DEVFN void quad_transpose(uint4 (&v)[4]) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(v);
-  const bool odd = lane_id() & 1, high = lane_id() & 2;
-#pragma unroll
-  for (int k = 0; k < 4; k += 2)  // chunks k, k + 1 with the neighbour
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? w[4 * k + e] : w[4 * k + 4 + e], 1);
-      w[4 * k + e] = odd ? got : w[4 * k + e];
-      w[4 * k + 4 + e] = odd ? w[4 * k + 4 + e] : got;
-    }
-#pragma unroll
-  for (int k = 0; k < 2; ++k)  // chunks k, k + 2 with the lane two on
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? w[4 * k + e] : w[4 * k + 8 + e], 2);
-      w[4 * k + e] = high ? got : w[4 * k + e];
-      w[4 * k + 8 + e] = high ? w[4 * k + 8 + e] : got;
-    }
-}
-
 // A value of V that is not finite, in a slot that some rows of a tile see and
 // others do not, spoils the products of those others too (0 * inf).  So rows
 // whose O is not finite look whether such a slot lies behind their last one;
 // if one does, their O is computed again from the slots they see alone.  Whole
 // warps call it, `bad` marks the lanes with such a row.
 template <int D, bool BF16>
-__noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int jb, int end, bool bad, int lim, int row,
-                                         int hq, float m, const ChunkSink& sink) {
+__noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int jb, int step, int end, bool bad, int lim,
+                                         int row, int hq, float m, const ChunkSink& sink) {
   constexpr int E = D / 32;
   const tkb_kv_cache& c = p.c;
   const int lane = lane_id();
@@ -457,6 +453,7 @@ __noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int
   const int from = __reduce_min_sync(0xffffffffu, bad ? max(lim, jb * kChunkBlock) : end);
   int last = -1;  // the last slot with a value of V that is not finite
   for (int j = from; j < end; ++j) {
+    if ((j / kChunkBlock - jb) % step) continue;  // the other warpgroup's
     const int page = page_at(j);
     if (page < 0) continue;
     float v[E];
@@ -485,6 +482,7 @@ __noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int
       o[2 * e] = o[2 * e + 1] = 0.f;
     }
     for (int j = jb * kChunkBlock; j < min(rl, end); ++j) {
+      if ((j / kChunkBlock - jb) % step) continue;
       const int page = page_at(j);
       if (page < 0) continue;
       float k[E], v[E], s = 0.f;
@@ -810,11 +808,10 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         ++no;
         tc_fence_after();
       }
-      // ---- the warpgroups' halves of a single tile meet: the second hands over its m, l and O, 32 columns at a time
-      const bool meet = !it.pair && it.je - it.jb > 1;
-      float f0 = 1.f, f1 = 0.f;
-      bool sees0 = true, sees1 = false;  // a half that saw nothing has an O of masked values alone
-      if (!it.pair && w == 1) {
+      // ---- the warpgroups' halves of a whole unit of one tile meet: the second hands over its m, l and O, 32 columns
+      // at a time.  (Of a part, each leaves its own half in the workspace.)
+      const bool whole = it.whole(), meet = !it.pair && whole && it.je - it.jb > 1;
+      if (!it.pair && w == 1 && whole) {
         if (meet) {
           xml[r] = make_float2(m, l);
 #pragma unroll 1
@@ -833,11 +830,11 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         }
         continue;
       }
-      // ---- the tile's rows go out
+      // ---- the tile's rows go out (loops that are not unrolled: this code runs once a unit, from a cold instruction cache)
       ChunkSink sink;
-      sink.part = !it.whole();
+      sink.part = !whole;
       const int which = it.jb > 0 ? 0 : 1;
-      sink.slot = ((2ll * blockIdx.x + which) * 2 + tile) * 128 + r;
+      sink.slot = ((2ll * blockIdx.x + which) * 2 + w) * 128 + r;
       if (sink.part) {
         flags |= which ? SPAN_BEGINS : SPAN_GOES_ON | (it.je == it.nb[1] ? SPAN_ENDS : 0);
         if (which) {
@@ -847,21 +844,21 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         }
       }
       const int row = s.first + tok;
-      sink.out = static_cast<uint16_t*>(p.out) + (valid ? row * p.out_stride + static_cast<long long>(hq) * D : 0);
-      bool odd = false;
-      // four lanes write one row's 64 bytes: where the rows of this lane's quad go (16 bytes a lane), null for none
-      uint16_t* rows4[4];
+      sink.out = valid ? static_cast<uint16_t*>(p.out) + row * p.out_stride + static_cast<long long>(hq) * D : nullptr;
+      // two lanes write 32 bytes of a row: where this lane's 16 bytes of its pair's two rows go
+      uint16_t* rows2[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        rows4[i] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(valid ? sink.out : nullptr),
-                                                           (lane & ~3) + i));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (rows4[i]) rows4[i] += (lane & 3) * 8;
+      for (int i = 0; i < 2; ++i) {
+        rows2[i] = reinterpret_cast<uint16_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(sink.out), (lane & ~1) + i));
+        if (rows2[i]) rows2[i] += (lane & 1) * 8;
+      }
       float4* part = p.part + (sink.slot >> 7) * (D / 4) * 128 + r;
+      float f0 = 1.f, f1 = 0.f, zero = 0.f;
+      bool sees0 = true, sees1 = false;  // a half that saw nothing has an O of masked values alone
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        if (meet) {  // the other's columns
+      for (int c = 0; c < D / 16; ++c) {
+        if (meet && !(c & 1)) {  // the other's columns
           if (!(ok = mbar_wait_warp(x_full, nx & 1, abort_flag))) break;
           if (c == 0) {
             const float2 ml = xml[r];
@@ -880,53 +877,56 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
             if (sink.part) p.part_ml[sink.slot] = make_float2(m, l);
             else if (p.lse) p.lse[static_cast<long long>(row) * p.Hq + hq] = (m + lg2(l)) * 0.69314718055994531f;
           }
+          if (!has) break;  // a tile whose blocks lie before the run's
         }
-        if (has) {
-          uint32_t o[32];
-          tmem_ld32(tO + c * 32, o);
-          wait_ld_dep(o);
-          if (meet) {
+        uint32_t o[16];
+        tmem_ld16(tO + c * 16, o);
+        wait_ld16_dep(o);
+        if (meet) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 x = xo[i * 128 + r];
-              const float b[4] = {x.x, x.y, x.z, x.w};
+          for (int i = 0; i < 4; ++i) {
+            const float4 x = xo[((c & 1) * 4 + i) * 128 + r];
+            const float b[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o[4 * i + e] = __float_as_uint((sees0 ? f0 * __uint_as_float(o[4 * i + e]) : 0.f) + (sees1 ? f1 * b[e] : 0.f));
-            }
+            for (int e = 0; e < 4; ++e)
+              o[4 * i + e] = __float_as_uint((sees0 ? f0 * __uint_as_float(o[4 * i + e]) : 0.f) + (sees1 ? f1 * b[e] : 0.f));
           }
+          if (c & 1) {
+            mbar_arrive(x_empty);
+            ++nx;
+          }
+        }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) odd |= !(fabsf(__uint_as_float(o[i])) < INFINITY);
-          if (sink.part) {
-            if (valid) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                part[(c * 8 + i) * 128] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                      __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-            }
-          } else {
-            uint4 v[4];
-            uint32_t* vw = reinterpret_cast<uint32_t*>(v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              vw[i] = sink.inv == 0.f ? 0u : pack2<BF16>(__uint_as_float(o[2 * i]) * sink.inv, __uint_as_float(o[2 * i + 1]) * sink.inv);
-            quad_transpose(v);
+        for (int i = 0; i < 16; ++i) zero = fmaf(__uint_as_float(o[i]), 0.f, zero);  // NaN once a value is not finite
+        if (sink.part) {
+          if (valid) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (rows4[i]) *reinterpret_cast<uint4*>(rows4[i] + c * 32) = v[i];
+              part[(c * 4 + i) * 128] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                    __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
           }
-        }
-        if (meet) {
-          mbar_arrive(x_empty);
-          ++nx;
+        } else {
+          uint32_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            v[i] = sink.inv == 0.f ? 0u : pack2<BF16>(__uint_as_float(o[2 * i]) * sink.inv, __uint_as_float(o[2 * i + 1]) * sink.inv);
+          const bool odd = lane & 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // lane i of the pair: 16 bytes i of both rows
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[4 + i], 1);
+            v[i] = odd ? got : v[i];
+            v[4 + i] = odd ? v[4 + i] : got;
+          }
+          if (rows2[0]) *reinterpret_cast<uint4*>(rows2[0] + c * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+          if (rows2[1]) *reinterpret_cast<uint4*>(rows2[1] + c * 16) = make_uint4(v[4], v[5], v[6], v[7]);
         }
       }
       if (!ok) break;
       // O that is not finite though l is: look behind the row's last slot
       const int last = min(end * kChunkBlock, s.held);
-      const bool bad = has && odd && valid && l > 0.f && lim < last;
+      const bool bad = has && !(zero == 0.f) && valid && l > 0.f && lim < last;
       if (__any_sync(0xffffffffu, bad))
-        chunk_again<D, BF16>(p, it.b, it.hg / p.hb, it.jb, last, bad, lim, row, hq, m, sink);
+        chunk_again<D, BF16>(p, it.b, it.hg / p.hb, meet ? it.jb : j0, meet ? 1 : step, last, bad, lim, row, hq, m, sink);
     }
     if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(ok ? flags : 0, span_b, span_hg, span_u);
   }
@@ -941,42 +941,74 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
 
 // Joins the parts of units that span CTAs: the block of CTA c takes the unit
 // that begins there and goes on behind it, with the parts of the CTAs that
-// follow up to the one that ends it, in their order.  A thread has one row and
-// 32 columns; blockIdx.y is tile and column group.
+// follow up to the one that ends it, in their order; of a unit of one tile each
+// CTA has left two, its warpgroups'.  A thread has one row and 32 columns;
+// blockIdx.y is tile and column group.
 template <int D, typename T>
 __global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+  __shared__ int s_part[kChunkGrid], s_count[4], s_end;
   grid_wait();
-  const int c = blockIdx.x, w = blockIdx.y / (D / 32), cg = blockIdx.y % (D / 32), r = threadIdx.x;
+  const int c = blockIdx.x, w = blockIdx.y / (D / 32), cg = blockIdx.y % (D / 32), r = threadIdx.x, lane = lane_id();
   const int4 span = p.span[c];
   if (!(span.x & SPAN_BEGINS)) return;
+  if (r == 0) s_end = gridDim.x - 1;
+  __syncthreads();
   const ChunkSeq s = chunk_seq(p, span.y);
   const int t0 = span.w * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
+  const bool pair = tokens > p.tt;
+  if (!pair && w) return;
+  int parts = 0;  // the list of parts, 128 CTAs at a time up to the one that ends the unit
+#pragma unroll 1
+  for (int x0 = c; x0 < gridDim.x; x0 += 128) {
+    const int x = x0 + r;
+    const int flags = x == c || x >= gridDim.x ? 0 : p.span[x].x;
+    if ((flags & (SPAN_GOES_ON | SPAN_ENDS)) == (SPAN_GOES_ON | SPAN_ENDS)) atomicMin(&s_end, x);
+    __syncthreads();
+    const bool mine = x == c || (x <= s_end && flags & SPAN_GOES_ON);
+    const unsigned there = __ballot_sync(0xffffffffu, mine);
+    if (lane == 0) s_count[warp_id()] = __popc(there);
+    __syncthreads();
+    int at = parts + __popc(there & ((1u << lane) - 1));
+    for (int i = 0; i < 4; ++i) {
+      if (i < warp_id()) at += s_count[i];
+      parts += s_count[i];
+    }
+    if (mine) s_part[at] = 2 * x + (x == c);
+    __syncthreads();
+    if (s_end < x0 + 128) break;
+  }
   int tok, hq;
   if (!chunk_row(p, s, span.z, t0, tokens, w, r, tok, hq)) return;
-  // CTA c's second part, then the first parts of those that follow
-  float m = -INFINITY, l = 0.f, o[32];
+  // part i of this row: of a pair its own tile's, else both warpgroups' in turn
+  const int n = pair ? parts : 2 * parts;
+  auto slot_of = [&](int i) { return pair ? 2ll * s_part[i] + w : 2ll * s_part[i >> 1] + (i & 1); };
+  float m = -INFINITY;
+  bool nan = false;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float x = p.part_ml[slot_of(i) * 128 + r].x;
+    nan |= x != x;
+    m = fmaxf(m, x);
+  }
+  if (nan) m = NAN;
+  float l = 0.f, o[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) o[i] = 0.f;
-  int flags = 0;
-  for (int x = c; x < gridDim.x && !(flags & SPAN_ENDS); ++x) {
-    if (x > c) {
-      flags = p.span[x].x;
-      if (!(flags & SPAN_GOES_ON)) continue;  // a run too short to hold a block
-    }
-    const long long slot = ((2ll * x + (x == c ? 1 : 0)) * 2 + w) * 128;
-    const float2 ml = p.part_ml[slot + r];
-    if (ml.x == -INFINITY) continue;  // it saw nothing
-    const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : ex2(m - mm), f1 = ex2(ml.x - mm);
-    l = f0 * l + f1 * ml.y;
-    m = mm;
-    const float4* part = p.part + slot / 128 * (D / 4) * 128 + cg * 8 * 128 + r;
+#pragma unroll 2
+  for (int k = 0; k < n; ++k) {
+    const long long slot = slot_of(k);
+    const float2 ml = p.part_ml[slot * 128 + r];
+    const float4* part = p.part + slot * (D / 4) * 128 + cg * 8 * 128 + r;
+    const bool sees = ml.x != -INFINITY;  // else its O is of masked values alone, or not written
+    const float f = sees ? ex2(ml.x - m) : 0.f;
+    l = fmaf(f, ml.y, l);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float4 v = part[i * 128];
-      o[4 * i] = fmaf(f1, v.x, f0 * o[4 * i]);
-      o[4 * i + 1] = fmaf(f1, v.y, f0 * o[4 * i + 1]);
-      o[4 * i + 2] = fmaf(f1, v.z, f0 * o[4 * i + 2]);
-      o[4 * i + 3] = fmaf(f1, v.w, f0 * o[4 * i + 3]);
+      const float4 v = sees ? part[i * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+      o[4 * i] = fmaf(f, v.x, o[4 * i]);
+      o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]);
+      o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
     }
   }
   const long long row = s.first + tok;
