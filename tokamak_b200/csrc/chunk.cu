@@ -60,34 +60,12 @@ TKB_DEVFN void chunk_rows(const int32_t* row_start, int rows, int b, int& first,
 }
 
 // ============================================================ the deal
-// sum over i < n of floor((a i + b) / m); a, b >= 0
-TKB_DEVFN long long floor_sum(long long n, unsigned m, unsigned a, long long b) {
-  long long sum = 0;
-  while (true) {
-    if (a >= m) {
-      sum += n * (n - 1) / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += n * (b / m);
-      b %= m;
-    }
-    const long long y = static_cast<long long>(a) * n + b;
-    if (y < m) return sum;
-    n = y / m;
-    b = y % m;
-    const unsigned was = m;
-    m = a;
-    a = was;
-  }
-}
-
 constexpr int kChunkGrid = 148;   // one CTA per SM
 constexpr int kChunkBlock = 128;  // slots per block
 // What a block costs beside a block of a single tile: with two tiles twice the
 // products; and what a unit costs on top (its queries' load, its rows' output).
-constexpr int kCostPair = 2, kCostUnit = 2;
-constexpr int kCostLeast = 6;     // a CTA's run at least: shorter ones cost more to join than they save
+constexpr int kCostPair = 2, kCostUnit = 4;
+constexpr int kCostLeast = 12;    // a CTA's run at least, unless it has a unit of its own: shorter parts cost more to join than they save
 
 // A sequence: its rows, how many slots its first row sees less one (may be
 // negative), what it holds, and its units.
@@ -98,9 +76,18 @@ struct ChunkSeq {
 TKB_DEVFN int chunk_blocks(int base, int upto) {  // blocks for a row that sees base + upto slots; at least one
   return 1 + (max(base, 0) + upto - 1) / kChunkBlock;
 }
-__noinline__ __device__ long long chunk_cost_before(int per, int base, int u) {  // of the first u (full) units
-  return static_cast<long long>(u) * (kCostUnit + kCostPair) +
-         kCostPair * floor_sum(u, kChunkBlock, per, static_cast<long long>(max(base, 0)) + per - 1);
+// Cost of the first u (full) units: the sum over v < u of floor((per v + c) / 128), from the sum of the dividends and that
+// of their remainders, which repeat after 128 / gcd(per, 128) terms, taking each value of their class mod the gcd once.
+__noinline__ __device__ long long chunk_cost_before(int per, int base, int u) {
+  const int c = max(base, 0) + per - 1, g = min(per & -per, kChunkBlock), period = kChunkBlock / g;
+  const int turns = u / period;
+  int rest = 0;
+  long long rests = static_cast<long long>(turns) * (period * (c & (g - 1)) + g * (period * (period - 1) / 2));
+#pragma unroll 1
+  for (int v = turns * period; v < u; ++v) rest += (per * v + c) & (kChunkBlock - 1);
+  rests += rest;
+  const long long n = u, sum = (per * (n * (n - 1) / 2) + n * c - rests) / kChunkBlock;
+  return n * (kCostUnit + kCostPair) + kCostPair * sum;
 }
 TKB_DEVFN int chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
   const int t0 = u * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
@@ -108,8 +95,8 @@ TKB_DEVFN int chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
 }
 TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   ChunkSeq s;
+  const int held = max(p.c.seq_lens[b], -(1 << 30)), most = p.c.max_pages * p.c.page_size;
   chunk_rows(p.row_start, p.rows, b, s.first, s.n);
-  const int most = p.c.max_pages * p.c.page_size, held = max(p.c.seq_lens[b], -(1 << 30));
   // rows without a slot see none, rows past the table all of it
   if (held < s.n || held > most) {
     if (s.n) atomicOr(&g_device_error, ERR_BAD_INDEX);
@@ -125,59 +112,84 @@ TKB_DEVFN long long chunk_seq_cost(const ChunkParams& p, const ChunkSeq& s) {  /
 
 // One unit's share of a CTA's run.
 struct ChunkItem {
+  ChunkSeq s;
+  int more;                // 0: the run has ended
   int b, hg, u;            // sequence, head group (kv head, block of query heads), unit of the sequence
   int t0, tokens;          // its tokens among the sequence's rows
-  int nb[2];               // blocks of its tiles (the second's are all the unit's)
+  int nb0, nb1;            // blocks of its tiles (the second's are all the unit's)
   int jb, je;              // the run's blocks
-  bool pair;               // two tiles
-  TKB_DEVFN bool whole() const { return jb == 0 && je == nb[1]; }
+  TKB_DEVFN bool pair(const ChunkParams& p) const { return tokens > p.tt; }  // two tiles
+  TKB_DEVFN bool whole() const { return jb == 0 && je == nb1; }
 };
 // Walks the items of a run.  Every warp walks for itself, its state in shared
-// memory: a lane steps it, and the registers are the softmax's.
+// memory: a lane steps it, ahead of its use, and the registers are the softmax's.
 struct ChunkWalk {
-  ChunkSeq s;
-  ChunkItem it;
-  int b, hg, u;
-  int more;
+  ChunkItem it[2];
+  int b, hg, u, k;
   long long at, x0, x1;    // cost where the unit starts, where the run does and ends
-  TKB_DEVFN bool next(const ChunkParams& p) {
-    __syncwarp();
-    if (lane_id() == 0) more = step(p);
-    __syncwarp();
-    return more;
-  }
-  TKB_DEVFN bool step(const ChunkParams& p) {
-    while (at < x1) {
-      if (u == s.units) {
-        u = 0;
-        if (++hg == p.c.Hkv * p.hb) {
-          hg = 0;
+  // The item at hand; of the one after it once ahead() has been called.
+  TKB_DEVFN const ChunkItem& item() const { return it[k & 1]; }
+  TKB_DEVFN void step(const ChunkParams& p) {  // one lane: the item after the one at hand
+    const int from = k & 1;
+    ChunkSeq s = it[from].s;
+    int b_ = b, hg_ = hg, u_ = u;
+    long long at_ = at;
+    const long long x0_ = x0, x1_ = x1;
+    ChunkItem n;
+    n.more = 0;
+    while (at_ < x1_) {
+      if (u_ == s.units) {
+        u_ = 0;
+        if (++hg_ == p.c.Hkv * p.hb) {
+          hg_ = 0;
           do {
-            if (++b >= p.c.B) return false;
-            s = chunk_seq(p, b);
+            if (++b_ >= p.c.B) break;
+            s = chunk_seq(p, b_);
           } while (s.n == 0);
+          if (b_ >= p.c.B) break;
         }
       }
-      const int cost = chunk_cost(p, s, u);
-      it.b = b;
-      it.hg = hg;
-      it.u = u;
-      it.t0 = u * 2 * p.tt;
-      it.tokens = min(2 * p.tt, s.n - it.t0);
-      it.pair = it.tokens > p.tt;
-      it.nb[0] = chunk_blocks(s.base, it.t0 + min(it.tokens, p.tt));
-      it.nb[1] = chunk_blocks(s.base, it.t0 + it.tokens);
-      auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later, x below its cost
+      n.u = u_;
+      n.t0 = u_ * 2 * p.tt;
+      n.tokens = min(2 * p.tt, s.n - n.t0);
+      const bool two = n.tokens > p.tt;
+      n.nb0 = chunk_blocks(s.base, n.t0 + min(n.tokens, p.tt));
+      n.nb1 = chunk_blocks(s.base, n.t0 + n.tokens);
+      const int cost = kCostUnit + (two ? kCostPair : 1) * n.nb1;
+      auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later
+        if (x <= kCostUnit) return 0;
+        if (x >= cost) return n.nb1;
         const int y = static_cast<int>(x) - kCostUnit;
-        return it.pair ? (y + kCostPair - 1) / kCostPair : y;
+        return two ? (y + kCostPair - 1) / kCostPair : y;
       };
-      it.jb = x0 <= at + kCostUnit ? 0 : x0 - at >= cost ? it.nb[1] : block_at(x0 - at);
-      it.je = x1 <= at + kCostUnit ? 0 : x1 - at >= cost ? it.nb[1] : block_at(x1 - at);
-      at += cost;
-      ++u;
-      if (it.jb < it.je) return true;
+      n.jb = block_at(x0_ - at_);
+      n.je = block_at(x1_ - at_);
+      at_ += cost;
+      ++u_;
+      if (n.jb < n.je) {
+        n.more = 1;
+        break;
+      }
     }
-    return false;
+    n.s = s;
+    n.b = b_;
+    n.hg = hg_;
+    it[from ^ 1] = n;
+    b = b_;
+    hg = hg_;
+    u = u_;
+    at = at_;
+  }
+  TKB_DEVFN void ahead(const ChunkParams& p) {  // a whole warp
+    if (lane_id() == 0) step(p);
+  }
+  TKB_DEVFN bool next() {  // a whole warp, after ahead()
+    __syncwarp();
+    const int now = k + 1;
+    __syncwarp();
+    if (lane_id() == 0) k = now;
+    __syncwarp();
+    return item().more;
   }
 };
 
@@ -185,26 +197,62 @@ struct ChunkWalk {
 template <int NT_>
 TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
   __shared__ long long s_sum[NT_ / 32], s_x;
-  __shared__ int s_at[3];
+  __shared__ int s_units[NT_ / 32], s_at[3];
   __shared__ ChunkSeq s_seq;
   const int tid = threadIdx.x, lane = lane_id(), wid = warp_id();
   const int per = (p.c.B + NT_ - 1) / NT_, b0 = min(tid * per, p.c.B), b1 = min(b0 + per, p.c.B);
   const int groups = p.c.Hkv * p.hb;
-  long long at = 0, x0 = 0, x1 = 0;
-  // first the costs of this thread's sequences, then, with the sums over all, the one the run starts in
+  // the costs of this thread's sequences, and their sums over the block
+  ChunkSeq s;
+  long long cost = 0, mine = 0, total = 0;
+  int units = 0;
 #pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    long long upto = at;
+  for (int b = b0; b < b1; ++b) {
+    s = chunk_seq(p, b);
+    cost = chunk_seq_cost(p, s);
+    mine += cost * groups;
+    units = min(units + min(s.units, 0xFFFF) * groups, 0xFFFF);
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += y;
+  }
+  units = __reduce_add_sync(0xffffffffu, units);
+  if (lane == 31) {
+    s_sum[wid] = upto;
+    s_units[wid] = units;
+  }
+  __syncthreads();
+  units = 0;
+#pragma unroll 1
+  for (int i = 0; i < NT_ / 32; ++i) {
+    if (i == wid) upto += total;
+    total += s_sum[i];
+    units += s_units[i];
+  }
+  int ctas = gridDim.x;
+  if (total < static_cast<long long>(ctas) * kCostLeast)
+    ctas = min(ctas, max(units, (static_cast<int>(total) + kCostLeast - 1) / kCostLeast));
+  const int c = blockIdx.x;
+  if (c >= ctas) return false;
+  // total * c / ctas
+  const long long each = total / ctas;
+  const int rest = static_cast<int>(total - each * ctas);
+  const long long x0 = each * c + rest * c / ctas, x1 = each * (c + 1) + rest * (c + 1) / ctas;
+  upto -= mine;
+  if (upto <= x0 && x0 < upto + mine) {  // the run starts in one of this thread's sequences
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
-      const ChunkSeq s = chunk_seq(p, b);
-      const long long cost = chunk_seq_cost(p, s);
-      if (pass && upto <= x0 && x0 < upto + cost * groups) {
+      if (per > 1) {
+        s = chunk_seq(p, b);
+        cost = chunk_seq_cost(p, s);
+      }
+      if (x0 < upto + cost * groups) {
         int hg = 0;
-        while (x0 >= upto + cost) {
-          upto += cost;
-          ++hg;
-        }
+#pragma unroll 1
+        for (; x0 >= upto + cost; ++hg) upto += cost;
         int lo = 0, hi = s.units - 1;  // last unit that starts at x0 or before
 #pragma unroll 1
         while (lo < hi) {
@@ -221,30 +269,6 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
       }
       upto += cost * groups;
     }
-    if (pass) break;
-    const long long mine = upto;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += y;
-    }
-    if (lane == 31) s_sum[wid] = upto;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll 1
-    for (int i = 0; i < NT_ / 32; ++i) {
-      if (i == wid) upto += total;
-      total += s_sum[i];
-    }
-    const int ctas = total < static_cast<long long>(gridDim.x) * kCostLeast
-                         ? (static_cast<int>(total) + kCostLeast - 1) / kCostLeast : gridDim.x;
-    const int c = blockIdx.x;
-    if (c >= ctas) return false;
-    // total * c / ctas
-    const long long each = total / ctas, rest = total - each * ctas;
-    x0 = each * c + static_cast<int>(rest) * c / ctas;
-    x1 = each * (c + 1) + static_cast<int>(rest) * (c + 1) / ctas;
-    at = upto - mine;
   }
   __syncthreads();
   if (lane == 0) {
@@ -254,8 +278,10 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
     w.at = s_x;
     w.x0 = x0;
     w.x1 = x1;
-    w.s = s_seq;
+    w.it[0].s = s_seq;
+    w.k = 0;
   }
+  __syncwarp();
   return true;
 }
 
@@ -263,12 +289,15 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
 // first part of a unit that goes on in later ones.
 enum ChunkSpan : int { SPAN_GOES_ON = 1, SPAN_ENDS = 2, SPAN_BEGINS = 4 };
 
-// The (sequence row, query head) of row r of tile w of a unit; false where there is none.
-TKB_DEVFN bool chunk_row(const ChunkParams& p, const ChunkSeq& s, int hg, int t0, int tokens, int w, int r, int& tok,
-                         int& hq) {
-  const int t = r / p.gb, g = (hg % p.hb) * p.gb + r % p.gb;
+// The (sequence row, query head) of row r of tile w of a unit, r = (t, g) in tokens and heads; false where there is none.
+TKB_DEVFN bool chunk_row(const ChunkParams& p, int hg, int t0, int tokens, int w, int t, int g, int& tok, int& hq) {
+  int h = hg;
+  if (p.hb > 1) {
+    h = hg / p.hb;
+    g += (hg - h * p.hb) * p.gb;
+  }
   tok = t0 + w * p.tt + t;
-  hq = (hg / p.hb) * p.G + g;
+  hq = h * p.G + g;
   return t < p.tt && w * p.tt + t < tokens && g < p.G;
 }
 
@@ -557,7 +586,6 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
   }
   grid_wait();
   ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * static_cast<int>(sizeof(ChunkWalk)));
-  const ChunkItem& it = walk.it;
   const bool any = chunk_deal<320>(p, walk);
   tc_fence_before();
   __syncthreads();
@@ -575,9 +603,12 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     const uint32_t q_bytes = static_cast<uint32_t>(p.gb) * p.tt * D * 2;
     int nq = 0, nk = 0, nv = 0;  // loads issued
     bool ok = true;
-    while (ok && walk.next(p)) {
-      const int h = it.hg / p.hb, hq0 = h * p.G + (it.hg % p.hb) * p.gb;
-      const ChunkSeq& s = walk.s;
+    walk.ahead(p);
+    while (ok && walk.next()) {
+      const ChunkItem& it = walk.item();
+      const ChunkSeq& s = it.s;
+      const int h = it.hg / p.hb, hq0 = h * p.G + (it.hg % p.hb) * p.gb, jb = it.jb, je = it.je;
+      const bool pair = it.pair(p);
       // read once by a unit alone, or by the units that follow too
       const uint64_t pol_q = policy_evict_first(), pol_kv = s.units > 1 ? policy_evict_last() : policy_evict_first();
       const int32_t* table = p.c.block_table + static_cast<long long>(it.b) * p.c.max_pages;
@@ -591,21 +622,22 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         return bad ? p.c.n_pages : pg;
       };
       bool bad;
-      int page = page_in(it.jb, bad);
+      int page = page_in(jb, bad);
       if (!(ok = mbar_wait_warp(q_empty, (nq & 1) ^ 1, abort_flag))) break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (it.pair ? 2 : 1) * q_bytes);
-        for (int w = 0; w < (it.pair ? 2 : 1); ++w)
+        mbar_arrive_expect_tx(q_full, (pair ? 2 : 1) * q_bytes);
+        for (int w = 0; w < (pair ? 2 : 1); ++w)
 #pragma unroll
           for (int x = 0; x < D / 64; ++x)
             tma_load_3d(smem + C::OFF_Q + w * C::TILE + x * C::SLAB, &p.tmQ, q_full, x * 64, hq0,
                         s.first + it.t0 + w * p.tt, pol_q);
       }
       ++nq;
-      for (int j = it.jb; j < it.je; ++j) {
+      walk.ahead(p);
+      for (int j = jb; j < je; ++j) {
         bool bad_next = false;
         int next = 0;
-        if (j + 1 < it.je) next = page_in(j + 1, bad_next);
+        if (j + 1 < je) next = page_in(j + 1, bad_next);
         const int in_head = (j * kChunkBlock + gi * box_rows) % p.c.page_size + h * p.c.page_size;
         // bits of the 16-slot groups that lie in bad pages
         const unsigned lost = __reduce_or_sync(0xffffffffu, bad ? ((1u << (box_rows / 16)) - 1) << (gi * box_rows / 16) : 0u);
@@ -680,14 +712,15 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
         issue_PV(w, nv % C::NST, half, acc);
         return true;
       };
-      while (ok && walk.step(p)) {
+      for (walk.step(p), ++walk.k; ok && walk.item().more; walk.step(p), ++walk.k) {
+        const ChunkItem& it = walk.item();
         if (!(ok = mbar_wait(q_full, nq & 1, abort_flag))) break;
         ++nq;
         tc_fence_after();
         const int jb = it.jb, je = it.je;
-        if (it.pair) {
+        if (it.pair(p)) {
           // both warpgroups meet the same blocks, each with its own tile; the first tile's may end earlier
-          const int end[2] = {min(je, it.nb[0]), je};
+          const int end[2] = {min(je, it.nb0), je};
           if (!wait_k()) break;
           for (int w = 0; w < 2; ++w)
             if (jb < end[w]) issue_S(w, w, nk % C::NST);
@@ -764,15 +797,19 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     int ns = 0, no = 0, nb = 0, nx = 0;  // blocks of this warpgroup, items with blocks of it, blocks of the CTA, exchanges
     int flags = 0, span_b = 0, span_hg = 0, span_u = 0;
     bool ok = true;
-    while (ok && walk.next(p)) {
-      const ChunkSeq& s = walk.s;
-      const int tile = it.pair ? w : 0;
+    const int row_t = r / p.gb, row_g = r - row_t * p.gb;
+    walk.ahead(p);
+    while (ok && walk.next()) {
+      const ChunkItem& it = walk.item();
+      const ChunkSeq& s = it.s;
+      const bool pair = it.pair(p);
+      const int tile = pair ? w : 0;
       int tok, hq;
-      const bool valid = chunk_row(p, s, it.hg, it.t0, it.tokens, tile, r, tok, hq);
+      const bool valid = chunk_row(p, it.hg, it.t0, it.tokens, tile, row_t, row_g, tok, hq);
       const int lim = valid ? min(max(s.base + tok + 1, 0), s.held) : 0;
       const bool busy = __any_sync(0xffffffffu, valid);  // a warp without rows leaves its P as it is: nobody reads its O
       const int tile_lim = min(max(s.base + it.t0 + tile * p.tt + 1, 0), s.held);  // what the tile's first row sees
-      const int step = it.pair ? 1 : 2, j0 = it.jb + (it.pair ? 0 : w), end = it.pair ? min(it.je, it.nb[w]) : it.je;
+      const int step = pair ? 1 : 2, j0 = it.jb + (pair ? 0 : w), end = pair && w == 0 ? min(it.je, it.nb0) : it.je;
       float m = -INFINITY, l = 0.f;
       for (int j = j0; j < end; j += step) {
         const int at = j * kChunkBlock, nth = nb + j - it.jb;
@@ -802,6 +839,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       }
       if (!ok) break;
       nb += it.je - it.jb;
+      walk.ahead(p);  // while the last products run
       const bool has = j0 < end;
       if (has) {
         if (!(ok = mbar_wait_warp(&o_done[w], no & 1, abort_flag))) break;
@@ -810,8 +848,8 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       }
       // ---- the warpgroups' halves of a whole unit of one tile meet: the second hands over its m, l and O, 32 columns
       // at a time.  (Of a part, each leaves its own half in the workspace.)
-      const bool whole = it.whole(), meet = !it.pair && whole && it.je - it.jb > 1;
-      if (!it.pair && w == 1 && whole) {
+      const bool whole = it.whole(), meet = !pair && whole && it.je - it.jb > 1;
+      if (!pair && w == 1 && whole) {
         if (meet) {
           xml[r] = make_float2(m, l);
 #pragma unroll 1
@@ -836,7 +874,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       const int which = it.jb > 0 ? 0 : 1;
       sink.slot = ((2ll * blockIdx.x + which) * 2 + w) * 128 + r;
       if (sink.part) {
-        flags |= which ? SPAN_BEGINS : SPAN_GOES_ON | (it.je == it.nb[1] ? SPAN_ENDS : 0);
+        flags |= which ? SPAN_BEGINS : SPAN_GOES_ON | (it.je == it.nb1 ? SPAN_ENDS : 0);
         if (which) {
           span_b = it.b;
           span_hg = it.hg;
@@ -978,7 +1016,7 @@ __global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__
     if (s_end < x0 + 128) break;
   }
   int tok, hq;
-  if (!chunk_row(p, s, span.z, t0, tokens, w, r, tok, hq)) return;
+  if (!chunk_row(p, span.z, t0, tokens, w, r / p.gb, r % p.gb, tok, hq)) return;
   // part i of this row: of a pair its own tile's, else both warpgroups' in turn
   const int n = pair ? parts : 2 * parts;
   auto slot_of = [&](int i) { return pair ? 2ll * s_part[i] + w : 2ll * s_part[i >> 1] + (i & 1); };
