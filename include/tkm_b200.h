@@ -412,7 +412,8 @@ int tkb_kv_pages(int32_t *block_table, int32_t *held, const int32_t *lens, int32
  * rounded once.  adapter[b] = -1: out_r = y_r.  Rows of no sequence are left
  * as they were.  An adapter that does not exist counts as -1 and sets bit 2 of
  * the device error word.  K, N and the strides: multiples of 16 bytes, the
- * pointers 16-byte aligned; R a multiple of 8 up to 128.
+ * pointers 16-byte aligned; R a multiple of 8 up to 128; B at most 4096, rows at
+ * most 2^21.
  * The plan sorts the rows by adapter: tkb_lora_plan writes it from adapter [B]
  * and row_start (as for tkb_kv_append), once for all projections that take
  * the same rows, and tkb_lora_add reads it.  plan: tkb_lora_plan_bytes,

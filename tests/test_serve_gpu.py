@@ -227,8 +227,9 @@ def test_lora_bad_adapters_and_row_starts():
         plan = ops().lora_plan(on_gpu(adapter), 2, 10, row_start=on_gpu([0, 4, 10]))
         out = ops().lora_add(plan, x, a, b, y, out=torch.empty_like(y))
         assert device_error() == 4 and torch.equal(out[:4], y[:4]) and not torch.equal(out[4:], y[4:])
-    for start in ([0, 4, 99], [0, 8, 6], [-3, 4, 10]):
-        plan = ops().lora_plan(on_gpu([0, 1]), 2, 10, row_start=on_gpu(start))
+    for start in ([0, 4, 99], [0, 8, 6], [-3, 4, 10], [0, 10, 0, 10], [0, 7, 2, 9]):
+        ids = [0, 1, 1][:len(start) - 1]
+        plan = ops().lora_plan(on_gpu(ids), 2, 10, row_start=on_gpu(start))
         ops().lora_add(plan, x, a, b, y, out=torch.empty_like(y))
         assert device_error() == 4, start
 

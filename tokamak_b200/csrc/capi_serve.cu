@@ -14,6 +14,15 @@ int batch_check(const char* who, const void* row_start, int rows, int B) {
   return TKB_OK;
 }
 
+constexpr int kLoraRows = 1 << 21;  // rows of a plan: its tiles are counted in a grid's second dimension
+int lora_check(const char* who, const void* row_start, int rows, int B, int n_adapters) {
+  int rc = batch_check(who, row_start, rows, B);
+  if (rc) return rc;
+  if (n_adapters <= 0) return fail(TKB_ERR_ARG, "%s: n_adapters must be positive", who);
+  if (rows > kLoraRows) return fail(TKB_ERR_UNSUPPORTED, "%s: %d rows > 2^21", who, rows);
+  return TKB_OK;
+}
+
 int chunk_check(const char* who, const tkb_kv_cache* c, int rows, int Hq) {
   int rc = cache_check(who, c);
   if (rc) return rc;
@@ -89,50 +98,47 @@ int tkb_kv_pages(int32_t* block_table, int32_t* held, const int32_t* lens, int32
 
 size_t tkb_lora_plan_bytes(int B, int rows, int n_adapters) {
   const char* who = "tkb_lora_plan_bytes";
-  if (batch_check(who, who, rows, B)) return 0;
-  if (n_adapters <= 0) {
-    fail(TKB_ERR_ARG, "%s: n_adapters must be positive", who);
-    return 0;
-  }
-  return round256(static_cast<size_t>(rows) * 4);
+  if (lora_check(who, who, rows, B, n_adapters)) return 0;
+  return lora_plan_at(B, rows, n_adapters).bytes;
 }
 
 int tkb_lora_plan(const int32_t* adapter, const int32_t* row_start, int B, int rows, int n_adapters, void* plan,
                   size_t plan_bytes, void* stream) {
   const char* who = "tkb_lora_plan";
-  int rc = batch_check(who, row_start, rows, B);
+  int rc = lora_check(who, row_start, rows, B, n_adapters);
   if (rc) return rc;
-  if (n_adapters <= 0) return fail(TKB_ERR_ARG, "%s: n_adapters must be positive", who);
   if (!adapter) return fail(TKB_ERR_ARG, "%s: null pointer", who);
   const size_t need = tkb_lora_plan_bytes(B, rows, n_adapters);
   if (!plan || plan_bytes < need || (reinterpret_cast<uintptr_t>(plan) & 255))
     return fail(TKB_ERR_WORKSPACE, "%s: plan of %zu bytes, 256-byte aligned, required", who, need);
-  const LoraPlanParams p = {adapter, row_start, static_cast<int32_t*>(plan), B, rows, n_adapters};
-  return cuda_status(launch_early(lora_plan_kernel, dim3((rows + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream), p),
-                     who, 1);
+  const LoraPlanAt at = lora_plan_at(B, rows, n_adapters);
+  uint8_t* base = static_cast<uint8_t*>(plan);
+  const LoraPlanParams p = {adapter, row_start, static_cast<int*>(plan), reinterpret_cast<LoraTile*>(base + 256),
+                            reinterpret_cast<int32_t*>(base + at.rows), B, rows, n_adapters, at.tm, 0};
+  return cuda_status(lora_plan(p, static_cast<cudaStream_t>(stream)), who, 1);
 }
 
 size_t tkb_lora_workspace(int rows, int R) {
-  if (rows <= 0 || R <= 0) {
-    fail(TKB_ERR_ARG, "tkb_lora_workspace: rows and R must be positive");
+  if (rows <= 0 || rows > kLoraRows || R <= 0 || R > 128) {
+    fail(TKB_ERR_ARG, "tkb_lora_workspace: rows are 1 to 2^21, R 1 to 128");
     return 0;
   }
-  return round256(static_cast<size_t>(rows) * R * 4);
+  return round256(lora_ws_bytes(rows, R));
 }
 
 int tkb_lora_add(const void* plan, const void* x, long long x_stride, const void* A, const void* B_, const float* scale,
                  const void* y, long long y_stride, void* out, long long out_stride, int B, int rows, int n_adapters,
                  int K, int N, int R, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "tkb_lora_add";
-  int rc = batch_check(who, plan, rows, B);
+  if (!plan || !x || !A || !B_ || !y || !out) return fail(TKB_ERR_ARG, "%s: null pointer", who);
+  int rc = lora_check(who, plan, rows, B, n_adapters);
   if (rc) return rc;
   if (!dtype_ok(dtype)) return fail(TKB_ERR_ARG, "%s: bad dtype %d", who, dtype);
-  if (n_adapters <= 0 || K <= 0 || N <= 0) return fail(TKB_ERR_ARG, "%s: n_adapters, K and N must be positive", who);
+  if (K <= 0 || N <= 0) return fail(TKB_ERR_ARG, "%s: K and N must be positive", who);
   if (R <= 0 || R % 8 || R > 128) return fail(TKB_ERR_UNSUPPORTED, "%s: rank %d is not a multiple of 8 up to 128", who, R);
   const int e = dtype_bytes(dtype);
   if (static_cast<long long>(K) * e % 16 || static_cast<long long>(N) * e % 16 || K > (1 << 26) || N > (1 << 26))
     return fail(TKB_ERR_ARG, "%s: K and N must be multiples of 16 bytes", who);
-  if (!plan || !x || !A || !B_ || !y || !out) return fail(TKB_ERR_ARG, "%s: null pointer", who);
   if ((rc = rows_check(who, "x", x, x_stride, K, dtype)) || (rc = rows_check(who, "y", y, y_stride, N, dtype)) ||
       (rc = rows_check(who, "out", out, out_stride, N, dtype)))
     return rc;
@@ -141,10 +147,29 @@ int tkb_lora_add(const void* plan, const void* x, long long x_stride, const void
   const size_t need = tkb_lora_workspace(rows, R);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return fail(TKB_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, required", who, need);
-  const LoraParams p = {static_cast<const int32_t*>(plan), x, A, B_, y, out, scale, static_cast<float*>(workspace),
-                        x_stride, y_stride, out_stride, rows, K, N, R};
+  const LoraPlanAt at = lora_plan_at(B, rows, n_adapters);
+  const uint8_t* base = static_cast<const uint8_t*>(plan);
+  LoraParams p;
+  memset(&p, 0, sizeof(p));
+  p.n_tiles = static_cast<const int*>(plan);
+  p.tiles = reinterpret_cast<const LoraTile*>(base + 256);
+  p.row_of = reinterpret_cast<const int32_t*>(base + at.rows);
+  p.x = x;
+  p.a = A;
+  p.b = B_;
+  p.y = y;
+  p.out = out;
+  p.scale = scale;
+  p.t = static_cast<float*>(workspace);
+  p.x_stride = x_stride;
+  p.y_stride = y_stride;
+  p.out_stride = out_stride;
+  p.rows = rows;
+  p.K = K;
+  p.N = N;
+  p.R = R;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CALL(T) lora_add_t<T>(p, st)
+#define CALL(T) lora_add_t<T>(p, at, st)
   return cuda_status(TKB_BY_DTYPE(dtype, CALL), who, 2);
 #undef CALL
 }

@@ -1,92 +1,633 @@
-// lora.cu -- low-rank adapters of many requests beside a shared projection.
+// lora.cu -- low-rank adapters of many requests beside a shared projection:
+// out = y + scale (x A) B with each row's own adapter.
+//
+// 4 R FLOP a value of x or y read: HBM bounds it for prompts (x, y and out move
+// once, the adapters stay in L2), the chain of launches for single tokens.  The
+// plan sorts the rows by adapter and cuts them into tiles of one adapter each
+// (16 rows, or 64 where the adapters have that many), so that an adapter is
+// read once a tile and its products run on m16n8k16 instructions.  Two
+// kernels: t = x A, cut over K when there are few tiles, its fp32 parts in the
+// workspace; then out, cut over the columns.  The first product's result goes into the second as two
+// 16-bit values, the rounding and the rest, so that only out is rounded.
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
 namespace tkb {
 
+// ============================================================ the plan
+// Layout: number of tiles (256 bytes), the tiles, then the row of every sorted place.
+struct LoraTile {
+  int adapter, at, count, unused;  // -1: rows without one; first sorted place, rows
+};
+struct LoraPlanAt {
+  int tm, tiles;                   // rows per tile, tiles at most
+  size_t rows, bytes;              // offset of the rows
+};
+static LoraPlanAt lora_plan_at(int B, int rows, int n_adapters) {
+  LoraPlanAt a;
+  const long long groups = n_adapters < B ? n_adapters + 1ll : B;
+  // Tiles of 64 rows read an adapter a quarter as often; where adapters have fewer rows, most of such a tile is empty.
+  a.tm = rows >= 32 * groups ? 64 : 16;
+  a.tiles = static_cast<int>(rows / a.tm + (groups < rows ? groups : rows));
+  a.rows = 256 + static_cast<size_t>(a.tiles) * sizeof(LoraTile);
+  a.bytes = (a.rows + static_cast<size_t>(rows) * 4 + 255) & ~size_t(255);
+  return a;
+}
+
 struct LoraPlanParams {
   const int32_t* adapter;
   const int32_t* row_start;
-  int32_t* of_row;
-  int B, rows, n_adapters;
+  int* n_tiles;
+  LoraTile* tiles;
+  int32_t* row_of;
+  int B, rows, n_adapters, tm, sorted;  // sorted: power of two >= B
 };
+constexpr int kLoraPlanRows = 8192;     // sorted places per CTA
 
-// The adapter of every row: -1 none, -2 a row of no sequence.
-__global__ void lora_plan_kernel(const __grid_constant__ LoraPlanParams p) {
+// Every CTA sorts the sequences by adapter (bitonic, in shared memory) and
+// finds its share of the rows; the first writes the tiles.
+__global__ void __launch_bounds__(kPagesThreads) lora_plan_kernel(const __grid_constant__ LoraPlanParams p) {
+  extern __shared__ unsigned long long s_key[];         // [sorted] adapter + 1, sequence
+  int* s_pos = reinterpret_cast<int*>(s_key + p.sorted);  // [sorted + 1] first sorted place
+  int* s_group = s_pos + p.sorted + 1;                  // [sorted + 1] first sorted sequence of each group
+  int* s_tile = s_group + p.sorted + 1;                 // [sorted + 1] its first tile
+  __shared__ int s_warp[32];
+  const int tid = threadIdx.x, n = p.sorted;
   grid_wait();
-  if (p.row_start && blockIdx.x == 0)
-    for (int b = threadIdx.x; b < p.B; b += blockDim.x)
-      if (p.row_start[b] < 0 || p.row_start[b + 1] < p.row_start[b] || p.row_start[b + 1] > p.rows)
+  for (int b = tid; b < n; b += kPagesThreads) {
+    unsigned long long key = ~0ull;
+    if (b < p.B) {
+      int first, count, a = p.adapter[b];
+      chunk_rows(p.row_start, p.rows, b, first, count);
+      if (a < -1 || a >= p.n_adapters) {
         atomicOr(&g_device_error, ERR_BAD_INDEX);
-  for (int row = blockIdx.x * blockDim.x + threadIdx.x; row < p.rows; row += gridDim.x * blockDim.x) {
-    int b = row;
-    bool has = true;
-    if (p.row_start) {
-      int lo = 0, hi = p.B - 1;
+        a = -1;
+      }
+      if (count) key = static_cast<unsigned long long>(a + 1) << 32 | static_cast<unsigned>(b);
+    }
+    s_key[b] = key;
+  }
+  __syncthreads();
+  for (int size = 2; size <= n; size <<= 1)
+    for (int stride = size >> 1; stride; stride >>= 1) {
+      for (int i = tid; i < n / 2; i += kPagesThreads) {
+        const int lo = (i / stride) * 2 * stride + i % stride, hi = lo + stride;
+        const unsigned long long a = s_key[lo], b = s_key[hi];
+        if ((a > b) == !(lo & size)) {
+          s_key[lo] = b;
+          s_key[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+  // places, groups and tiles by sums over the sorted sequences
+  int count[kPagesSeqs], lead[kPagesSeqs], sum = 0, leads = 0;
+#pragma unroll
+  for (int i = 0; i < kPagesSeqs; ++i) {
+    const int k = tid * kPagesSeqs + i;
+    count[i] = lead[i] = 0;
+    if (k >= n || s_key[k] == ~0ull) continue;
+    int first;
+    chunk_rows(p.row_start, p.rows, static_cast<int>(s_key[k] & 0xffffffffu), first, count[i]);
+    lead[i] = k == 0 || s_key[k] >> 32 != s_key[k - 1] >> 32;
+    sum += count[i];
+    leads += lead[i];
+  }
+  int total, groups;
+  int at = pages_scan(sum, s_warp, total), g = pages_scan(leads, s_warp, groups);
+  if (total > p.rows) {  // sequences that share rows: those that do not fit are left out
+    if (tid == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
+    total = p.rows;
+  }
+#pragma unroll
+  for (int i = 0; i < kPagesSeqs; ++i) {
+    const int k = tid * kPagesSeqs + i;
+    if (k >= n) break;
+    s_pos[k] = min(at, total);
+    if (lead[i]) s_group[g++] = k;
+    at += count[i];
+  }
+  if (tid == 0) s_pos[n] = total;
+  __syncthreads();
+  auto group_end = [&](int i) { return i + 1 < groups ? s_pos[s_group[i + 1]] : total; };
+  if (blockIdx.x == 0) {
+    int tiles[kPagesSeqs], mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kPagesSeqs; ++i) {
+      const int k = tid * kPagesSeqs + i;
+      tiles[i] = k < groups ? (group_end(k) - s_pos[s_group[k]] + p.tm - 1) / p.tm : 0;
+      mine += tiles[i];
+    }
+    int t = pages_scan(mine, s_warp, all);
+#pragma unroll
+    for (int i = 0; i < kPagesSeqs; ++i) {
+      const int k = tid * kPagesSeqs + i;
+      if (k < groups) s_tile[k] = t;
+      t += tiles[i];
+    }
+    if (tid == 0) *p.n_tiles = all;
+    __syncthreads();
+    for (int i = tid; i < all; i += kPagesThreads) {
+      int lo = 0, hi = groups - 1;  // last group that starts at tile i or before
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (p.row_start[mid] <= row) lo = mid;
+        if (s_tile[mid] <= i) lo = mid;
         else hi = mid - 1;
       }
-      b = lo;
-      has = p.row_start[b] <= row && row < p.row_start[b + 1];
+      LoraTile t;
+      t.adapter = static_cast<int>(s_key[s_group[lo]] >> 32) - 1;
+      t.at = s_pos[s_group[lo]] + (i - s_tile[lo]) * p.tm;
+      t.count = min(p.tm, group_end(lo) - t.at);
+      t.unused = 0;
+      p.tiles[i] = t;
     }
-    int a = p.adapter[b];
-    if (a < -1 || a >= p.n_adapters) {
-      atomicOr(&g_device_error, ERR_BAD_INDEX);
-      a = -1;
+  }
+  const int first = blockIdx.x * kLoraPlanRows, last = min(first + kLoraPlanRows, total);
+  for (int i = first + tid; i < last; i += kPagesThreads) {
+    int lo = 0, hi = n - 1;  // last sorted sequence that starts at place i or before; those behind the rows start at `total`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_pos[mid] <= i) lo = mid;
+      else hi = mid - 1;
     }
-    p.of_row[row] = has ? a : -2;
+    int row0, rows;
+    chunk_rows(p.row_start, p.rows, static_cast<int>(s_key[lo] & 0xffffffffu), row0, rows);
+    p.row_of[i] = row0 + i - s_pos[lo];
   }
 }
 
+static cudaError_t lora_plan(LoraPlanParams p, cudaStream_t st) {
+  p.sorted = 2;
+  while (p.sorted < p.B) p.sorted *= 2;
+  const size_t smem = p.sorted * 8 + (p.sorted + 1) * 3 * sizeof(int);
+  const cudaError_t e = allow_smem<lora_plan_kernel>(kPagesThreads * kPagesSeqs * 20 + 16);
+  if (e != cudaSuccess) return e;
+  return launch_early(lora_plan_kernel, dim3((p.rows + kLoraPlanRows - 1) / kLoraPlanRows), kPagesThreads, smem, st, p);
+}
+
+// ============================================================ the products
 struct LoraParams {
-  const int32_t* of_row;
+  const int* n_tiles;
+  const LoraTile* tiles;
+  const int32_t* row_of;
   const void *x, *a, *b, *y;
   void* out;
   const float* scale;
-  float* t;  // [rows][R]: scale * x A
+  float* t;                // [splits][rows][RP] by sorted place
   long long x_stride, y_stride, out_stride;
   int rows, K, N, R;
+  int splits, k_per;       // parts of K and columns of each (a multiple of a chunk)
+  int chunks;              // chunks of columns per CTA of the second kernel
 };
+constexpr int kLoraThreads = 128;
 
-template <typename T>
-__global__ void __launch_bounds__(256) lora_down_kernel(const __grid_constant__ LoraParams p) {
+// Byte offset of 16-byte piece `ch` of row r in a tile of RB-byte rows, so that
+// eight rows' equal pieces (ldmatrix) lie in different banks.
+template <int RB>
+TKB_DEVFN int lora_swz(int r, int ch) {
+  return r * RB + ((ch ^ (RB == 32 ? r >> 2 & 1 : r & 7)) << 4);
+}
+
+// t = x A over one part of K.  A warp holds 16 rows; tiles of 16 rows give each
+// warp a quarter of every chunk of K instead.
+template <typename T, int RP, int TM>
+struct LoraDown {
+  static constexpr int KC = 64, ST = 4;                  // columns of K per chunk, chunks in flight
+  static constexpr int XB = TM * KC * 2, AB = KC * RP * 2, STAGE = XB + AB;
+  static constexpr int SUM = TM == 16 ? 4 * 16 * RP * 4 : 0;
+  static constexpr int SMEM = ST * STAGE > SUM ? ST * STAGE : SUM;
+};
+template <typename T, int RP, int TM>
+__global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraDown<T, RP, TM>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ int s_row[TM];
   grid_wait();
-  const int row = blockIdx.x, a = p.of_row[row];
-  if (a < 0) return;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-  const T* A = static_cast<const T*>(p.a) + static_cast<long long>(a) * p.K * p.R;
-  for (int r = warp_id(); r < p.R; r += 8) {
-    float s = 0.f;
-    for (int k = lane_id(); k < p.K; k += 32) s = fmaf(static_cast<float>(x[k]), static_cast<float>(A[static_cast<long long>(k) * p.R + r]), s);
-    s = warp_sum(s);
-    if (lane_id() == 0) p.t[static_cast<long long>(row) * p.R + r] = s * (p.scale ? p.scale[a] : 1.f);
+  if (static_cast<int>(blockIdx.x) >= *p.n_tiles) return;
+  const LoraTile tile = p.tiles[blockIdx.x];
+  if (tile.adapter < 0) return;
+  const int tid = threadIdx.x, lane = lane_id(), w = warp_id();
+  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
+  __syncthreads();
+  const int k0 = blockIdx.y * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
+  const T* A = static_cast<const T*>(p.a) + static_cast<long long>(tile.adapter) * p.K * p.R;
+  auto load = [&](int c) {
+    if (c < n) {
+      uint8_t* s = s_ring + c % C::ST * C::STAGE;
+      const int k = k0 + c * C::KC;
+      for (int i = tid; i < TM * 8; i += kLoraThreads) {
+        const int r = i >> 3, ch = i & 7, kk = k + ch * 8;
+        const bool in = r < tile.count && kk < k1;
+        cp_async16(smem_u32(s + lora_swz<128>(r, ch)), static_cast<const T*>(p.x) + s_row[r] * p.x_stride + (in ? kk : 0), in ? 16 : 0);
+      }
+      for (int i = tid; i < C::KC * RP / 8; i += kLoraThreads) {
+        const int r = i / (RP / 8), ch = i % (RP / 8);
+        const bool in = k + r < k1 && ch * 8 < p.R;
+        cp_async16(smem_u32(s + C::XB + lora_swz<RP * 2>(r, ch)), A + (in ? static_cast<long long>(k + r) * p.R + ch * 8 : 0), in ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  float acc[RP / 8][4];
+#pragma unroll
+  for (int i = 0; i < RP / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  for (int c = 0; c < C::ST - 1; ++c) load(c);
+  const int mi = lane >> 3, ri = lane & 7, r0 = TM == 16 ? 0 : w * 16;
+  for (int c = 0; c < n; ++c) {
+    cp_async_wait<C::ST - 2>();
+    __syncthreads();
+    load(c + C::ST - 1);
+    const uint32_t xs = smem_u32(s_ring + c % C::ST * C::STAGE), as = xs + C::XB;
+#pragma unroll
+    for (int kk = 0; kk < C::KC / 16; ++kk) {
+      if (TM == 16 && kk != w) continue;
+      uint32_t a[4];
+      ldsm4(xs + lora_swz<128>(r0 + ri + (mi & 1) * 8, kk * 2 + (mi >> 1)), a);
+#pragma unroll
+      for (int j = 0; j < RP / 16; ++j) {
+        uint32_t b[4];
+        ldsm4_t(as + lora_swz<RP * 2>(kk * 16 + ri + (mi & 1) * 8, j * 2 + (mi >> 1)), b);
+        mma16816<BF16>(acc[2 * j], a, b[0], b[1]);
+        mma16816<BF16>(acc[2 * j + 1], a, b[2], b[3]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  const int g = lane >> 2, c2 = (lane & 3) * 2;
+  float* out = p.t + (static_cast<long long>(blockIdx.y) * p.rows + tile.at) * RP;
+  if constexpr (TM == 16) {
+    // the warps' quarters meet
+    __syncthreads();
+    float* s = reinterpret_cast<float*>(s_ring);
+#pragma unroll
+    for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[(w * 16 + g + (e >> 1) * 8) * RP + j * 8 + c2 + (e & 1)] = acc[j][e];
+    __syncthreads();
+    for (int i = tid; i < tile.count * RP; i += kLoraThreads)
+      out[i] = (s[i] + s[16 * RP + i]) + (s[32 * RP + i] + s[48 * RP + i]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const int r = r0 + g + (e >> 1) * 8;
+        if (r < tile.count) *reinterpret_cast<float2*>(out + r * RP + j * 8 + c2) = make_float2(acc[j][e], acc[j][e + 1]);
+      }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) lora_up_kernel(const __grid_constant__ LoraParams p) {
+// out = y + t B for one tile and `chunks` times 64 columns.  A warp has 16 rows,
+// or of tiles of 16 rows a quarter of the columns.
+template <typename T, int RP, int TM>
+struct LoraUp {
+  static constexpr int NC = 64, ST = 3;
+  static constexpr int YB = TM * NC * 2, BB = RP * NC * 2, STAGE = YB + BB, SMEM = ST * STAGE;
+};
+template <typename T, int RP, int TM>
+__global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraUp<T, RP, TM>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ int s_row[TM];
   grid_wait();
-  const int row = blockIdx.x, a = p.of_row[row];
-  if (a == -2) return;
-  const T* y = static_cast<const T*>(p.y) + row * p.y_stride;
-  T* out = static_cast<T*>(p.out) + row * p.out_stride;
-  const T* Bm = static_cast<const T*>(p.b) + static_cast<long long>(max(a, 0)) * p.R * p.N;
-  for (int n = threadIdx.x; n < p.N; n += 256) {
-    float s = static_cast<float>(y[n]);
-    if (a >= 0)
-      for (int r = 0; r < p.R; ++r)
-        s = fmaf(p.t[static_cast<long long>(row) * p.R + r], static_cast<float>(Bm[static_cast<long long>(r) * p.N + n]), s);
-    out[n] = static_cast<T>(s);
+  if (static_cast<int>(blockIdx.y) >= *p.n_tiles) return;
+  const LoraTile tile = p.tiles[blockIdx.y];
+  if (tile.adapter < 0 && p.out == p.y) return;
+  const int tid = threadIdx.x, lane = lane_id(), w = warp_id();
+  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
+  __syncthreads();
+  const int n0 = blockIdx.x * p.chunks * C::NC, n = min(p.chunks, (p.N - n0 + C::NC - 1) / C::NC);
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  if (tile.adapter < 0) {  // no adapter: the rows as they are
+    const int pieces = min(n * C::NC, p.N - n0) / 8;
+    for (int i = tid; i < tile.count * pieces; i += kLoraThreads) {
+      const int r = s_row[i / pieces], col = n0 + i % pieces * 8;
+      *reinterpret_cast<uint4*>(out + r * p.out_stride + col) = *reinterpret_cast<const uint4*>(y + r * p.y_stride + col);
+    }
+    return;
+  }
+  const T* Bm = static_cast<const T*>(p.b) + static_cast<long long>(tile.adapter) * p.R * p.N;
+  auto load = [&](int c) {
+    if (c < n) {
+      uint8_t* s = s_ring + c % C::ST * C::STAGE;
+      const int col = n0 + c * C::NC;
+      for (int i = tid; i < TM * 8; i += kLoraThreads) {
+        const int r = i >> 3, ch = i & 7, cc = col + ch * 8;
+        const bool in = r < tile.count && cc < p.N;
+        cp_async16(smem_u32(s + lora_swz<128>(r, ch)), y + s_row[r] * p.y_stride + (in ? cc : 0), in ? 16 : 0);
+      }
+      for (int i = tid; i < RP * 8; i += kLoraThreads) {
+        const int r = i >> 3, ch = i & 7, cc = col + ch * 8;
+        const bool in = r < p.R && cc < p.N;
+        cp_async16(smem_u32(s + C::YB + lora_swz<128>(r, ch)), Bm + (in ? static_cast<long long>(r) * p.N + cc : 0), in ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  for (int c = 0; c < C::ST - 1; ++c) load(c);
+  // t of this thread's rows g and g + 8: the parts summed in their order, times the adapter's scale
+  const int g = lane >> 2, c2 = (lane & 3) * 2, r0 = TM == 16 ? 0 : w * 16;
+  const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
+  float up[2] = {1.f, 1.f};  // f16: t goes in as multiples of a power of two near the row's largest, so that it fits the type
+  uint32_t hi[RP / 16][4], lo[RP / 16][4];
+  {
+    float t[RP / 16][8];
+    float top[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + g + (i & 1) * 8;
+        float2 s = make_float2(0.f, 0.f);
+        if (r < tile.count) {
+          const float* src = p.t + (static_cast<long long>(tile.at) + r) * RP + k * 16 + (i >> 1) * 8 + c2;
+          for (int part = 0; part < p.splits; ++part) {
+            const float2 v = *reinterpret_cast<const float2*>(src + static_cast<long long>(part) * p.rows * RP);
+            s.x += v.x;
+            s.y += v.y;
+          }
+        }
+        t[k][2 * i] = s.x * scale;
+        t[k][2 * i + 1] = s.y * scale;
+        top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(t[k][2 * i]), fabsf(t[k][2 * i + 1])));
+      }
+    float down[2] = {1.f, 1.f};
+    if (!BF16) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        if (top[i] > 1e-30f && top[i] < 1e30f) {  // else 0, infinite, or next to either
+          const int e = (__float_as_int(top[i]) >> 23) - 127;
+          up[i] = __int_as_float((e + 127) << 23);
+          down[i] = __int_as_float((127 - e) << 23);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = t[k][2 * i] * down[i & 1], b = t[k][2 * i + 1] * down[i & 1];
+        hi[k][i] = pack2<BF16>(a, b);
+        const float2 h = unpack2<BF16>(hi[k][i]);
+        lo[k][i] = pack2<BF16>(a - h.x, b - h.y);
+      }
+  }
+  const int mi = lane >> 3, ri = lane & 7;
+  constexpr int NT8 = TM == 16 ? 2 : 8;  // 8-column products of this warp
+  const int j0 = TM == 16 ? w * 2 : 0;
+  for (int c = 0; c < n; ++c) {
+    cp_async_wait<C::ST - 2>();
+    __syncthreads();
+    load(c + C::ST - 1);
+    uint8_t* ys = s_ring + c % C::ST * C::STAGE;
+    const uint32_t bs = smem_u32(ys) + C::YB;
+    float acc[NT8][4];
+#pragma unroll
+    for (int j = 0; j < NT8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+      for (int j = 0; j < NT8; j += 2) {
+        uint32_t b[4];
+        ldsm4_t(bs + lora_swz<128>(k * 16 + ri + (mi & 1) * 8, j0 + j + (mi >> 1)), b);
+        mma16816<BF16>(acc[j], hi[k], b[0], b[1]);
+        mma16816<BF16>(acc[j + 1], hi[k], b[2], b[3]);
+        mma16816<BF16>(acc[j], lo[k], b[0], b[1]);
+        mma16816<BF16>(acc[j + 1], lo[k], b[2], b[3]);
+      }
+    // added to y where it lies in shared memory, by the threads that hold the products
+#pragma unroll
+    for (int j = 0; j < NT8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(ys + lora_swz<128>(r0 + g + (e >> 1) * 8, j0 + j) + c2 * 2);
+        const float2 v = unpack2<BF16>(*at);
+        *at = pack2<BF16>(fmaf(acc[j][e], up[e >> 1], v.x), fmaf(acc[j][e + 1], up[e >> 1], v.y));
+      }
+    __syncwarp();
+    const int col = n0 + c * C::NC;
+#pragma unroll
+    for (int i = lane; i < 16 * NT8; i += 32) {
+      const int r = r0 + i / NT8, ch = j0 + i % NT8;
+      if (r < tile.count && col + ch * 8 < p.N)
+        *reinterpret_cast<uint4*>(out + s_row[r] * p.out_stride + col + ch * 8) = *reinterpret_cast<const uint4*>(ys + lora_swz<128>(r, ch));
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ------------------------------------------------------------ fp32: FMA
+template <int RP, int TM>
+struct LoraDown<float, RP, TM> {
+  static constexpr int KC = 32, ST = 3;
+  static constexpr int XS = KC + 4;                      // floats from row to row: eight rows in different banks
+  static constexpr int XB = TM * XS * 4, AB = KC * RP * 4, STAGE = XB + AB, SMEM = ST * STAGE;
+};
+template <int RP, int TM>
+__global__ void __launch_bounds__(kLoraThreads) lora_down_f32_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraDown<float, RP, TM>;
+  constexpr int CG = RP / 4, RG = kLoraThreads / CG < TM ? kLoraThreads / CG : TM, PER = TM / RG;  // threads along R and rows, rows each
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ int s_row[TM];
+  grid_wait();
+  if (static_cast<int>(blockIdx.x) >= *p.n_tiles) return;
+  const LoraTile tile = p.tiles[blockIdx.x];
+  if (tile.adapter < 0) return;
+  const int tid = threadIdx.x;
+  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
+  __syncthreads();
+  const int k0 = blockIdx.y * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
+  const float* A = static_cast<const float*>(p.a) + static_cast<long long>(tile.adapter) * p.K * p.R;
+  auto load = [&](int c) {
+    if (c < n) {
+      uint8_t* s = s_ring + c % C::ST * C::STAGE;
+      const int k = k0 + c * C::KC;
+      for (int i = tid; i < TM * 8; i += kLoraThreads) {
+        const int r = i >> 3, kk = k + (i & 7) * 4;
+        const bool in = r < tile.count && kk < k1;
+        cp_async16(smem_u32(s + (r * C::XS + (i & 7) * 4) * 4), static_cast<const float*>(p.x) + s_row[r] * p.x_stride + (in ? kk : 0), in ? 16 : 0);
+      }
+      for (int i = tid; i < C::KC * RP / 4; i += kLoraThreads) {
+        const int r = i / CG, ch = i % CG * 4;
+        const bool in = k + r < k1 && ch < p.R;
+        cp_async16(smem_u32(s + C::XB + i * 16), A + (in ? static_cast<long long>(k + r) * p.R + ch : 0), in ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  const int cg = tid % CG, rg = tid / CG;
+  const bool busy = rg < RG;
+  float acc[PER][4];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  for (int c = 0; c < C::ST - 1; ++c) load(c);
+  for (int c = 0; c < n; ++c) {
+    cp_async_wait<C::ST - 2>();
+    __syncthreads();
+    load(c + C::ST - 1);
+    const float* xs = reinterpret_cast<const float*>(s_ring + c % C::ST * C::STAGE);
+    const float4* as = reinterpret_cast<const float4*>(s_ring + c % C::ST * C::STAGE + C::XB);
+    if (busy)
+#pragma unroll 2
+      for (int k = 0; k < C::KC; k += 4) {
+        float4 a[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = as[(k + e) * CG + cg];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(xs + (i * RG + rg) * C::XS + k);
+          const float xv[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[i][0] = fmaf(xv[e], a[e].x, acc[i][0]);
+            acc[i][1] = fmaf(xv[e], a[e].y, acc[i][1]);
+            acc[i][2] = fmaf(xv[e], a[e].z, acc[i][2]);
+            acc[i][3] = fmaf(xv[e], a[e].w, acc[i][3]);
+          }
+        }
+      }
+  }
+  cp_async_wait<0>();
+  float* out = p.t + (static_cast<long long>(blockIdx.y) * p.rows + tile.at) * RP;
+  if (busy)
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i * RG + rg < tile.count)
+        *reinterpret_cast<float4*>(out + (i * RG + rg) * RP + cg * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+}
+
+template <int RP, int TM>
+struct LoraUp<float, RP, TM> {
+  static constexpr int NC = 64, TS = RP + 4;
+  static constexpr int TB = TM * TS * 4, BB = RP * NC * 4, SMEM = TB + BB;
+};
+template <int RP, int TM>
+__global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraUp<float, RP, TM>;
+  constexpr int PER = TM / 8;  // rows per thread: 16 threads of 4 columns, 8 of rows
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ int s_row[TM];
+  grid_wait();
+  if (static_cast<int>(blockIdx.y) >= *p.n_tiles) return;
+  const LoraTile tile = p.tiles[blockIdx.y];
+  if (tile.adapter < 0 && p.out == p.y) return;
+  const int tid = threadIdx.x, cg = tid % 16, rg = tid / 16;
+  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
+  float* ts = reinterpret_cast<float*>(s_ring);
+  float* bs = reinterpret_cast<float*>(s_ring + C::TB);
+  if (tile.adapter >= 0) {
+    const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
+    for (int i = tid; i < TM * RP; i += kLoraThreads) {
+      const int r = i / RP, k = i % RP;
+      float s = 0.f;
+      if (r < tile.count)
+        for (int part = 0; part < p.splits; ++part)
+          s += p.t[(static_cast<long long>(part) * p.rows + tile.at + r) * RP + k];
+      ts[r * C::TS + k] = s * scale;
+    }
+  }
+  const float* y = static_cast<const float*>(p.y);
+  float* out = static_cast<float*>(p.out);
+  const float* Bm = static_cast<const float*>(p.b) + static_cast<long long>(max(tile.adapter, 0)) * p.R * p.N;
+  const int n0 = blockIdx.x * p.chunks * C::NC;
+  for (int c = 0; c < p.chunks; ++c) {
+    const int base = n0 + c * C::NC, col = base + cg * 4;
+    if (base >= p.N) break;
+    __syncthreads();
+    if (tile.adapter >= 0)
+      for (int i = tid; i < RP * 16; i += kLoraThreads) {
+        const int r = i / 16, cc = base + i % 16 * 4;
+        const bool in = r < p.R && cc < p.N;
+        cp_async16(smem_u32(bs + i * 4), Bm + (in ? static_cast<long long>(r) * p.N + cc : 0), in ? 16 : 0);
+      }
+    cp_async_commit();
+    float4 v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      v[i] = col < p.N && i * 8 + rg < tile.count
+                 ? *reinterpret_cast<const float4*>(y + s_row[i * 8 + rg] * p.y_stride + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+    cp_async_wait<0>();
+    __syncthreads();
+    if (tile.adapter >= 0)
+#pragma unroll 2
+      for (int k = 0; k < RP; k += 4) {
+        float4 b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = *reinterpret_cast<const float4*>(bs + (k + e) * C::NC + cg * 4);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float4 t = *reinterpret_cast<const float4*>(ts + (i * 8 + rg) * C::TS + k);
+          const float tv[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[i].x = fmaf(tv[e], b[e].x, v[i].x);
+            v[i].y = fmaf(tv[e], b[e].y, v[i].y);
+            v[i].z = fmaf(tv[e], b[e].z, v[i].z);
+            v[i].w = fmaf(tv[e], b[e].w, v[i].w);
+          }
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (col < p.N && i * 8 + rg < tile.count)
+        *reinterpret_cast<float4*>(out + s_row[i * 8 + rg] * p.out_stride + col) = v[i];
   }
 }
 
+// ------------------------------------------------------------ launches
+// Parts of K while the tiles alone leave SMs idle: CTAs to fill the GPU twice, of at least 256 columns.
+constexpr int kLoraFill = 296;
+static int lora_rank(int R) { return R <= 16 ? 16 : R <= 64 ? 64 : 128; }
+static size_t lora_ws_bytes(int rows, int R) {
+  // splits * tiles <= kLoraFill unless splits is 1, and a tile has at most 64 rows
+  return (static_cast<size_t>(rows) + kLoraFill * 64) * lora_rank(R) * 4;
+}
+
+template <typename T, int RP, int TM>
+static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) {
+  const int cols = (p.N + 63) / 64, per = (cols + p.chunks - 1) / p.chunks;
+  cudaError_t e;
+  if constexpr (sizeof(T) == 4) {
+    e = allow_smem<lora_down_f32_kernel<RP, TM>>(LoraDown<T, RP, TM>::SMEM);
+    if (e == cudaSuccess) e = allow_smem<lora_up_f32_kernel<RP, TM>>(LoraUp<T, RP, TM>::SMEM);
+    if (e == cudaSuccess) e = launch_early(lora_down_f32_kernel<RP, TM>, dim3(tiles, p.splits), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p);
+    if (e == cudaSuccess) e = launch_early(lora_up_f32_kernel<RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
+  } else {
+    e = allow_smem<lora_down_kernel<T, RP, TM>>(LoraDown<T, RP, TM>::SMEM);
+    if (e == cudaSuccess) e = allow_smem<lora_up_kernel<T, RP, TM>>(LoraUp<T, RP, TM>::SMEM);
+    if (e == cudaSuccess) e = launch_early(lora_down_kernel<T, RP, TM>, dim3(tiles, p.splits), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p);
+    if (e == cudaSuccess) e = launch_early(lora_up_kernel<T, RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
+  }
+  return e;
+}
+
 template <typename T>
-static cudaError_t lora_add_t(const LoraParams& p, cudaStream_t st) {
-  cudaError_t e = launch_early(lora_down_kernel<T>, dim3(p.rows), 256, 0, st, p);
-  if (e != cudaSuccess) return e;
-  return launch_early(lora_up_kernel<T>, dim3(p.rows), 256, 0, st, p);
+static cudaError_t lora_add_t(LoraParams& p, const LoraPlanAt& plan, cudaStream_t st) {
+  const int tiles = plan.tiles, rank = lora_rank(p.R);
+  p.splits = kLoraFill / tiles;
+  if (p.splits > (p.K + 255) / 256) p.splits = (p.K + 255) / 256;
+  if (p.splits < 1) p.splits = 1;
+  p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
+  p.splits = (p.K + p.k_per - 1) / p.k_per;
+  // columns of out per CTA: up to 512, while there are CTAs to fill the GPU four times
+  p.chunks = static_cast<int>(static_cast<long long>(tiles) * ((p.N + 63) / 64) / (148 * 4));
+  p.chunks = p.chunks < 1 ? 1 : p.chunks > 8 ? 8 : p.chunks;
+#define LAUNCH(RP) return plan.tm == 64 ? lora_launch<T, RP, 64>(p, tiles, st) : lora_launch<T, RP, 16>(p, tiles, st)
+  if (rank == 16) LAUNCH(16);
+  if (rank == 64) LAUNCH(64);
+  LAUNCH(128);
+#undef LAUNCH
 }
 
 }  // namespace tkb
