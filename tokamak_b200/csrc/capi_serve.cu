@@ -93,7 +93,9 @@ int tkb_kv_pages(int32_t* block_table, int32_t* held, const int32_t* lens, int32
   if (reinterpret_cast<uintptr_t>(slots) & 7) return fail(TKB_ERR_ARG, "%s: slots must be 8-byte aligned", who);
   const PagesParams p = {block_table, held, lens, free_pages, n_free, granted, reinterpret_cast<long long*>(slots),
                          row_start, slots ? rows : 0, B, max_pages, page_size, n_pages};
-  return cuda_status(kv_pages(p, static_cast<cudaStream_t>(stream)), who, 1);
+  unsigned kernels = 0;
+  const cudaError_t e = kv_pages(p, static_cast<cudaStream_t>(stream), kernels);
+  return cuda_status(e, who, kernels);
 }
 
 size_t tkb_lora_plan_bytes(int B, int rows, int n_adapters) {
@@ -115,7 +117,7 @@ int tkb_lora_plan(const int32_t* adapter, const int32_t* row_start, int B, int r
   uint8_t* base = static_cast<uint8_t*>(plan);
   const LoraPlanParams p = {adapter, row_start, static_cast<int*>(plan), reinterpret_cast<LoraTile*>(base + 256),
                             reinterpret_cast<int32_t*>(base + at.rows), B, rows, n_adapters, at.tm, 0};
-  return cuda_status(lora_plan(p, static_cast<cudaStream_t>(stream)), who, 1);
+  return cuda_status(lora_plan(p, at.tiles * at.tm, static_cast<cudaStream_t>(stream)), who, 1);
 }
 
 size_t tkb_lora_workspace(int rows, int R) {
@@ -123,7 +125,7 @@ size_t tkb_lora_workspace(int rows, int R) {
     fail(TKB_ERR_ARG, "tkb_lora_workspace: rows are 1 to 2^21, R 1 to 128");
     return 0;
   }
-  return round256(lora_ws_bytes(rows, R));
+  return round256(static_cast<size_t>(rows) * lora_rank(R) * 4);
 }
 
 int tkb_lora_add(const void* plan, const void* x, long long x_stride, const void* A, const void* B_, const float* scale,

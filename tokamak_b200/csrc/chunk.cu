@@ -24,6 +24,10 @@
 
 namespace tkb {
 
+// Lets the next launch of the stream come up from here on, when all CTAs of this
+// one have started; its grid_wait() still waits for this one's end.
+TKB_DEVFN void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 struct alignas(64) ChunkParams {
   CUtensorMap tmQ, tmK, tmV;  // 16-bit types
   tkb_kv_cache c;
@@ -585,6 +589,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
     tmem_relinquish();
   }
   grid_wait();
+  grid_go();
   ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * static_cast<int>(sizeof(ChunkWalk)));
   const bool any = chunk_deal<320>(p, walk);
   tc_fence_before();
@@ -986,6 +991,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
   __shared__ int s_part[kChunkGrid], s_count[4], s_end;
   grid_wait();
+  grid_go();
   const int c = blockIdx.x, w = blockIdx.y / (D / 32), cg = blockIdx.y % (D / 32), r = threadIdx.x, lane = lane_id();
   const int4 span = p.span[c];
   if (!(span.x & SPAN_BEGINS)) return;

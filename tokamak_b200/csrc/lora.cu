@@ -6,16 +6,17 @@
 // plan sorts the rows by adapter and cuts them into tiles of one adapter each
 // (16 rows, or 64 where the adapters have that many), so that an adapter is
 // read once a tile and its products run on m16n8k16 instructions.  Two
-// kernels: t = x A, cut over K when there are few tiles, its fp32 parts in the
-// workspace; then out, cut over the columns.  The first product's result goes into the second as two
-// 16-bit values, the rounding and the rest, so that only out is rounded.
+// kernels: t = x A in fp32, cut over K into the CTAs of a cluster, which sum
+// their parts in order through their shared memories; then out, cut over the
+// columns.  t goes into the second product as two 16-bit values, the rounding
+// and the rest, so that only out is rounded.
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
 namespace tkb {
 
 // ============================================================ the plan
-// Layout: number of tiles (256 bytes), the tiles, then the row of every sorted place.
+// Layout: number of tiles (256 bytes), the tiles, then the tiles' rows, tm entries each.
 struct LoraTile {
   int adapter, at, count, unused;  // -1: rows without one; first sorted place, rows
 };
@@ -30,7 +31,7 @@ static LoraPlanAt lora_plan_at(int B, int rows, int n_adapters) {
   a.tm = rows >= 32 * groups ? 64 : 16;
   a.tiles = static_cast<int>(rows / a.tm + (groups < rows ? groups : rows));
   a.rows = 256 + static_cast<size_t>(a.tiles) * sizeof(LoraTile);
-  a.bytes = (a.rows + static_cast<size_t>(rows) * 4 + 255) & ~size_t(255);
+  a.bytes = (a.rows + static_cast<size_t>(a.tiles) * a.tm * 4 + 255) & ~size_t(255);
   return a;
 }
 
@@ -42,127 +43,146 @@ struct LoraPlanParams {
   int32_t* row_of;
   int B, rows, n_adapters, tm, sorted;  // sorted: power of two >= B
 };
-constexpr int kLoraPlanRows = 8192;     // sorted places per CTA
+constexpr int kLoraPlanRows = 8192;     // entries of row_of per CTA
 
-// Every CTA sorts the sequences by adapter (bitonic, in shared memory) and
-// finds its share of the rows; the first writes the tiles.
-__global__ void __launch_bounds__(kPagesThreads) lora_plan_kernel(const __grid_constant__ LoraPlanParams p) {
-  extern __shared__ unsigned long long s_key[];         // [sorted] adapter + 1, sequence
-  int* s_pos = reinterpret_cast<int*>(s_key + p.sorted);  // [sorted + 1] first sorted place
-  int* s_group = s_pos + p.sorted + 1;                  // [sorted + 1] first sorted sequence of each group
-  int* s_tile = s_group + p.sorted + 1;                 // [sorted + 1] its first tile
-  __shared__ int s_warp[32];
+// Every CTA sorts the sequences by adapter in shared memory, up to 256 of them
+// by counting the smaller ones of each, more by a bitonic network; the sums over the
+// sorted ones give places, groups of one adapter and tiles; then it writes its
+// share of the tiles and rows.
+template <int THREADS, int SEQS>
+__global__ void __launch_bounds__(THREADS) lora_plan_kernel(const __grid_constant__ LoraPlanParams p) {
+  extern __shared__ unsigned long long s_key[];           // [sorted] adapter + 1, sequence
   const int tid = threadIdx.x, n = p.sorted;
+  int2* s_rows = reinterpret_cast<int2*>(s_key + n);      // [sorted] first row and number, by sequence
+  int* s_pos = reinterpret_cast<int*>(s_rows + n);        // [sorted + 1] first sorted place
+  int* s_group = s_pos + n + 1;                           // [sorted + 1] first sorted sequence of each group
+  int* s_tile = s_group + n + 1;                          // [sorted + 1] its first tile
+  __shared__ unsigned long long s_warp[32];
   grid_wait();
-  for (int b = tid; b < n; b += kPagesThreads) {
-    unsigned long long key = ~0ull;
+  grid_go();
+  for (int b = tid; b < n; b += THREADS) {
+    unsigned long long key = ~0ull << 16 | b;             // behind all others, and no two alike
     if (b < p.B) {
-      int first, count, a = p.adapter[b];
-      chunk_rows(p.row_start, p.rows, b, first, count);
+      int2 r;
+      int a = p.adapter[b];
+      chunk_rows(p.row_start, p.rows, b, r.x, r.y);
       if (a < -1 || a >= p.n_adapters) {
         atomicOr(&g_device_error, ERR_BAD_INDEX);
         a = -1;
       }
-      if (count) key = static_cast<unsigned long long>(a + 1) << 32 | static_cast<unsigned>(b);
+      if (r.y) key = static_cast<unsigned long long>(a + 1) << 32 | static_cast<unsigned>(b);
+      s_rows[b] = r;
     }
     s_key[b] = key;
   }
   __syncthreads();
-  for (int size = 2; size <= n; size <<= 1)
-    for (int stride = size >> 1; stride; stride >>= 1) {
-      for (int i = tid; i < n / 2; i += kPagesThreads) {
-        const int lo = (i / stride) * 2 * stride + i % stride, hi = lo + stride;
-        const unsigned long long a = s_key[lo], b = s_key[hi];
-        if ((a > b) == !(lo & size)) {
-          s_key[lo] = b;
-          s_key[hi] = a;
+  if constexpr (SEQS == 1) {
+    const unsigned long long key = tid < n ? s_key[tid] : 0;
+    int rank = 0;
+    if (tid < n)
+      for (int i = 0; i < n; ++i) rank += s_key[i] < key;
+    __syncthreads();
+    if (tid < n) s_key[rank] = key;
+    __syncthreads();
+  } else {
+    for (int size = 2; size <= n; size <<= 1)
+      for (int stride = size >> 1; stride; stride >>= 1) {
+        for (int i = tid; i < n / 2; i += THREADS) {
+          const int lo = (i / stride) * 2 * stride + i % stride, hi = lo + stride;
+          const unsigned long long a = s_key[lo], b = s_key[hi];
+          if ((a > b) == !(lo & size)) {
+            s_key[lo] = b;
+            s_key[hi] = a;
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
-    }
-  // places, groups and tiles by sums over the sorted sequences
-  int count[kPagesSeqs], lead[kPagesSeqs], sum = 0, leads = 0;
+  }
+  auto holds = [&](int k) { return k < n && s_key[k] >> 48 != 0xffff; };
+  auto seq_of = [&](int k) { return static_cast<int>(s_key[k] & 0xffffffffu); };
+  int count[SEQS], lead[SEQS], sum = 0, leads = 0;
 #pragma unroll
-  for (int i = 0; i < kPagesSeqs; ++i) {
-    const int k = tid * kPagesSeqs + i;
+  for (int i = 0; i < SEQS; ++i) {
+    const int k = tid * SEQS + i;
     count[i] = lead[i] = 0;
-    if (k >= n || s_key[k] == ~0ull) continue;
-    int first;
-    chunk_rows(p.row_start, p.rows, static_cast<int>(s_key[k] & 0xffffffffu), first, count[i]);
+    if (!holds(k)) continue;
+    count[i] = s_rows[seq_of(k)].y;
     lead[i] = k == 0 || s_key[k] >> 32 != s_key[k - 1] >> 32;
     sum += count[i];
     leads += lead[i];
   }
-  int total, groups;
-  int at = pages_scan(sum, s_warp, total), g = pages_scan(leads, s_warp, groups);
-  if (total > p.rows) {  // sequences that share rows: those that do not fit are left out
-    if (tid == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
-    total = p.rows;
-  }
+  // rows in the upper half: sequences that share rows can have 4096 times as many as there are
+  unsigned long long all;
+  const unsigned long long before = block_scan<THREADS>(static_cast<unsigned long long>(sum) << 16 | leads, s_warp, all);
+  const int groups = static_cast<int>(all & 0xffff);
+  const bool over = all >> 16 > static_cast<unsigned>(p.rows);
+  const int total = over ? p.rows : static_cast<int>(all >> 16);
+  if (over && tid == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);  // those that do not fit are left out
+  long long at = static_cast<long long>(before >> 16);
+  int g = static_cast<int>(before & 0xffff);
 #pragma unroll
-  for (int i = 0; i < kPagesSeqs; ++i) {
-    const int k = tid * kPagesSeqs + i;
+  for (int i = 0; i < SEQS; ++i) {
+    const int k = tid * SEQS + i;
     if (k >= n) break;
-    s_pos[k] = min(at, total);
+    s_pos[k] = static_cast<int>(min(at, static_cast<long long>(total)));
     if (lead[i]) s_group[g++] = k;
     at += count[i];
   }
   if (tid == 0) s_pos[n] = total;
   __syncthreads();
-  auto group_end = [&](int i) { return i + 1 < groups ? s_pos[s_group[i + 1]] : total; };
-  if (blockIdx.x == 0) {
-    int tiles[kPagesSeqs], mine = 0, all;
+  auto group_start = [&](int i) { return i < groups ? s_pos[s_group[i]] : total; };
+  int tiles[SEQS], mine = 0;
 #pragma unroll
-    for (int i = 0; i < kPagesSeqs; ++i) {
-      const int k = tid * kPagesSeqs + i;
-      tiles[i] = k < groups ? (group_end(k) - s_pos[s_group[k]] + p.tm - 1) / p.tm : 0;
-      mine += tiles[i];
-    }
-    int t = pages_scan(mine, s_warp, all);
-#pragma unroll
-    for (int i = 0; i < kPagesSeqs; ++i) {
-      const int k = tid * kPagesSeqs + i;
-      if (k < groups) s_tile[k] = t;
-      t += tiles[i];
-    }
-    if (tid == 0) *p.n_tiles = all;
-    __syncthreads();
-    for (int i = tid; i < all; i += kPagesThreads) {
-      int lo = 0, hi = groups - 1;  // last group that starts at tile i or before
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_tile[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      LoraTile t;
-      t.adapter = static_cast<int>(s_key[s_group[lo]] >> 32) - 1;
-      t.at = s_pos[s_group[lo]] + (i - s_tile[lo]) * p.tm;
-      t.count = min(p.tm, group_end(lo) - t.at);
-      t.unused = 0;
-      p.tiles[i] = t;
-    }
+  for (int i = 0; i < SEQS; ++i) {
+    const int k = tid * SEQS + i;
+    tiles[i] = k < groups ? (group_start(k + 1) - group_start(k) + p.tm - 1) / p.tm : 0;
+    mine += tiles[i];
   }
-  const int first = blockIdx.x * kLoraPlanRows, last = min(first + kLoraPlanRows, total);
-  for (int i = first + tid; i < last; i += kPagesThreads) {
-    int lo = 0, hi = n - 1;  // last sorted sequence that starts at place i or before; those behind the rows start at `total`
+  int t = static_cast<int>(block_scan<THREADS>(static_cast<unsigned long long>(mine), s_warp, all));
+  const int n_tiles = static_cast<int>(all);
+#pragma unroll
+  for (int i = 0; i < SEQS; ++i) {
+    const int k = tid * SEQS + i;
+    if (k < groups) s_tile[k] = t;
+    t += tiles[i];
+  }
+  if (tid == 0 && blockIdx.x == 0) *p.n_tiles = n_tiles;
+  __syncthreads();
+  auto last_from = [](const int* from, int m, int x) {  // last of m ascending values that is x or less
+    int lo = 0, hi = m - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (s_pos[mid] <= i) lo = mid;
+      if (from[mid] <= x) lo = mid;
       else hi = mid - 1;
     }
-    int row0, rows;
-    chunk_rows(p.row_start, p.rows, static_cast<int>(s_key[lo] & 0xffffffffu), row0, rows);
-    p.row_of[i] = row0 + i - s_pos[lo];
+    return lo;
+  };
+  const int e0 = blockIdx.x * kLoraPlanRows, e1 = min(e0 + kLoraPlanRows, n_tiles * p.tm);
+  for (int e = e0 + tid; e < e1; e += THREADS) {
+    const int i = e / p.tm, r = e - i * p.tm, grp = last_from(s_tile, groups, i);
+    const int place = group_start(grp) + (i - s_tile[grp]) * p.tm, rows = min(p.tm, group_start(grp + 1) - place);
+    if (r == 0) {
+      LoraTile tile;
+      tile.adapter = static_cast<int>(s_key[s_group[grp]] >> 32) - 1;
+      tile.at = place;
+      tile.count = rows;
+      tile.unused = 0;
+      p.tiles[i] = tile;
+    }
+    const int x = place + min(r, rows - 1);  // entries behind the tile's rows repeat the last
+    const int k = last_from(s_pos, n, x);    // sequences behind the rows start at `total`
+    p.row_of[e] = s_rows[seq_of(k)].x + x - s_pos[k];
   }
 }
 
-static cudaError_t lora_plan(LoraPlanParams p, cudaStream_t st) {
+static cudaError_t lora_plan(LoraPlanParams p, int entries, cudaStream_t st) {
   p.sorted = 2;
   while (p.sorted < p.B) p.sorted *= 2;
-  const size_t smem = p.sorted * 8 + (p.sorted + 1) * 3 * sizeof(int);
-  const cudaError_t e = allow_smem<lora_plan_kernel>(kPagesThreads * kPagesSeqs * 20 + 16);
-  if (e != cudaSuccess) return e;
-  return launch_early(lora_plan_kernel, dim3((p.rows + kLoraPlanRows - 1) / kLoraPlanRows), kPagesThreads, smem, st, p);
+  const size_t smem = p.sorted * 16 + (p.sorted + 1) * 3 * sizeof(int);
+  const dim3 grid((entries + kLoraPlanRows - 1) / kLoraPlanRows);
+  if (p.B <= 256) return launch_early(lora_plan_kernel<256, 1>, grid, 256, smem, st, p);
+  const cudaError_t e = allow_smem<lora_plan_kernel<1024, 4>>(4096 * 28 + 16);
+  return e != cudaSuccess ? e : launch_early(lora_plan_kernel<1024, 4>, grid, 1024, smem, st, p);
 }
 
 // ============================================================ the products
@@ -173,10 +193,10 @@ struct LoraParams {
   const void *x, *a, *b, *y;
   void* out;
   const float* scale;
-  float* t;                // [splits][rows][RP] by sorted place
+  float* t;                // [rows][RP] by sorted place
   long long x_stride, y_stride, out_stride;
   int rows, K, N, R;
-  int splits, k_per;       // parts of K and columns of each (a multiple of a chunk)
+  int splits, k_per;       // parts of K, the CTAs of a cluster, and columns of each (a multiple of a chunk)
   int chunks;              // chunks of columns per CTA of the second kernel
 };
 constexpr int kLoraThreads = 128;
@@ -188,13 +208,38 @@ TKB_DEVFN int lora_swz(int r, int ch) {
   return r * RB + ((ch ^ (RB == 32 ? r >> 2 & 1 : r & 7)) << 4);
 }
 
+// The parts of a tile of t, [count][RP] floats in each CTA's shared memory at
+// the same place, summed in the order of the cluster's ranks; each CTA writes its share.
+TKB_DEVFN void lora_meet(const float* mine, float* out, int values, int ctas) {
+  if (ctas > 1) cluster_sync();
+  else __syncthreads();
+  const uint32_t here = smem_u32(mine);
+  const int rank = blockIdx.x;  // the grid's first dimension is the cluster
+  for (int i = (rank * kLoraThreads + threadIdx.x) * 4; i < values; i += ctas * kLoraThreads * 4) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < ctas; ++c) {
+      float4 v;
+      if (ctas == 1) v = *reinterpret_cast<const float4*>(mine + i);
+      else
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(here + i * 4, c)) : "memory");
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+    *reinterpret_cast<float4*>(out + i) = sum;
+  }
+  if (ctas > 1) cluster_sync();  // the others have read this CTA's part
+}
+
 // t = x A over one part of K.  A warp holds 16 rows; tiles of 16 rows give each
 // warp a quarter of every chunk of K instead.
 template <typename T, int RP, int TM>
 struct LoraDown {
   static constexpr int KC = 64, ST = 4;                  // columns of K per chunk, chunks in flight
   static constexpr int XB = TM * KC * 2, AB = KC * RP * 2, STAGE = XB + AB;
-  static constexpr int SUM = TM == 16 ? 4 * 16 * RP * 4 : 0;
+  static constexpr int SUM = (TM == 16 ? 5 : 4) * 16 * RP * 4;  // the warps' quarters and their sum, or the tile
   static constexpr int SMEM = ST * STAGE > SUM ? ST * STAGE : SUM;
 };
 template <typename T, int RP, int TM>
@@ -204,13 +249,14 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ int s_row[TM];
   grid_wait();
-  if (static_cast<int>(blockIdx.x) >= *p.n_tiles) return;
-  const LoraTile tile = p.tiles[blockIdx.x];
-  if (tile.adapter < 0) return;
+  grid_go();
+  const int n_tiles = *p.n_tiles;
+  const LoraTile tile = p.tiles[blockIdx.y];  // read beside the number: behind it lies what an earlier plan left
+  if (threadIdx.x < TM) s_row[threadIdx.x] = p.row_of[blockIdx.y * TM + threadIdx.x];
+  if (static_cast<int>(blockIdx.y) >= n_tiles || tile.adapter < 0) return;
   const int tid = threadIdx.x, lane = lane_id(), w = warp_id();
-  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
   __syncthreads();
-  const int k0 = blockIdx.y * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
+  const int k0 = blockIdx.x * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
   const T* A = static_cast<const T*>(p.a) + static_cast<long long>(tile.adapter) * p.K * p.R;
   auto load = [&](int c) {
     if (c < n) {
@@ -256,28 +302,22 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
     }
   }
   cp_async_wait<0>();
+  __syncthreads();
   const int g = lane >> 2, c2 = (lane & 3) * 2;
-  float* out = p.t + (static_cast<long long>(blockIdx.y) * p.rows + tile.at) * RP;
+  float* s = reinterpret_cast<float*>(s_ring);
+#pragma unroll
+  for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2)
+      *reinterpret_cast<float2*>(s + (w * 16 + g + (e >> 1) * 8) * RP + j * 8 + c2) = make_float2(acc[j][e], acc[j][e + 1]);
   if constexpr (TM == 16) {
-    // the warps' quarters meet
-    __syncthreads();
-    float* s = reinterpret_cast<float*>(s_ring);
-#pragma unroll
-    for (int j = 0; j < RP / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[(w * 16 + g + (e >> 1) * 8) * RP + j * 8 + c2 + (e & 1)] = acc[j][e];
+    // the warps' quarters of every chunk
     __syncthreads();
     for (int i = tid; i < tile.count * RP; i += kLoraThreads)
-      out[i] = (s[i] + s[16 * RP + i]) + (s[32 * RP + i] + s[48 * RP + i]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < RP / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const int r = r0 + g + (e >> 1) * 8;
-        if (r < tile.count) *reinterpret_cast<float2*>(out + r * RP + j * 8 + c2) = make_float2(acc[j][e], acc[j][e + 1]);
-      }
+      s[64 * RP + i] = (s[i] + s[16 * RP + i]) + (s[32 * RP + i] + s[48 * RP + i]);
+    s += 64 * RP;
   }
+  lora_meet(s, p.t + static_cast<long long>(tile.at) * RP, tile.count * RP, p.splits);
 }
 
 // out = y + t B for one tile and `chunks` times 64 columns.  A warp has 16 rows,
@@ -294,11 +334,12 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_cons
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ int s_row[TM];
   grid_wait();
-  if (static_cast<int>(blockIdx.y) >= *p.n_tiles) return;
+  grid_go();
+  const int n_tiles = *p.n_tiles;
   const LoraTile tile = p.tiles[blockIdx.y];
-  if (tile.adapter < 0 && p.out == p.y) return;
+  if (threadIdx.x < TM) s_row[threadIdx.x] = p.row_of[blockIdx.y * TM + threadIdx.x];
+  if (static_cast<int>(blockIdx.y) >= n_tiles || (tile.adapter < 0 && p.out == p.y)) return;
   const int tid = threadIdx.x, lane = lane_id(), w = warp_id();
-  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
   __syncthreads();
   const int n0 = blockIdx.x * p.chunks * C::NC, n = min(p.chunks, (p.N - n0 + C::NC - 1) / C::NC);
   const T* y = static_cast<const T*>(p.y);
@@ -330,7 +371,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_cons
     cp_async_commit();
   };
   for (int c = 0; c < C::ST - 1; ++c) load(c);
-  // t of this thread's rows g and g + 8: the parts summed in their order, times the adapter's scale
+  // t of this thread's rows g and g + 8, times the adapter's scale
   const int g = lane >> 2, c2 = (lane & 3) * 2, r0 = TM == 16 ? 0 : w * 16;
   const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
   float up[2] = {1.f, 1.f};  // f16: t goes in as multiples of a power of two near the row's largest, so that it fits the type
@@ -344,14 +385,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_cons
       for (int i = 0; i < 4; ++i) {
         const int r = r0 + g + (i & 1) * 8;
         float2 s = make_float2(0.f, 0.f);
-        if (r < tile.count) {
-          const float* src = p.t + (static_cast<long long>(tile.at) + r) * RP + k * 16 + (i >> 1) * 8 + c2;
-          for (int part = 0; part < p.splits; ++part) {
-            const float2 v = *reinterpret_cast<const float2*>(src + static_cast<long long>(part) * p.rows * RP);
-            s.x += v.x;
-            s.y += v.y;
-          }
-        }
+        if (r < tile.count)
+          s = *reinterpret_cast<const float2*>(p.t + (static_cast<long long>(tile.at) + r) * RP + k * 16 + (i >> 1) * 8 + c2);
         t[k][2 * i] = s.x * scale;
         t[k][2 * i + 1] = s.y * scale;
         top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(t[k][2 * i]), fabsf(t[k][2 * i + 1])));
@@ -430,7 +465,8 @@ template <int RP, int TM>
 struct LoraDown<float, RP, TM> {
   static constexpr int KC = 32, ST = 3;
   static constexpr int XS = KC + 4;                      // floats from row to row: eight rows in different banks
-  static constexpr int XB = TM * XS * 4, AB = KC * RP * 4, STAGE = XB + AB, SMEM = ST * STAGE;
+  static constexpr int XB = TM * XS * 4, AB = KC * RP * 4, STAGE = XB + AB;
+  static constexpr int SMEM = ST * STAGE > TM * RP * 4 ? ST * STAGE : TM * RP * 4;
 };
 template <int RP, int TM>
 __global__ void __launch_bounds__(kLoraThreads) lora_down_f32_kernel(const __grid_constant__ LoraParams p) {
@@ -439,13 +475,14 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_f32_kernel(const __gri
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ int s_row[TM];
   grid_wait();
-  if (static_cast<int>(blockIdx.x) >= *p.n_tiles) return;
-  const LoraTile tile = p.tiles[blockIdx.x];
-  if (tile.adapter < 0) return;
+  grid_go();
+  const int n_tiles = *p.n_tiles;
+  const LoraTile tile = p.tiles[blockIdx.y];  // read beside the number: behind it lies what an earlier plan left
+  if (threadIdx.x < TM) s_row[threadIdx.x] = p.row_of[blockIdx.y * TM + threadIdx.x];
+  if (static_cast<int>(blockIdx.y) >= n_tiles || tile.adapter < 0) return;
   const int tid = threadIdx.x;
-  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
   __syncthreads();
-  const int k0 = blockIdx.y * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
+  const int k0 = blockIdx.x * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + C::KC - 1) / C::KC);
   const float* A = static_cast<const float*>(p.a) + static_cast<long long>(tile.adapter) * p.K * p.R;
   auto load = [&](int c) {
     if (c < n) {
@@ -499,12 +536,13 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_f32_kernel(const __gri
       }
   }
   cp_async_wait<0>();
-  float* out = p.t + (static_cast<long long>(blockIdx.y) * p.rows + tile.at) * RP;
+  __syncthreads();
+  float* s = reinterpret_cast<float*>(s_ring);
   if (busy)
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (i * RG + rg < tile.count)
-        *reinterpret_cast<float4*>(out + (i * RG + rg) * RP + cg * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+      *reinterpret_cast<float4*>(s + (i * RG + rg) * RP + cg * 4) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  lora_meet(s, p.t + static_cast<long long>(tile.at) * RP, tile.count * RP, p.splits);
 }
 
 template <int RP, int TM>
@@ -519,22 +557,19 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_
   extern __shared__ __align__(128) uint8_t s_ring[];
   __shared__ int s_row[TM];
   grid_wait();
-  if (static_cast<int>(blockIdx.y) >= *p.n_tiles) return;
+  grid_go();
+  const int n_tiles = *p.n_tiles;
   const LoraTile tile = p.tiles[blockIdx.y];
-  if (tile.adapter < 0 && p.out == p.y) return;
+  if (threadIdx.x < TM) s_row[threadIdx.x] = p.row_of[blockIdx.y * TM + threadIdx.x];
+  if (static_cast<int>(blockIdx.y) >= n_tiles || (tile.adapter < 0 && p.out == p.y)) return;
   const int tid = threadIdx.x, cg = tid % 16, rg = tid / 16;
-  if (tid < TM) s_row[tid] = p.row_of[tile.at + min(tid, tile.count - 1)];
   float* ts = reinterpret_cast<float*>(s_ring);
   float* bs = reinterpret_cast<float*>(s_ring + C::TB);
   if (tile.adapter >= 0) {
     const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
     for (int i = tid; i < TM * RP; i += kLoraThreads) {
       const int r = i / RP, k = i % RP;
-      float s = 0.f;
-      if (r < tile.count)
-        for (int part = 0; part < p.splits; ++part)
-          s += p.t[(static_cast<long long>(part) * p.rows + tile.at + r) * RP + k];
-      ts[r * C::TS + k] = s * scale;
+      ts[r * C::TS + k] = r < tile.count ? p.t[(static_cast<long long>(tile.at) + r) * RP + k] * scale : 0.f;
     }
   }
   const float* y = static_cast<const float*>(p.y);
@@ -586,13 +621,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_
 }
 
 // ------------------------------------------------------------ launches
-// Parts of K while the tiles alone leave SMs idle: CTAs to fill the GPU twice, of at least 256 columns.
-constexpr int kLoraFill = 296;
 static int lora_rank(int R) { return R <= 16 ? 16 : R <= 64 ? 64 : 128; }
-static size_t lora_ws_bytes(int rows, int R) {
-  // splits * tiles <= kLoraFill unless splits is 1, and a tile has at most 64 rows
-  return (static_cast<size_t>(rows) + kLoraFill * 64) * lora_rank(R) * 4;
-}
 
 template <typename T, int RP, int TM>
 static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) {
@@ -601,12 +630,12 @@ static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) 
   if constexpr (sizeof(T) == 4) {
     e = allow_smem<lora_down_f32_kernel<RP, TM>>(LoraDown<T, RP, TM>::SMEM);
     if (e == cudaSuccess) e = allow_smem<lora_up_f32_kernel<RP, TM>>(LoraUp<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = launch_early(lora_down_f32_kernel<RP, TM>, dim3(tiles, p.splits), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p);
+    if (e == cudaSuccess) e = launch_early(lora_down_f32_kernel<RP, TM>, dim3(p.splits, tiles), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p, p.splits);
     if (e == cudaSuccess) e = launch_early(lora_up_f32_kernel<RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
   } else {
     e = allow_smem<lora_down_kernel<T, RP, TM>>(LoraDown<T, RP, TM>::SMEM);
     if (e == cudaSuccess) e = allow_smem<lora_up_kernel<T, RP, TM>>(LoraUp<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = launch_early(lora_down_kernel<T, RP, TM>, dim3(tiles, p.splits), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p);
+    if (e == cudaSuccess) e = launch_early(lora_down_kernel<T, RP, TM>, dim3(p.splits, tiles), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p, p.splits);
     if (e == cudaSuccess) e = launch_early(lora_up_kernel<T, RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
   }
   return e;
@@ -615,13 +644,12 @@ static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) 
 template <typename T>
 static cudaError_t lora_add_t(LoraParams& p, const LoraPlanAt& plan, cudaStream_t st) {
   const int tiles = plan.tiles, rank = lora_rank(p.R);
-  p.splits = kLoraFill / tiles;
-  if (p.splits > (p.K + 255) / 256) p.splits = (p.K + 255) / 256;
-  if (p.splits < 1) p.splits = 1;
+  // parts of K: CTAs to fill the GPU four times, each of at least 256 columns, a cluster of eight at most
+  p.splits = 1;
+  while (p.splits < 8 && static_cast<long long>(tiles) * p.splits < 148 * 4 && p.K >= 512 * p.splits) p.splits *= 2;
   p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
-  p.splits = (p.K + p.k_per - 1) / p.k_per;
-  // columns of out per CTA: up to 512, while there are CTAs to fill the GPU four times
-  p.chunks = static_cast<int>(static_cast<long long>(tiles) * ((p.N + 63) / 64) / (148 * 4));
+  // columns of out per CTA: up to 512, while there are CTAs to fill the GPU eight times
+  p.chunks = static_cast<int>(static_cast<long long>(tiles) * ((p.N + 63) / 64) / (148 * 8));
   p.chunks = p.chunks < 1 ? 1 : p.chunks > 8 ? 8 : p.chunks;
 #define LAUNCH(RP) return plan.tm == 64 ? lora_launch<T, RP, 64>(p, tiles, st) : lora_launch<T, RP, 16>(p, tiles, st)
   if (rank == 16) LAUNCH(16);

@@ -5,10 +5,12 @@
 namespace tkb {
 
 // Latency bounds it: some 20 bytes a sequence and 8 a page moved.  One launch
-// of one cluster: every CTA sums the sequences' needs for itself (two scans over
-// at most 4096 of them, in shared memory), so that the CTAs share nothing but
-// the order of three phases, kept by cluster barriers: all have read the state;
-// surplus pages are on the stack; the missing ones are in the table.
+// of one cluster (one CTA up to 256 sequences): every CTA sums the sequences'
+// needs for itself (a scan over at most 4096 of them, in shared memory), so
+// that the CTAs share nothing but the order of three phases, kept by cluster
+// barriers: all have read the state; surplus pages are on the stack; the
+// missing ones are in the table.  The slots of many rows are a second launch
+// over all SMs (1000 sequences, 190 k rows: 84 us in the cluster's eight).
 struct PagesParams {
   int32_t* table;
   int32_t* held;
@@ -21,49 +23,82 @@ struct PagesParams {
   int rows, B, max_pages, page_size, n_pages;
 };
 
-constexpr int kPagesThreads = 1024;
-constexpr int kPagesSeqs = 4;  // sequences per thread of the scans: 4096 in all
-
 // Exclusive sums over the block of each thread's value, and the total.
-TKB_DEVFN int pages_scan(int v, int* s_warp, int& total) {
+template <int THREADS, typename V>
+TKB_DEVFN V block_scan(V v, V* s_warp, V& total) {
+  constexpr int W = THREADS / 32;
   const int lane = lane_id(), w = warp_id();
-  int x = v;
+  V x = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    const V y = __shfl_up_sync(0xffffffffu, x, d);
     if (lane >= d) x += y;
   }
   __syncthreads();
   if (lane == 31) s_warp[w] = x;
   __syncthreads();
-  int sum = s_warp[lane];
-  int upto = sum;
+  const V sum = lane < W ? s_warp[lane] : V(0);
+  V upto = sum;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, upto, d);
+  for (int d = 1; d < W; d <<= 1) {
+    const V y = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += y;
   }
-  total = __shfl_sync(0xffffffffu, upto, 31);
-  const int before = __shfl_sync(0xffffffffu, upto - sum, w);
+  total = __shfl_sync(0xffffffffu, upto, W - 1);
+  const V before = __shfl_sync(0xffffffffu, upto - sum, w);
   return before + x - v;
 }
 
-__global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(const __grid_constant__ PagesParams p) {
+// The slot of a row that belongs to sequence b, `back` rows before its sequence's end.
+TKB_DEVFN long long page_slot(const PagesParams& p, int b, int back, int pages) {
+  const long long slot = static_cast<long long>(__ldg(p.lens + b)) - back;
+  if (slot < 0 || slot >= static_cast<long long>(pages) * p.page_size) return -1;
+  const int i = static_cast<int>(slot) / p.page_size;
+  const int page = __ldcg(p.table + static_cast<long long>(b) * p.max_pages + i);
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.n_pages)) return -1;
+  return static_cast<long long>(page) * p.page_size + (static_cast<int>(slot) - i * p.page_size);
+}
+// The sequence of a row: the last b with row_start[b] <= row; false where the row is not its own.
+TKB_DEVFN bool row_seq(const int32_t* row_start, int B, int row, int& b, int& back) {
+  b = row;
+  back = 1;
+  if (!row_start) return true;
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(row_start + mid) <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  b = lo;
+  const int end = __ldg(row_start + b + 1);
+  back = end - row;
+  return __ldg(row_start + b) <= row && row < end;
+}
+
+constexpr int kPagesSlots = 4096;  // rows whose slots the same launch finds
+
+// SEQS sequences a thread.
+template <int THREADS, int SEQS>
+__global__ void __launch_bounds__(THREADS) kv_pages_kernel(const __grid_constant__ PagesParams p) {
   // per sequence: pages kept, pages to give back (with a minus sign) or to take, and where they go on or come off the stack
   extern __shared__ int s_seq[];
-  __shared__ int s_warp[32];
+  __shared__ unsigned long long s_warp[32];
   int* s_kept = s_seq;
   int* s_move = s_seq + p.B;
   int* s_at = s_seq + 2 * p.B;
   const int tid = threadIdx.x, lane = lane_id();
   const int rank = blockIdx.x, ctas = gridDim.x;  // the grid is one cluster
+  auto together = [&]() {
+    if (SEQS > 1) cluster_sync();
+    else __syncthreads();
+  };
   grid_wait();
-  int kept[kPagesSeqs], back[kPagesSeqs], need[kPagesSeqs], sum_back = 0, sum_need = 0;
-  bool odd = false, room[kPagesSeqs];
+  int kept[SEQS], back[SEQS], need[SEQS], sum_back = 0, sum_need = 0;
+  bool odd = false, room[SEQS];
   const long long most = static_cast<long long>(p.max_pages) * p.page_size;
 #pragma unroll
-  for (int i = 0; i < kPagesSeqs; ++i) {
-    const int b = tid * kPagesSeqs + i;
+  for (int i = 0; i < SEQS; ++i) {
+    const int b = tid * SEQS + i;
     kept[i] = back[i] = need[i] = 0;
     room[i] = true;
     if (b >= p.B) continue;
@@ -82,16 +117,17 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(const __grid_co
   int n_free = *p.n_free;
   odd |= n_free < 0 || n_free > p.n_pages;
   n_free = min(max(n_free, 0), p.n_pages);
-  int all_back, all_need;
-  int at_back = n_free + pages_scan(sum_back, s_warp, all_back);
-  int at_need = pages_scan(sum_need, s_warp, all_need);
+  unsigned long long all;
+  const unsigned long long at = block_scan<THREADS>(static_cast<unsigned long long>(sum_back) << 32 | static_cast<unsigned>(sum_need), s_warp, all);
+  const int all_back = static_cast<int>(all >> 32);
+  int at_back = n_free + static_cast<int>(at >> 32), at_need = static_cast<int>(at & 0xffffffffu);
   odd |= n_free + all_back > p.n_pages;
   const int height = min(n_free + all_back, p.n_pages);
-  cluster_sync();  // all have read held and n_free
+  together();  // all have read held and n_free
   int taken = 0;
 #pragma unroll
-  for (int i = 0; i < kPagesSeqs; ++i) {
-    const int b = tid * kPagesSeqs + i;
+  for (int i = 0; i < SEQS; ++i) {
+    const int b = tid * SEQS + i;
     if (b >= p.B) break;
     const bool fits = need[i] == 0 || at_need + need[i] <= height;
     s_kept[b] = kept[i];
@@ -107,15 +143,15 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(const __grid_co
   }
   taken = __reduce_max_sync(0xffffffffu, taken);
   __syncthreads();
-  if (lane == 0) s_warp[warp_id()] = taken;
+  if (lane == 0) s_warp[warp_id()] = static_cast<unsigned>(taken);
   __syncthreads();
   if (tid == 0 && rank == 0) {
-    for (int w = 0; w < kPagesThreads / 32; ++w) taken = max(taken, s_warp[w]);
+    for (int w = 0; w < THREADS / 32; ++w) taken = max(taken, static_cast<int>(s_warp[w]));
     *p.n_free = height - taken;
   }
   if (odd && rank == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
   // a warp a sequence
-  const int w0 = rank * (kPagesThreads / 32) + warp_id(), warps = ctas * (kPagesThreads / 32);
+  const int w0 = rank * (THREADS / 32) + warp_id(), warps = ctas * (THREADS / 32);
   for (int b = w0; b < p.B; b += warps) {
     const int n = -s_move[b], at = s_at[b];
     int32_t* t = p.table + static_cast<long long>(b) * p.max_pages + s_kept[b];
@@ -124,47 +160,45 @@ __global__ void __launch_bounds__(kPagesThreads) kv_pages_kernel(const __grid_co
       t[e] = -1;
     }
   }
-  cluster_sync();  // the stack is whole
+  together();  // the stack is whole
   for (int b = w0; b < p.B; b += warps) {
     const int n = s_move[b], at = s_at[b];
     int32_t* t = p.table + static_cast<long long>(b) * p.max_pages + s_kept[b];
     for (int e = lane; e < n; e += 32) t[e] = __ldcg(p.free_pages + at - e);
   }
   if (!p.slots) return;
-  cluster_sync();  // the table is whole
-  for (int row = rank * kPagesThreads + tid; row < p.rows; row += ctas * kPagesThreads) {
-    int b = row, back = 1;
-    bool has = true;
-    if (p.row_start) {
-      int lo = 0, hi = p.B - 1;  // last b with row_start[b] <= row
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(p.row_start + mid) <= row) lo = mid;
-        else hi = mid - 1;
-      }
-      b = lo;
-      const int end = __ldg(p.row_start + b + 1);
-      has = __ldg(p.row_start + b) <= row && row < end;
-      back = end - row;
-    }
-    const long long slot = static_cast<long long>(__ldg(p.lens + b)) - back;
-    const int pages = s_kept[b] + max(s_move[b], 0);
-    long long to = -1;
-    if (has && slot >= 0 && slot < static_cast<long long>(pages) * p.page_size) {
-      const int i = static_cast<int>(slot / p.page_size);
-      const int page = __ldcg(p.table + static_cast<long long>(b) * p.max_pages + i);
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(p.n_pages))
-        to = static_cast<long long>(page) * p.page_size + slot % p.page_size;
-    }
-    p.slots[row] = to;
+  together();  // the table is whole
+  for (int row = rank * THREADS + tid; row < p.rows; row += ctas * THREADS) {
+    int b, back;
+    const bool has = row_seq(p.row_start, p.B, row, b, back);
+    p.slots[row] = has ? page_slot(p, b, back, s_kept[b] + max(s_move[b], 0)) : -1;
   }
 }
 
-static cudaError_t kv_pages(const PagesParams& p, cudaStream_t st) {
-  const int ctas = p.B > 128 || p.rows > 4096 ? 8 : 1;
-  const cudaError_t e = allow_smem<kv_pages_kernel>(3 * sizeof(int) * kPagesThreads * kPagesSeqs);
-  if (e != cudaSuccess) return e;
-  return launch_early(kv_pages_kernel, dim3(ctas), kPagesThreads, 3 * sizeof(int) * p.B, st, p, ctas);
+__global__ void __launch_bounds__(256) kv_slots_kernel(const __grid_constant__ PagesParams p) {
+  grid_wait();
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= p.rows) return;
+  int b, back;
+  const bool has = row_seq(p.row_start, p.B, row, b, back);
+  p.slots[row] = has ? page_slot(p, b, back, p.held[b]) : -1;
+}
+
+static cudaError_t kv_pages(const PagesParams& p, cudaStream_t st, unsigned& kernels) {
+  PagesParams first = p;
+  const bool apart = p.slots && p.rows > kPagesSlots;
+  if (apart) first.slots = nullptr;
+  const size_t smem = 3 * sizeof(int) * p.B;
+  cudaError_t e = cudaSuccess;
+  if (p.B <= 256) {
+    e = launch_early(kv_pages_kernel<256, 1>, dim3(1), 256, smem, st, first);
+  } else {
+    e = allow_smem<kv_pages_kernel<1024, 4>>(3 * sizeof(int) * 4096);
+    if (e == cudaSuccess) e = launch_early(kv_pages_kernel<1024, 4>, dim3(8), 1024, smem, st, first, 8);
+  }
+  kernels = apart ? 2 : 1;
+  if (apart && e == cudaSuccess) e = launch_early(kv_slots_kernel, dim3((p.rows + 255) / 256), 256, 0, st, p);
+  return e;
 }
 
 }  // namespace tkb
