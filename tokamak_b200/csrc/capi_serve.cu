@@ -72,11 +72,9 @@ int tkb_paged_attn_chunk(const tkb_kv_cache* cache, const void* q, long long q_s
   p.G = Hq / cache->Hkv;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  unsigned kernels = 0;
-#define CALL(T) paged_chunk_t<T>(p, workspace, st, kernels)
-  const cudaError_t e = TKB_BY_DTYPE(cache->dtype, CALL);
+#define CALL(T) paged_chunk_t<T>(p, workspace, st)
+  return cuda_status(TKB_BY_DTYPE(cache->dtype, CALL), who, 2);
 #undef CALL
-  return cuda_status(e, who, kernels);
 }
 
 int tkb_kv_pages(int32_t* block_table, int32_t* held, const int32_t* lens, int32_t* free_pages, int32_t* n_free,

@@ -38,7 +38,7 @@ struct alignas(64) ChunkParams {
   long long q_stride, out_stride;
   int rows, Hq, G;
   int gb, hb;          // query heads per tile, blocks of them per kv head (G <= hb * gb)
-  int tt;              // tokens per tile: 128 / gb
+  int tt;              // tokens per tile: 128 / gb, of fp32 64 / gb
   int gran;            // slots per TMA box: what divides both a page and a block of 128
   float scale_log2;
   float4* part;        // [2 * grid][2 tiles][D / 4][128 rows] unnormalised parts
@@ -1069,69 +1069,250 @@ __global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__
 }
 
 // ============================================================ fp32
-template <typename T, int E>
-TKB_DEVFN void lane_values(const T* p, float (&f)[E]) {
+// The same units and parts on FMA instructions, two at a time (f32x2): a CTA of
+// 256 threads holds up to 128 packed rows (two tiles of 64) against 64 slots.
+// Thread (tr, tc) of 16 x 16 has rows tr + 16 i, i < MR, and slots tc + 16 e of the scores,
+// and columns 4 tc .. 4 tc + 3 of every 64 of the output, so that a row's
+// scores, weights and sums stay in one half of a warp.  MR follows the unit's
+// rows: with 128 of them FMA issue bounds it, with 16 or fewer the reads of K
+// and V from shared memory, a little below HBM's rate.
+template <int D>
+struct ChunkF32 {
+  static constexpr int TS = 64;                            // slots at a time
+  static constexpr int KS = D + 4, PS = TS + 4;            // floats from row to row: neighbours in different banks
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 128 * KS * 4;
+  static constexpr int OFF_V = OFF_K + TS * KS * 4;
+  static constexpr int OFF_P = OFF_V + TS * D * 4;
+  static constexpr int OFF_WALK = OFF_P + 128 * PS * 4;
+  static constexpr int OFF_AT = OFF_WALK + 8 * sizeof(ChunkWalk);  // [2][TS] element offsets of the slots, -1 for none
+  static constexpr int SMEM = OFF_AT + 2 * TS * 8;
+  static_assert(SMEM <= 232448 && sizeof(ChunkWalk) % 8 == 0, "shared memory");
+};
+
+// The blocks of one item for MR rows a thread.
+template <int D, int MR>
+__noinline__ __device__ void chunk_f32_item(const ChunkParams& p, const ChunkItem& it, uint8_t* smem) {
+  using C = ChunkF32<D>;
+  constexpr int DC = D / 64;  // groups of four columns a thread
+  const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;
+  float* sq = reinterpret_cast<float*>(smem + C::OFF_Q);
+  float* sk = reinterpret_cast<float*>(smem + C::OFF_K);
+  float* sv = reinterpret_cast<float*>(smem + C::OFF_V);
+  float* sp = reinterpret_cast<float*>(smem + C::OFF_P);
+  long long* s_at = reinterpret_cast<long long*>(smem + C::OFF_AT);
+  const ChunkSeq s = it.s;
+  const int h = it.hg / p.hb, b = it.b;
+  // row r of the CTA: tile r / 64, and its token and head in the tile
+  auto row_of = [&](int r, int& tok, int& hq) {
+    const int rr = r & 63, t = rr / p.gb;
+    return chunk_row(p, it.hg, it.t0, it.tokens, r >> 6, t, rr - t * p.gb, tok, hq);
+  };
+  auto places = [&](int sub) {  // of the slots of 64 from sub * 64 on
+    if (tid < C::TS) {
+      const int slot = sub * C::TS + tid;
+      long long at = -1;
+      if (slot < s.held) {
+        const int page = page_of(p.c, b, slot / p.c.page_size);
+        if (page >= 0) at = page_offset(p.c, page, h) + static_cast<long long>(slot % p.c.page_size) * D;
+      }
+      s_at[(sub & 1) * C::TS + tid] = at;
+    }
+  };
+  auto fetch = [&](const void* pool, float* to, int stride, int sub, bool any) {
+    if (any)
+      for (int i = tid; i < C::TS * D / 4; i += 256) {
+        const int r = i / (D / 4), c = i % (D / 4) * 4;
+        const long long at = s_at[(sub & 1) * C::TS + r];
+        cp_async16(smem_u32(to + r * stride + c), static_cast<const float*>(pool) + (at < 0 ? 0 : at + c), at < 0 ? 0 : 16);
+      }
+    cp_async_commit();
+  };
+  const int sub0 = it.jb * (kChunkBlock / C::TS), sub1 = it.je * (kChunkBlock / C::TS);
+  __syncthreads();  // the item before is through with shared memory
+  places(sub0);
+  for (int i = tid; i < 16 * MR * D / 4; i += 256) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    int tok, hq;
+    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row_of(r, tok, hq))
+      q = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + (s.first + tok) * p.q_stride + static_cast<long long>(hq) * D + c);
+    *reinterpret_cast<float4*>(sq + r * C::KS + c) = q;
+  }
+  __syncthreads();
+  fetch(p.c.k, sk, C::KS, sub0, true);
+  fetch(p.c.v, sv, D, sub0, true);
+  int lim[MR];
+  float m[MR], l[MR];
+  uint64_t o[MR][2 * DC];
+  int first_lim = 0x7fffffff;
 #pragma unroll
-  for (int e = 0; e < E; ++e) f[e] = static_cast<float>(p[e]);
+  for (int i = 0; i < MR; ++i) {
+    int tok, hq;
+    const bool valid = row_of(tr + 16 * i, tok, hq);
+    lim[i] = valid ? min(max(s.base + tok + 1, 0), s.held) : 0;
+    if (valid) first_lim = min(first_lim, lim[i]);
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 2 * DC; ++c) o[i][c] = f2(0.f, 0.f);
+  }
+#pragma unroll 1
+  for (int sub = sub0; sub < sub1; ++sub) {
+    const bool more = sub + 1 < sub1;
+    if (more) places(sub + 1);
+    cp_async_wait<1>();
+    __syncthreads();
+    // ---- scores: even and odd columns summed apart
+    uint64_t acc[MR][4];
+#pragma unroll
+    for (int i = 0; i < MR; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = f2(0.f, 0.f);
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+      ulonglong2 k[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k[e] = *reinterpret_cast<const ulonglong2*>(sk + (tc + 16 * e) * C::KS + d);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sq + (tr + 16 * i) * C::KS + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = fma_f2(q.y, k[e].y, fma_f2(q.x, k[e].x, acc[i][e]));
+      }
+    }
+    bool there[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) there[e] = s_at[(sub & 1) * C::TS + tc + 16 * e] >= 0;
+    __syncthreads();
+    fetch(p.c.k, sk, C::KS, sub + 1, more);
+    // ---- softmax
+#pragma unroll
+    for (int i = 0; i < MR; ++i) {
+      float x[4], mx = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float a, c;
+        f2_split(acc[i][e], a, c);
+        x[e] = there[e] && sub * C::TS + tc + 16 * e < lim[i] ? (a + c) * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, x[e]);
+      }
+#pragma unroll
+      for (int d = 8; d; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn, f = ex2(m[i] - base);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = ex2(x[e] - base);
+        sum += x[e];
+        sp[(tr + 16 * i) * C::PS + tc + 16 * e] = x[e];
+      }
+#pragma unroll
+      for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      l[i] = fmaf(l[i], f, sum);
+      m[i] = mn;
+      if (f != 1.f) {
+        const uint64_t ff = f2(f, f);
+#pragma unroll
+        for (int c = 0; c < 2 * DC; ++c) o[i][c] = mul_f2(o[i][c], ff);
+      }
+    }
+    cp_async_wait<1>();
+    __syncthreads();
+    // ---- O += P V; slots that a row does not see are left out of its sum, where V may hold anything
+    const bool cut = (sub + 1) * C::TS > first_lim;
+#pragma unroll 2
+    for (int j = 0; j < C::TS; j += 4) {
+      ulonglong2 v[4][DC];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) v[e][c] = *reinterpret_cast<const ulonglong2*>(sv + (j + e) * D + c * 64 + tc * 4);
+#pragma unroll
+      for (int i = 0; i < MR; ++i) {
+        const float4 pr = *reinterpret_cast<const float4*>(sp + (tr + 16 * i) * C::PS + j);
+        const float pv[4] = {pr.x, pr.y, pr.z, pr.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (cut && sub * C::TS + j + e >= lim[i]) continue;
+          const uint64_t pp = f2(pv[e], pv[e]);
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            o[i][2 * c] = fma_f2(pp, v[e][c].x, o[i][2 * c]);
+            o[i][2 * c + 1] = fma_f2(pp, v[e][c].y, o[i][2 * c + 1]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    fetch(p.c.v, sv, D, sub + 1, more);
+  }
+  cp_async_wait<0>();
+  const bool part = !it.whole();
+#pragma unroll
+  for (int i = 0; i < MR; ++i) {
+    const int r = tr + 16 * i;
+    int tok, hq;
+    if (!row_of(r, tok, hq)) continue;
+    const long long row = s.first + tok;
+    if (part) {
+      const long long slot = (2ll * blockIdx.x + (it.jb > 0 ? 0 : 1)) * 2 + (r >> 6);
+      if (tc == 0) {
+        p.part_ml[slot * 128 + (r & 63)] = make_float2(m[i], l[i]);
+        if (!it.pair(p)) p.part_ml[(slot + 1) * 128 + (r & 63)] = make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        float4 v;
+        f2_split(o[i][2 * c], v.x, v.y);
+        f2_split(o[i][2 * c + 1], v.z, v.w);
+        p.part[slot * (D / 4) * 128 + (c * 16 + tc) * 128 + (r & 63)] = v;
+      }
+    } else {
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      float* out = static_cast<float*>(p.out) + row * p.out_stride + static_cast<long long>(hq) * D;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) {
+        float4 v;
+        f2_split(o[i][2 * c], v.x, v.y);
+        f2_split(o[i][2 * c + 1], v.z, v.w);
+        v = l[i] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        *reinterpret_cast<float4*>(out + c * 64 + tc * 4) = v;
+      }
+      if (tc == 0 && p.lse) p.lse[row * p.Hq + hq] = (m[i] + lg2(l[i])) * 0.6931471805599453f;
+    }
+  }
 }
 
-// One query row of one head by a warp, slot by slot.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) chunk_simple_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr int E = D / 32;
-  const int lane = lane_id(), row = blockIdx.x;
-  const tkb_kv_cache& c = p.c;
+template <int D>
+__global__ void __launch_bounds__(256, 1) chunk_f32_kernel(const __grid_constant__ ChunkParams p) {
+  using C = ChunkF32<D>;
+  extern __shared__ __align__(128) uint8_t s_ring[];
   grid_wait();
-  int b = row, first = row, n = 1;
-  if (p.row_start) {
-    int lo = 0, hi = c.B;  // last b with row_start[b] <= row
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (p.row_start[mid] <= row) lo = mid;
-      else hi = mid - 1;
+  grid_go();
+  ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(s_ring + C::OFF_WALK + warp_id() * static_cast<int>(sizeof(ChunkWalk)));
+  int flags = 0, span_b = 0, span_hg = 0, span_u = 0;
+  if (chunk_deal<256>(p, walk)) {
+    walk.ahead(p);
+    while (walk.next()) {
+      const ChunkItem& it = walk.item();
+      // rows that the unit's tokens take up, the second tile's behind 64
+      const int rows = it.pair(p) ? 64 + (it.tokens - p.tt) * p.gb : it.tokens * p.gb;
+      if (rows <= 16) chunk_f32_item<D, 1>(p, it, s_ring);
+      else if (rows <= 64) chunk_f32_item<D, 4>(p, it, s_ring);
+      else chunk_f32_item<D, 8>(p, it, s_ring);
+      if (!it.whole()) {
+        const bool begins = it.jb == 0;
+        flags |= begins ? SPAN_BEGINS : SPAN_GOES_ON | (it.je == it.nb1 ? SPAN_ENDS : 0);
+        if (begins) {
+          span_b = it.b;
+          span_hg = it.hg;
+          span_u = it.u;
+        }
+      }
+      walk.ahead(p);
     }
-    b = lo;
-    if (b >= c.B) return;
-    chunk_rows(p.row_start, p.rows, b, first, n);
-    if (row < first || row >= first + n) return;
   }
-  const int held = c.seq_lens[b], most = c.max_pages * c.page_size;
-  int upto = held - n + (row - first) + 1;  // slots this row sees
-  if (upto <= 0 || upto > most) {
-    if (lane == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
-    upto = min(max(upto, 0), most);
-  }
-  for (int hq = warp_id(); hq < p.Hq; hq += 8) {
-    const int h = hq / p.G;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-    lane_values(static_cast<const T*>(p.q) + row * p.q_stride + static_cast<long long>(hq) * D + lane * E, q);
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    int page = -1;
-    for (int j = 0; j < upto; ++j) {
-      const int in = j % c.page_size;
-      if (in == 0) page = page_of(c, b, j / c.page_size);
-      if (page < 0) continue;
-      const long long at = page_offset(c, page, h) + static_cast<long long>(in) * D + lane * E;
-      float k[E], v[E], s = 0.f;
-      lane_values(static_cast<const T*>(c.k) + at, k);
-      lane_values(static_cast<const T*>(c.v) + at, v);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
-      s = warp_sum(s) * p.scale_log2;
-      const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2(m - base), w = ex2(s - base);
-      l = l * f + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e] * f);
-      m = mn;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* out = static_cast<T*>(p.out) + row * p.out_stride + static_cast<long long>(hq) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = static_cast<T>(o[e] * inv);
-    if (p.lse && lane == 0) p.lse[static_cast<long long>(row) * p.Hq + hq] = (m + lg2(l)) * 0.6931471805599453f;
-  }
+  if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(flags, span_b, span_hg, span_u);
 }
 
 template <int D, typename T>
@@ -1172,31 +1353,37 @@ static ChunkWs chunk_ws(const tkb_kv_cache& c) {
   return w;
 }
 
-// Launches, and how many kernels they were.
+template <int D>
+static cudaError_t chunk_f32(const ChunkParams& p, cudaStream_t st) {
+  cudaError_t e = allow_smem<chunk_f32_kernel<D>>(ChunkF32<D>::SMEM);
+  if (e == cudaSuccess) e = launch_early(chunk_f32_kernel<D>, dim3(kChunkGrid), 256, ChunkF32<D>::SMEM, st, p);
+  if (e == cudaSuccess) e = launch_early(chunk_join_kernel<D, float>, dim3(kChunkGrid, 2 * D / 32), 128, 0, st, p);
+  return e;
+}
+
+// Two launches.
 template <typename T>
-static cudaError_t paged_chunk_t(ChunkParams& p, void* workspace, cudaStream_t st, unsigned& kernels) {
+static cudaError_t paged_chunk_t(ChunkParams& p, void* workspace, cudaStream_t st) {
+  constexpr int tile = sizeof(T) == 4 ? 64 : 128;  // packed rows of a tile
   const int D = p.c.D;
+  const ChunkWs w = chunk_ws(p.c);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part = reinterpret_cast<float4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+  p.span = reinterpret_cast<int4*>(ws + w.span);
+  p.hb = (p.G + tile - 1) / tile;
+  p.gb = (p.G + p.hb - 1) / p.hb;
+  p.tt = tile / p.gb;
   if constexpr (sizeof(T) == 4) {
-    kernels = 1;
-    return D == 64 ? launch_early(chunk_simple_kernel<T, 64>, dim3(p.rows), 256, 0, st, p)
-                   : launch_early(chunk_simple_kernel<T, 128>, dim3(p.rows), 256, 0, st, p);
+    return D == 64 ? chunk_f32<64>(p, st) : chunk_f32<128>(p, st);
   } else {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    const ChunkWs w = chunk_ws(p.c);
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    p.part = reinterpret_cast<float4*>(ws);
-    p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
-    p.span = reinterpret_cast<int4*>(ws + w.span);
-    p.hb = (p.G + 127) / 128;
-    p.gb = (p.G + p.hb - 1) / p.hb;
-    p.tt = 128 / p.gb;
     p.gran = kChunkBlock;
     while (p.c.page_size % p.gran) p.gran /= 2;
     cudaError_t e = chunk_tmap(&p.tmQ, p.q, BF16, {D, p.Hq, p.rows}, {D, p.q_stride}, p.gb, p.tt);
     const long long heads = static_cast<long long>(p.c.Hkv) * p.c.page_size;
     if (e == cudaSuccess) e = chunk_tmap(&p.tmK, p.c.k, BF16, {D, heads, p.c.n_pages}, {D, p.c.page_stride}, p.gran, 1);
     if (e == cudaSuccess) e = chunk_tmap(&p.tmV, p.c.v, BF16, {D, heads, p.c.n_pages}, {D, p.c.page_stride}, p.gran, 1);
-    kernels = 2;
     if (e != cudaSuccess) return e;
     return D == 64 ? chunk_tc<64, T>(p, st) : chunk_tc<128, T>(p, st);
   }

@@ -43,7 +43,7 @@ struct LoraPlanParams {
   int32_t* row_of;
   int B, rows, n_adapters, tm, sorted;  // sorted: power of two >= B
 };
-constexpr int kLoraPlanRows = 8192;     // entries of row_of per CTA
+constexpr int kLoraPlanRows = 1024;     // entries of row_of per CTA: its sort is done again by each
 
 // Every CTA sorts the sequences by adapter in shared memory, up to 256 of them
 // by counting the smaller ones of each, more by a bitonic network; the sums over the
@@ -237,7 +237,7 @@ TKB_DEVFN void lora_meet(const float* mine, float* out, int values, int ctas) {
 // warp a quarter of every chunk of K instead.
 template <typename T, int RP, int TM>
 struct LoraDown {
-  static constexpr int KC = 64, ST = 4;                  // columns of K per chunk, chunks in flight
+  static constexpr int KC = 64, ST = 3;                  // columns of K per chunk, chunks in flight
   static constexpr int XB = TM * KC * 2, AB = KC * RP * 2, STAGE = XB + AB;
   static constexpr int SUM = (TM == 16 ? 5 : 4) * 16 * RP * 4;  // the warps' quarters and their sum, or the tile
   static constexpr int SMEM = ST * STAGE > SUM ? ST * STAGE : SUM;
@@ -623,9 +623,23 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_
 // ------------------------------------------------------------ launches
 static int lora_rank(int R) { return R <= 16 ? 16 : R <= 64 ? 64 : 128; }
 
+// CTAs that run at the same time, by their shared memory.
+constexpr int lora_resident(int smem) { return 148 * (232448 / (smem + 1280) < 12 ? 232448 / (smem + 1280) : 12); }
+
 template <typename T, int RP, int TM>
-static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) {
-  const int cols = (p.N + 63) / 64, per = (cols + p.chunks - 1) / p.chunks;
+static cudaError_t lora_launch(LoraParams& p, int tiles, cudaStream_t st) {
+  // Parts of K: as many CTAs as run at the same time (a few more would be a second wave of their own), each of at
+  // least 256 columns, a cluster of eight at most.  12.4 k rows of 2048 and 5632 columns, R = 16: 19 and 45 us in 1.1 waves.
+  constexpr int down = lora_resident(LoraDown<T, RP, TM>::SMEM);
+  p.splits = 1;
+  while (p.splits < 8 && tiles * 2ll * p.splits <= down && p.K >= 512 * p.splits) p.splits *= 2;
+  p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
+  // columns of out per CTA: up to 512, while there are three waves of CTAs; of tiles of 16 rows, whose start weighs more
+  // than their work, eight CTAs an SM (64 rows, 11264 columns: 6.1 us; 7.6 with 64 columns a CTA)
+  const int cols = (p.N + 63) / 64;
+  const long long fit = static_cast<long long>(tiles) * cols / (TM == 16 ? 148 * 8 : 3 * lora_resident(LoraUp<T, RP, TM>::SMEM));
+  p.chunks = fit < 1 ? 1 : fit > 8 ? 8 : static_cast<int>(fit);
+  const int per = (cols + p.chunks - 1) / p.chunks;
   cudaError_t e;
   if constexpr (sizeof(T) == 4) {
     e = allow_smem<lora_down_f32_kernel<RP, TM>>(LoraDown<T, RP, TM>::SMEM);
@@ -644,13 +658,6 @@ static cudaError_t lora_launch(const LoraParams& p, int tiles, cudaStream_t st) 
 template <typename T>
 static cudaError_t lora_add_t(LoraParams& p, const LoraPlanAt& plan, cudaStream_t st) {
   const int tiles = plan.tiles, rank = lora_rank(p.R);
-  // parts of K: CTAs to fill the GPU four times, each of at least 256 columns, a cluster of eight at most
-  p.splits = 1;
-  while (p.splits < 8 && static_cast<long long>(tiles) * p.splits < 148 * 4 && p.K >= 512 * p.splits) p.splits *= 2;
-  p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
-  // columns of out per CTA: up to 512, while there are CTAs to fill the GPU eight times
-  p.chunks = static_cast<int>(static_cast<long long>(tiles) * ((p.N + 63) / 64) / (148 * 8));
-  p.chunks = p.chunks < 1 ? 1 : p.chunks > 8 ? 8 : p.chunks;
 #define LAUNCH(RP) return plan.tm == 64 ? lora_launch<T, RP, 64>(p, tiles, st) : lora_launch<T, RP, 16>(p, tiles, st)
   if (rank == 16) LAUNCH(16);
   if (rank == 64) LAUNCH(64);
