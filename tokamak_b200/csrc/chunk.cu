@@ -28,6 +28,16 @@ namespace tkb {
 // one have started; its grid_wait() still waits for this one's end.
 TKB_DEVFN void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// What the deal reckons with: a block of a unit of two tiles, of one, of one of
+// at most 16 rows; a unit on top (its queries' load, its rows' output); and a
+// CTA's run at least, unless it has a unit of its own (shorter parts cost more
+// to join than they save).  In 16 bits a block of one tile is a warpgroup's, of
+// two both's; in fp32 the rows' products are what takes time.
+struct ChunkCost {
+  int pair, one, few, unit, least;
+};
+constexpr ChunkCost kCost16 = {2, 1, 1, 4, 12}, kCost32 = {8, 4, 1, 2, 8};
+
 struct alignas(64) ChunkParams {
   CUtensorMap tmQ, tmK, tmV;  // 16-bit types
   tkb_kv_cache c;
@@ -40,6 +50,7 @@ struct alignas(64) ChunkParams {
   int gb, hb;          // query heads per tile, blocks of them per kv head (G <= hb * gb)
   int tt;              // tokens per tile: 128 / gb, of fp32 64 / gb
   int gran;            // slots per TMA box: what divides both a page and a block of 128
+  ChunkCost cost;
   float scale_log2;
   float4* part;        // [2 * grid][2 tiles][D / 4][128 rows] unnormalised parts
   float2* part_ml;     // [2 * grid][2][128] their maxima (in powers of 2) and sums
@@ -66,10 +77,6 @@ TKB_DEVFN void chunk_rows(const int32_t* row_start, int rows, int b, int& first,
 // ============================================================ the deal
 constexpr int kChunkGrid = 148;   // one CTA per SM
 constexpr int kChunkBlock = 128;  // slots per block
-// What a block costs beside a block of a single tile: with two tiles twice the
-// products; and what a unit costs on top (its queries' load, its rows' output).
-constexpr int kCostPair = 2, kCostUnit = 4;
-constexpr int kCostLeast = 12;    // a CTA's run at least, unless it has a unit of its own: shorter parts cost more to join than they save
 
 // A sequence: its rows, how many slots its first row sees less one (may be
 // negative), what it holds, and its units.
@@ -82,7 +89,8 @@ TKB_DEVFN int chunk_blocks(int base, int upto) {  // blocks for a row that sees 
 }
 // Cost of the first u (full) units: the sum over v < u of floor((per v + c) / 128), from the sum of the dividends and that
 // of their remainders, which repeat after 128 / gcd(per, 128) terms, taking each value of their class mod the gcd once.
-__noinline__ __device__ long long chunk_cost_before(int per, int base, int u) {
+__noinline__ __device__ long long chunk_cost_before(const ChunkParams& p, int base, int u) {
+  const int per = 2 * p.tt;
   const int c = max(base, 0) + per - 1, g = min(per & -per, kChunkBlock), period = kChunkBlock / g;
   const int turns = u / period;
   int rest = 0;
@@ -91,11 +99,14 @@ __noinline__ __device__ long long chunk_cost_before(int per, int base, int u) {
   for (int v = turns * period; v < u; ++v) rest += (per * v + c) & (kChunkBlock - 1);
   rests += rest;
   const long long n = u, sum = (per * (n * (n - 1) / 2) + n * c - rests) / kChunkBlock;
-  return n * (kCostUnit + kCostPair) + kCostPair * sum;
+  return n * (p.cost.unit + p.cost.pair) + p.cost.pair * sum;
+}
+TKB_DEVFN int chunk_block_cost(const ChunkParams& p, int tokens) {
+  return tokens > p.tt ? p.cost.pair : tokens * p.gb > 16 ? p.cost.one : p.cost.few;
 }
 TKB_DEVFN int chunk_cost(const ChunkParams& p, const ChunkSeq& s, int u) {
   const int t0 = u * 2 * p.tt, tokens = min(2 * p.tt, s.n - t0);
-  return kCostUnit + (tokens > p.tt ? kCostPair : 1) * chunk_blocks(s.base, t0 + tokens);
+  return p.cost.unit + chunk_block_cost(p, tokens) * chunk_blocks(s.base, t0 + tokens);
 }
 TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   ChunkSeq s;
@@ -111,7 +122,7 @@ TKB_DEVFN ChunkSeq chunk_seq(const ChunkParams& p, int b) {
   return s;
 }
 TKB_DEVFN long long chunk_seq_cost(const ChunkParams& p, const ChunkSeq& s) {  // of one head group
-  return s.n ? chunk_cost_before(2 * p.tt, s.base, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
+  return s.n ? chunk_cost_before(p, s.base, s.units - 1) + chunk_cost(p, s, s.units - 1) : 0;
 }
 
 // One unit's share of a CTA's run.
@@ -156,15 +167,14 @@ struct ChunkWalk {
       n.u = u_;
       n.t0 = u_ * 2 * p.tt;
       n.tokens = min(2 * p.tt, s.n - n.t0);
-      const bool two = n.tokens > p.tt;
+      const int each = chunk_block_cost(p, n.tokens);
       n.nb0 = chunk_blocks(s.base, n.t0 + min(n.tokens, p.tt));
       n.nb1 = chunk_blocks(s.base, n.t0 + n.tokens);
-      const int cost = kCostUnit + (two ? kCostPair : 1) * n.nb1;
+      const int cost = p.cost.unit + each * n.nb1;
       auto block_at = [&](long long x) {  // first block that starts at cost x of the unit or later
-        if (x <= kCostUnit) return 0;
+        if (x <= p.cost.unit) return 0;
         if (x >= cost) return n.nb1;
-        const int y = static_cast<int>(x) - kCostUnit;
-        return two ? (y + kCostPair - 1) / kCostPair : y;
+        return (static_cast<int>(x) - p.cost.unit + each - 1) / each;
       };
       n.jb = block_at(x0_ - at_);
       n.je = block_at(x1_ - at_);
@@ -237,8 +247,8 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
     units += s_units[i];
   }
   int ctas = gridDim.x;
-  if (total < static_cast<long long>(ctas) * kCostLeast)
-    ctas = min(ctas, max(units, (static_cast<int>(total) + kCostLeast - 1) / kCostLeast));
+  if (total < static_cast<long long>(ctas) * p.cost.least)
+    ctas = min(ctas, max(units, (static_cast<int>(total) + p.cost.least - 1) / p.cost.least));
   const int c = blockIdx.x;
   if (c >= ctas) return false;
   // total * c / ctas
@@ -261,13 +271,13 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
 #pragma unroll 1
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
-          if (upto + chunk_cost_before(2 * p.tt, s.base, mid) <= x0) lo = mid;
+          if (upto + chunk_cost_before(p, s.base, mid) <= x0) lo = mid;
           else hi = mid - 1;
         }
         s_at[0] = b;
         s_at[1] = hg;
         s_at[2] = lo;
-        s_x = upto + chunk_cost_before(2 * p.tt, s.base, lo);
+        s_x = upto + chunk_cost_before(p, s.base, lo);
         s_seq = s;
         break;
       }
@@ -1374,6 +1384,7 @@ static cudaError_t paged_chunk_t(ChunkParams& p, void* workspace, cudaStream_t s
   p.hb = (p.G + tile - 1) / tile;
   p.gb = (p.G + p.hb - 1) / p.hb;
   p.tt = tile / p.gb;
+  p.cost = sizeof(T) == 4 ? kCost32 : kCost16;
   if constexpr (sizeof(T) == 4) {
     return D == 64 ? chunk_f32<64>(p, st) : chunk_f32<128>(p, st);
   } else {
