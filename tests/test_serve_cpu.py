@@ -162,3 +162,52 @@ def test_oracle_of_the_pages_keeps_every_page_once():
         used = [int(p) for b in range(6) for p in table[b, :held[b]]]
         assert sorted(used + stack) == list(range(17)) and (table[np.arange(5) >= held[:, None]] == -1).all()
         assert all(bool(g) == (h * 16 >= n) for g, h, n in zip(granted, held, lens))
+
+
+def small(**more):
+    from tests.test_generate_cpu import small_generator
+    return small_generator(**more)
+
+
+def test_generator_refusals():
+    from tokamak_b200 import TkbError
+    for bad in (dict(chunk=-1), dict(pool=-1)):
+        with pytest.raises(TkbError):
+            small(**bad)
+    cfg, gen = small()
+    for pieces in ([[1]], [[], []], [[1], [2], [3]]):
+        with pytest.raises(TkbError, match="extend"):
+            gen.extend(pieces)
+    with pytest.raises(TkbError, match="max_tokens"):
+        gen.extend([[1] * 65, []])
+    with pytest.raises(TkbError, match="token ids"):
+        gen.extend([[], [cfg["vocab"]]])
+    for bad in ([2], [-1]):
+        with pytest.raises(TkbError, match="release"):
+            gen.release(bad)
+    _, gen = small(pool=1, page_size=16)
+    for call in (lambda: gen.prefill([[1] * 9, [2]]), lambda: gen.extend([[1], [2]]), lambda: gen.generate([[1], [2]], 4)):
+        with pytest.raises(TkbError, match="2 pages are needed, the pool has 1"):
+            call()
+
+
+def test_adapter_refusals(tmp_path):
+    from tokamak_b200 import TkbError, configs, generate
+    cfg = dict(configs.C1, layers=1)
+    z = lambda *s: np.zeros(s, np.float32)  # noqa: E731
+    good = (z(3, 256, 8), z(3, 8, 256))
+    assert generate.Adapters(cfg, [dict(wo=good)], scale=z(3)).rank == 8
+    for layers in ([], [{}], [dict(wo=good)] * 2, [dict(wq=good)], [dict(wo=(good[0], z(3, 16, 256)))],
+                   [dict(wo=(z(3, 128, 8), good[1]))], [dict(wo=good, wd=(z(2, 688, 8), z(2, 8, 256)))],
+                   [dict(wo=(z(256, 8), good[1]))]):
+        with pytest.raises(TkbError):
+            generate.Adapters(cfg, layers)
+    with pytest.raises(TkbError):
+        generate.Adapters(cfg, [dict(wo=good)], scale=z(2))
+    path = tmp_path / "a.npz"
+    np.savez(path, **{"0.wo.A": good[0], "0.wo.B": good[1]})
+    assert generate.Adapters.load(cfg, path).n == 3
+    for arrays in ({"0.wo.A": good[0]}, {"1.wo.A": good[0], "1.wo.B": good[1]}, {"wo.A": good[0]}, {}):
+        np.savez(path, **arrays)
+        with pytest.raises(TkbError):
+            generate.Adapters.load(cfg, path)
