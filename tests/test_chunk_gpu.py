@@ -138,6 +138,25 @@ def test_large_scores(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_many_small_weights_beside_a_large_one(dtype):
+    """One key of weight 1 and 12000 of weight 2^-26, together 2^-12.4 of it: less than f16 can hold one by one, but not less
+    than its step.  V is 1 for the small ones and 0 for the large one, so the output is their sum alone."""
+    n, D = 12001, 64
+    c = Cache(dtype, [n], 1, D, 64).fill([n])
+    t, j = c.table[0].long(), torch.arange(n, device="cuda")
+    c.k[t[j // 64], 0, j % 64] = 0.0
+    c.v[t[j // 64], 0, j % 64] = 1.0
+    c.k[t[5 // 64], 0, 5, 0] = 144.25   # scaled: 18.03, e^-18.03 = 2^-26.01
+    c.v[t[5 // 64], 0, 5] = 0.0
+    q = torch.zeros(3, D, dtype=dtype, device="cuda")
+    q[:, 0] = 1.0
+    out, _ = ops().paged_attn_chunk(c.handle, q, 1, row_start=on_gpu([0, 3]))
+    big = float(c.k[t[0], 0, 5, 0].double()) / 8
+    small = np.arange(n - 3, n) * np.exp(-big)
+    assert rel_l2(num(out), np.repeat((small / (1 + small))[:, None], D, 1)) < 2 * ATTN[dtype]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 def test_values_out_of_sight_do_not_matter(dtype, D, bad):

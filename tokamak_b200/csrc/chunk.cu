@@ -225,7 +225,7 @@ TKB_DEVFN bool chunk_deal(const ChunkParams& p, ChunkWalk& w) {
     s = chunk_seq(p, b);
     cost = chunk_seq_cost(p, s);
     mine += cost * groups;
-    units = min(units + min(s.units, 0xFFFF) * groups, 0xFFFF);
+    units = static_cast<int>(min(units + static_cast<long long>(s.units) * groups, 0xFFFFll));
   }
   long long upto = mine;
 #pragma unroll
@@ -388,7 +388,10 @@ TKB_DEVFN void chunk_softmax(uint32_t tS, uint32_t tO, float sl2, bool first, bo
   }
   mx0 = fmax3(mx0, sv[124], sv[125]);
   mx1 = fmax3(mx1, sv[126], sv[127]);
-  const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;
+  // m is kept UP below the maximum, so that f16 weights, at most 2^(8 + UP), lie as far as they can above the type's
+  // smallest value, 2^-24: what is rounded to 0 is below 2^-31 of the largest
+  constexpr float UP = BF16 ? 0.f : 7.f;
+  const float mx = fmaf(fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)), sl2, -UP);
   float resc = 1.f;
   bool raised = false;
   if (first) {
