@@ -169,9 +169,11 @@ int tkb_lora_add(const void* plan, const void* x, long long x_stride, const void
   p.N = N;
   p.R = R;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CALL(T) lora_add_t<T>(p, at, st)
-  return cuda_status(TKB_BY_DTYPE(dtype, CALL), who, 2);
+  unsigned kernels = 0;
+#define CALL(T) lora_add_t<T>(p, at, st, kernels)
+  const cudaError_t status = TKB_BY_DTYPE(dtype, CALL);
 #undef CALL
+  return cuda_status(status, who, kernels);
 }
 
 }  // extern "C"

@@ -5,11 +5,13 @@
 // once, the adapters stay in L2), the chain of launches for single tokens.  The
 // plan sorts the rows by adapter and cuts them into tiles of one adapter each
 // (16 rows, or 64 where the adapters have that many), so that an adapter is
-// read once a tile and its products run on m16n8k16 instructions.  Two
-// kernels: t = x A in fp32, cut over K into the CTAs of a cluster, which sum
+// read once a tile and its products run on m16n8k16 instructions.  Tiles of 64
+// rows, and fp32, take two kernels: t = x A in fp32, cut over K into the CTAs of a cluster, which sum
 // their parts in order through their shared memories; then out, cut over the
 // columns.  t goes into the second product as two 16-bit values, the rounding
-// and the rest, so that only out is rounded.
+// and the rest, so that only out is rounded.  Tiles of 16 rows, where launches
+// and first loads are what takes time, take one: the cluster that has summed t
+// goes on with the columns of out.
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
@@ -233,8 +235,8 @@ TKB_DEVFN void lora_meet(const float* mine, float* out, int values, int ctas) {
   if (ctas > 1) cluster_sync();  // the others have read this CTA's part
 }
 
-// t = x A over one part of K.  A warp holds 16 rows; tiles of 16 rows give each
-// warp a quarter of every chunk of K instead.
+// t = x A over one part of K.  A warp holds 16 rows (of tiles of 16 rows, in
+// lora_one_kernel, each has a quarter of every chunk of K instead).
 template <typename T, int RP, int TM>
 struct LoraDown {
   static constexpr int KC = 64, ST = 3;                  // columns of K per chunk, chunks in flight
@@ -242,8 +244,9 @@ struct LoraDown {
   static constexpr int SUM = (TM == 16 ? 5 : 4) * 16 * RP * 4;  // the warps' quarters and their sum, or the tile
   static constexpr int SMEM = ST * STAGE > SUM ? ST * STAGE : SUM;
 };
-template <typename T, int RP, int TM>
+template <typename T, int RP>
 __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int TM = 64;
   using C = LoraDown<T, RP, TM>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(128) uint8_t s_ring[];
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
   for (int c = 0; c < C::ST - 1; ++c) load(c);
-  const int mi = lane >> 3, ri = lane & 7, r0 = TM == 16 ? 0 : w * 16;
+  const int mi = lane >> 3, ri = lane & 7, r0 = w * 16;
   for (int c = 0; c < n; ++c) {
     cp_async_wait<C::ST - 2>();
     __syncthreads();
@@ -289,7 +292,6 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
     const uint32_t xs = smem_u32(s_ring + c % C::ST * C::STAGE), as = xs + C::XB;
 #pragma unroll
     for (int kk = 0; kk < C::KC / 16; ++kk) {
-      if (TM == 16 && kk != w) continue;
       uint32_t a[4];
       ldsm4(xs + lora_swz<128>(r0 + ri + (mi & 1) * 8, kk * 2 + (mi >> 1)), a);
 #pragma unroll
@@ -310,25 +312,91 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
 #pragma unroll
     for (int e = 0; e < 4; e += 2)
       *reinterpret_cast<float2*>(s + (w * 16 + g + (e >> 1) * 8) * RP + j * 8 + c2) = make_float2(acc[j][e], acc[j][e + 1]);
-  if constexpr (TM == 16) {
-    // the warps' quarters of every chunk
-    __syncthreads();
-    for (int i = tid; i < tile.count * RP; i += kLoraThreads)
-      s[64 * RP + i] = (s[i] + s[16 * RP + i]) + (s[32 * RP + i] + s[48 * RP + i]);
-    s += 64 * RP;
-  }
   lora_meet(s, p.t + static_cast<long long>(tile.at) * RP, tile.count * RP, p.splits);
 }
 
-// out = y + t B for one tile and `chunks` times 64 columns.  A warp has 16 rows,
-// or of tiles of 16 rows a quarter of the columns.
+// t of rows g and g + 8 of a warp's 16 as operands of the second product: the 16-bit rounding and the rest.  f16 takes it as
+// multiples `up` of a power of two near the row's largest, so that it fits the type.  at(r, k): t of row r, columns k, k + 1.
+template <bool BF16, int RP, typename At>
+TKB_DEVFN void lora_split(At&& at, float (&up)[2], uint32_t (&hi)[RP / 16][4], uint32_t (&lo)[RP / 16][4]) {
+  const int g = lane_id() >> 2, c2 = (lane_id() & 3) * 2;
+  float t[RP / 16][8], top[2] = {0.f, 0.f}, down[2] = {1.f, 1.f};
+  up[0] = up[1] = 1.f;
+#pragma unroll
+  for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 s = at(g + (i & 1) * 8, k * 16 + (i >> 1) * 8 + c2);
+      t[k][2 * i] = s.x;
+      t[k][2 * i + 1] = s.y;
+      top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(s.x), fabsf(s.y)));
+    }
+  if (!BF16) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+      if (top[i] > 1e-30f && top[i] < 1e30f) {  // else 0, infinite, or next to either
+        const int e = (__float_as_int(top[i]) >> 23) - 127;
+        up[i] = __int_as_float((e + 127) << 23);
+        down[i] = __int_as_float((127 - e) << 23);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = t[k][2 * i] * down[i & 1], b = t[k][2 * i + 1] * down[i & 1];
+      hi[k][i] = pack2<BF16>(a, b);
+      const float2 h = unpack2<BF16>(hi[k][i]);
+      lo[k][i] = pack2<BF16>(a - h.x, b - h.y);
+    }
+}
+// acc = t B for NT8 times 8 columns from piece j0 on of a [RP][64] tile of B.
+template <bool BF16, int RP, int NT8>
+TKB_DEVFN void lora_columns(uint32_t bs, int j0, const uint32_t (&hi)[RP / 16][4], const uint32_t (&lo)[RP / 16][4],
+                            float (&acc)[NT8][4]) {
+  const int mi = lane_id() >> 3, ri = lane_id() & 7;
+#pragma unroll
+  for (int j = 0; j < NT8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < RP / 16; ++k)
+#pragma unroll
+    for (int j = 0; j < NT8; j += 2) {
+      uint32_t b[4];
+      ldsm4_t(bs + lora_swz<128>(k * 16 + ri + (mi & 1) * 8, j0 + j + (mi >> 1)), b);
+      mma16816<BF16>(acc[j], hi[k], b[0], b[1]);
+      mma16816<BF16>(acc[j + 1], hi[k], b[2], b[3]);
+      mma16816<BF16>(acc[j], lo[k], b[0], b[1]);
+      mma16816<BF16>(acc[j + 1], lo[k], b[2], b[3]);
+    }
+}
+// acc added to y where it lies in shared memory, rows r0 .., by the threads that hold the products.
+template <bool BF16, int NT8>
+TKB_DEVFN void lora_onto(uint8_t* ys, int r0, int j0, const float (&up)[2], const float (&acc)[NT8][4]) {
+  const int g = lane_id() >> 2, c2 = (lane_id() & 3) * 2;
+#pragma unroll
+  for (int j = 0; j < NT8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(ys + lora_swz<128>(r0 + g + (e >> 1) * 8, j0 + j) + c2 * 2);
+      const float2 v = unpack2<BF16>(*at);
+      *at = pack2<BF16>(fmaf(acc[j][e], up[e >> 1], v.x), fmaf(acc[j][e + 1], up[e >> 1], v.y));
+    }
+}
+
+// out = y + t B for one tile of 64 rows and `chunks` times 64 columns, 16 rows a warp.
 template <typename T, int RP, int TM>
 struct LoraUp {
   static constexpr int NC = 64, ST = 3;
   static constexpr int YB = TM * NC * 2, BB = RP * NC * 2, STAGE = YB + BB, SMEM = ST * STAGE;
 };
-template <typename T, int RP, int TM>
+template <typename T, int RP>
 __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_constant__ LoraParams p) {
+  constexpr int TM = 64;
   using C = LoraUp<T, RP, TM>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(128) uint8_t s_ring[];
@@ -371,93 +439,193 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_cons
     cp_async_commit();
   };
   for (int c = 0; c < C::ST - 1; ++c) load(c);
-  // t of this thread's rows g and g + 8, times the adapter's scale
-  const int g = lane >> 2, c2 = (lane & 3) * 2, r0 = TM == 16 ? 0 : w * 16;
+  const int r0 = w * 16;
   const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
-  float up[2] = {1.f, 1.f};  // f16: t goes in as multiples of a power of two near the row's largest, so that it fits the type
+  float up[2];
   uint32_t hi[RP / 16][4], lo[RP / 16][4];
-  {
-    float t[RP / 16][8];
-    float top[2] = {0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < RP / 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + g + (i & 1) * 8;
-        float2 s = make_float2(0.f, 0.f);
-        if (r < tile.count)
-          s = *reinterpret_cast<const float2*>(p.t + (static_cast<long long>(tile.at) + r) * RP + k * 16 + (i >> 1) * 8 + c2);
-        t[k][2 * i] = s.x * scale;
-        t[k][2 * i + 1] = s.y * scale;
-        top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(t[k][2 * i]), fabsf(t[k][2 * i + 1])));
-      }
-    float down[2] = {1.f, 1.f};
-    if (!BF16) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        if (top[i] > 1e-30f && top[i] < 1e30f) {  // else 0, infinite, or next to either
-          const int e = (__float_as_int(top[i]) >> 23) - 127;
-          up[i] = __int_as_float((e + 127) << 23);
-          down[i] = __int_as_float((127 - e) << 23);
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < RP / 16; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = t[k][2 * i] * down[i & 1], b = t[k][2 * i + 1] * down[i & 1];
-        hi[k][i] = pack2<BF16>(a, b);
-        const float2 h = unpack2<BF16>(hi[k][i]);
-        lo[k][i] = pack2<BF16>(a - h.x, b - h.y);
-      }
-  }
-  const int mi = lane >> 3, ri = lane & 7;
-  constexpr int NT8 = TM == 16 ? 2 : 8;  // 8-column products of this warp
-  const int j0 = TM == 16 ? w * 2 : 0;
+  lora_split<BF16, RP>([&](int r, int k) {
+    float2 s = make_float2(0.f, 0.f);
+    if (r0 + r < tile.count) s = *reinterpret_cast<const float2*>(p.t + (static_cast<long long>(tile.at) + r0 + r) * RP + k);
+    return make_float2(s.x * scale, s.y * scale);
+  }, up, hi, lo);
   for (int c = 0; c < n; ++c) {
     cp_async_wait<C::ST - 2>();
     __syncthreads();
     load(c + C::ST - 1);
     uint8_t* ys = s_ring + c % C::ST * C::STAGE;
-    const uint32_t bs = smem_u32(ys) + C::YB;
-    float acc[NT8][4];
-#pragma unroll
-    for (int j = 0; j < NT8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-#pragma unroll
-    for (int k = 0; k < RP / 16; ++k)
-#pragma unroll
-      for (int j = 0; j < NT8; j += 2) {
-        uint32_t b[4];
-        ldsm4_t(bs + lora_swz<128>(k * 16 + ri + (mi & 1) * 8, j0 + j + (mi >> 1)), b);
-        mma16816<BF16>(acc[j], hi[k], b[0], b[1]);
-        mma16816<BF16>(acc[j + 1], hi[k], b[2], b[3]);
-        mma16816<BF16>(acc[j], lo[k], b[0], b[1]);
-        mma16816<BF16>(acc[j + 1], lo[k], b[2], b[3]);
-      }
-    // added to y where it lies in shared memory, by the threads that hold the products
-#pragma unroll
-    for (int j = 0; j < NT8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(ys + lora_swz<128>(r0 + g + (e >> 1) * 8, j0 + j) + c2 * 2);
-        const float2 v = unpack2<BF16>(*at);
-        *at = pack2<BF16>(fmaf(acc[j][e], up[e >> 1], v.x), fmaf(acc[j][e + 1], up[e >> 1], v.y));
-      }
+    float acc[8][4];
+    lora_columns<BF16, RP, 8>(smem_u32(ys) + C::YB, 0, hi, lo, acc);
+    lora_onto<BF16, 8>(ys, r0, 0, up, acc);
     __syncwarp();
     const int col = n0 + c * C::NC;
 #pragma unroll
-    for (int i = lane; i < 16 * NT8; i += 32) {
-      const int r = r0 + i / NT8, ch = j0 + i % NT8;
+    for (int i = lane; i < 16 * 8; i += 32) {
+      const int r = r0 + (i >> 3), ch = i & 7;
       if (r < tile.count && col + ch * 8 < p.N)
         *reinterpret_cast<uint4*>(out + s_row[r] * p.out_stride + col + ch * 8) = *reinterpret_cast<const uint4*>(ys + lora_swz<128>(r, ch));
     }
   }
   cp_async_wait<0>();
+}
+
+// ------------------------------------------------------------ tiles of 16 rows in one kernel
+// A cluster per tile: its CTAs take parts of K, sum t through their shared
+// memories, and then parts of the columns, whose first loads have been under
+// way since the start.  A warp walks over columns on its own, 64 at a time.
+template <typename T, int RP>
+struct LoraOne {
+  static constexpr int ST = RP == 16 ? 3 : 2, STAGE = 16 * 128 + RP * 128;  // per warp: y and B
+  static constexpr int DOWN = LoraDown<T, RP, 16>::SMEM, OFF_T = DOWN, OFF_UP = OFF_T + 16 * RP * 4;
+  static constexpr int SMEM = OFF_UP + 4 * ST * STAGE;
+  static_assert(SMEM <= 232448 - 1024, "shared memory");
+};
+template <typename T, int RP>
+__global__ void __launch_bounds__(kLoraThreads) lora_one_kernel(const __grid_constant__ LoraParams p) {
+  using C = LoraOne<T, RP>;
+  using Dn = LoraDown<T, RP, 16>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  __shared__ int s_row[16];
+  grid_wait();
+  grid_go();
+  const int n_tiles = *p.n_tiles;
+  const LoraTile tile = p.tiles[blockIdx.y];  // read beside the number: behind it lies what an earlier plan left
+  if (threadIdx.x < 16) s_row[threadIdx.x] = p.row_of[blockIdx.y * 16 + threadIdx.x];
+  if (static_cast<int>(blockIdx.y) >= n_tiles || (tile.adapter < 0 && p.out == p.y)) return;
+  const int tid = threadIdx.x, lane = lane_id(), w = warp_id(), ctas = p.splits, rank = blockIdx.x;
+  __syncthreads();
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  const int c0 = rank * p.chunks, c1 = min(c0 + p.chunks, (p.N + 63) / 64);  // chunks of 64 columns
+  if (tile.adapter < 0) {  // no adapter: the rows as they are
+    const int n0 = c0 * 64, pieces = max(0, min(c1 * 64, p.N) - n0) / 8;
+    for (int i = tid; i < tile.count * pieces; i += kLoraThreads) {
+      const int r = s_row[i / pieces], col = n0 + i % pieces * 8;
+      *reinterpret_cast<uint4*>(out + r * p.out_stride + col) = *reinterpret_cast<const uint4*>(y + r * p.y_stride + col);
+    }
+    return;
+  }
+  const T* A = static_cast<const T*>(p.a) + static_cast<long long>(tile.adapter) * p.K * p.R;
+  const T* Bm = static_cast<const T*>(p.b) + static_cast<long long>(tile.adapter) * p.R * p.N;
+  uint8_t* mine = s_ring + C::OFF_UP + w * C::ST * C::STAGE;
+  auto load_up = [&](int i) {  // the warp's i-th chunk
+    const int c = c0 + w + 4 * i;
+    if (c < c1) {
+      uint8_t* s = mine + i % C::ST * C::STAGE;
+      for (int e = lane; e < 16 * 8; e += 32) {
+        const int r = e >> 3, ch = e & 7, cc = c * 64 + ch * 8;
+        const bool in = r < tile.count && cc < p.N;
+        cp_async16(smem_u32(s + lora_swz<128>(r, ch)), y + s_row[r] * p.y_stride + (in ? cc : 0), in ? 16 : 0);
+      }
+      for (int e = lane; e < RP * 8; e += 32) {
+        const int r = e >> 3, ch = e & 7, cc = c * 64 + ch * 8;
+        const bool in = r < p.R && cc < p.N;
+        cp_async16(smem_u32(s + 16 * 128 + lora_swz<128>(r, ch)), Bm + (in ? static_cast<long long>(r) * p.N + cc : 0), in ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  const int k0 = rank * p.k_per, k1 = min(p.K, k0 + p.k_per), n = max(0, (k1 - k0 + Dn::KC - 1) / Dn::KC);
+  auto load_down = [&](int c) {
+    if (c < n) {
+      uint8_t* s = s_ring + c % Dn::ST * Dn::STAGE;
+      const int k = k0 + c * Dn::KC, r = tid >> 3, ch = tid & 7, kk = k + ch * 8;
+      const bool in = r < tile.count && kk < k1;
+      cp_async16(smem_u32(s + lora_swz<128>(r, ch)), static_cast<const T*>(p.x) + s_row[r] * p.x_stride + (in ? kk : 0), in ? 16 : 0);
+      for (int i = tid; i < Dn::KC * RP / 8; i += kLoraThreads) {
+        const int ar = i / (RP / 8), ac = i % (RP / 8);
+        const bool there = k + ar < k1 && ac * 8 < p.R;
+        cp_async16(smem_u32(s + Dn::XB + lora_swz<RP * 2>(ar, ac)), A + (there ? static_cast<long long>(k + ar) * p.R + ac * 8 : 0), there ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  };
+  // ---- t: this CTA's part of K, a quarter of every chunk a warp
+  for (int i = 0; i < C::ST - 1; ++i) load_up(i);
+  for (int c = 0; c < Dn::ST - 1; ++c) load_down(c);
+  const int mi = lane >> 3, ri = lane & 7, g = lane >> 2, c2 = (lane & 3) * 2;
+  {
+    float acc[RP / 8][4];
+#pragma unroll
+    for (int i = 0; i < RP / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+    for (int c = 0; c < n; ++c) {
+      cp_async_wait<Dn::ST - 2>();
+      __syncthreads();
+      load_down(c + Dn::ST - 1);
+      const uint32_t xs = smem_u32(s_ring + c % Dn::ST * Dn::STAGE), as = xs + Dn::XB;
+      uint32_t a[4];
+      ldsm4(xs + lora_swz<128>(ri + (mi & 1) * 8, w * 2 + (mi >> 1)), a);
+#pragma unroll
+      for (int j = 0; j < RP / 16; ++j) {
+        uint32_t b[4];
+        ldsm4_t(as + lora_swz<RP * 2>(w * 16 + ri + (mi & 1) * 8, j * 2 + (mi >> 1)), b);
+        mma16816<BF16>(acc[2 * j], a, b[0], b[1]);
+        mma16816<BF16>(acc[2 * j + 1], a, b[2], b[3]);
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    float* s = reinterpret_cast<float*>(s_ring);
+#pragma unroll
+    for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2)
+        *reinterpret_cast<float2*>(s + (w * 16 + g + (e >> 1) * 8) * RP + j * 8 + c2) = make_float2(acc[j][e], acc[j][e + 1]);
+    __syncthreads();
+    for (int i = tid; i < 16 * RP; i += kLoraThreads)
+      s[64 * RP + i] = (s[i] + s[16 * RP + i]) + (s[32 * RP + i] + s[48 * RP + i]);
+    // every CTA sums the cluster's parts for itself, in the order of the ranks
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
+    const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
+    float* st = reinterpret_cast<float*>(s_ring + C::OFF_T);
+    const uint32_t here = smem_u32(s + 64 * RP);
+    for (int i = tid * 4; i < 16 * RP; i += kLoraThreads * 4) {
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < ctas; ++c) {
+        float4 v;
+        if (ctas == 1) v = *reinterpret_cast<const float4*>(s + 64 * RP + i);
+        else
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(mapa_shared(here + i * 4, c)) : "memory");
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      *reinterpret_cast<float4*>(st + i) = make_float4(sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale);
+    }
+    __syncthreads();
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' parts have been read
+  }
+  // ---- out
+  float up[2];
+  uint32_t hi[RP / 16][4], lo[RP / 16][4];
+  const float* st = reinterpret_cast<const float*>(s_ring + C::OFF_T);
+  lora_split<BF16, RP>([&](int r, int k) { return *reinterpret_cast<const float2*>(st + r * RP + k); }, up, hi, lo);
+  for (int i = 0; c0 + w + 4 * i < c1; ++i) {
+    // the chunks asked for at the start are here; from then on the ring's own
+    cp_async_wait<C::ST - 2>();
+    __syncwarp();
+    load_up(i + C::ST - 1);
+    uint8_t* ys = mine + i % C::ST * C::STAGE;
+    float acc[8][4];
+    lora_columns<BF16, RP, 8>(smem_u32(ys) + 16 * 128, 0, hi, lo, acc);
+    lora_onto<BF16, 8>(ys, 0, 0, up, acc);
+    __syncwarp();
+    const int col = (c0 + w + 4 * i) * 64;
+#pragma unroll
+    for (int e = lane; e < 16 * 8; e += 32) {
+      const int r = e >> 3, ch = e & 7;
+      if (r < tile.count && col + ch * 8 < p.N)
+        *reinterpret_cast<uint4*>(out + s_row[r] * p.out_stride + col + ch * 8) = *reinterpret_cast<const uint4*>(ys + lora_swz<128>(r, ch));
+    }
+    __syncwarp();  // before the stage is loaded again
+  }
+  cp_async_wait<0>();
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others have read this CTA's part
 }
 
 // ------------------------------------------------------------ fp32: FMA
@@ -627,38 +795,53 @@ static int lora_rank(int R) { return R <= 16 ? 16 : R <= 64 ? 64 : 128; }
 constexpr int lora_resident(int smem) { return 148 * (232448 / (smem + 1280) < 12 ? 232448 / (smem + 1280) : 12); }
 
 template <typename T, int RP, int TM>
-static cudaError_t lora_launch(LoraParams& p, int tiles, cudaStream_t st) {
-  // Parts of K: as many CTAs as run at the same time (a few more would be a second wave of their own), each of at
-  // least 256 columns, a cluster of eight at most.  12.4 k rows of 2048 and 5632 columns, R = 16: 19 and 45 us in 1.1 waves.
-  constexpr int down = lora_resident(LoraDown<T, RP, TM>::SMEM);
-  p.splits = 1;
-  while (p.splits < 8 && tiles * 2ll * p.splits <= down && p.K >= 512 * p.splits) p.splits *= 2;
-  p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
-  // columns of out per CTA: up to 512, while there are three waves of CTAs; of tiles of 16 rows, whose start weighs more
-  // than their work, eight CTAs an SM (64 rows, 11264 columns: 6.1 us; 7.6 with 64 columns a CTA)
+static cudaError_t lora_launch(LoraParams& p, int tiles, cudaStream_t st, unsigned& kernels) {
   const int cols = (p.N + 63) / 64;
-  const long long fit = static_cast<long long>(tiles) * cols / (TM == 16 ? 148 * 8 : 3 * lora_resident(LoraUp<T, RP, TM>::SMEM));
-  p.chunks = fit < 1 ? 1 : fit > 8 ? 8 : static_cast<int>(fit);
-  const int per = (cols + p.chunks - 1) / p.chunks;
-  cudaError_t e;
-  if constexpr (sizeof(T) == 4) {
-    e = allow_smem<lora_down_f32_kernel<RP, TM>>(LoraDown<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = allow_smem<lora_up_f32_kernel<RP, TM>>(LoraUp<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = launch_early(lora_down_f32_kernel<RP, TM>, dim3(p.splits, tiles), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p, p.splits);
-    if (e == cudaSuccess) e = launch_early(lora_up_f32_kernel<RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
+  p.splits = 1;
+  if constexpr (TM == 16 && sizeof(T) == 2) {
+    // clusters until there are four CTAs an SM, of a chunk of K and of columns each at least
+    while (p.splits < 8 && tiles * 2ll * p.splits <= 148 * 4 && p.K >= 128 * p.splits && cols >= 2 * p.splits) p.splits *= 2;
+    p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
+    p.chunks = (cols + p.splits - 1) / p.splits;
+    kernels = 1;
+    const cudaError_t e = allow_smem<lora_one_kernel<T, RP>>(LoraOne<T, RP>::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_early(lora_one_kernel<T, RP>, dim3(p.splits, tiles), kLoraThreads, LoraOne<T, RP>::SMEM, st, p, p.splits);
   } else {
-    e = allow_smem<lora_down_kernel<T, RP, TM>>(LoraDown<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = allow_smem<lora_up_kernel<T, RP, TM>>(LoraUp<T, RP, TM>::SMEM);
-    if (e == cudaSuccess) e = launch_early(lora_down_kernel<T, RP, TM>, dim3(p.splits, tiles), kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p, p.splits);
-    if (e == cudaSuccess) e = launch_early(lora_up_kernel<T, RP, TM>, dim3(per, tiles), kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
+    // Parts of K: as many CTAs as run at the same time (a few more would be a second wave of their own), each of at
+    // least 256 columns, a cluster of eight at most.  12.4 k rows of 2048 and 5632 columns, R = 16: 19 and 45 us in 1.1
+    // waves, 15 and 35 in less than one.
+    while (p.splits < 8 && tiles * 2ll * p.splits <= lora_resident(LoraDown<T, RP, TM>::SMEM) && p.K >= 512 * p.splits) p.splits *= 2;
+    p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
+    // columns of out per CTA: up to 512, while there are three waves of CTAs
+    const long long fit = static_cast<long long>(tiles) * cols / (3 * lora_resident(LoraUp<T, RP, TM>::SMEM));
+    p.chunks = fit < 1 ? 1 : fit > 8 ? 8 : static_cast<int>(fit);
+    const dim3 down(p.splits, tiles), up((cols + p.chunks - 1) / p.chunks, tiles);
+    void (*first)(LoraParams);
+    void (*second)(LoraParams);
+    cudaError_t e;
+    if constexpr (sizeof(T) == 4) {
+      first = lora_down_f32_kernel<RP, TM>;
+      second = lora_up_f32_kernel<RP, TM>;
+      e = allow_smem<lora_down_f32_kernel<RP, TM>>(LoraDown<T, RP, TM>::SMEM);
+      if (e == cudaSuccess) e = allow_smem<lora_up_f32_kernel<RP, TM>>(LoraUp<T, RP, TM>::SMEM);
+    } else {
+      first = lora_down_kernel<T, RP>;
+      second = lora_up_kernel<T, RP>;
+      e = allow_smem<lora_down_kernel<T, RP>>(LoraDown<T, RP, TM>::SMEM);
+      if (e == cudaSuccess) e = allow_smem<lora_up_kernel<T, RP>>(LoraUp<T, RP, TM>::SMEM);
+    }
+    kernels = 2;
+    if (e == cudaSuccess) e = launch_early(first, down, kLoraThreads, LoraDown<T, RP, TM>::SMEM, st, p, p.splits);
+    if (e == cudaSuccess) e = launch_early(second, up, kLoraThreads, LoraUp<T, RP, TM>::SMEM, st, p);
+    return e;
   }
-  return e;
 }
 
 template <typename T>
-static cudaError_t lora_add_t(LoraParams& p, const LoraPlanAt& plan, cudaStream_t st) {
+static cudaError_t lora_add_t(LoraParams& p, const LoraPlanAt& plan, cudaStream_t st, unsigned& kernels) {
   const int tiles = plan.tiles, rank = lora_rank(p.R);
-#define LAUNCH(RP) return plan.tm == 64 ? lora_launch<T, RP, 64>(p, tiles, st) : lora_launch<T, RP, 16>(p, tiles, st)
+#define LAUNCH(RP) return plan.tm == 64 ? lora_launch<T, RP, 64>(p, tiles, st, kernels) : lora_launch<T, RP, 16>(p, tiles, st, kernels)
   if (rank == 16) LAUNCH(16);
   if (rank == 64) LAUNCH(64);
   LAUNCH(128);
