@@ -495,16 +495,20 @@ def lora_add(plan, x, A, B, y, scale=None, out=None, workspace=None):
     B [n_adapters, R, N], y [rows, N], scale [n_adapters] fp32 or None; y itself where no out is given.  Returns out."""
     out = y if out is None else out
     n, K, R = A.shape
-    N = B.shape[2]
+    N, rows, dtype = B.shape[2], plan.rows, x.dtype
     if n != plan.n_adapters:
         raise TkbError(f"lora_add: {n} adapters, the plan is for {plan.n_adapters}")
-    _expect(A, "A", (n, K, R), x.dtype)
-    _expect(B, "B", (n, R, N), x.dtype)
+    # all at once for the calls that pass; what is wrong is found below
+    if not (A.dtype == dtype and B.dtype == dtype and y.dtype == dtype and out.dtype == dtype and B.shape[:2] == (n, R) and
+            A.is_contiguous() and B.is_contiguous() and x.shape == (rows, K) and y.shape == (rows, N) and
+            out.shape == (rows, N) and x.stride(1) == 1 and y.stride(1) == 1 and out.stride(1) == 1):
+        _expect(A, "A", (n, K, R), dtype)
+        _expect(B, "B", (n, R, N), dtype)
+        for t, name, width in ((x, "x", K), (y, "y", N), (out, "out", N)):
+            if t.shape != (rows, width) or t.dtype != dtype or t.stride(1) != 1:
+                raise TkbError(f"lora_add: {name} is {t.dtype} {tuple(t.shape)}, not {dtype} {(rows, width)} with "
+                               "contiguous columns")
     _vec(scale, "scale", n, torch.float32)
-    for t, name, width in ((x, "x", K), (y, "y", N), (out, "out", N)):
-        if t.shape != (plan.rows, width) or t.dtype != x.dtype or (width > 1 and t.stride(1) != 1):
-            raise TkbError(f"lora_add: {name} is {t.dtype} {tuple(t.shape)}, not {x.dtype} {(plan.rows, width)} with "
-                           "contiguous columns")
     if workspace is None:
         workspace = lora_workspace(plan.rows, R, x.device)
     stream = _launch_stream("lora_add", x, A, B, y, out, scale, plan.buffer, workspace)
