@@ -13,8 +13,8 @@
 // equal runs, whatever the lengths, to one CTA per SM; a unit that spans CTAs
 // leaves unnormalised parts in the workspace, which a second kernel joins in
 // the order of the run.  Inside a CTA the roles are those of the prompt's own
-// attention (attn_fwd.cu): one warp issues TMA, one the tcgen05 products, two
-// warpgroups hold a query row a thread and do the softmax.  A unit of two tiles
+// attention (attn_fwd.cu): a warp each issues the TMA loads of Q and K and of V, one the
+// tcgen05 products, two warpgroups hold a query row a thread and do the softmax.  A unit of two tiles
 // gives each warpgroup one of them; a unit of one gives them its blocks in
 // turn, and their two results meet in shared memory at its end.
 // TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [256+D,256+2D),
@@ -316,6 +316,7 @@ TKB_DEVFN bool chunk_row(const ChunkParams& p, int hg, int t0, int tokens, int w
 }
 
 // ============================================================ 16-bit types: tcgen05
+constexpr int kChunkThreads = 352;  // softmax 0-7, Q and K loads 8, products 9, V loads 10
 template <int D>
 struct ChunkCfg {
   static constexpr int TILE = 128 * D * 2;  // bytes of one 128-row x D tile
@@ -333,7 +334,7 @@ struct ChunkCfg {
   static constexpr int NMASK = 16;                       // page marks of the newest blocks (more than are in flight)
   static constexpr int OFF_MASK = OFF_BAR + NBAR * 8;
   static constexpr int OFF_WALK = (OFF_MASK + NMASK * 4 + 7) / 8 * 8;
-  static constexpr int OFF_MISC = OFF_WALK + 10 * sizeof(ChunkWalk);
+  static constexpr int OFF_MISC = OFF_WALK + kChunkThreads / 32 * sizeof(ChunkWalk);
   static constexpr int SMEM = OFF_MISC + 16 + 1024;      // + slack for 1024-byte alignment
   static_assert(SMEM <= 232448, "tiles exceed 227 KB of shared memory");
   static constexpr uint32_t TM_S0 = 0, TM_S1 = 128, TM_O0 = 256, TM_O1 = 256 + D;
@@ -556,7 +557,7 @@ __noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid_constant__ ChunkParams p) {
   using C = ChunkCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -604,7 +605,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
   grid_wait();
   grid_go();
   ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * static_cast<int>(sizeof(ChunkWalk)));
-  const bool any = chunk_deal<320>(p, walk);
+  const bool any = chunk_deal<kChunkThreads>(p, walk);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -612,14 +613,20 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
 
   if (!any) {
     if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(0, 0, 0, 0);
-  } else if (warp == 8) {
-    // ------------------------------------------------------------ TMA producer
-    // A lane issues one box: `gran` slots of one 64-column slab of K or V.
+  } else if (warp == 8 || warp == 10) {
+    // ------------------------------------------------------------ TMA producers
+    // A lane issues one box: `gran` slots of one 64-column slab of K or V.  Two warps, because boxes of 16 slots are 16 to
+    // 32 of these instructions a block, some 0.1 us each from one warp.
+    const bool keys = warp == 8;
+    uint64_t* full = keys ? k_full : v_full;
+    uint64_t* empty = keys ? k_empty : v_empty;
+    const CUtensorMap* map = keys ? &p.tmK : &p.tmV;
+    uint8_t* ring = smem + (keys ? C::OFF_K : C::OFF_V);
     const int boxes = kChunkBlock / p.gran, nl = boxes * (D / 64);
     const int gi = lane % boxes, hh = lane / boxes;
     const int box_rows = p.gran;
     const uint32_t q_bytes = static_cast<uint32_t>(p.gb) * p.tt * D * 2;
-    int nq = 0, nk = 0, nv = 0;  // loads issued
+    int nq = 0, nb = 0;  // loads issued
     bool ok = true;
     walk.ahead(p);
     while (ok && walk.next()) {
@@ -641,44 +648,40 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       };
       bool bad;
       int page = page_in(jb, bad);
-      if (!(ok = mbar_wait_warp(q_empty, (nq & 1) ^ 1, abort_flag))) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (pair ? 2 : 1) * q_bytes);
-        for (int w = 0; w < (pair ? 2 : 1); ++w)
+      if (keys) {
+        if (!(ok = mbar_wait_warp(q_empty, (nq & 1) ^ 1, abort_flag))) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, (pair ? 2 : 1) * q_bytes);
+          for (int w = 0; w < (pair ? 2 : 1); ++w)
 #pragma unroll
-          for (int x = 0; x < D / 64; ++x)
-            tma_load_3d(smem + C::OFF_Q + w * C::TILE + x * C::SLAB, &p.tmQ, q_full, x * 64, hq0,
-                        s.first + it.t0 + w * p.tt, pol_q);
+            for (int x = 0; x < D / 64; ++x)
+              tma_load_3d(smem + C::OFF_Q + w * C::TILE + x * C::SLAB, &p.tmQ, q_full, x * 64, hq0,
+                          s.first + it.t0 + w * p.tt, pol_q);
+        }
+        ++nq;
       }
-      ++nq;
       walk.ahead(p);
       for (int j = jb; j < je; ++j) {
         bool bad_next = false;
         int next = 0;
         if (j + 1 < je) next = page_in(j + 1, bad_next);
         const int in_head = (j * kChunkBlock + gi * box_rows) % p.c.page_size + h * p.c.page_size;
-        // bits of the 16-slot groups that lie in bad pages
-        const unsigned lost = __reduce_or_sync(0xffffffffu, bad ? ((1u << (box_rows / 16)) - 1) << (gi * box_rows / 16) : 0u);
-        if (lost && lane == 0) atomicOr(&g_device_error, ERR_BAD_INDEX);
-        const int sk = nk % C::NST;
-        if (!(ok = mbar_wait_warp(&k_empty[sk], ((nk / C::NST) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0) {
-          marks[nk % C::NMASK] = ~lost;
-          mbar_arrive_expect_tx(&k_full[sk], C::TILE);
+        const int stage = nb % C::NST;
+        if (!(ok = mbar_wait_warp(&empty[stage], ((nb / C::NST) & 1) ^ 1, abort_flag))) break;
+        if (keys) {
+          // bits of the 16-slot groups that lie in bad pages
+          const unsigned lost = __reduce_or_sync(0xffffffffu, bad ? ((1u << (box_rows / 16)) - 1) << (gi * box_rows / 16) : 0u);
+          if (lane == 0) {
+            if (lost) atomicOr(&g_device_error, ERR_BAD_INDEX);
+            marks[nb % C::NMASK] = ~lost;
+          }
         }
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], C::TILE);
         __syncwarp();
         if (lane < nl)
-          tma_load_3d(smem + C::OFF_K + sk * C::TILE + hh * C::SLAB + gi * box_rows * 128, &p.tmK, &k_full[sk], hh * 64,
-                      in_head, page, pol_kv);
-        ++nk;
-        const int sv = nv % C::NST;
-        if (!(ok = mbar_wait_warp(&v_empty[sv], ((nv / C::NST) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0) mbar_arrive_expect_tx(&v_full[sv], C::TILE);
-        __syncwarp();
-        if (lane < nl)
-          tma_load_3d(smem + C::OFF_V + sv * C::TILE + hh * C::SLAB + gi * box_rows * 128, &p.tmV, &v_full[sv], hh * 64,
-                      in_head, page, pol_kv);
-        ++nv;
+          tma_load_3d(ring + stage * C::TILE + hh * C::SLAB + gi * box_rows * 128, map, &full[stage], hh * 64, in_head, page,
+                      pol_kv);
+        ++nb;
         page = next;
         bad = bad_next;
       }
@@ -687,8 +690,7 @@ __global__ void __launch_bounds__(320, 1) chunk_tc_kernel(const __grid_constant_
       // Let every copy this CTA started land before the CTA exits.
       volatile int never = 0;
       if (nq) mbar_wait(q_full, (nq - 1) & 1, &never);
-      for (int i = max(0, nk - C::NST); i < nk; ++i) mbar_wait(&k_full[i % C::NST], (i / C::NST) & 1, &never);
-      for (int i = max(0, nv - C::NST); i < nv; ++i) mbar_wait(&v_full[i % C::NST], (i / C::NST) & 1, &never);
+      for (int i = max(0, nb - C::NST); i < nb; ++i) mbar_wait(&full[i % C::NST], (i / C::NST) & 1, &never);
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
@@ -1332,7 +1334,7 @@ template <int D, typename T>
 static cudaError_t chunk_tc(const ChunkParams& p, cudaStream_t st) {
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   cudaError_t e = allow_smem<chunk_tc_kernel<D, BF16>>(ChunkCfg<D>::SMEM);
-  if (e == cudaSuccess) e = launch_early(chunk_tc_kernel<D, BF16>, dim3(kChunkGrid), 320, ChunkCfg<D>::SMEM, st, p);
+  if (e == cudaSuccess) e = launch_early(chunk_tc_kernel<D, BF16>, dim3(kChunkGrid), kChunkThreads, ChunkCfg<D>::SMEM, st, p);
   if (e == cudaSuccess) e = launch_early(chunk_join_kernel<D, T>, dim3(kChunkGrid, 2 * D / 32), 128, 0, st, p);
   return e;
 }
