@@ -34,7 +34,9 @@ struct LoraPlanAt {
 static LoraPlanAt lora_plan_at(int B, int rows, int n_adapters) {
   LoraPlanAt a;
   const long long groups = n_adapters < B ? n_adapters + 1ll : B;
-  // Tiles of 64 rows read an adapter a quarter as often; where adapters have fewer rows, most of such a tile is empty.
+  // Tiles of 64 rows read an adapter a quarter as often; where adapters have few rows, most of such a tile is empty.  16 and
+  // 64 rows: 1.6 k rows of 33 adapters of rank 64 73 and 37 us, 12.4 k rows of 8 315 and 204, 548 of 16 (rank 16) 11.4 and
+  // 13.5, 64 of 16 27 and 37.
   a.tm = rows >= 32 * groups ? 64 : 16;
   a.tiles = static_cast<int>(rows / a.tm + (groups < rows ? groups : rows));
   a.rows = 256 + static_cast<size_t>(a.tiles) * sizeof(LoraTile);
