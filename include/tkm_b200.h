@@ -274,7 +274,8 @@ int tkb_lmhead_ce(const void *X, long long ldx, const void *W, long long ldw, co
  * CUDA graph follows the lengths and tables.  A page outside [0, n_pages)
  * or a length above max_pages * page_size sets bit 2 of the device error
  * word: such slots count as not held, such rows are not written.  Sequences
- * may share pages that only tkb_paged_attn_decode without `accumulate` reads. */
+ * may share pages that only tkb_paged_attn_decode without `accumulate` and
+ * tkb_paged_attn_chunk read. */
 typedef struct {
     void *k, *v;
     int32_t *pos;
