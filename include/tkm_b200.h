@@ -312,7 +312,8 @@ int tkb_kv_lens(int32_t *seq_lens, int32_t *seen, const int32_t *row_start, int 
  * columns, or with out_full the whole packed row, as tkb_gqa_attn_fwd and
  * tkb_paged_attn_decode take it.  Rows that have no slot (n_b > seq_lens[b],
  * a slot past max_pages * page_size, a bad page) are not stored and set bit 2
- * of the device error word; their out is written. */
+ * of the device error word; their out is written.  A sequence with seen[b]
+ * below 0 takes no part: its rows are not stored and set no bit. */
 int tkb_kv_append(const tkb_kv_cache *cache, const void *qkv, long long qkv_stride, const float *bias,
                   const float *qk_gain, void *out, long long out_stride, int out_full, const int32_t *row_start,
                   const int32_t *seen, int rows, int Hq, int has_qknorm, int has_rope, float theta,

@@ -683,3 +683,24 @@ def test_decode_infinite_values_stay_infinite(dtype, Hkv, G, D, lens):
     out = out.view(B, Hkv, G, D)
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(), want.nan_to_num())
     assert torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("held", [0, 20])
+def test_append_leaves_out_sequences_that_take_no_part(dtype, held):
+    """seen below 0: nothing stored and no bit set, whatever the sequence holds; the other rows as ever."""
+    c = Cache(dtype, [9, held, 33], 2, 64, 16).fill([9, held, 33])
+    c.table[1] = -1
+    seen = torch.tensor([9, -1, 33], dtype=torch.int32, device="cuda")
+    before = [t.clone() for t in (c.k, c.v, c.pos, c.weight)]
+    rows = c.randn(3, 8 * 64, dtype=dtype)
+    out = ops().kv_append(c.handle, rows, 4, seen=seen, rope=False)
+    assert device_error() == 0 and torch.equal(out, rows[:, :256])
+    for t, part in ((before[0], rows[:, 256:384]), (before[1], rows[:, 384:])):
+        for b, slot in ((0, 8), (2, 32)):
+            t[c.table[b, slot // 16].long(), :, slot % 16] = part[b].view(2, 64)
+    for b, slot in ((0, 8), (2, 32)):
+        before[2][c.table[b, slot // 16].long(), :, slot % 16] = slot
+        before[3][c.table[b, slot // 16].long(), :, slot % 16] = 0
+    for got, want in zip((c.k, c.v, c.pos, c.weight), before):
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())

@@ -191,6 +191,72 @@ def test_generator_refusals():
             call()
 
 
+def test_released_sequences_take_no_part_in_steps(monkeypatch):
+    """Lengths, positions and pages of a batch whose sequences end, wait and start again, the calls restated on the host: a
+    sequence that holds nothing after a release, or after an extend that brought it nothing, gets no token from a step."""
+    torch = pytest.importorskip("torch")
+    from tokamak_b200 import TkbError, generate
+
+    def kv_lens(lens, limit=None, seen=None, add=0, row_start=None):
+        n = torch.full_like(lens, add) if row_start is None else row_start.diff()
+        lens += n
+        seen += n
+
+    def kv_pages(table, held, lens, free, n_free, page):
+        stack = free[:int(n_free)].tolist()
+        t, h, stack, _ = ref.pages(table.numpy(), held.numpy(), lens.tolist(), stack, page)
+        table.copy_(torch.from_numpy(t))
+        held.copy_(torch.from_numpy(h))
+        free[:len(stack)] = torch.tensor(stack, dtype=torch.int32)
+        n_free.fill_(len(stack))
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(generate.ops, "kv_lens", kv_lens)
+    monkeypatch.setattr(generate.ops, "kv_pages", kv_pages)
+    monkeypatch.setattr(generate.ops, "paged_attn_chunk_workspace", lambda *a: None)
+    monkeypatch.setattr(generate.ops, "gemm", lambda x, w, **more: torch.zeros(x.shape[0], w.shape[1]))
+    for pool in (0, 2):
+        cfg, gen = small(pool=pool, page_size=16)
+        gen._forward = lambda x, attend, row_start=None: torch.zeros(x.shape[0], cfg["d_model"])
+        gen.extend([[1] * 5, [2] * 7])
+        assert gen.lens.tolist() == gen.held == [5, 7]
+        gen.release([1])
+        for n in (6, 7, 8):
+            gen.decode()
+            assert gen.lens.tolist() == gen.held == [n, 0] and int(gen.seen[0]) == n
+            assert int(gen.seen[1]) < 0  # the append leaves such a sequence out
+            if pool:
+                assert gen.pages_held.tolist() == [1, 0]
+        gen.release([1])  # once more
+        gen.extend([[], [3, 4]])
+        assert gen.lens.tolist() == gen.seen.tolist() == gen.held == [8, 2]
+        gen.decode()
+        assert gen.lens.tolist() == gen.seen.tolist() == gen.held == [9, 3]
+        # a full pool refuses only steps that need a page
+        gen.release([0])
+        gen.extend([[], [5] * 14])
+        assert gen.held == [0, 17]
+        gen.decode()
+        assert gen.lens.tolist() == gen.held == [0, 18]
+        if pool:
+            with pytest.raises(TkbError, match="3 pages are needed"):
+                gen.extend([[1], []])
+            assert gen.lens.tolist() == gen.held == [0, 18] and int(gen.seen[0]) < 0
+        gen.prefill([[1], [2]])
+        gen.decode()
+        assert gen.lens.tolist() == gen.seen.tolist() == gen.held == [2, 2]
+        # slots that no request has taken yet wait too; without any request, steps start from self.token
+        _, gen = small(pool=pool, page_size=16)
+        gen._forward = lambda x, attend, row_start=None: torch.zeros(x.shape[0], cfg["d_model"])
+        gen.decode()
+        assert gen.lens.tolist() == gen.seen.tolist() == gen.held == [1, 1]
+        _, gen = small(pool=pool, page_size=16)
+        gen._forward = lambda x, attend, row_start=None: torch.zeros(x.shape[0], cfg["d_model"])
+        gen.extend([[], [3] * 4])
+        gen.decode()
+        assert gen.lens.tolist() == gen.held == [0, 5]
+
+
 def test_adapter_refusals(tmp_path):
     from tokamak_b200 import TkbError, configs, generate
     cfg = dict(configs.C1, layers=1)

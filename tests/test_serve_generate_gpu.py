@@ -91,6 +91,55 @@ def test_a_shared_pool_gives_the_same_tokens():
     assert gen.held == [42, 25, 40] and device_error() == 0
 
 
+@pytest.mark.parametrize("pool", [0, 12])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_released_sequence_stays_empty(pool, captured):
+    """A request ends while the others decode; the next one in its place gets the logits of its tokens alone, and the others
+    those of a batch where nobody left."""
+    from tokamak_b200 import generate
+    cfg = make(gqa=True)
+    ckpt, embed, rng = weights(cfg), table(cfg), np.random.default_rng(3)
+    said = [rng.integers(0, cfg["vocab"], n).tolist() for n in (30, 16, 5)]
+    gen = generate.Generator(cfg, ckpt, embed, 3, 128, page_size=16, pool=pool)
+    gen.prefill(said)
+    said[1] = []
+    graph, logits = torch.cuda.CUDAGraph(), None
+    if captured:  # while all three are there
+        gen.token.zero_()
+        gen.decode()
+        said = [s + [0] if s else s for s in said]
+        with torch.cuda.graph(graph):
+            logits = gen.decode()
+    gen.release([1])
+
+    def step(tokens):
+        gen.token.copy_(torch.tensor(tokens))
+        if not captured:
+            return num(gen.decode())
+        graph.replay()
+        gen.held = [n + a for n, a in zip(gen.held, gen.live)]
+        return num(logits)
+
+    def alone(b):
+        return num(generate.Generator(cfg, ckpt, embed, 1, 128, page_size=16).prefill([said[b]]))[0]
+
+    for s in range(20):
+        got = step([s, 100 + s, 50 + s])
+        said = [t + [n] if t else t for t, n in zip(said, (s, 0, 50 + s))]
+        assert gen.lens.tolist() == gen.held == [len(t) for t in said]
+        if pool:
+            assert gen.pages_held.tolist() == [-(-n // 16) for n in gen.held]
+    assert rel_l2(got[0], alone(0)) < LOGITS and rel_l2(got[2], alone(2)) < LOGITS
+    said[1] = rng.integers(0, cfg["vocab"], 21).tolist()
+    got = num(gen.extend([[], said[1], []]))
+    assert rel_l2(got[1], alone(1)) < LOGITS and gen.held == [len(t) for t in said]
+    got = step([7, 8, 9])
+    said = [t + [n] for t, n in zip(said, (7, 8, 9))]
+    for b in range(3):
+        assert rel_l2(got[b], alone(b)) < LOGITS
+    assert gen.lens.tolist() == gen.seen.tolist() == gen.held and device_error() == 0
+
+
 def test_pool_and_budget():
     """Evictions give pages back."""
     from tokamak_b200 import generate

@@ -177,8 +177,10 @@ __global__ void __launch_bounds__(NT) kv_append_kernel(const __grid_constant__ A
     }
     const int held = c.seq_lens[b], slot = held - back;
     int page = -1;
-    if (has && slot >= 0 && slot < c.max_pages * c.page_size) page = page_of(c, b, slot / c.page_size);
-    else atomicOr(&g_device_error, ERR_BAD_INDEX);
+    if (!has || !p.seen || p.seen[b] >= 0) {  // else the sequence takes no part
+      if (has && slot >= 0 && slot < c.max_pages * c.page_size) page = page_of(c, b, slot / c.page_size);
+      else atomicOr(&g_device_error, ERR_BAD_INDEX);
+    }
     const int in_page = slot % c.page_size;
     s_kv[tid] = page < 0 ? -1 : page_offset(c, page, 0) + static_cast<long long>(in_page) * D;
     s_meta[tid] = page < 0 ? -1 : meta_offset(c, page, 0) + in_page;

@@ -162,7 +162,9 @@ class Generator:
             self.low = [{k: tuple(torch.as_tensor(m, dtype=torch.bfloat16, device=device).contiguous() for m in ab)
                          for k, ab in w.items()} for w in adapters.layers]
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)   # tokens held in the cache
-        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)   # tokens so far
+        self.seen = torch.zeros(batch, dtype=torch.int32, device=device)   # tokens so far; -1: takes no part in steps
+        self.live = [True] * batch                                         # takes part in steps
+        self.step_rows = torch.arange(batch + 1, dtype=torch.int32, device=device)  # row starts of a step's new tokens
         self.caches = []
         for _ in self.layers:
             k, v = (torch.zeros(n_pages, Hkv, page_size, D, dtype=torch.bfloat16, device=device) for _ in "kv")
@@ -220,6 +222,17 @@ class Generator:
         if self.pool:
             ops.kv_pages(self.table, self.pages_held, self.lens, self.free_pages, self.n_free, self.page_size)
 
+    def _take_part(self, live):
+        """Which sequences take part in decode steps.  Captured steps follow: they read step_rows and seen.  Those that
+        change hold nothing."""
+        if live == self.live:
+            return
+        for b, (was, now) in enumerate(zip(self.live, live)):
+            if was != now:
+                self.seen[b:b + 1].fill_(0 if now else -1)
+        self.live = live
+        self.step_rows.copy_(torch.from_numpy(np.concatenate(([0], np.cumsum(live))).astype(np.int32)))
+
     def _append(self, i, qkv, **more):
         return ops.kv_append(self.caches[i], qkv, self.Hq, seen=self.seen, bias=self.layers[i]["bqkv"],
                              theta=float(self.cfg["theta"]), **more)
@@ -245,6 +258,7 @@ class Generator:
             raise TkbError("prefill: one prompt of 1 to max_tokens tokens per sequence")
         self._check_tokens("prefill", prompts)
         self._room(n)
+        self._take_part([True] * self.batch)
         self.lens.zero_()
         self.seen.zero_()
         self.held = [0] * self.batch
@@ -324,8 +338,9 @@ class Generator:
     def extend(self, pieces):
         """Conversations go on: new tokens of each sequence (lists of token ids, empty for those that bring none) enter
         behind what it holds, in pieces of at most `chunk` tokens; returns the logits [batch, vocab] after each one's last
-        (0 for sequences without new tokens).  A sequence that holds nothing starts with them.  With a budget, a
-        piece adds the attention of its last `window` tokens to the weights."""
+        (0 for sequences without new tokens).  A sequence that holds nothing starts with them; those that still hold
+        nothing take no part in decode steps until they get some.  With a budget, a piece adds the attention of its last
+        `window` tokens to the weights."""
         n = [len(p) for p in pieces]
         if len(n) != self.batch or max(n) < 1:
             raise TkbError("extend: a list of tokens per sequence, one of them not empty")
@@ -334,6 +349,7 @@ class Generator:
             raise TkbError("extend: more tokens than max_tokens")
         self._check_tokens("extend", pieces)
         self._room(held)
+        self._take_part([h > 0 for h in held])
         step = self.chunk or max(n)
         if step >= max(n):
             return self._enter(pieces)
@@ -346,23 +362,26 @@ class Generator:
         return logits
 
     def release(self, sequences):
-        """These sequences (indices) end: they hold nothing, and their pages go back to the pool.  Each starts again with
-        extend."""
+        """These sequences (indices) end: they hold nothing, their pages go back to the pool, and decode steps leave them out
+        until they start again with extend."""
         which = sorted(set(int(b) for b in sequences))
         if which and (which[0] < 0 or which[-1] >= self.batch):
             raise TkbError(f"release: sequences are 0 to {self.batch - 1}")
         for b in which:
             self.lens[b:b + 1].zero_()
-            self.seen[b:b + 1].zero_()
             self.held[b] = 0
+        self._take_part([a and b not in which for b, a in enumerate(self.live)])
         self._pages()
 
     def decode(self):
-        """One step: the tokens in self.token (rows of embed) enter the caches; returns the next logits [batch, vocab]."""
+        """One step: the tokens in self.token (rows of embed) enter the caches; returns the next logits [batch, vocab].  The
+        rows of sequences that have been released, or have had nothing from extend yet, mean nothing: their tokens enter
+        nowhere."""
         if not torch.cuda.is_current_stream_capturing():  # a captured step's lengths are its replays'
-            self._room([n + 1 for n in self.held])
-            self.held = [n + 1 for n in self.held]
-        ops.kv_lens(self.lens, seen=self.seen, add=1)
+            held = [n + a for n, a in zip(self.held, self.live)]
+            self._room(held)
+            self.held = held
+        ops.kv_lens(self.lens, seen=self.seen, row_start=self.step_rows)
         self._pages()
 
         def attend(i, qkv):
