@@ -333,3 +333,62 @@ def test_many_sequences():
     out, lse = ops().paged_attn_chunk(c.handle, q, 2, row_start=on_gpu(start))
     check(c, q, 2, lens.tolist(), start, out, lse, torch.bfloat16)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_nan_scores_reach_rows_that_span_ctas(dtype, D):
+    """Rows whose slots are dealt out to several CTAs, every score of some of the parts NaN: a query of NaN, and sequences
+    that end in a block of one slot whose key is NaN.  None of them may look like a part that sees nothing."""
+    lens = [3000, 20000]
+    c = Cache(dtype, lens, 1, D, 16).fill(lens)
+    q = c.randn(5, 2 * D, dtype=dtype)
+    q[0, :D] = float("nan")
+    q[4, D + 3] = float("nan")
+    out, lse = ops().paged_attn_chunk(c.handle, q, 2, row_start=on_gpu([0, 2, 5]))
+    lost = np.zeros((5, 2), bool)
+    lost[0, 0] = lost[4, 1] = True
+    assert np.array_equal(np.isnan(num(out).reshape(5, 2, D)), np.repeat(lost[:, :, None], D, 2))
+    assert np.array_equal(np.isnan(num(lse)), lost)
+    lens = [128 * k + 1 for k in range(2, 42)]
+    c = Cache(dtype, lens, 1, D, 16).fill(lens)
+    for b, n in enumerate(lens):
+        c.k[c.table[b, (n - 1) // 16].long(), 0, (n - 1) % 16] = float("nan")
+    q = c.randn(len(lens), D, dtype=dtype)
+    out, lse = ops().paged_attn_chunk(c.handle, q, 1)
+    assert num(out).shape == (40, D) and np.isnan(num(out)).all() and np.isnan(num(lse)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,G,n,rows", [(64, 1, 100000, 20), (128, 1, 100000, 20), (128, 4, 60000, 50), (64, 8, 130000, 9)])
+def test_a_value_out_of_sight_in_a_long_context(dtype, D, G, n, rows):
+    """A value of V that is not finite near the end of long contexts, in a call that gives every CTA several of them and short
+    sequences behind: rows before it as ever, the others lose its column alone, the other sequences nothing, and no
+    wait runs out.  (The sequences share their pages.)"""
+    B, page, few = 320 // G, 64, 64
+    pages = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(pages + few, 1, page, D, generator=g, device="cuda").to(dtype) for _ in "kv")
+    table = torch.full((B + few, pages), -1, dtype=torch.int32, device="cuda")
+    table[:B] = torch.arange(pages, device="cuda")
+    table[B:, 0] = torch.arange(pages, pages + few, device="cuda")
+    c = ops().KVCache(k, v, table, on_gpu([n] * B + [40] * few))
+    start = on_gpu(starts([rows] * B + [3] * few))
+    q = torch.randn(B * rows + 3 * few, G * D, generator=g, device="cuda").to(dtype)
+    clean, clean_lse = ops().paged_attn_chunk(c, q, G, row_start=start)
+    spoilt = []
+    for slot, d, bad in ((n - rows // 2, 5, float("nan")), (n - 2, D - 1, float("inf"))):
+        v[slot // page, 0, slot % page, d] = bad
+        spoilt.append((slot - (n - rows), d))
+    out, lse = ops().paged_attn_chunk(c, q, G, row_start=start)
+    again, _ = ops().paged_attn_chunk(c, q, G, row_start=start)
+    assert device_error() == 0
+    assert torch.equal(out[B * rows:], clean[B * rows:]) and torch.equal(lse, clean_lse)
+    lost = torch.zeros(B, rows, G, D, dtype=torch.bool, device="cuda")
+    for row, d in spoilt:
+        lost[:, row:, :, d] = True
+    out, again, clean = (t[:B * rows].view(B, rows, G, D) for t in (out, again, clean))
+    assert torch.equal(out.isfinite(), ~lost)
+    assert torch.equal(out[~lost], again[~lost])
+    want = clean[~lost].double()
+    assert float((out[~lost].double() - want).norm() / want.norm()) < ATTN[dtype]

@@ -150,6 +150,7 @@ struct ChunkWalk {
   ChunkItem it[2];
   int b, hg, u, k;
   long long at, x0, x1;    // cost where the unit starts, where the run does and ends
+  int count[6];            // what the warp has counted when its run is done, for a second walk
   // The item at hand; of the one after it once ahead() has been called.
   TKB_DEVFN const ChunkItem& item() const { return it[k & 1]; }
   TKB_DEVFN void step(const ChunkParams& p) {  // one lane: the item after the one at hand
@@ -479,20 +480,41 @@ TKB_DEVFN void chunk_put4(const ChunkParams& p, const ChunkSink& k, int col4, fl
 }
 
 // A value of V that is not finite, in a slot that some rows of a tile see and
-// others do not, spoils the products of those others too (0 * inf).  So rows
-// whose O is not finite look whether such a slot lies behind their last one;
-// if one does, their O is computed again from the slots they see alone.  Whole
-// warps call it, `bad` marks the lanes with such a row.
+// others do not, spoils the products of those others too (0 * inf).  A CTA that
+// meets a row whose O is not finite though its sum is, and which has slots of its
+// item behind its last one, walks its run a second time, with care: in slots that
+// not all rows of a unit see, such values become 0 in shared memory before their
+// products, and once a row is written, those that it does see are added to it.
+// (2 x 1.7 k tokens over 16 k, such a value near each end: 1.72 -> 3.55 ms.  No
+// wait of the run, bounded as they are, has to cover more than a block of it.)
+// 128 threads: the values of slots from .. upto - 1 of a stage of V.
 template <int D, bool BF16>
-__noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int jb, int step, int end, bool bad, int lim,
-                                         int row, int hq, float m, const ChunkSink& sink) {
+__noinline__ __device__ void chunk_take_out(uint8_t* stage, int from, int upto, int r) {
+  constexpr uint32_t EXP = BF16 ? 0x7f80u : 0x7c00u;  // all ones: an infinity or NaN
+  for (int i = from * 8 + r; i < upto * 8; i += 128)
+#pragma unroll 1
+    for (int x = 0; x < D / 64; ++x) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(stage + x * 128 * 128 + i * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t v = at[e];
+        uint32_t keep = 0u;
+        if ((v & EXP) != EXP) keep |= 0xffffu;
+        if ((v >> 16 & EXP) != EXP) keep |= 0xffff0000u;
+        if (~keep) at[e] = v & keep;
+      }
+    }
+}
+// Whole warps, a row a lane: the values taken out of blocks j0, j0 + step, ... below slot `last`, from slot `from` on.
+template <int D, bool BF16>
+__noinline__ __device__ void chunk_add_back(const ChunkParams& p, int b, int h, int j0, int step, int from, int last, int lim,
+                                            int row, int hq, float m, const ChunkSink& sink) {
   constexpr int E = D / 32;
   const tkb_kv_cache& c = p.c;
   const int lane = lane_id();
   using U = typename std::conditional<E == 4, uint2, uint32_t>::type;
-  auto load = [&](const void* pool, int page, int in, float (&f)[E]) {
-    const U u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(pool) + page_offset(c, page, h) +
-                                            static_cast<long long>(in) * D + lane * E);
+  auto load = [&](const void* pool, long long at, float (&f)[E]) {
+    const U u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(pool) + at + lane * E);
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) {
@@ -501,124 +523,93 @@ __noinline__ __device__ void chunk_again(const ChunkParams& p, int b, int h, int
       f[2 * e + 1] = x.y;
     }
   };
-  auto page_at = [&](int j) {
+  __syncwarp();  // the rows' other lanes have written them
+#pragma unroll 1
+  for (int j = max(from, j0 * kChunkBlock); j < last; ++j) {
+    if ((j / kChunkBlock - j0) % step) continue;  // the other warpgroup's
     const int pg = c.block_table[static_cast<long long>(b) * c.max_pages + j / c.page_size];
-    return static_cast<unsigned>(pg) < static_cast<unsigned>(c.n_pages) ? pg : -1;
-  };
-  const int from = __reduce_min_sync(0xffffffffu, bad ? max(lim, jb * kChunkBlock) : end);
-  int last = -1;  // the last slot with a value of V that is not finite
-  for (int j = from; j < end; ++j) {
-    if ((j / kChunkBlock - jb) % step) continue;  // the other warpgroup's
-    const int page = page_at(j);
-    if (page < 0) continue;
-    float v[E];
-    load(c.v, page, j % c.page_size, v);
+    if (static_cast<unsigned>(pg) >= static_cast<unsigned>(c.n_pages)) continue;
+    const long long at = page_offset(c, pg, h) + static_cast<long long>(j % c.page_size) * D;
+    float k[E], v[E];
+    load(c.v, at, v);
     bool odd = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) odd |= !(fabsf(v[e]) < INFINITY);
-    if (__any_sync(0xffffffffu, odd)) last = j;
-  }
-  unsigned todo = __ballot_sync(0xffffffffu, bad && last >= lim);
-  for (; todo; todo &= todo - 1) {
-    const int src = __ffs(todo) - 1;
-    const int rl = __shfl_sync(0xffffffffu, lim, src), rr = __shfl_sync(0xffffffffu, row, src),
-              rh = __shfl_sync(0xffffffffu, hq, src);
-    const float rm = __shfl_sync(0xffffffffu, m, src);
-    const float base = rm == -INFINITY ? 0.f : rm;
-    float q[E], o[E];
-    const U u = *reinterpret_cast<const U*>(static_cast<const uint16_t*>(p.q) + rr * p.q_stride +
-                                            static_cast<long long>(rh) * D + lane * E);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float2 x = unpack2<BF16>(w[e]);
-      q[2 * e] = x.x;
-      q[2 * e + 1] = x.y;
-      o[2 * e] = o[2 * e + 1] = 0.f;
-    }
-    for (int j = jb * kChunkBlock; j < min(rl, end); ++j) {
-      if ((j / kChunkBlock - jb) % step) continue;
-      const int page = page_at(j);
-      if (page < 0) continue;
-      float k[E], v[E], s = 0.f;
-      load(c.k, page, j % c.page_size, k);
-      load(c.v, page, j % c.page_size, v);
+    if (!__any_sync(0xffffffffu, odd)) continue;
+    load(c.k, at, k);
+#pragma unroll 1
+    for (unsigned todo = __ballot_sync(0xffffffffu, lim > j); todo; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1, rr = __shfl_sync(0xffffffffu, row, src), rh = __shfl_sync(0xffffffffu, hq, src);
+      const float rm = __shfl_sync(0xffffffffu, m, src), inv = __shfl_sync(0xffffffffu, sink.inv, src);
+      const long long slot = __shfl_sync(0xffffffffu, sink.slot, src);
+      float q[E], s = 0.f;
+      load(p.q, rr * p.q_stride + static_cast<long long>(rh) * D, q);
 #pragma unroll
       for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
-      const float pr = ex2(fmaf(warp_sum(s), p.scale_log2, -base));
+      const float pr = ex2(fmaf(warp_sum(s), p.scale_log2, rm == -INFINITY ? 0.f : -rm));
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(pr, v[e], o[e]);
-    }
-    ChunkSink to;
-    to.part = sink.part;
-    to.slot = __shfl_sync(0xffffffffu, sink.slot, src);
-    to.inv = __shfl_sync(0xffffffffu, sink.inv, src);
-    to.out = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(sink.out), src));
-    __syncwarp();
-    if constexpr (E == 4) {
-      chunk_put4<D, BF16>(p, to, lane, o[0], o[1], o[2], o[3]);
-    } else {
-      const float a = __shfl_down_sync(0xffffffffu, o[0], 1), d = __shfl_down_sync(0xffffffffu, o[1], 1);
-      if (!(lane & 1)) chunk_put4<D, BF16>(p, to, lane >> 1, o[0], o[1], a, d);
+      for (int e = 0; e < E; ++e) {
+        if (fabsf(v[e]) < INFINITY) continue;
+        const int col = lane * E + e;
+        if (sink.part) {
+          float* o = reinterpret_cast<float*>(p.part + (slot >> 7) * (D / 4) * 128 + (col >> 2) * 128 + (slot & 127)) + (col & 3);
+          *o = fmaf(pr, v[e], *o);
+        } else {
+          uint16_t* o = static_cast<uint16_t*>(p.out) + rr * p.out_stride + static_cast<long long>(rh) * D + col;
+          *o = static_cast<uint16_t>(pack2<BF16>(fmaf(pr * inv, v[e], unpack2<BF16>(*o).x), 0.f));
+        }
+      }
     }
   }
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid_constant__ ChunkParams p) {
-  using C = ChunkCfg<D>;
+// Where things lie in shared memory.
+TKB_DEVFN uint8_t* chunk_smem() {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+}
+template <int D>
+struct ChunkShared {
+  using C = ChunkCfg<D>;
+  uint64_t *q_full, *q_empty, *k_full, *k_empty, *v_full, *v_empty, *s_full, *p_ready, *o_done, *x_full, *x_empty, *mma_drain;
+  uint32_t *marks, *tmem_slot;
+  volatile int *abort_flag, *again_flag;
+  ChunkWalk* walk;
+  TKB_DEVFN explicit ChunkShared(uint8_t* smem) {
+    q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    q_empty = q_full + 1;
+    k_full = q_full + 2;
+    k_empty = k_full + C::NST;
+    v_full = k_empty + C::NST;
+    v_empty = v_full + C::NST;
+    s_full = v_empty + C::NST;
+    p_ready = s_full + 2;  // [w][half]
+    o_done = p_ready + 4;
+    x_full = o_done + 2;
+    x_empty = x_full + 1;
+    mma_drain = x_empty + 1;
+    marks = reinterpret_cast<uint32_t*>(smem + C::OFF_MASK);
+    tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+    abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+    again_flag = abort_flag + 1;
+    walk = reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK) + warp_id();
+  }
+};
+
+// The roles of a CTA over its run.  CAREFUL: the second walk, which counts on from the first.
+template <int D, bool BF16, bool CAREFUL>
+TKB_DEVFN void chunk_tc_run(const ChunkParams& p, uint8_t* smem, uint32_t tmem, bool any) {
+  using C = ChunkCfg<D>;
   const uint32_t sbase = smem_u32(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;
-  uint64_t* k_empty = k_full + C::NST;
-  uint64_t* v_full = k_empty + C::NST;
-  uint64_t* v_empty = v_full + C::NST;
-  uint64_t* s_full = v_empty + C::NST;
-  uint64_t* p_ready = s_full + 2;  // [w][half]
-  uint64_t* o_done = p_ready + 4;
-  uint64_t* x_full = o_done + 2;
-  uint64_t* x_empty = x_full + 1;
-  uint64_t* mma_drain = x_empty + 1;
-  uint32_t* marks = reinterpret_cast<uint32_t*>(smem + C::OFF_MASK);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+  const ChunkShared<D> sh(smem);
+  uint64_t *const q_full = sh.q_full, *const q_empty = sh.q_empty, *const k_full = sh.k_full, *const k_empty = sh.k_empty,
+           *const v_full = sh.v_full, *const v_empty = sh.v_empty, *const s_full = sh.s_full, *const p_ready = sh.p_ready,
+           *const o_done = sh.o_done, *const x_full = sh.x_full, *const x_empty = sh.x_empty, *const mma_drain = sh.mma_drain;
+  uint32_t* const marks = sh.marks;
+  volatile int *const abort_flag = sh.abort_flag, *const again_flag = sh.again_flag;
+  ChunkWalk& walk = *sh.walk;
   const int warp = warp_id(), lane = lane_id();
-
-  if (threadIdx.x == 0) {
-    for (uint64_t* x : {q_full, q_empty, mma_drain}) mbar_init(x, 1);
-    for (int s = 0; s < C::NST; ++s)
-      for (uint64_t* x : {k_full, k_empty, v_full, v_empty}) mbar_init(x + s, 1);
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(&s_full[w], 1);
-      mbar_init(&p_ready[2 * w], 128);
-      mbar_init(&p_ready[2 * w + 1], 128);
-      mbar_init(&o_done[w], 1);
-    }
-    mbar_init(x_full, 128);
-    mbar_init(x_empty, 128);
-    *abort_flag = 0;
-    fence_barrier_init();
-    prefetch_tmap(&p.tmQ);
-    prefetch_tmap(&p.tmK);
-    prefetch_tmap(&p.tmV);
-  }
-  if (warp == 9) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  grid_wait();
-  grid_go();
-  ChunkWalk& walk = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * static_cast<int>(sizeof(ChunkWalk)));
-  const bool any = chunk_deal<kChunkThreads>(p, walk);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
+  auto counted = [&](int i) { return CAREFUL ? walk.count[i] : 0; };
   if (!any) {
     if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(0, 0, 0, 0);
   } else if (warp == 8 || warp == 10) {
@@ -634,7 +625,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
     const int gi = lane % boxes, hh = lane / boxes;
     const int box_rows = p.gran;
     const uint32_t q_bytes = static_cast<uint32_t>(p.gb) * p.tt * D * 2;
-    int nq = 0, nb = 0;  // loads issued
+    int nq = counted(0), nb = counted(1);  // loads issued
     bool ok = true;
     walk.ahead(p);
     while (ok && walk.next()) {
@@ -694,6 +685,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
         bad = bad_next;
       }
     }
+    __syncwarp();
+    if (!CAREFUL && lane == 0) {
+      walk.count[0] = nq;
+      walk.count[1] = nb;
+    }
     if (*abort_flag) {
       // Let every copy this CTA started land before the CTA exits.
       volatile int never = 0;
@@ -726,8 +722,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
                   (acc || kk > 0) ? 1u : 0u);
         }
       };
-      int nq = 0, nk = 0, nv = 0;  // Q tiles, K and V blocks met so far
-      int np[2] = {0, 0};          // blocks of each warpgroup whose P has been used
+      int nq = counted(0), nk = counted(1), nv = counted(2);  // Q tiles, K and V blocks met so far
+      int np[2] = {counted(3), counted(4)};  // blocks of each warpgroup whose P has been used
       bool ok = true;
       auto wait_k = [&]() {
         if (!(ok = mbar_wait(&k_full[nk % C::NST], (nk / C::NST) & 1, abort_flag))) return false;
@@ -806,6 +802,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
           }
         }
       }
+      if (!CAREFUL) {
+        walk.count[0] = nq;
+        walk.count[1] = nk;
+        walk.count[2] = nv;
+        walk.count[3] = np[0];
+        walk.count[4] = np[1];
+      }
       if (!ok) {
         // Make sure no MMA is still running when TMEM is released.
         volatile int never = 0;
@@ -822,7 +825,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
     float4* xo = reinterpret_cast<float4*>(smem + C::OFF_X);
     float2* xml = reinterpret_cast<float2*>(smem + C::OFF_XML);
     const float sl2 = p.scale_log2;
-    int ns = 0, no = 0, nb = 0, nx = 0;  // blocks of this warpgroup, items with blocks of it, blocks of the CTA, exchanges
+    // blocks of this warpgroup, items with blocks of it, blocks of the CTA, exchanges
+    int ns = counted(0), no = counted(1), nb = counted(2), nx = counted(3);
     int flags = 0, span_b = 0, span_hg = 0, span_u = 0;
     bool ok = true;
     const int row_t = r / p.gb, row_g = r - row_t * p.gb;
@@ -843,11 +847,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
         const int at = j * kChunkBlock, nth = nb + j - it.jb;
         if (!(ok = mbar_wait_warp(&s_full[w], ns & 1, abort_flag))) break;
         tc_fence_after();
-        if (at + kChunkBlock > s.held) {
+        const int all_see = CAREFUL ? min(max(s.base + it.t0 + 1, 0), s.held) : s.held;  // what the unit's first row sees
+        if (at + kChunkBlock > all_see) {
           // slots of the last page behind the sequence's end may hold anything, and 0 * NaN is NaN: V there becomes 0
           const int stage = nth % C::NST;
           if (!(ok = mbar_wait_warp(&v_full[stage], (nth / C::NST) & 1, abort_flag))) break;
           const int from = max(s.held - at, 0);
+          if constexpr (CAREFUL)
+            chunk_take_out<D, BF16>(smem + C::OFF_V + stage * C::TILE, max(all_see - at, 0), min(from, kChunkBlock), r);
           for (int i = from * 8 + r; i < kChunkBlock * 8; i += 128)
 #pragma unroll
             for (int x = 0; x < D / 64; ++x)
@@ -988,20 +995,81 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid
         }
       }
       if (!ok) break;
-      // O that is not finite though l is: look behind the row's last slot
       const int last = min(end * kChunkBlock, s.held);
-      const bool bad = has && !(zero == 0.f) && valid && l > 0.f && lim < last;
-      if (__any_sync(0xffffffffu, bad))
-        chunk_again<D, BF16>(p, it.b, it.hg / p.hb, meet ? it.jb : j0, meet ? 1 : step, last, bad, lim, row, hq, m, sink);
+      if constexpr (CAREFUL) {
+        chunk_add_back<D, BF16>(p, it.b, it.hg / p.hb, meet ? it.jb : j0, meet ? 1 : step,
+                                min(max(s.base + it.t0 + 1, 0), s.held), last, lim, row, hq, m, sink);
+      } else if (has && !(zero == 0.f) && valid && l > 0.f && lim < last) {
+        *again_flag = 1;  // O is not finite though l is
+      }
+    }
+    __syncwarp();
+    if (!CAREFUL && lane == 0) {
+      walk.count[0] = ns;
+      walk.count[1] = no;
+      walk.count[2] = nb;
+      walk.count[3] = nx;
     }
     if (threadIdx.x == 0) p.span[blockIdx.x] = make_int4(ok ? flags : 0, span_b, span_hg, span_u);
   }
+}
+template <int D, bool BF16>
+__noinline__ __device__ void chunk_tc_again(const ChunkParams& p) {
+  uint8_t* smem = chunk_smem();
+  const ChunkShared<D> sh(smem);
+  const bool any = chunk_deal<kChunkThreads>(p, *sh.walk);
+  chunk_tc_run<D, BF16, true>(p, smem, *sh.tmem_slot, any);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kChunkThreads, 1) chunk_tc_kernel(const __grid_constant__ ChunkParams p) {
+  using C = ChunkCfg<D>;
+  uint8_t* smem = chunk_smem();
+  const ChunkShared<D> sh(smem);
+  const int warp = warp_id();
+
+  if (threadIdx.x == 0) {
+    for (uint64_t* x : {sh.q_full, sh.q_empty, sh.mma_drain}) mbar_init(x, 1);
+    for (int s = 0; s < C::NST; ++s)
+      for (uint64_t* x : {sh.k_full, sh.k_empty, sh.v_full, sh.v_empty}) mbar_init(x + s, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh.s_full[w], 1);
+      mbar_init(&sh.p_ready[2 * w], 128);
+      mbar_init(&sh.p_ready[2 * w + 1], 128);
+      mbar_init(&sh.o_done[w], 1);
+    }
+    mbar_init(sh.x_full, 128);
+    mbar_init(sh.x_empty, 128);
+    *sh.abort_flag = 0;
+    *sh.again_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&p.tmQ);
+    prefetch_tmap(&p.tmK);
+    prefetch_tmap(&p.tmV);
+  }
+  if (warp == 9) {
+    tmem_alloc(sh.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  grid_wait();
+  grid_go();
+  const bool any = chunk_deal<kChunkThreads>(p, *sh.walk);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  chunk_tc_run<D, BF16, false>(p, smem, *sh.tmem_slot, any);
 
   tc_fence_before();
   __syncthreads();
+  if (*sh.again_flag && !*sh.abort_flag) {
+    tc_fence_after();
+    chunk_tc_again<D, BF16>(p);
+    tc_fence_before();
+    __syncthreads();
+  }
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*sh.tmem_slot, 512);
   }
 }
 
