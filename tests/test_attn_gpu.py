@@ -186,3 +186,42 @@ def test_attn_long_sequence_ds_path_vs_recompute():
                            ("dQ", d_ds.view(B, S, Hq + 2 * Hkv, D)[0, :, h].float(), rdq[0, 0])):
         err = (torch.linalg.vector_norm(got - ref) / torch.linalg.vector_norm(ref)).item()
         assert err < TOL16, (name, err)
+
+
+def _plain(qkv, S, Hq, Hkv, D, causal):
+    """(out [S, Hq * D], lse [Hq, S]) of one batch in 64 bits."""
+    x = qkv.astype(np.float64).reshape(S, Hq + 2 * Hkv, D)
+    out, lse = np.zeros((S, Hq, D)), np.zeros((Hq, S))
+    for h in range(Hq):
+        g = h // (Hq // Hkv)
+        s = x[:, h] @ x[:, Hq + g].T * D ** -0.5
+        if causal:
+            s[np.triu_indices(S, 1)] = -np.inf
+        top = s.max(1, keepdims=True)
+        p = np.exp(s - top)
+        out[:, h] = (p / p.sum(1, keepdims=True)) @ x[:, Hq + Hkv + g]
+        lse[h] = top[:, 0] + np.log(p.sum(1))
+    return out.reshape(S, Hq * D), lse
+
+
+# P and the output are each rounded to the type, by half a step at most: 2^-8 and 2^-8 of bf16, 2^-11 and 2^-11 of f16.
+# Scores up to 500 in fp32 are off by some 500 * 2^-23 = 6e-5, and so are the weights, and lse by as much.
+LOW = {torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("low", [-8.0, -12.0, -80.0, -500.0])
+def test_attn_fwd_scores_far_below_zero(D, causal, dtype, low):
+    """All scores of every row near `low`: the weights hang on their differences alone."""
+    S, Hq, Hkv = 300, 4, 2
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(S, Hq + 2 * Hkv, D, generator=g)
+    x[:, :Hq, 0] = 16.0
+    x[:, Hq:Hq + Hkv, 0] = low * D ** 0.5 / 16.0
+    x = x.to(dtype).reshape(1, S, -1)
+    want_o, want_l = _plain(x.double().numpy(), S, Hq, Hkv, D, causal)
+    o, lse = _ops().gqa_attn_fwd(x.cuda(), 1, S, Hq, Hkv, D, D ** -0.5, causal)
+    assert rel_l2(o.double().cpu().numpy().reshape(S, -1), want_o) < LOW[dtype]
+    assert np.abs(lse.cpu().numpy().reshape(Hq, S) - want_l).max() < 1e-3

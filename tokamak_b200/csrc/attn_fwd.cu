@@ -118,12 +118,14 @@ TKB_DEVFN void softmax_block(uint32_t tS, uint32_t tO, float sl2, int j, int qt,
   }
   float mx0 = sv[0], mx1 = sv[1], mx2 = sv[2], mx3 = sv[3];
 #pragma unroll
-  for (int c = 4; c < 128; c += 8) {
+  for (int c = 4; c < 124; c += 8) {
     mx0 = fmax3(mx0, sv[c], sv[c + 1]);
     mx1 = fmax3(mx1, sv[c + 2], sv[c + 3]);
     mx2 = fmax3(mx2, sv[c + 4], sv[c + 5]);
     mx3 = fmax3(mx3, sv[c + 6], sv[c + 7]);
   }
+  mx0 = fmax3(mx0, sv[124], sv[125]);
+  mx1 = fmax3(mx1, sv[126], sv[127]);
   const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;
   // Raise the running max when this block's exceeds it by more than 8
   // (2^8 headroom in fp32): the row sum now, the partial O row below,
