@@ -225,3 +225,26 @@ def test_attn_fwd_scores_far_below_zero(D, causal, dtype, low):
     o, lse = _ops().gqa_attn_fwd(x.cuda(), 1, S, Hq, Hkv, D, D ** -0.5, causal)
     assert rel_l2(o.double().cpu().numpy().reshape(S, -1), want_o) < LOW[dtype]
     assert np.abs(lse.cpu().numpy().reshape(Hq, S) - want_l).max() < 1e-3
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attn_fwd_scores_of_minus_infinity_before_low_ones(D, dtype):
+    """260 keys whose scores are -inf take no weight: rows that see them alone give 0 and -inf, the scores behind
+    them, far below zero, count in full."""
+    S = 400
+    g = torch.Generator().manual_seed(4)
+    x = torch.zeros(S, 3, D)
+    x[:, 0, 0] = 1.0
+    x[:, 0, 1] = 30.0 * (D / 64) ** 0.5
+    x[:, 1, 1] = -50.0
+    x[:260, 1, 0] = -float("inf")
+    x[:, 2] = torch.randn(S, D, generator=g)
+    x = x.to(dtype)
+    o, lse = _ops().gqa_attn_fwd(x.reshape(1, S, -1).cuda(), 1, S, 1, 1, D, D ** -0.5, True)
+    o, lse, v = o.double().cpu().numpy().reshape(S, D), lse.double().cpu().numpy().ravel(), x[:, 2].double().numpy()
+    assert (o[:260] == 0).all() and np.isneginf(lse[:260]).all()
+    want = np.array([v[260:i + 1].mean(0) for i in range(260, S)])
+    assert rel_l2(o[260:], want) < LOW[dtype]
+    score = float(x[0, 0, 1].double()) * -50.0 * D ** -0.5
+    assert np.abs(lse[260:] - score - np.log(np.arange(1, S - 259))).max() < 1e-3

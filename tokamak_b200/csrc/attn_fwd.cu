@@ -134,21 +134,22 @@ TKB_DEVFN void softmax_block(uint32_t tS, uint32_t tO, float sl2, int j, int qt,
   float resc = 1.f;
   bool raised = false;
   if (j == 0) {
-    m_used = (mx == -INFINITY) ? 0.f : mx;
-  } else if (mx > m_used + 8.0f) {
+    m_used = mx;
+  } else if (mx > m_used + 8.0f) {  // from -inf (scores of -inf alone so far) too
     resc = ex2(m_used - mx);  // may be 0 for a jump past 2^126: O is then cleared
     l *= resc;
     m_used = mx;
     raised = true;
   }
-  const uint64_t sl2x2 = f2(sl2, sl2), nmx2 = f2(-m_used, -m_used);
+  const float base = m_used == -INFINITY ? 0.f : -m_used;
+  const uint64_t sl2x2 = f2(sl2, sl2), nmx2 = f2(base, base);
   uint32_t pk0[32], pk1[32];
   uint64_t ls0 = f2(0.f, 0.f), ls1 = f2(0.f, 0.f);
-  // exponentials of keys 2i, 2i+1 (pair i of the half at sv + base): the
+  // exponentials of keys 2i, 2i+1 (pair i of the half at sv + from): the
   // scale and the row sums in packed f32x2 instructions
-  auto exp_pair = [&](int base, int i, uint32_t& pk, uint64_t& ls) {
+  auto exp_pair = [&](int from, int i, uint32_t& pk, uint64_t& ls) {
     float x0, x1, a, c;
-    f2_split(fma_f2(f2(sv[base + 2 * i], sv[base + 2 * i + 1]), sl2x2, nmx2), x0, x1);
+    f2_split(fma_f2(f2(sv[from + 2 * i], sv[from + 2 * i + 1]), sl2x2, nmx2), x0, x1);
     a = ex2(x0);
     c = ex2(x1);
     ls = add_f2(ls, f2(a, c));
