@@ -410,8 +410,12 @@ int tkb_kv_pages(int32_t *block_table, int32_t *held, const int32_t *lens, int32
  * with x [rows][K], y (the shared projection's output) and out [rows][N] (out
  * may be y, at the same stride), A [n_adapters][K][R] and B [n_adapters][R][N],
  * all of one dtype, rows x_stride, y_stride, out_stride elements apart; scale
- * [n_adapters] fp32 (NULL: 1).  Products and sums are fp32, the result is
- * rounded once.  adapter[b] = -1: out_r = y_r.  Rows of no sequence are left
+ * [n_adapters] fp32 (NULL: 1).  Products and sums are fp32 and the result is
+ * rounded once; in 16-bit types x A enters the second product as two 16-bit
+ * parts, off by at most 2^-16 of it in bf16 and 2^-22 in f16.  NaN and
+ * infinities in x, A and y reach their rows as the formula has them; those of
+ * B do too, but in 16-bit types an infinite value may give NaN.
+ * adapter[b] = -1: out_r = y_r.  Rows of no sequence are left
  * as they were.  An adapter that does not exist counts as -1 and sets bit 2 of
  * the device error word.  K, N and the strides: multiples of 16 bytes, the
  * pointers 16-byte aligned; R a multiple of 8 up to 128; B at most 4096, rows at

@@ -221,6 +221,40 @@ def test_lora_nan_stays_in_its_rows(dtype):
     assert out[20].isnan().all() and out[:7].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R", [8, 16, 24, 64, 72])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_lora_infinities_keep_their_sign(dtype, R, rows):
+    """An infinite x beside adapters of one sign: rows of infinities, as in the formula; a scale below 0 turns them; a rank
+    that is padded does not make them NaN, and neither does another large value of the row."""
+    K, N = 128, 72
+    x, y, a, b, _, start = lora_case(dtype, [0, 1], [rows, rows], 2, K, N, R)
+    a, b, scale = a.abs() + 0.01, b.abs() + 0.01, on_gpu([1.0, -0.5], torch.float32)
+    plan = ops().lora_plan(on_gpu([0, 1]), 2, 2 * rows, row_start=on_gpu(start))
+    clean = ops().lora_add(plan, x, a, b, y, scale=scale, out=torch.empty_like(y))
+    want = torch.full_like(y, float("inf"))
+    x[1, 7], x[2, K - 1], x[rows + 3, 0] = float("inf"), -float("inf"), float("inf")
+    x[2, 3] = 60000.0 if dtype == torch.float16 else 1e30
+    want[2], want[rows + 3] = -float("inf"), -float("inf")
+    out = ops().lora_add(plan, x, a, b, y, scale=scale, out=torch.empty_like(y))
+    lost = torch.zeros(2 * rows, dtype=torch.bool, device="cuda")
+    lost[[1, 2, rows + 3]] = True
+    assert torch.equal(out[lost], want[lost]) and torch.equal(out[~lost], clean[~lost])
+
+
+def test_lora_products_above_the_largest_bf16():
+    """x A between the largest bf16 and the largest fp32, times a small B: finite."""
+    K, N, R = 64, 64, 16
+    x, y, a, b, _, start = lora_case(torch.bfloat16, [0], [3], 1, K, N, R)
+    x.zero_()
+    x[1, 0], x[1, 1] = torch.finfo(torch.bfloat16).max, 1e36
+    a.fill_(1.0)
+    b.fill_(2.0 ** -20)
+    plan = ops().lora_plan(on_gpu([0]), 1, 3, row_start=on_gpu(start))
+    out = ops().lora_add(plan, x, a, b, y, out=torch.empty_like(y))
+    rows_close(num(out), ref.lora(num(x), num(a), num(b), num(y), [0], start, None), torch.bfloat16)
+
+
 def test_lora_bad_adapters_and_row_starts():
     x, y, a, b, scale, _ = lora_case(torch.bfloat16, [0, 1], [4, 6], 2, 64, 64, 8)
     for adapter in ([2, 1], [-2, 1], [1 << 30, 1]):

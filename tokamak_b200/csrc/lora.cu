@@ -322,8 +322,10 @@ __global__ void __launch_bounds__(kLoraThreads) lora_down_kernel(const __grid_co
   lora_meet(s, p.t + static_cast<long long>(tile.at) * RP, tile.count * RP, p.splits);
 }
 
-// t of rows g and g + 8 of a warp's 16 as operands of the second product: the 16-bit rounding and the rest.  f16 takes it as
-// multiples `up` of a power of two near the row's largest, so that it fits the type.  at(r, k): t of row r, columns k, k + 1.
+// t of rows g and g + 8 of a warp's 16 as operands of the second product: the 16-bit rounding and the rest, which leave out
+// 2^-16 of it in bf16 and 2^-22 in f16 at most.  f16 takes it as multiples `up` of a power of two near the row's largest, so
+// that it fits the type.  The rounding is a finite one, so that the rest of an infinite t, or of one that would round to an
+// infinity, is what it should be.  at(r, k): t of row r, columns k, k + 1.
 template <bool BF16, int RP, typename At>
 TKB_DEVFN void lora_split(At&& at, float (&up)[2], uint32_t (&hi)[RP / 16][4], uint32_t (&lo)[RP / 16][4]) {
   const int g = lane_id() >> 2, c2 = (lane_id() & 3) * 2;
@@ -336,14 +338,17 @@ TKB_DEVFN void lora_split(At&& at, float (&up)[2], uint32_t (&hi)[RP / 16][4], u
       const float2 s = at(g + (i & 1) * 8, k * 16 + (i >> 1) * 8 + c2);
       t[k][2 * i] = s.x;
       t[k][2 * i + 1] = s.y;
-      top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(s.x), fabsf(s.y)));
+      if (!BF16) {
+        if (fabsf(s.x) < INFINITY) top[i & 1] = fmaxf(top[i & 1], fabsf(s.x));
+        if (fabsf(s.y) < INFINITY) top[i & 1] = fmaxf(top[i & 1], fabsf(s.y));
+      }
     }
   if (!BF16) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
       top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      if (top[i] > 1e-30f && top[i] < 1e30f) {  // else 0, infinite, or next to either
+      if (top[i] > 1e-30f && top[i] < 1e30f) {  // else 0, or next to it or to the largest there is
         const int e = (__float_as_int(top[i]) >> 23) - 127;
         up[i] = __int_as_float((e + 127) << 23);
         down[i] = __int_as_float((127 - e) << 23);
@@ -354,8 +359,9 @@ TKB_DEVFN void lora_split(At&& at, float (&up)[2], uint32_t (&hi)[RP / 16][4], u
   for (int k = 0; k < RP / 16; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      constexpr float MOST = BF16 ? 3.38953139e38f : 65504.f;
       const float a = t[k][2 * i] * down[i & 1], b = t[k][2 * i + 1] * down[i & 1];
-      hi[k][i] = pack2<BF16>(a, b);
+      hi[k][i] = pack2<BF16>(fminf(fmaxf(a, -MOST), MOST), fminf(fmaxf(b, -MOST), MOST));
       const float2 h = unpack2<BF16>(hi[k][i]);
       lo[k][i] = pack2<BF16>(a - h.x, b - h.y);
     }
@@ -452,7 +458,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_kernel(const __grid_cons
   uint32_t hi[RP / 16][4], lo[RP / 16][4];
   lora_split<BF16, RP>([&](int r, int k) {
     float2 s = make_float2(0.f, 0.f);
-    if (r0 + r < tile.count) s = *reinterpret_cast<const float2*>(p.t + (static_cast<long long>(tile.at) + r0 + r) * RP + k);
+    // columns behind the rank are sums of zeros, or of zeros times an infinity
+    if (r0 + r < tile.count && k < p.R) s = *reinterpret_cast<const float2*>(p.t + (static_cast<long long>(tile.at) + r0 + r) * RP + k);
     return make_float2(s.x * scale, s.y * scale);
   }, up, hi, lo);
   for (int c = 0; c < n; ++c) {
@@ -611,7 +618,9 @@ __global__ void __launch_bounds__(kLoraThreads) lora_one_kernel(const __grid_con
   float up[2];
   uint32_t hi[RP / 16][4], lo[RP / 16][4];
   const float* st = reinterpret_cast<const float*>(s_ring + C::OFF_T);
-  lora_split<BF16, RP>([&](int r, int k) { return *reinterpret_cast<const float2*>(st + r * RP + k); }, up, hi, lo);
+  lora_split<BF16, RP>([&](int r, int k) {
+    return k < p.R ? *reinterpret_cast<const float2*>(st + r * RP + k) : make_float2(0.f, 0.f);
+  }, up, hi, lo);
   for (int i = 0; c0 + w + 4 * i < c1; ++i) {
     // the chunks asked for at the start are here; from then on the ring's own
     cp_async_wait<C::ST - 2>();
@@ -744,7 +753,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_
     const float scale = p.scale ? p.scale[tile.adapter] : 1.f;
     for (int i = tid; i < TM * RP; i += kLoraThreads) {
       const int r = i / RP, k = i % RP;
-      ts[r * C::TS + k] = r < tile.count ? p.t[(static_cast<long long>(tile.at) + r) * RP + k] * scale : 0.f;
+      ts[r * C::TS + k] = r < tile.count && k < p.R ? p.t[(static_cast<long long>(tile.at) + r) * RP + k] * scale : 0.f;
     }
   }
   const float* y = static_cast<const float*>(p.y);
