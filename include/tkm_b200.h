@@ -397,8 +397,12 @@ int tkb_paged_attn_chunk(const tkb_kv_cache *cache, const void *q, long long q_s
  * the pool, page * page_size + slot in the page, for callers that move tokens
  * themselves: row_start as for tkb_kv_append, lens counting the new rows; -1
  * for a row without a place.  One call for a cache serves all layers that
- * share the table.  Lengths below 0, counts outside their range and pages
- * above n_pages set bit 2 of the device error word and are cut to the range.
+ * share the table.  Lengths below 0, counts outside their range and more free
+ * pages than n_pages set bit 2 of the device error word and are cut to the
+ * range.  A number outside [0, n_pages) among the pages that move or that hold
+ * a row sets it too: it moves like the others, its rows have no place, and a
+ * sequence that is given one is not granted (what it held before is not
+ * looked at).
  * B at most 4096, B * max_pages below 2^30, page_size 1 to 1024. */
 int tkb_kv_pages(int32_t *block_table, int32_t *held, const int32_t *lens, int32_t *free_pages, int32_t *n_free,
                  int32_t *granted, int64_t *slots, const int32_t *row_start, int rows, int B, int max_pages,

@@ -108,6 +108,33 @@ def test_bad_counts_are_cut():
         assert (guard[:4] == 77).all() and guard[11] == 77
 
 
+@pytest.mark.parametrize("B", [3, 300])
+@pytest.mark.parametrize("bad", [-1, 16, 1 << 30])
+def test_numbers_that_name_no_page(B, bad):
+    """A held entry that names no page: bit 2 when a row lies in it, when it is given back, and when another sequence gets
+    it, which is then not granted; the other sequences are."""
+    t = torch.full((B, 3), -1, dtype=torch.int32, device="cuda")
+    t[0, :2], t[1, 0] = on_gpu([4, bad]), 7
+    held, free, n_free = on_gpu([2, 1] + [0] * (B - 2)), torch.full((16,), -5, dtype=torch.int32, device="cuda"), on_gpu([0])
+
+    def step(lens, rows=None):
+        start = np.concatenate(([0], np.cumsum(rows))) if rows else None
+        granted, slots = ops().kv_pages(t, held, on_gpu(lens + [0] * (B - len(lens))), free, n_free, 16,
+                                        row_start=None if rows is None else on_gpu(list(start) + [start[-1]] * (B - len(rows))),
+                                        rows=None if rows is None else int(start[-1]))
+        return granted[:3].tolist(), None if slots is None else slots.tolist()
+
+    assert step([32, 16]) == ([1, 1, 1], None) and device_error() == 0     # nothing moves
+    assert step([18, 16], rows=[3, 1]) == ([1, 1, 1], [4 * 16 + 15, -1, -1, 7 * 16 + 15]) and device_error() == 4
+    assert step([16, 16])[0] == [1, 1, 1] and device_error() == 4          # given back
+    assert int(n_free) == 1 and int(free[0]) == bad
+    assert step([16, 16, 5], rows=[0, 1, 5]) == ([1, 1, 0], [7 * 16 + 15] + [-1] * 5) and device_error() == 4
+    assert held[:3].tolist() == [1, 1, 1] and int(n_free) == 0
+    assert step([16, 16])[0] == [1, 1, 1] and device_error() == 4          # and back again
+    free[0] = 9
+    assert step([16, 16, 5])[0] == [1, 1, 1] and device_error() == 0
+
+
 def test_pages_captured():
     """A captured call follows the lengths; the pages it takes are those of plain calls."""
     B, most, page = 9, 8, 16

@@ -49,13 +49,19 @@ TKB_DEVFN V block_scan(V v, V* s_warp, V& total) {
   return before + x - v;
 }
 
+// Whether a number names a page; the error bit where it does not.
+TKB_DEVFN bool page_ok(const PagesParams& p, int page) {
+  if (static_cast<unsigned>(page) < static_cast<unsigned>(p.n_pages)) return true;
+  atomicOr(&g_device_error, ERR_BAD_INDEX);
+  return false;
+}
 // The slot of a row that belongs to sequence b, `back` rows before its sequence's end.
 TKB_DEVFN long long page_slot(const PagesParams& p, int b, int back, int pages) {
   const long long slot = static_cast<long long>(__ldg(p.lens + b)) - back;
   if (slot < 0 || slot >= static_cast<long long>(pages) * p.page_size) return -1;
   const int i = static_cast<int>(slot) / p.page_size;
   const int page = __ldcg(p.table + static_cast<long long>(b) * p.max_pages + i);
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.n_pages)) return -1;
+  if (!page_ok(p, page)) return -1;
   return static_cast<long long>(page) * p.page_size + (static_cast<int>(slot) - i * p.page_size);
 }
 // The sequence of a row: the last b with row_start[b] <= row; false where the row is not its own.
@@ -159,7 +165,9 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(const __grid_constant
     const int n = -s_move[b], at = s_at[b];
     int32_t* t = p.table + static_cast<long long>(b) * p.max_pages + s_kept[b];
     for (int e = lane; e < n; e += 32) {
-      if (at + e < p.n_pages) p.free_pages[at + e] = t[e];
+      const int page = t[e];
+      page_ok(p, page);
+      if (at + e < p.n_pages) p.free_pages[at + e] = page;
       t[e] = -1;
     }
   }
@@ -167,7 +175,11 @@ __global__ void __launch_bounds__(THREADS) kv_pages_kernel(const __grid_constant
   for (int b = w0; b < p.B; b += warps) {
     const int n = s_move[b], at = s_at[b];
     int32_t* t = p.table + static_cast<long long>(b) * p.max_pages + s_kept[b];
-    for (int e = lane; e < n; e += 32) t[e] = __ldcg(p.free_pages + at - e);
+    for (int e = lane; e < n; e += 32) {
+      const int page = __ldcg(p.free_pages + at - e);
+      if (!page_ok(p, page) && p.granted) p.granted[b] = 0;
+      t[e] = page;
+    }
   }
   if (!p.slots) return;
   together();  // the table is whole
