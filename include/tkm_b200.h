@@ -396,7 +396,9 @@ int tkb_paged_attn_chunk(const tkb_kv_cache *cache, const void *q, long long q_s
  * slots (may be NULL) gets, for each of `rows` rows, the place of its token in
  * the pool, page * page_size + slot in the page, for callers that move tokens
  * themselves: row_start as for tkb_kv_append, lens counting the new rows; -1
- * for a row without a place.  One call for a cache serves all layers that
+ * for a row without a place.  (Without slots, rows only helps to choose the
+ * launch: about how many tokens have come and gone since the call before; 0
+ * for a step.)  One call for a cache serves all layers that
  * share the table.  Lengths below 0, counts outside their range and more free
  * pages than n_pages set bit 2 of the device error word and are cut to the
  * range.  A number outside [0, n_pages) among the pages that move or that hold

@@ -202,7 +202,7 @@ def test_released_sequences_take_no_part_in_steps(monkeypatch):
         lens += n
         seen += n
 
-    def kv_pages(table, held, lens, free, n_free, page):
+    def kv_pages(table, held, lens, free, n_free, page, tokens=0):
         stack = free[:int(n_free)].tolist()
         t, h, stack, _ = ref.pages(table.numpy(), held.numpy(), lens.tolist(), stack, page)
         table.copy_(torch.from_numpy(t))

@@ -108,6 +108,23 @@ def test_bad_counts_are_cut():
         assert (guard[:4] == 77).all() and guard[11] == 77
 
 
+@pytest.mark.parametrize("B", [1, 48, 49, 128, 129, 256, 257])
+def test_pages_whatever_the_launch(B):
+    """`tokens` chooses a launch; the tables are the same for every number, beside the oracle's."""
+    rng, most, page = np.random.default_rng(B), 30, 16
+    lens = rng.integers(0, most * page + 1, B)
+    pool = Pool(B, most, page, lens, free=4 * B)
+    for tokens in (0, 1024, 1025, 4096 * page + page, 1 << 40):
+        new = np.where(rng.random(B) < 0.2, 0, np.minimum(most * page, lens + rng.integers(0, 3 * page, B)))
+        granted, slots = ops().kv_pages(pool.t, pool.h, on_gpu(new), pool.f, pool.n, page, tokens=tokens)
+        pool.table, pool.held, pool.stack, want = ref.pages(pool.table, pool.held, new, pool.stack, page)
+        assert slots is None and granted.tolist() == want
+        assert np.array_equal(pool.t.cpu().numpy(), pool.table) and np.array_equal(pool.h.cpu().numpy(), pool.held)
+        assert int(pool.n) == len(pool.stack) and pool.f[:len(pool.stack)].tolist() == pool.stack
+        lens = np.where(np.array(want) > 0, new, np.minimum(new, pool.held * page))
+    assert device_error() == 0
+
+
 @pytest.mark.parametrize("B", [3, 300])
 @pytest.mark.parametrize("bad", [-1, 16, 1 << 30])
 def test_numbers_that_name_no_page(B, bad):

@@ -90,7 +90,7 @@ int tkb_kv_pages(int32_t* block_table, int32_t* held, const int32_t* lens, int32
     return fail(TKB_ERR_UNSUPPORTED, "%s: B * max_pages or n_pages above 2^30", who);
   if (reinterpret_cast<uintptr_t>(slots) & 7) return fail(TKB_ERR_ARG, "%s: slots must be 8-byte aligned", who);
   const PagesParams p = {block_table, held, lens, free_pages, n_free, granted, reinterpret_cast<long long*>(slots),
-                         row_start, slots ? rows : 0, B, max_pages, page_size, n_pages};
+                         row_start, rows > 0 ? rows : 0, B, max_pages, page_size, n_pages};
   unsigned kernels = 0;
   const cudaError_t e = kv_pages(p, static_cast<cudaStream_t>(stream), kernels);
   return cuda_status(e, who, kernels);

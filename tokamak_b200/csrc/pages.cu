@@ -20,7 +20,8 @@ struct PagesParams {
   int32_t* granted;
   long long* slots;
   const int32_t* row_start;
-  int rows, B, max_pages, page_size, n_pages;
+  int rows;  // without slots: about how many tokens come and go
+  int B, max_pages, page_size, n_pages;
 };
 
 // Exclusive sums over the block of each thread's value, and the total.
@@ -81,10 +82,18 @@ TKB_DEVFN bool row_seq(const int32_t* row_start, int B, int row, int& b, int& ba
   return __ldg(row_start + b) <= row && row < end;
 }
 
-// Few rows and sequences take one CTA of 256 threads (64 sequences of a row each: 6.2 us with the case's copy, the cluster
-// 8.2).  From 1024 rows on there are pages to move as well, and their slots are the second launch's (64 sequences, 10 k
-// rows: one CTA 18 us, the cluster 12.3, 11.1 with the slots apart).
+// One CTA of 256 threads or the cluster, us a call in a graph without slots, B sequences of which each moves so many pages:
+//   B          16            32            48            64            96            128           256
+//   none   1.8   4.1     2.1   4.2     2.5   4.3     2.8   4.2     3.3   4.2     3.9   4.2     6.3   4.2
+//   8      2.3   4.5     3.0   4.6     3.7   4.6     4.5   4.6     6.0   4.8     7.4   4.5    13.6   4.5
+//   128    3.4   5.1     5.2   5.2     7.0   5.3     8.8   5.3    12.7   5.3    16.2   5.2    30.8   5.3
+//   512    8.0   7.4    14.2   7.9    20.7   7.9    26.5   8.0    39.1   8.1    51.4   7.9     101   8.1
+// Up to kPagesFew rows are steps, which move next to nothing.  More are prompts, and of those the slots are a second launch
+// (64 sequences, 10 k rows: in one CTA 18 us, in the cluster 12.3, apart 11.1).
 constexpr int kPagesFew = 1024;
+static bool pages_one_cta(const PagesParams& p) {
+  return p.rows <= kPagesFew ? p.B <= 128 : p.B <= 48 && p.rows / p.page_size <= 4096;
+}
 
 // SEQS sequences a thread.
 template <int THREADS, int SEQS>
@@ -205,7 +214,7 @@ static cudaError_t kv_pages(const PagesParams& p, cudaStream_t st, unsigned& ker
   if (apart) first.slots = nullptr;
   const size_t smem = 3 * sizeof(int) * p.B;
   cudaError_t e = cudaSuccess;
-  if (p.B <= 256 && p.rows <= kPagesFew) {
+  if (pages_one_cta(p)) {
     e = launch_early(kv_pages_kernel<256, 1>, dim3(1), 256, smem, st, first);
   } else {
     e = allow_smem<kv_pages_kernel<1024, 4>>(3 * sizeof(int) * 4096);

@@ -217,10 +217,10 @@ class Generator:
         if self.pool and need > self.pool:
             raise TkbError(f"Generator: {need} pages are needed, the pool has {self.pool}")
 
-    def _pages(self):
-        """The pages of the sequences as their lengths want them now."""
+    def _pages(self, tokens=0):
+        """The pages of the sequences as their lengths want them now, about so many tokens after the last time."""
         if self.pool:
-            ops.kv_pages(self.table, self.pages_held, self.lens, self.free_pages, self.n_free, self.page_size)
+            ops.kv_pages(self.table, self.pages_held, self.lens, self.free_pages, self.n_free, self.page_size, tokens=tokens)
 
     def _take_part(self, live):
         """Which sequences take part in decode steps.  Captured steps follow: they read step_rows and seen.  Those that
@@ -261,10 +261,10 @@ class Generator:
         self._take_part([True] * self.batch)
         self.lens.zero_()
         self.seen.zero_()
-        self.held = [0] * self.batch
+        left, self.held = sum(self.held), [0] * self.batch
         if self.chunk and max(n) > self.chunk:
             logits = torch.empty(self.batch, self.cfg["vocab"], dtype=torch.float32, device=self.token.device)
-            self._pages()  # what the sequences held goes back before the first piece
+            self._pages(left)  # what the sequences held goes back before the first piece
             for at in range(0, max(n), self.chunk):
                 pieces = [p[at:at + self.chunk] for p in prompts]
                 got, last = self._enter(pieces), [b for b, p in enumerate(pieces) if p and at + self.chunk >= n[b]]
@@ -276,7 +276,7 @@ class Generator:
         row_start = torch.from_numpy(start).to(dev)
         tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.int64, device=dev)
         ops.kv_lens(self.lens, seen=self.seen, row_start=row_start)
-        self._pages()
+        self._pages(left + sum(n))
         self.held = list(n)
         if self.budget and max(n) > self.budget:
             ends, upto = self._last(start, n)
@@ -312,7 +312,7 @@ class Generator:
         row_start = torch.from_numpy(start).to(dev)
         tokens = torch.tensor([t for p in pieces for t in p], dtype=torch.int64, device=dev)
         ops.kv_lens(self.lens, seen=self.seen, row_start=row_start)
-        self._pages()
+        self._pages(sum(n))
         self.held = [h + m for h, m in zip(self.held, n)]
         workspace = ops.paged_attn_chunk_workspace(self.caches[0], len(tokens), self.Hq)
         if self.budget:
@@ -367,11 +367,12 @@ class Generator:
         which = sorted(set(int(b) for b in sequences))
         if which and (which[0] < 0 or which[-1] >= self.batch):
             raise TkbError(f"release: sequences are 0 to {self.batch - 1}")
+        left = sum(self.held[b] for b in which)
         for b in which:
             self.lens[b:b + 1].zero_()
             self.held[b] = 0
         self._take_part([a and b not in which for b, a in enumerate(self.live)])
-        self._pages()
+        self._pages(left)
 
     def decode(self):
         """One step: the tokens in self.token (rows of embed) enter the caches; returns the next logits [batch, vocab].  The
@@ -402,7 +403,7 @@ class Generator:
             ops.kv_evict(c, self.budget, self.seen, recent=self.recent, sinks=self.sinks,
                          workspace=self.evict_workspace)
         ops.kv_lens(self.lens, self.budget)
-        self._pages()
+        self._pages(sum(max(0, n - self.budget) for n in self.held))
         self.held = [min(n, self.budget) for n in self.held]
 
     def generate(self, prompts, steps, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):

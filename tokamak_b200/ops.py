@@ -440,10 +440,11 @@ def paged_attn_chunk(cache, q, Hq, row_start=None, scale=None, out=None, lse=Non
     return out, lse
 
 
-def kv_pages(block_table, held, lens, free_pages, n_free, page_size, row_start=None, rows=None):
+def kv_pages(block_table, held, lens, free_pages, n_free, page_size, row_start=None, rows=None, tokens=0):
     """Pages for sequences of `lens` tokens (tkb_kv_pages): block_table [B, max_pages], held [B], the stack free_pages
     [n_pages] and its height n_free [1] are brought up to date, all int32.  Returns (granted [B] int32, slots): with
-    `rows`, slots [rows] int64 is each new row's place in the pool (row_start as in kv_append), else None."""
+    `rows`, slots [rows] int64 is each new row's place in the pool (row_start as in kv_append), else None; `tokens` is then
+    about how many tokens come and go (0: a step), for the launch."""
     B, max_pages = block_table.shape
     _expect(block_table, "block_table", (B, max_pages), torch.int32)
     _vec(held, "held", B, torch.int32)
@@ -455,7 +456,7 @@ def kv_pages(block_table, held, lens, free_pages, n_free, page_size, row_start=N
     granted = torch.empty_like(held)
     slots = None if rows is None else torch.empty(rows, dtype=torch.int64, device=held.device)
     check(lib().tkb_kv_pages(_ptr(block_table), _ptr(held), _ptr(lens), _ptr(free_pages), _ptr(n_free), _ptr(granted),
-                             _ptr(slots), _ptr(row_start), 0 if rows is None else rows, B, max_pages, page_size,
+                             _ptr(slots), _ptr(row_start), min(int(tokens), 0x7FFFFFFF) if rows is None else rows, B, max_pages, page_size,
                              free_pages.numel(), stream), "tkb_kv_pages")
     return granted, slots
 
