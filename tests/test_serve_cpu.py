@@ -277,3 +277,19 @@ def test_adapter_refusals(tmp_path):
         np.savez(path, **arrays)
         with pytest.raises(TkbError):
             generate.Adapters.load(cfg, path)
+
+
+def test_adapters_of_ranks_that_no_kernel_has_are_refused_at_once():
+    """Before a forward pass has counted tokens that it cannot take."""
+    from tokamak_b200 import TkbError, configs, generate
+    cfg = dict(configs.C1, layers=1)
+
+    def build(R):
+        return generate.Adapters(cfg, [dict(wo=(np.zeros((3, 256, R), np.float32), np.zeros((3, R, 256), np.float32)))])
+    for R in (8, 24, 128):
+        assert build(R).rank == R
+    for R in (0, 4, 12, 136, 256):
+        with pytest.raises(TkbError, match="rank"):
+            build(R)
+    with pytest.raises(TkbError):
+        generate.Adapters(cfg, [dict(wo=(np.zeros((0, 256, 8), np.float32), np.zeros((0, 8, 256), np.float32)))])

@@ -63,8 +63,10 @@ ADAPTED = ("wqkv", "wo", "wgu", "wd")  # the projections of a layer that may hav
 
 class Adapters:
     """Low-rank adapters of a configuration's layers: layers[i][name] = (A [n, in, R], B [n, R, out]) for the projections
-    of layer i that have them (names of ADAPTED; wgu is the fused [gate | up] matrix), all of n adapters and one rank;
-    scale [n] is usually alpha / R."""
+    of layer i that have them (names of ADAPTED; wgu is the fused [gate | up] matrix), all of n adapters and one rank, a
+    multiple of 8 up to 128; scale [n] is usually alpha / R.  Where a layer has adapters of wgu, its gate and up values are
+    rounded to bf16 once more for every sequence, also for those without one: the adapters' sum comes between the matrix
+    and the activation."""
 
     def __init__(self, cfg, layers, scale=None):
         d, F = cfg["d_model"], cfg["ffn"]
@@ -74,6 +76,8 @@ class Adapters:
         if len(layers) != cfg["layers"] or first is None or np.ndim(first) != 3:
             raise TkbError("Adapters: one dictionary of (A, B) for every layer, one of them at least")
         self.n, _, self.rank = first.shape
+        if self.n < 1 or self.rank % 8 or not 8 <= self.rank <= 128:
+            raise TkbError(f"Adapters: {self.n} of rank {self.rank}; one at least, and ranks are multiples of 8 up to 128")
         for w in layers:
             for name, (a, b) in w.items():
                 if name not in sizes:
