@@ -293,3 +293,14 @@ def test_adapters_of_ranks_that_no_kernel_has_are_refused_at_once():
             build(R)
     with pytest.raises(TkbError):
         generate.Adapters(cfg, [dict(wo=(np.zeros((0, 256, 8), np.float32), np.zeros((0, 8, 256), np.float32)))])
+
+
+def test_arrays_beside_an_adapters_are_not_passed_over(tmp_path):
+    """A misnamed array beside a good pair would be left out without a word."""
+    from tokamak_b200 import TkbError, configs, generate
+    cfg, path = dict(configs.C1, layers=1), tmp_path / "a.npz"
+    a, b = np.zeros((3, 256, 8), np.float32), np.zeros((3, 8, 256), np.float32)
+    for name in ("0.wo.", "0.wo.AB", "0.wo.C", "00.wo.A", "².wo.A"):
+        np.savez(path, **{"0.wo.A": a, "0.wo.B": b, name: a})
+        with pytest.raises(TkbError, match="unexpected array"):
+            generate.Adapters.load(cfg, path)

@@ -99,7 +99,7 @@ class Adapters:
                 part = key.split(".")
                 if key == "scale":
                     continue
-                if len(part) != 3 or part[2] not in "AB" or not part[0].isdigit() or int(part[0]) >= len(layers) or \
+                if len(part) != 3 or part[2] not in ("A", "B") or part[0] not in map(str, range(len(layers))) or \
                         f"{part[0]}.{part[1]}.{'B' if part[2] == 'A' else 'A'}" not in f.files:
                     raise TkbError(f"{path}: unexpected array {key}")
                 if part[2] == "A":
