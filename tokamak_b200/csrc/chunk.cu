@@ -20,13 +20,14 @@
 // TMEM (512 columns): S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [256+D,256+2D),
 // P as 16-bit pairs over the first half of S.
 //
-// Measured: 2 x 1.5-1.8 k tokens over 14-16 k, 64/8 heads of 128, bf16: 1710 us, 910
-// TFLOP/s (2.6 us a block of 256 rows x 128 slots; the chain S, softmax, P V bounds
-// it, as it does the prompt's own attention).  8 x 3-6 tokens over 12-16 k (471 MB):
-// 99 us, 0.73 of HBM.  32 ragged sequences up to 2048 with 1-100 tokens, 32/8 x 64:
-// 93.5 us: 8 us until the first scores, 4-5 a unit.  fp32, 3 x 1-129 tokens over
-// 300-1025, 16 heads of 128: 153 us, FMA issue.  A warp a (row, head), slot by slot,
-// took 309 ms, 92 ms, 9.0 ms and 0.9 ms.
+// Measured: 2 x 1.5-1.8 k tokens over 14-16 k, 64/8 heads of 128, bf16: 1755-1800 us
+// (SM clock 1.66-1.6 GHz under the power limit), 890-865 TFLOP/s (2.6 us a block of
+// 256 rows x 128 slots; the chain S, softmax, P V bounds it, as it does the prompt's
+// own attention).  8 x 3-6 tokens over 12-16 k (471 MB): 101-107 us, 0.67-0.71 of
+// HBM.  32 ragged sequences up to 2048 with 1-100 tokens, 32/8 x 64: 92 us: 8 us
+// until the first scores, 4-5 a unit.  fp32, 3 x 1-129 tokens over 300-1025, 16 heads of 128: 154 us, with issue
+// slots 42 % and the FMA pipe 27 % busy: eight warps an SM do not fill them.  A warp
+// a (row, head), slot by slot, took 309 ms, 92 ms, 9.0 ms and 0.9 ms.
 #include "tkb_common.cuh"
 #include "../../include/tkm_b200.h"
 
@@ -40,7 +41,12 @@ TKB_DEVFN void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: 
 // at most 16 rows; a unit on top (its queries' load, its rows' output); and a
 // CTA's run at least, unless it has a unit of its own (shorter parts cost more
 // to join than they save).  In 16 bits a block of one tile is a warpgroup's, of
-// two both's; in fp32 the rows' products are what takes time.
+// two both's; in fp32 the rows' products are what takes time.  Other 16-bit weights,
+// us for 32 ragged sequences, 8 x 3-6 tokens over 12-16 k, 8 prompts of 1000-2048:
+//   as below 92, 100, 186      unit 0   135, 103, 214    unit 2  99, 102, 195
+//   unit 8   92,  98, 187      pair 1    96, 102, 190    one 2   99, 136, 190
+// least: one sequence of 5 tokens over 333 16 us, 20 with 4, 16 with 24; the others
+// are the same with 4 to 48.
 struct ChunkCost {
   int pair, one, few, unit, least;
 };
@@ -362,7 +368,11 @@ TKB_DEVFN void wait_ld16_dep(uint32_t (&r)[16]) {
 // running maximum raised when this block's exceeds it by more than 8
 // (rescaling O in TMEM), P written over S in two halves, release(h) once half
 // h is in TMEM.  P is rounded to the type (half a step; the row sum is that of
-// the unrounded values).
+// the unrounded values): the error against 64 bits is 0.0021-0.0023 in bf16 where
+// the output's own rounding is 0.0016-0.0017.  P in two 16-bit parts and a second
+// product with V, in units of one tile alone, leave the output's rounding, but
+// their instructions take 32 ragged sequences from 92 to 142 us, 8 x 3-6 tokens
+// over 12-16 k from 101 to 141 and 64 single tokens from 87 to 143.
 template <int D, bool BF16, typename Release>
 TKB_DEVFN void chunk_softmax(uint32_t tS, uint32_t tO, float sl2, bool first, bool cut, int lim, unsigned there,
                              float& m_used, float& l, Release&& release) {
@@ -1165,9 +1175,9 @@ __global__ void __launch_bounds__(128) chunk_join_kernel(const __grid_constant__
 // Thread (tr, tc) of 16 x 16 has rows tr + 16 i, i < MR, and slots tc + 16 e of the scores,
 // and columns 4 tc .. 4 tc + 3 of every 64 of the output, so that a row's
 // scores, weights and sums stay in one half of a warp.  MR follows the unit's
-// rows: with 128 of them FMA issue bounds it, with 16 or fewer the reads of K
-// and V from shared memory.  8 sequences of 2-4 k, 8 kv heads of 128: 4 tokens x 2
-// heads 174 us (MR 1; 294 with 4, 521 with 8), 30 x 2 454 us (MR 4; 8: 782).
+// rows: with few of them the reads of K and V from shared memory are most of it.
+// 8 sequences of 2-4 k, 8 kv heads of 128: 4 tokens x 2 heads 174 us (MR 1; 294 with
+// 4, 521 with 8), 30 x 2 454 us (MR 4; 8: 782).
 template <int D>
 struct ChunkF32 {
   static constexpr int TS = 64;                            // slots at a time

@@ -807,7 +807,8 @@ __global__ void __launch_bounds__(kLoraThreads) lora_up_f32_kernel(const __grid_
 // ------------------------------------------------------------ launches
 static int lora_rank(int R) { return R <= 16 ? 16 : R <= 64 ? 64 : 128; }
 
-// CTAs that run at the same time, by their shared memory.
+// CTAs that run at the same time, by their shared memory; twelve an SM at most, by the registers of the kernels that need
+// little of it (fp32, 40 a thread).
 constexpr int lora_resident(int smem) { return 148 * (232448 / (smem + 1280) < 12 ? 232448 / (smem + 1280) : 12); }
 
 template <typename T, int RP, int TM>
@@ -815,7 +816,9 @@ static cudaError_t lora_launch(LoraParams& p, int tiles, cudaStream_t st, unsign
   const int cols = (p.N + 63) / 64;
   p.splits = 1;
   if constexpr (TM == 16 && sizeof(T) == 2) {
-    // clusters until there are four CTAs an SM, of a chunk of K and of columns each at least
+    // Clusters until there are four CTAs an SM, of a chunk of K and of columns each at least.  One, two, four and eight parts,
+    // 64 tokens of 16 adapters of 16: K 5632, N 2048 22.6, 13.1, 8.0 and 6.5 us; 1024 x 1024 8.1, 5.8, 4.4, 4.8; 256 x 256 3.4,
+    // 4.0, 3.9, 4.6; 256 tokens of 64 adapters, 2048 x 2048 14.8, 9.4, 7.6, 10.9 (four are the rule's).
     while (p.splits < 8 && tiles * 2ll * p.splits <= 148 * 4 && p.K >= 128 * p.splits && cols >= 2 * p.splits) p.splits *= 2;
     p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
     p.chunks = (cols + p.splits - 1) / p.splits;
@@ -826,10 +829,13 @@ static cudaError_t lora_launch(LoraParams& p, int tiles, cudaStream_t st, unsign
   } else {
     // Parts of K: as many CTAs as run at the same time (a few more would be a second wave of their own), each of at
     // least 256 columns, a cluster of eight at most.  12.4 k rows of 2048 and 5632 columns, R = 16: 19 and 45 us in 1.1
-    // waves, 15 and 35 in less than one.
+    // waves, 15 and 35 in less than one.  Both kernels with one, two, four and eight parts: 1.6 k rows of 33 adapters of 64,
+    // 4096 x 4096 86, 49, 39 and 31 us; 800 rows of 8 of 16, K 2048 24.4, 14.2, 9.5, 8.4; K 1024 11.4, 8.5, 7.5, 7.1; K 512
+    // 7.6, 7.2, 6.1, 6.1 (four and two are the rule's: short sums leave a microsecond, of which fewer CTAs take less room).
     while (p.splits < 8 && tiles * 2ll * p.splits <= lora_resident(LoraDown<T, RP, TM>::SMEM) && p.K >= 512 * p.splits) p.splits *= 2;
     p.k_per = ((p.K + p.splits - 1) / p.splits + 63) / 64 * 64;
-    // columns of out per CTA: up to 512, while there are three waves of CTAs
+    // Columns of out per CTA: up to 512, while there are three waves of CTAs.  64, 128, 256 and 512 of them: 12 k rows, N
+    // 11264 138, 116, 110 and 113 us with x A (the rule: 108); 800 rows, N 2048 8.4, 9.5, 10.5, 14.3 (the rule: 8.4).
     const long long fit = static_cast<long long>(tiles) * cols / (3 * lora_resident(LoraUp<T, RP, TM>::SMEM));
     p.chunks = fit < 1 ? 1 : fit > 8 ? 8 : static_cast<int>(fit);
     const dim3 down(p.splits, tiles), up((cols + p.chunks - 1) / p.chunks, tiles);
